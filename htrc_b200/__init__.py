@@ -6,8 +6,11 @@ sm_100a kernels.  See include/htrc_flat.h for the C ABI.
 """
 from .flat import (PROD, dequant_rows, fake_quant, flat_attention, flat_attention_heads,  # noqa: F401
                    flat_attention_prod, forward_into, run_stages, workspace_bytes)
+from .rotary import (grid_positions, rotary_axes, rotary_axes_backward, rotary_qk,  # noqa: F401
+                     rotary_qk_backward)
 from .runner import CHUNKS, MODES, FlatRunner, plan_chunk, predicted_peak_mib  # noqa: F401
 
 __all__ = ["PROD", "MODES", "CHUNKS", "flat_attention", "flat_attention_heads", "flat_attention_prod", "FlatRunner",
            "plan_chunk",
-           "predicted_peak_mib", "run_stages", "workspace_bytes", "forward_into", "fake_quant", "dequant_rows"]
+           "predicted_peak_mib", "run_stages", "workspace_bytes", "forward_into", "fake_quant", "dequant_rows",
+           "grid_positions", "rotary_axes", "rotary_axes_backward", "rotary_qk", "rotary_qk_backward"]

@@ -1,4 +1,5 @@
-"""ctypes binding of libhtrc_flat.so (the C ABI declared in include/htrc_flat.h and include/htrc_tree.h).
+"""ctypes binding of libhtrc_flat.so (the C ABI declared in include/htrc_flat.h, include/htrc_tree.h
+and include/htrc_layer.h).
 
 The library is built in-tree (``python -m htrc_b200.build``) and loaded from this package directory.
 There is no fallback: if the library is missing, every operator call raises.
@@ -53,7 +54,30 @@ class HtrcTreeDims(ctypes.Structure):
 TREE_MAX_LEVELS, TREE_MAX_CENTRES, TREE_KMEANS_CENTRES = 16, 256, 32
 TREE_STAGE_ACCEPT, TREE_STAGE_LEAVES, TREE_STAGE_FINAL, TREE_STAGE_ALL = 1, 2, 4, 7
 
-# name -> (restype, argtypes); every symbol include/htrc_flat.h and include/htrc_tree.h declare
+# element types of include/htrc_layer.h
+LAYER_F32, LAYER_BF16, LAYER_F16, LAYER_I32 = range(4)
+ROTARY_MAX_AXES, ROTARY_MAX_DIM, ROTARY_MAX_HEADS = 4, 256, 1024
+ROTARY_PAIRS = {"interleaved": 0, "half": 1}
+_i64x3 = _i64 * 3
+
+
+class HtrcRotaryTensor(ctypes.Structure):
+    """Mirror of include/htrc_layer.h HtrcRotaryTensor."""
+    _fields_ = [("in_", _p), ("in_stride", _i64x3), ("out", _p), ("out_stride", _i64x3), ("x", _p),
+                ("x_stride", _i64x3), ("weight", _p), ("dweight", _p), ("weight_dtype", _i32), ("heads", _i32)]
+
+
+class HtrcRotaryArgs(ctypes.Structure):
+    """Mirror of include/htrc_layer.h HtrcRotaryArgs."""
+    _fields_ = [("tensor", HtrcRotaryTensor * 2), ("n_tensors", _i32), ("dtype", _i32), ("batch", _i64),
+                ("tokens", _i64), ("dim", _i32), ("n_axes", _i32), ("axis_width", _i32 * 4), ("pairs", _i32),
+                ("positions", _p), ("position_dtype", _i32), ("position_stride", _i64x3), ("theta", ctypes.c_double),
+                ("freqs", ctypes.POINTER(ctypes.c_double)), ("eps", _f32), ("workspace", _p),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
+# name -> (restype, argtypes); every symbol include/htrc_flat.h, include/htrc_tree.h and include/htrc_layer.h
+# declare
 SIGNATURES = {
     "htrc_leaf_pitch": (_i64, [_i64]),
     "htrc_flat_workspace_size": (ctypes.c_int, [ctypes.POINTER(HtrcFlatArgs), ctypes.POINTER(ctypes.c_size_t)]),
@@ -105,6 +129,10 @@ SIGNATURES = {
                                         ctypes.c_size_t, _p, _p, _p, _i32, _p]),
     "htrc_tree_centres_scratch_size": (ctypes.c_int, [_i64, ctypes.POINTER(ctypes.c_size_t)]),
     "htrc_tree_centres": (ctypes.c_int, [_p, _i32, _i64, _f32, _p, _p, _p, ctypes.c_size_t, _p]),
+    # operators around the flat attention (include/htrc_layer.h)
+    "htrc_rotary_forward": (ctypes.c_int, [ctypes.POINTER(HtrcRotaryArgs), _p]),
+    "htrc_rotary_workspace_size": (ctypes.c_int, [ctypes.POINTER(HtrcRotaryArgs), ctypes.POINTER(ctypes.c_size_t)]),
+    "htrc_rotary_backward": (ctypes.c_int, [ctypes.POINTER(HtrcRotaryArgs), _p]),
 }
 
 _lib = None

@@ -6,6 +6,13 @@
 
 namespace htrc {
 
+// the current device, and the tensor-map encoder, for the C entries outside api.cu (defined there)
+bool device_ok();
+int sm_count();
+// rank-2..5 tiled map; dims innermost first, strides in bytes for dims 1..rank-1
+bool make_tiled_map(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
+                    const uint64_t* strides, const uint32_t* box, bool swizzle128);
+
 // precision "tf32": a float32 operand's value as the tensor cores read it in tf32 (low 13 mantissa bits cleared)
 constexpr uint32_t kTf32Mask = 0xFFFFE000u;
 

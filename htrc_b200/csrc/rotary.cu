@@ -1,0 +1,596 @@
+// Rotary positions over several axes, with the per-head RMS norm before them, forward and backward, and the
+// C entries of include/htrc_layer.h for them.
+//
+// Forward, per row of dim elements (one token, one head):  u = x * rsqrt(mean(x^2) + eps) * w  (or u = x), then
+// every pair (a, b) of the rotated width becomes (a cos - b sin, a sin + b cos).  Backward:  g = the transposed
+// rotation of dy;  dw = sum g x r;  h = g w;  dx = r (h - x r^2 mean(h x)),  r = rsqrt(mean(x^2) + eps).
+//
+// Both only move bytes: a row is read once and written once (backward with a norm: two reads), all arithmetic is
+// float32 in registers.  A warp holds 32 / LPR rows of one token at a time, LPR lanes of 8 elements each, and walks
+// the heads of its token, so the 4 cosines and sines that a lane needs are computed once per token and stay in
+// registers.  The output's strides carry the token-major -> head-major reorder.
+//
+// Angles: an int32 position times the frequency in revolutions as a 64-bit fixed-point fraction, modulo 2^64, is the
+// exactly reduced turn for every int32 position (float32 positions: the product in two floats, its whole turns
+// dropped), so late positions lose no accuracy.
+#include <cmath>
+
+#include "../../include/htrc_layer.h"
+#include "common.cuh"
+#include "kernels.cuh"
+
+namespace htrc {
+
+namespace {
+
+constexpr int kRotWarps = 8;
+constexpr int kRotMaxPairs = HTRC_ROTARY_MAX_DIM / 2;
+constexpr int kRotUnroll = 4;         // row batches whose loads are in flight together
+
+struct RotaryRows {
+  const void* in;
+  void* out;
+  const void* x;
+  const void* weight;
+  int64_t is[3], os[3], xs[3];
+  int heads, weight_dtype;
+  int chunk, chunks;                  // heads per task, tasks per token
+};
+
+struct RotaryParams {
+  RotaryRows t[2];
+  const void* positions;
+  int64_t ps[3];
+  int64_t batch, tokens;
+  int dim, npairs;
+  float eps;
+  bool float_positions;
+  uint64_t turn[kRotMaxPairs];        // frequency in revolutions: 0.64 fixed point, or (hi, lo) floats
+  uint8_t axis[kRotMaxPairs];
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ float load_weight(const void* w, int dtype, int i) {
+  if (dtype == HTRC_LAYER_F32) return __ldg(static_cast<const float*>(w) + i);
+  if (dtype == HTRC_LAYER_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
+  return __half2float(static_cast<const __half*>(w)[i]);
+}
+
+// cosine and sine of pair i of a token whose positions start at pos
+__device__ __forceinline__ float2 pair_turn(const RotaryParams& p, int64_t pos, int i) {
+  const int64_t at = pos + p.axis[i] * p.ps[2];
+  const uint64_t f = p.turn[i];
+  float turns;
+  if (!p.float_positions) {
+    const int32_t n = __ldg(static_cast<const int32_t*>(p.positions) + at);
+    const uint64_t frac = static_cast<uint64_t>(static_cast<int64_t>(n)) * f;      // modulo one revolution
+    turns = static_cast<float>(static_cast<int32_t>(frac >> 32)) * 0x1p-32f;
+  } else {
+    const float n = __ldg(static_cast<const float*>(p.positions) + at);
+    const float hi = __uint_as_float(static_cast<uint32_t>(f >> 32)), lo = __uint_as_float(static_cast<uint32_t>(f));
+    const float t = n * hi;
+    turns = (t - rintf(t)) + fmaf(n, lo, fmaf(n, hi, -t));
+  }
+  float s, c;
+  sincospif(2.0f * turns, &s, &c);
+  return make_float2(c, s);
+}
+
+// A lane's 8 elements of a row: two groups of 4 at off0 and off1 (16-bit types: 8 bytes each, float32: 16).
+// Interleaved pairs: off1 = off0 + 4, one contiguous piece.
+template <typename T>
+struct Raw {
+  uint4 a;
+};
+template <>
+struct Raw<float> {
+  uint4 a, b;
+};
+template <typename T, bool HALF>
+__device__ __forceinline__ Raw<T> load_raw(const T* row, int off0, int off1) {
+  Raw<T> r;
+  if constexpr (sizeof(T) == 4) {
+    r.a = __ldg(reinterpret_cast<const uint4*>(row + off0));
+    r.b = __ldg(reinterpret_cast<const uint4*>(row + off1));
+  } else if constexpr (HALF) {
+    const uint2 lo = __ldg(reinterpret_cast<const uint2*>(row + off0));
+    const uint2 hi = __ldg(reinterpret_cast<const uint2*>(row + off1));
+    r.a = make_uint4(lo.x, lo.y, hi.x, hi.y);
+  } else {
+    r.a = __ldg(reinterpret_cast<const uint4*>(row + off0));
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) { return pack_f16x2(a, b); }
+
+template <typename T>
+__device__ __forceinline__ void unpack(const Raw<T>& r, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    v[0] = __uint_as_float(r.a.x); v[1] = __uint_as_float(r.a.y); v[2] = __uint_as_float(r.a.z);
+    v[3] = __uint_as_float(r.a.w); v[4] = __uint_as_float(r.b.x); v[5] = __uint_as_float(r.b.y);
+    v[6] = __uint_as_float(r.b.z); v[7] = __uint_as_float(r.b.w);
+  } else {
+    const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack2<T>(w[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+}
+template <typename T, bool HALF>
+__device__ __forceinline__ void store8(T* row, int off0, int off1, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(row + off0) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(row + off1) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    const uint4 w = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+    if constexpr (HALF) {
+      *reinterpret_cast<uint2*>(row + off0) = make_uint2(w.x, w.y);
+      *reinterpret_cast<uint2*>(row + off1) = make_uint2(w.z, w.w);
+    } else {
+      *reinterpret_cast<uint4*>(row + off0) = w;
+    }
+  }
+}
+
+// Rotates a lane's 8 elements in place; turned pairs only (a pair past the rotated width stays, whatever it holds).
+// HALF: pairs (v[i], v[4 + i]), all 4 turned or none; else (v[2 i], v[2 i + 1]), the first n turned.  BACK: by -angle.
+template <bool HALF, bool BACK>
+__device__ __forceinline__ void turn8(float (&v)[8], const float2 (&cs)[4], int n) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int ia = HALF ? i : 2 * i, ib = HALF ? i + 4 : 2 * i + 1;
+    const float a = v[ia], b = v[ib], c = cs[i].x, s = BACK ? -cs[i].y : cs[i].y;
+    if (i < n) {
+      v[ia] = fmaf(a, c, -b * s);
+      v[ib] = fmaf(a, s, b * c);
+    }
+  }
+}
+
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Rows whose pieces are 16-byte aligned, dim a multiple of 8 (HALF: the rotated width too).  blockIdx.y names the
+// tensor; a warp's task is a token and `chunk` of its heads.  BACK with a weight leaves the CTA's weight-gradient sums
+// at partial[(blockIdx.y * gridDim.x + blockIdx.x) * dim].
+template <typename T, int LPR, bool HALF, bool BACK>
+__global__ void __launch_bounds__(kRotWarps * 32)
+    rotary_kernel(const __grid_constant__ RotaryParams p, float* __restrict__ partial) {
+  __shared__ float sums[BACK ? kRotWarps * 32 * 8 : 1];
+  const RotaryRows& r = p.t[blockIdx.y];
+  constexpr int RPW = 32 / LPR;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int u = lane % LPR, sub = lane / LPR;
+  const int units = p.dim / 8;
+  const bool on = u < units;
+  // the lane's elements and the pairs they make
+  int off0 = 8 * u, off1 = 8 * u + 4, pair0 = 4 * u, turned;
+  if (HALF) {
+    const int rot = p.npairs / 4;
+    turned = u < rot ? 4 : 0;
+    if (u < rot) {
+      off0 = 4 * u;
+      off1 = p.npairs + 4 * u;
+    }
+  } else {
+    turned = min(4, max(0, p.npairs - pair0));
+  }
+  if (!on) turned = 0;
+  const bool norm = r.weight != nullptr;
+  float w[8], dw[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w[i] = norm && on ? load_weight(r.weight, r.weight_dtype, (i < 4 ? off0 : off1 - 4) + i) : 0.f;
+    dw[i] = 0.f;
+  }
+  const float inv_dim = 1.0f / static_cast<float>(p.dim);
+  const int64_t tasks = p.batch * p.tokens * r.chunks;
+  for (int64_t task = static_cast<int64_t>(blockIdx.x) * kRotWarps + warp; task < tasks;
+       task += static_cast<int64_t>(gridDim.x) * kRotWarps) {
+    const int64_t tok = task / r.chunks;
+    const int h0 = static_cast<int>(task - tok * r.chunks) * r.chunk, h1 = min(r.heads, h0 + r.chunk);
+    const int64_t b = tok / p.tokens, n = tok - b * p.tokens;
+    const T* in = static_cast<const T*>(r.in) + b * r.is[0] + n * r.is[1];
+    const T* x = BACK && norm ? static_cast<const T*>(r.x) + b * r.xs[0] + n * r.xs[1] : nullptr;
+    T* out = static_cast<T*>(r.out) + b * r.os[0] + n * r.os[1];
+    float2 cs[4];
+    const int64_t pos = b * p.ps[0] + n * p.ps[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cs[i] = i < turned ? pair_turn(p, pos, pair0 + i) : make_float2(1.f, 0.f);
+    for (int h = h0; h < h1; h += RPW * kRotUnroll) {
+      Raw<T> raw[kRotUnroll], rawx[BACK ? kRotUnroll : 1];
+#pragma unroll
+      for (int k = 0; k < kRotUnroll; ++k) {
+        const int hh = h + k * RPW + sub;
+        if (on && hh < h1) {
+          raw[k] = load_raw<T, HALF>(in + hh * r.is[2], off0, off1);
+          if (BACK && norm) rawx[k] = load_raw<T, HALF>(x + hh * r.xs[2], off0, off1);
+        } else {
+          raw[k] = Raw<T>{};
+          if (BACK) rawx[k] = Raw<T>{};
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kRotUnroll; ++k) {
+        const int hh = h + k * RPW + sub;
+        float v[8];
+        unpack<T>(raw[k], v);
+        if (!BACK) {
+          if (norm) {
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+            const float rs = rsqrtf(row_sum<LPR>(ss) * inv_dim + p.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = v[i] * rs * w[i];
+          }
+          turn8<HALF, false>(v, cs, turned);
+        } else {
+          turn8<HALF, true>(v, cs, turned);
+          if (norm) {
+            float xv[8], ss = 0.f, hx = 0.f;
+            unpack<T>(rawx[k], xv);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              ss = fmaf(xv[i], xv[i], ss);
+              hx = fmaf(v[i] * w[i], xv[i], hx);
+            }
+            const float rs = rsqrtf(row_sum<LPR>(ss) * inv_dim + p.eps);
+            const float back = row_sum<LPR>(hx) * inv_dim * rs * rs;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              dw[i] = fmaf(v[i], xv[i] * rs, dw[i]);
+              v[i] = rs * fmaf(-xv[i], back, v[i] * w[i]);
+            }
+          }
+        }
+        if (on && hh < h1) store8<T, HALF>(out + hh * r.os[2], off0, off1, v);
+      }
+    }
+  }
+  if (BACK && norm) {
+    // the CTA's sums, rows of a warp and then warps in order
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sums[threadIdx.x * 8 + i] = dw[i];
+    __syncthreads();
+    float* dst = partial + (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * p.dim;
+    if (threadIdx.x < LPR && on) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float s = 0.f;
+        for (int g = 0; g < kRotWarps * RPW; ++g) s += sums[(g * LPR + u) * 8 + i];
+        dst[(i < 4 ? off0 : off1 - 4) + i] = s;
+      }
+    }
+  }
+}
+
+// Any dim, alignment and rotated width: a warp per row, one element per lane and step, the normalised row in shared
+// memory while its pairs are formed.
+template <typename T, bool BACK>
+__global__ void __launch_bounds__(kRotWarps * 32)
+    rotary_any_kernel(const __grid_constant__ RotaryParams p, bool half, float* __restrict__ partial) {
+  constexpr int kMax = HTRC_ROTARY_MAX_DIM, kEl = kMax / 32;
+  __shared__ float rows[kRotWarps][kMax];
+  const RotaryRows& r = p.t[blockIdx.y];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool norm = r.weight != nullptr;
+  float dw[kEl];
+#pragma unroll
+  for (int k = 0; k < kEl; ++k) dw[k] = 0.f;
+  const float inv_dim = 1.0f / static_cast<float>(p.dim);
+  const int64_t tasks = p.batch * p.tokens * r.heads;
+  for (int64_t task = static_cast<int64_t>(blockIdx.x) * kRotWarps + warp; task < tasks;
+       task += static_cast<int64_t>(gridDim.x) * kRotWarps) {
+    const int64_t tok = task / r.heads, h = task - tok * r.heads, b = tok / p.tokens, n = tok - b * p.tokens;
+    const T* in = static_cast<const T*>(r.in) + b * r.is[0] + n * r.is[1] + h * r.is[2];
+    T* out = static_cast<T*>(r.out) + b * r.os[0] + n * r.os[1] + h * r.os[2];
+    const int64_t pos = b * p.ps[0] + n * p.ps[1];
+    float v[kEl], ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < kEl; ++k) {
+      const int e = lane + 32 * k;
+      v[k] = e < p.dim ? to_f<T>(in[e]) : 0.f;
+      ss = fmaf(v[k], v[k], ss);
+    }
+    if (!BACK && norm) {
+      const float rs = rsqrtf(row_sum<32>(ss) * inv_dim + p.eps);
+#pragma unroll
+      for (int k = 0; k < kEl; ++k) {
+        const int e = lane + 32 * k;
+        if (e < p.dim) v[k] *= rs * load_weight(r.weight, r.weight_dtype, e);
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < kEl; ++k) rows[warp][lane + 32 * k] = v[k];
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < kEl; ++k) {
+      const int e = lane + 32 * k;
+      if (e < 2 * p.npairs) {
+        const int i = half ? (e < p.npairs ? e : e - p.npairs) : e >> 1;
+        const bool second = half ? e >= p.npairs : (e & 1);
+        const float other = rows[warp][half ? (second ? i : i + p.npairs) : e ^ 1];
+        const float2 cs = pair_turn(p, pos, i);
+        const float s = (BACK != second) ? cs.y : -cs.y;     // forward: a c - b s and b c + a s
+        v[k] = fmaf(v[k], cs.x, other * s);
+      }
+    }
+    if (BACK && norm) {
+      const T* x = static_cast<const T*>(r.x) + b * r.xs[0] + n * r.xs[1] + h * r.xs[2];
+      float xv[kEl], hx = 0.f;
+      ss = 0.f;
+#pragma unroll
+      for (int k = 0; k < kEl; ++k) {
+        const int e = lane + 32 * k;
+        xv[k] = e < p.dim ? to_f<T>(x[e]) : 0.f;
+        ss = fmaf(xv[k], xv[k], ss);
+        if (e < p.dim) hx = fmaf(v[k] * load_weight(r.weight, r.weight_dtype, e), xv[k], hx);
+      }
+      const float rs = rsqrtf(row_sum<32>(ss) * inv_dim + p.eps);
+      const float back = row_sum<32>(hx) * inv_dim * rs * rs;
+#pragma unroll
+      for (int k = 0; k < kEl; ++k) {
+        const int e = lane + 32 * k;
+        if (e < p.dim) {
+          dw[k] = fmaf(v[k], xv[k] * rs, dw[k]);
+          v[k] = rs * fmaf(-xv[k], back, v[k] * load_weight(r.weight, r.weight_dtype, e));
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kEl; ++k) {
+      const int e = lane + 32 * k;
+      if (e < p.dim) out[e] = from_f<T>(v[k]);
+    }
+  }
+  if (BACK && norm) {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kEl; ++k) rows[warp][lane + 32 * k] = dw[k];
+    __syncthreads();
+    float* dst = partial + (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * p.dim;
+    for (int e = threadIdx.x; e < p.dim; e += blockDim.x) {
+      float s = 0.f;
+      for (int g = 0; g < kRotWarps; ++g) s += rows[g][e];
+      dst[e] = s;
+    }
+  }
+}
+
+// dweight[e] = the CTAs' partial sums in a fixed order: 32 interleaved sums, then those
+__global__ void __launch_bounds__(1024)
+    rotary_weight_kernel(const float* __restrict__ partial, int blocks, int dim, void* dw0, int dt0, void* dw1, int dt1) {
+  __shared__ float part[32][33];
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const int e = blockIdx.x * 32 + lane;
+  void* dst = blockIdx.y ? dw1 : dw0;
+  const int dt = blockIdx.y ? dt1 : dt0;
+  if (dst == nullptr) return;
+  const float* src = partial + static_cast<int64_t>(blockIdx.y) * blocks * dim;
+  float s = 0.f;
+  if (e < dim)
+    for (int g = row; g < blocks; g += 32) s += src[static_cast<int64_t>(g) * dim + e];
+  part[row][lane] = s;
+  __syncthreads();
+  if (row == 0 && e < dim) {
+    s = 0.f;
+    for (int g = 0; g < 32; ++g) s += part[g][lane];
+    if (dt == HTRC_LAYER_F32) static_cast<float*>(dst)[e] = s;
+    else if (dt == HTRC_LAYER_BF16) static_cast<__nv_bfloat16*>(dst)[e] = __float2bfloat16_rn(s);
+    else static_cast<__half*>(dst)[e] = __float2half_rn(s);
+  }
+}
+
+constexpr int kRotBlocksPerSm = 8;      // 256-thread CTAs per SM the grids are sized for
+
+int rotary_max_blocks() { return sm_count() * kRotBlocksPerSm; }
+
+int rotary_validate(const HtrcRotaryArgs* a, bool back, bool ptrs) {
+  if (a == nullptr || a->n_tensors < 1 || a->n_tensors > 2) return HTRC_ERR_ARG;
+  if (a->dtype < HTRC_LAYER_F32 || a->dtype > HTRC_LAYER_F16) return HTRC_ERR_ARG;
+  if (a->batch < 0 || a->tokens < 0) return HTRC_ERR_ARG;
+  if (a->tokens > 0 && a->batch > (int64_t(1) << 40) / a->tokens) return HTRC_ERR_ARG;
+  if (a->dim < 2 || a->n_axes < 1) return HTRC_ERR_ARG;
+  if (a->dim > HTRC_ROTARY_MAX_DIM || a->n_axes > HTRC_ROTARY_MAX_AXES) return HTRC_ERR_UNSUPPORTED;
+  int64_t width = 0;
+  for (int i = 0; i < a->n_axes; ++i) {
+    if (a->axis_width[i] < 0 || a->axis_width[i] % 2) return HTRC_ERR_ARG;
+    width += a->axis_width[i];
+  }
+  if (width > a->dim) return HTRC_ERR_ARG;
+  if (a->pairs != HTRC_ROTARY_INTERLEAVED && a->pairs != HTRC_ROTARY_HALF) return HTRC_ERR_ARG;
+  if (a->position_dtype != HTRC_LAYER_I32 && a->position_dtype != HTRC_LAYER_F32) return HTRC_ERR_ARG;
+  if (a->freqs == nullptr && !(a->theta > 0.0 && std::isfinite(a->theta))) return HTRC_ERR_ARG;
+  if (!(a->eps >= 0.0f) || !std::isfinite(a->eps)) return HTRC_ERR_ARG;
+  for (int i = 0; i < a->n_tensors; ++i) {
+    const HtrcRotaryTensor& t = a->tensor[i];
+    if (t.heads < 1) return HTRC_ERR_ARG;
+    if (t.heads > HTRC_ROTARY_MAX_HEADS) return HTRC_ERR_UNSUPPORTED;
+    if (t.weight_dtype < HTRC_LAYER_F32 || t.weight_dtype > HTRC_LAYER_F16) return HTRC_ERR_ARG;
+    if (!ptrs || a->batch * a->tokens == 0) continue;
+    if (!t.in || !t.out || !a->positions) return HTRC_ERR_ARG;
+    if (back && t.weight && (!t.x || !t.dweight)) return HTRC_ERR_ARG;
+  }
+  return HTRC_OK;
+}
+
+bool aligned16(const void* p, const int64_t* s, int es) {
+  if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  for (int i = 0; i < 3; ++i)
+    if (s[i] * es % 16) return false;
+  return true;
+}
+
+template <typename T, int LPR, bool HALF, bool BACK>
+void run_rows(const RotaryParams& p, dim3 grid, float* partial, cudaStream_t st) {
+  rotary_kernel<T, LPR, HALF, BACK><<<grid, kRotWarps * 32, 0, st>>>(p, partial);
+}
+
+template <typename T, bool BACK>
+void run_dim(const RotaryParams& p, bool half, dim3 grid, float* partial, cudaStream_t st) {
+  if (p.dim <= 64) {
+    half ? run_rows<T, 8, true, BACK>(p, grid, partial, st) : run_rows<T, 8, false, BACK>(p, grid, partial, st);
+  } else if (p.dim <= 128) {
+    half ? run_rows<T, 16, true, BACK>(p, grid, partial, st) : run_rows<T, 16, false, BACK>(p, grid, partial, st);
+  } else {
+    half ? run_rows<T, 32, true, BACK>(p, grid, partial, st) : run_rows<T, 32, false, BACK>(p, grid, partial, st);
+  }
+}
+
+template <bool BACK>
+int rotary_run(const HtrcRotaryArgs* a, cudaStream_t st) {
+  int rc = rotary_validate(a, BACK, true);
+  if (rc != HTRC_OK) return rc;
+  if (!device_ok()) return HTRC_ERR_DEVICE;
+  RotaryParams p{};
+  p.batch = a->batch;
+  p.tokens = a->tokens;
+  p.dim = a->dim;
+  p.eps = a->eps;
+  p.positions = a->positions;
+  p.float_positions = a->position_dtype == HTRC_LAYER_F32;
+  for (int i = 0; i < 3; ++i) p.ps[i] = a->position_stride[i];
+  for (int x = 0; x < a->n_axes; ++x)
+    for (int i = 0; i < a->axis_width[x] / 2; ++i, ++p.npairs) {
+      const double f = (a->freqs ? a->freqs[p.npairs] : std::pow(a->theta, -2.0 * i / a->axis_width[x])) *
+                       0.15915494309189533577;                        // 1 / (2 pi): revolutions per position
+      if (!std::isfinite(f)) return HTRC_ERR_ARG;
+      p.axis[p.npairs] = static_cast<uint8_t>(x);
+      if (p.float_positions) {
+        const float hi = static_cast<float>(f), lo = static_cast<float>(f - hi);
+        uint32_t h, l;
+        memcpy(&h, &hi, 4);
+        memcpy(&l, &lo, 4);
+        p.turn[p.npairs] = static_cast<uint64_t>(h) << 32 | l;
+      } else {
+        // the fraction of a revolution in 64 bits; whole revolutions per position turn nothing
+        const double whole = std::floor(f), top = (f - whole) * 0x1p32, hi = std::floor(top);
+        p.turn[p.npairs] = (static_cast<uint64_t>(hi) << 32) + static_cast<uint64_t>((top - hi) * 0x1p32);
+      }
+    }
+  const int es = a->dtype == HTRC_LAYER_F32 ? 4 : 2;
+  const bool half = a->pairs == HTRC_ROTARY_HALF;
+  bool vec = a->dim % 8 == 0 && (!half || p.npairs % 4 == 0), any_weight = false;
+  int64_t rows = a->batch * a->tokens;
+  for (int i = 0; i < a->n_tensors; ++i) {
+    const HtrcRotaryTensor& t = a->tensor[i];
+    RotaryRows& r = p.t[i];
+    r.in = t.in;
+    r.out = t.out;
+    r.x = t.x;
+    r.weight = t.weight;
+    r.weight_dtype = t.weight_dtype;
+    r.heads = t.heads;
+    for (int s = 0; s < 3; ++s) {
+      r.is[s] = t.in_stride[s];
+      r.os[s] = t.out_stride[s];
+      r.xs[s] = t.x_stride[s];
+    }
+    any_weight |= t.weight != nullptr;
+    vec = vec && aligned16(t.in, t.in_stride, es) && aligned16(t.out, t.out_stride, es) &&
+          (!(BACK && t.weight) || aligned16(t.x, t.x_stride, es));
+  }
+  const bool partials = BACK && any_weight;
+  size_t need = 0;
+  if (partials) {
+    htrc_rotary_workspace_size(a, &need);
+    if (a->workspace == nullptr || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16)
+      return HTRC_ERR_WORKSPACE;
+  }
+  const int lpr = a->dim <= 64 ? 8 : a->dim <= 128 ? 16 : 32;
+  int64_t blocks = 1;
+  for (int i = 0; i < a->n_tensors; ++i) {
+    RotaryRows& r = p.t[i];
+    // heads per warp: all of a token's, whose angles are then computed once, where the tokens alone fill the
+    // device; else one batch of rows, for the shortest chain
+    const int batch_rows = 32 / lpr;
+    r.chunk = rows >= 2 * sm_count() * kRotWarps ? r.heads : std::min<int>(r.heads, batch_rows);
+    r.chunks = (r.heads + r.chunk - 1) / r.chunk;
+    const int64_t tasks = rows * (vec ? r.chunks : r.heads);
+    blocks = std::max(blocks, (tasks + kRotWarps - 1) / kRotWarps);
+  }
+  blocks = std::min<int64_t>(blocks, rotary_max_blocks());
+  float* partial = static_cast<float*>(a->workspace);
+  const dim3 grid(static_cast<unsigned>(blocks), a->n_tensors);
+  if (rows > 0 || partials) {
+    auto go = [&](auto tag) {
+      using T = decltype(tag);
+      if (vec) run_dim<T, BACK>(p, half, grid, partial, st);
+      else rotary_any_kernel<T, BACK><<<grid, kRotWarps * 32, 0, st>>>(p, half, partial);
+    };
+    if (a->dtype == HTRC_LAYER_F32) go(float{});
+    else if (a->dtype == HTRC_LAYER_BF16) go(__nv_bfloat16{});
+    else go(__half{});
+    if (partials) {
+      const HtrcRotaryTensor &t0 = a->tensor[0], &t1 = a->tensor[a->n_tensors - 1];
+      rotary_weight_kernel<<<dim3((a->dim + 31) / 32, a->n_tensors), 1024, 0, st>>>(
+          partial, static_cast<int>(blocks), a->dim, t0.weight ? t0.dweight : nullptr, t0.weight_dtype,
+          t1.weight ? t1.dweight : nullptr, t1.weight_dtype);
+    }
+  }
+  return cudaGetLastError() == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
+}
+
+}  // namespace
+
+}  // namespace htrc
+
+extern "C" {
+
+int htrc_rotary_forward(const HtrcRotaryArgs* args, htrc_stream_t stream) {
+  return htrc::rotary_run<false>(args, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int htrc_rotary_workspace_size(const HtrcRotaryArgs* args, size_t* bytes) {
+  if (bytes == nullptr) return HTRC_ERR_ARG;
+  const int rc = htrc::rotary_validate(args, false, false);
+  if (rc != HTRC_OK) return rc;
+  *bytes = static_cast<size_t>(2) * htrc::rotary_max_blocks() * args->dim * sizeof(float);
+  return HTRC_OK;
+}
+
+int htrc_rotary_backward(const HtrcRotaryArgs* args, htrc_stream_t stream) {
+  return htrc::rotary_run<true>(args, reinterpret_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

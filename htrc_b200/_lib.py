@@ -55,10 +55,12 @@ TREE_MAX_LEVELS, TREE_MAX_CENTRES, TREE_KMEANS_CENTRES = 16, 256, 32
 TREE_STAGE_ACCEPT, TREE_STAGE_LEAVES, TREE_STAGE_FINAL, TREE_STAGE_ALL = 1, 2, 4, 7
 
 # element types of include/htrc_layer.h
-LAYER_F32, LAYER_BF16, LAYER_F16, LAYER_I32 = range(4)
+LAYER_F32, LAYER_BF16, LAYER_F16, LAYER_I32, LAYER_U8 = range(5)
+CROSS_MAX_DIM = 128
 ROTARY_MAX_AXES, ROTARY_MAX_DIM, ROTARY_MAX_HEADS = 4, 256, 1024
 ROTARY_PAIRS = {"interleaved": 0, "half": 1}
 _i64x3 = _i64 * 3
+_i64x4 = _i64 * 4
 
 
 class HtrcRotaryTensor(ctypes.Structure):
@@ -73,6 +75,17 @@ class HtrcRotaryArgs(ctypes.Structure):
                 ("tokens", _i64), ("dim", _i32), ("n_axes", _i32), ("axis_width", _i32 * 4), ("pairs", _i32),
                 ("positions", _p), ("position_dtype", _i32), ("position_stride", _i64x3), ("theta", ctypes.c_double),
                 ("freqs", ctypes.POINTER(ctypes.c_double)), ("eps", _f32), ("workspace", _p),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
+class HtrcCrossArgs(ctypes.Structure):
+    """Mirror of include/htrc_layer.h HtrcCrossArgs."""
+    _fields_ = [("q", _p), ("k", _p), ("v", _p), ("q_stride", _i64x3), ("k_stride", _i64x3), ("v_stride", _i64x3),
+                ("out", _p), ("out_stride", _i64x3), ("lse", _p), ("batch", _i64), ("queries", _i64), ("keys", _i64),
+                ("heads", _i32), ("kv_heads", _i32), ("dim", _i32), ("dtype", _i32), ("scale", _f32),
+                ("key_lengths", _p), ("mask", _p), ("mask_dtype", _i32), ("mask_stride", _i64x4), ("status", _p),
+                ("dout", _p), ("dout_stride", _i64x3), ("dlse", _p), ("dq", _p), ("dk", _p), ("dv", _p),
+                ("dq_stride", _i64x3), ("dk_stride", _i64x3), ("dv_stride", _i64x3), ("workspace", _p),
                 ("workspace_bytes", ctypes.c_size_t)]
 
 
@@ -133,6 +146,9 @@ SIGNATURES = {
     "htrc_rotary_forward": (ctypes.c_int, [ctypes.POINTER(HtrcRotaryArgs), _p]),
     "htrc_rotary_workspace_size": (ctypes.c_int, [ctypes.POINTER(HtrcRotaryArgs), ctypes.POINTER(ctypes.c_size_t)]),
     "htrc_rotary_backward": (ctypes.c_int, [ctypes.POINTER(HtrcRotaryArgs), _p]),
+    "htrc_cross_forward": (ctypes.c_int, [ctypes.POINTER(HtrcCrossArgs), _p]),
+    "htrc_cross_workspace_size": (ctypes.c_int, [ctypes.POINTER(HtrcCrossArgs), ctypes.POINTER(ctypes.c_size_t)]),
+    "htrc_cross_backward": (ctypes.c_int, [ctypes.POINTER(HtrcCrossArgs), _p]),
 }
 
 _lib = None

@@ -1,0 +1,125 @@
+// Shared by the cross-attention kernels (cross_fwd.cu, cross_bwd.cu): the masks, the element types, the shapes that
+// the C entries check, and the tensor maps of [batch][token][head][dim] operands.
+#pragma once
+#include "../../include/htrc_layer.h"
+#include "common.cuh"
+#include "kernels.cuh"
+
+namespace htrc {
+
+// How a launch's mask is read; the key lengths apply in every kind.
+enum CrossMask : int {
+  CROSS_NONE = 0,       // no mask
+  CROSS_KEYS = 1,       // the same for every query: a bias per key (0 / -inf from a bool mask)
+  CROSS_PAIRS = 2,      // bool, per query and key
+  CROSS_BIAS = 3,       // added, per query and key
+};
+
+struct CrossMaskView {
+  const void* p;
+  int64_t sb, sh, sn, sm;
+  int dtype;
+};
+
+// the mask's term at element offset i: -inf excludes
+__device__ __forceinline__ float mask_term(const void* p, int dtype, int64_t i) {
+  if (dtype == HTRC_LAYER_U8) return __ldg(static_cast<const uint8_t*>(p) + i) ? 0.f : -INFINITY;
+  if (dtype == HTRC_LAYER_F32) return __ldg(static_cast<const float*>(p) + i);
+  if (dtype == HTRC_LAYER_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+
+struct CrossShape {
+  int64_t batch, queries, keys;
+  int heads, kv_heads, group, dim;
+  float scale;                          // of the natural logits
+  const int32_t* lengths;
+  CrossMaskView mask;
+  // 1 where a tensor has that batch / head dimension, 0 where it is broadcast along it (the map then has one)
+  int q_b, q_h, k_b, k_h, v_b, v_h;
+};
+
+// keys of batch entry b
+__device__ __forceinline__ int key_count(const CrossShape& s, int b) {
+  if (s.lengths == nullptr) return static_cast<int>(s.keys);
+  const int n = __ldg(s.lengths + b);
+  return max(0, min(n, static_cast<int>(s.keys)));
+}
+
+template <bool BF>
+__device__ __forceinline__ uint32_t pack16x2(float lo, float hi) {
+  return BF ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
+}
+template <bool BF>
+__device__ __forceinline__ float2 unpack16x2(uint32_t w) {
+  if (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+template <bool BF>
+__host__ __device__ constexpr uint32_t idesc16(int M, int N, bool a_mn, bool b_mn) {
+  return BF ? idesc_bf16(M, N, a_mn, b_mn) : idesc_f16(M, N, a_mn, b_mn);
+}
+
+constexpr float kCrossLog2e = 1.4426950408889634f;
+constexpr float kCrossLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float cross_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
+}
+
+// A descriptor's constant words: K-major operand (LBO unused) and MN-major operand with 64-element chunks lbo apart
+__device__ __forceinline__ uint64_t desc_k(uint32_t smem) { return sw128_desc(smem, 16, 1024); }
+__device__ __forceinline__ uint64_t desc_mn(uint32_t smem, uint32_t lbo) { return sw128_desc(smem, lbo, 1024); }
+
+// Zeroes the rows of a staged [chunks][rows][64] tile (chunk_bytes apart) whose key is excluded for every query: past
+// the entry's keys or -inf in a per-key mask.  One warp; the writes are made visible to the tensor cores' reads.
+// Lane i decides keys key0 + 32 r + i.
+template <int ROWS, int CHUNKS>
+__device__ __forceinline__ void zero_excluded_rows(uint8_t* tile, uint32_t chunk_bytes, int key0, int count,
+                                                   const CrossShape& s, int64_t mask_at, bool keyed, int lane) {
+#pragma unroll
+  for (int r = 0; r < ROWS / 32; ++r) {
+    const int key = key0 + 32 * r + lane;
+    bool out = key >= count;
+    if (!out && keyed) out = mask_term(s.mask.p, s.mask.dtype, mask_at + static_cast<int64_t>(key) * s.mask.sm) == -INFINITY;
+    uint32_t todo = __ballot_sync(0xffffffffu, out);
+    while (todo) {
+      // four rows at a time: 8 lanes per 128-byte row
+      int row = -1;
+      uint32_t rest = todo;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int f = rest ? __ffs(rest) - 1 : -1;
+        if (rest) rest &= rest - 1;
+        if (lane / 8 == i) row = f;
+      }
+      todo = rest;
+      if (row >= 0) {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+          *reinterpret_cast<uint4*>(tile + c * chunk_bytes + (32 * r + row) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+int cross_validate(const HtrcCrossArgs* a, bool back, bool ptrs);
+CrossShape cross_shape(const HtrcCrossArgs* a);
+int cross_mask_kind(const HtrcCrossArgs* a);
+// [batch][token][head][dim] as a 4-d map (dim, token, head, batch), box (64, box_rows, 1, 1), 128-byte swizzle; *b and
+// *h are cleared for a dimension the tensor is broadcast along
+bool cross_map(CUtensorMap* m, const HtrcCrossArgs* a, const void* base, const int64_t* stride, int64_t rows, int heads,
+               int box_rows, int* b, int* h);
+
+}  // namespace htrc

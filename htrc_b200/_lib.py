@@ -7,6 +7,7 @@ There is no fallback: if the library is missing, every operator call raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).with_name("libhtrc_flat.so")
@@ -89,6 +90,13 @@ class HtrcCrossArgs(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_size_t)]
 
 
+# The same structs as one native-aligned pack of their fields in order: filling a ctypes structure field by field costs
+# several microseconds of the small calls.
+_ROTARY_TENSOR = "P3qP3qP3qPPii"
+ROTARY_ARGS = struct.Struct("@" + 2 * _ROTARY_TENSOR + "iiqqii4iiPi3qdPfPN0q")
+CROSS_ARGS = struct.Struct("@PPP3q3q3qP3qPqqqiiiifPPi4qPP3qPPPP3q3q3qPN0q")
+
+
 # name -> (restype, argtypes); every symbol include/htrc_flat.h, include/htrc_tree.h and include/htrc_layer.h
 # declare
 SIGNATURES = {
@@ -143,12 +151,13 @@ SIGNATURES = {
     "htrc_tree_centres_scratch_size": (ctypes.c_int, [_i64, ctypes.POINTER(ctypes.c_size_t)]),
     "htrc_tree_centres": (ctypes.c_int, [_p, _i32, _i64, _f32, _p, _p, _p, ctypes.c_size_t, _p]),
     # operators around the flat attention (include/htrc_layer.h)
-    "htrc_rotary_forward": (ctypes.c_int, [ctypes.POINTER(HtrcRotaryArgs), _p]),
-    "htrc_rotary_workspace_size": (ctypes.c_int, [ctypes.POINTER(HtrcRotaryArgs), ctypes.POINTER(ctypes.c_size_t)]),
-    "htrc_rotary_backward": (ctypes.c_int, [ctypes.POINTER(HtrcRotaryArgs), _p]),
-    "htrc_cross_forward": (ctypes.c_int, [ctypes.POINTER(HtrcCrossArgs), _p]),
-    "htrc_cross_workspace_size": (ctypes.c_int, [ctypes.POINTER(HtrcCrossArgs), ctypes.POINTER(ctypes.c_size_t)]),
-    "htrc_cross_backward": (ctypes.c_int, [ctypes.POINTER(HtrcCrossArgs), _p]),
+    # (their structs are passed as packed bytes, ROTARY_ARGS / CROSS_ARGS, or by reference)
+    "htrc_rotary_forward": (ctypes.c_int, [_p, _p]),
+    "htrc_rotary_workspace_size": (ctypes.c_int, [_p, ctypes.POINTER(ctypes.c_size_t)]),
+    "htrc_rotary_backward": (ctypes.c_int, [_p, _p]),
+    "htrc_cross_forward": (ctypes.c_int, [_p, _p]),
+    "htrc_cross_workspace_size": (ctypes.c_int, [_p, ctypes.POINTER(ctypes.c_size_t)]),
+    "htrc_cross_backward": (ctypes.c_int, [_p, _p]),
 }
 
 _lib = None
@@ -196,3 +205,9 @@ def stream_ptr(stream=None) -> int:
     import torch
     s = torch.cuda.current_stream() if stream is None else stream
     return int(s.cuda_stream)
+
+
+def raw_stream(index: int) -> int:
+    """The current stream's handle on CUDA device ``index``."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)

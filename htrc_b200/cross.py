@@ -21,11 +21,12 @@ import math
 import torch
 
 from . import _lib
-from ._lib import check, lib, ptr, stream_ptr
+from ._lib import check, lib
 
 _DTYPES = {torch.bfloat16: _lib.LAYER_BF16, torch.float16: _lib.LAYER_F16}
 _MASKS = {torch.bool: _lib.LAYER_U8, torch.float32: _lib.LAYER_F32, torch.bfloat16: _lib.LAYER_BF16,
           torch.float16: _lib.LAYER_F16}
+_LENGTHS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 _status = {}
 
 
@@ -46,23 +47,33 @@ def cross_status(device=None):
 
 
 def _rows(x):
-    """x where its rows are dense, 16-byte aligned and its own, else a contiguous copy."""
-    s = x.stride()
-    fine = (s[-1] == 1 or x.shape[-1] == 1) and x.data_ptr() % 16 == 0 and all(
-        n == 1 or (t % 8 == 0 and (t > 0 or i == 0)) for i, (n, t) in enumerate(zip(x.shape[:-1], s[:-1])))
-    return x if fine else x.contiguous()
+    """x where its rows are dense, 16-byte aligned and their own, else a contiguous copy."""
+    s0, s1, s2, s3 = x.stride()
+    if s3 == 1 and s1 > 0 and s2 > 0 and not (s0 | s1 | s2) & 7 and not x.data_ptr() & 15:
+        return x
+    x = x.contiguous()
+    return x if not x.data_ptr() & 15 else x.clone()
 
 
 def _strides(x, heads_first):
     """(batch, token, head) strides of a 4-d tensor."""
-    s = x.stride()
-    return (s[0], s[2], s[1]) if heads_first else (s[0], s[1], s[2])
+    s0, s1, s2, _ = x.stride()
+    return (s0, s2, s1) if heads_first else (s0, s1, s2)
+
+
+def _mask_strides(mask, want):
+    """The mask's strides over [batch, heads, queries, keys], 0 where it broadcasts."""
+    shape, stride = mask.shape, mask.stride()
+    if len(shape) > 4 or any(n != w and n != 1 for n, w in zip(reversed(shape), reversed(want))):
+        raise ValueError(f"mask {list(shape)} does not broadcast to {list(want)}")
+    strides = tuple(0 if n == 1 else t for n, t in zip(shape, stride))
+    return (0,) * (4 - len(strides)) + strides
 
 
 class _Call:
     """The checked arguments of one call: 4-d operands, shapes and the mask."""
-    __slots__ = ("q", "k", "v", "heads_first", "scale", "lengths", "mask", "batch", "queries", "keys", "heads",
-                 "kv_heads", "dim", "squeeze")
+    __slots__ = ("q", "k", "v", "heads_first", "lengths", "mask", "squeeze", "lse_shape", "shape_args", "mask_args",
+                 "device")
 
     def __init__(self, q, k, v, key_lengths, mask, scale, heads_first):
         for name, x in (("q", q), ("k", k), ("v", v)):
@@ -76,100 +87,106 @@ class _Call:
         self.squeeze = q.dim() == 3
         if self.squeeze:
             q, k, v = q[None], k[None], v[None]
-        self.heads_first = bool(heads_first)
-        t, h = (2, 1) if heads_first else (1, 2)
-        self.batch, self.queries, self.heads, self.dim = (int(q.shape[i]) for i in (0, t, h, 3))
-        self.keys, self.kv_heads = int(k.shape[t]), int(k.shape[h])
-        if k.shape != v.shape or int(k.shape[0]) != self.batch or int(k.shape[3]) != self.dim:
+        dev = self.device = q.device
+        if heads_first:
+            self.heads_first = True
+            batch, heads, queries, dim = q.shape
+            kb, kv_heads, keys, kd = k.shape
+        else:
+            self.heads_first = False
+            batch, queries, heads, dim = q.shape
+            kb, keys, kv_heads, kd = k.shape
+        if k.shape != v.shape or kb != batch or kd != dim:
             raise ValueError("k and v: q's batch and dim, and one shape, expected")
-        if self.kv_heads < 1 or self.heads < 1 or self.heads % self.kv_heads:
-            raise ValueError(f"{self.heads} query heads do not share {self.kv_heads} key heads evenly")
-        if self.dim % 8 or not 8 <= self.dim <= _lib.CROSS_MAX_DIM:
-            raise NotImplementedError(f"dim: a multiple of 8 up to {_lib.CROSS_MAX_DIM} is supported, got {self.dim}")
-        self.scale = 1.0 / math.sqrt(self.dim) if scale is None else float(scale)
-        if not (self.scale > 0 and math.isfinite(self.scale)):
+        if kv_heads < 1 or heads < 1 or heads % kv_heads:
+            raise ValueError(f"{heads} query heads do not share {kv_heads} key heads evenly")
+        if dim % 8 or not 8 <= dim <= _lib.CROSS_MAX_DIM:
+            raise NotImplementedError(f"dim: a multiple of 8 up to {_lib.CROSS_MAX_DIM} is supported, got {dim}")
+        scale = dim ** -0.5 if scale is None else float(scale)
+        if not (scale > 0 and math.isfinite(scale)):
             raise ValueError("scale must be positive and finite")
         if key_lengths is not None:
-            if not isinstance(key_lengths, torch.Tensor) or key_lengths.shape != (self.batch,) or \
-                    key_lengths.is_floating_point() or key_lengths.device != q.device:
+            if not isinstance(key_lengths, torch.Tensor) or key_lengths.dim() != 1 or key_lengths.shape[0] != batch or \
+                    key_lengths.dtype not in _LENGTHS or key_lengths.device != dev:
                 raise ValueError("key_lengths: [batch] integers on q's device expected")
-            key_lengths = key_lengths.to(torch.int32).contiguous()
+            if key_lengths.dtype is not torch.int32 or not key_lengths.is_contiguous():
+                # more keys than there are is all of them, whatever the wider type held
+                key_lengths = key_lengths.clamp(0, keys).to(torch.int32).contiguous()
         self.lengths = key_lengths
-        if mask is not None:
-            if not isinstance(mask, torch.Tensor) or mask.dtype not in _MASKS or mask.device != q.device:
-                raise ValueError("mask: a bool, float32, bfloat16 or float16 tensor on q's device expected")
-            try:
-                mask = mask.expand(self.batch, self.heads, self.queries, self.keys)
-            except RuntimeError as e:
-                raise ValueError(f"mask {list(mask.shape)} does not broadcast to "
-                                 f"{[self.batch, self.heads, self.queries, self.keys]}") from e
         self.mask = mask
+        self.mask_args = (0, 0, 0, 0, 0, 0)
+        if mask is not None:
+            if not isinstance(mask, torch.Tensor) or mask.dtype not in _MASKS or mask.device != dev:
+                raise ValueError("mask: a bool, float32, bfloat16 or float16 tensor on q's device expected")
+            self.mask_args = (mask.data_ptr(), _MASKS[mask.dtype], *_mask_strides(mask, (batch, heads, queries, keys)))
         self.q, self.k, self.v = _rows(q), _rows(k), _rows(v)
+        self.lse_shape = (batch, heads, queries)
+        self.shape_args = (batch, queries, keys, heads, kv_heads, dim, _DTYPES[q.dtype], scale,
+                           0 if key_lengths is None else key_lengths.data_ptr())
 
-    def args(self):
-        a = _lib.HtrcCrossArgs()
-        hf = self.heads_first
-        a.q, a.k, a.v = ptr(self.q), ptr(self.k), ptr(self.v)
-        a.q_stride[:], a.k_stride[:], a.v_stride[:] = (_strides(x, hf) for x in (self.q, self.k, self.v))
-        a.batch, a.queries, a.keys = self.batch, self.queries, self.keys
-        a.heads, a.kv_heads, a.dim, a.dtype = self.heads, self.kv_heads, self.dim, _DTYPES[self.q.dtype]
-        a.scale = self.scale
-        a.key_lengths = ptr(self.lengths)
-        if self.mask is not None:
-            a.mask, a.mask_dtype = ptr(self.mask), _MASKS[self.mask.dtype]
-            a.mask_stride[:] = self.mask.stride()
-        a.status = ptr(_status_word(self.q.device))
-        return a
+    def pack(self, out, lse, back=(0,) * 19):
+        hf, q, k, v = self.heads_first, self.q, self.k, self.v
+        return _lib.CROSS_ARGS.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), *_strides(q, hf), *_strides(k, hf), *_strides(v, hf),
+            out.data_ptr(), *_strides(out, hf), 0 if lse is None else lse.data_ptr(), *self.shape_args, *self.mask_args,
+            _status_word(self.device).data_ptr(), *back)
 
 
-def _forward(c):
-    q = c.q
-    with torch.cuda.device(q.device):
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty((c.batch, c.heads, c.queries), dtype=torch.float32, device=q.device)
-        a = c.args()
-        a.out, a.out_stride[:], a.lse = ptr(out), _strides(out, c.heads_first), ptr(lse)
-        check(lib().htrc_cross_forward(a, stream_ptr()), "htrc_cross_forward")
-    return out, lse
+def _guarded(call, device):
+    """call() with the tensors' device current."""
+    if torch.cuda.current_device() == device.index:
+        return call()
+    with torch.cuda.device(device):
+        return call()
+
+
+def _forward(c, want_lse):
+    def call():
+        out = torch.empty(c.q.shape, dtype=c.q.dtype, device=c.device)
+        lse = torch.empty(c.lse_shape, dtype=torch.float32, device=c.device) if want_lse else None
+        rc = lib().htrc_cross_forward(c.pack(out, lse), _lib.raw_stream(c.device.index))
+        if rc:
+            check(rc, "htrc_cross_forward")
+        return (out[0], None if lse is None else lse[0]) if c.squeeze else (out, lse)
+
+    return _guarded(call, c.device)
 
 
 def _backward(c, dout, out, lse, dlse):
     hf, q = c.heads_first, c.q
     if c.squeeze:
-        dout, out, lse = dout[None], out[None], lse.reshape(1, *lse.shape[-2:])
-        dlse = None if dlse is None else dlse.reshape(1, *dlse.shape[-2:])
+        dout, out, lse = dout[None], out[None], lse[None]
+        dlse = None if dlse is None else dlse[None]
     for name, x in (("dout", dout), ("out", out)):
-        if x.shape != q.shape or x.dtype != q.dtype or x.device != q.device:
+        if x.shape != q.shape or x.dtype != q.dtype or x.device != c.device:
             raise ValueError(f"{name}: q's shape, type and device expected")
     for name, x in (("lse", lse), ("dlse", dlse)):
-        if x is not None and (x.shape != (c.batch, c.heads, c.queries) or x.dtype != torch.float32 or
-                              x.device != q.device):
+        if x is not None and (x.shape != c.lse_shape or x.dtype != torch.float32 or x.device != c.device):
             raise ValueError(f"{name}: [batch, heads, queries] float32 on q's device expected")
-    with torch.cuda.device(q.device):
-        dout, out = _rows(dout), _rows(out)
-        lse = lse.contiguous()
-        dlse = None if dlse is None else dlse.contiguous()
-        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, c.k, c.v))
-        a = c.args()
-        a.out, a.out_stride[:], a.lse = ptr(out), _strides(out, hf), ptr(lse)
-        a.dout, a.dout_stride[:], a.dlse = ptr(dout), _strides(dout, hf), ptr(dlse)
-        a.dq, a.dk, a.dv = ptr(dq), ptr(dk), ptr(dv)
-        a.dq_stride[:], a.dk_stride[:], a.dv_stride[:] = (_strides(x, hf) for x in (dq, dk, dv))
+
+    def call():
+        do, o, z = _rows(dout), _rows(out), lse.contiguous()
+        dz = None if dlse is None else dlse.contiguous()
+        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=c.device) for x in (q, c.k, c.v))
+        back = [do.data_ptr(), *_strides(do, hf), 0 if dz is None else dz.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                dv.data_ptr(), *_strides(dq, hf), *_strides(dk, hf), *_strides(dv, hf), 0, 0]
         need = ctypes.c_size_t()
-        check(lib().htrc_cross_workspace_size(a, need), "htrc_cross_workspace_size")
-        ws = torch.empty(max(need.value, 256), dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = ptr(ws), int(ws.numel())
-        check(lib().htrc_cross_backward(a, stream_ptr()), "htrc_cross_backward")
-    return (dq[0], dk[0], dv[0]) if c.squeeze else (dq, dk, dv)
+        check(lib().htrc_cross_workspace_size(c.pack(o, z, back), need), "htrc_cross_workspace_size")
+        ws = torch.empty(need.value, dtype=torch.uint8, device=c.device)
+        back[-2:] = ws.data_ptr(), need.value
+        rc = lib().htrc_cross_backward(c.pack(o, z, back), _lib.raw_stream(c.device.index))
+        if rc:
+            check(rc, "htrc_cross_backward")
+        return (dq[0], dk[0], dv[0]) if c.squeeze else (dq, dk, dv)
+
+    return _guarded(call, c.device)
 
 
 class _Cross(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, key_lengths, mask, scale, heads_first):
         c = _Call(q, k, v, key_lengths, mask, scale, heads_first)
-        out, lse = _forward(c)
-        if c.squeeze:
-            out, lse = out[0], lse[0]
+        out, lse = _forward(c, True)
         ctx.save_for_backward(q, k, v, key_lengths, mask, out, lse)
         ctx.more = (scale, heads_first)
         ctx.set_materialize_grads(False)
@@ -192,10 +209,7 @@ def cross_attention(q, k, v, *, key_lengths=None, mask=None, scale=None, heads_f
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _Cross.apply(q, k, v, key_lengths, mask, scale, heads_first)
     else:
-        c = _Call(q, k, v, key_lengths, mask, scale, heads_first)
-        out, lse = _forward(c)
-        if c.squeeze:
-            out, lse = out[0], lse[0]
+        out, lse = _forward(_Call(q, k, v, key_lengths, mask, scale, heads_first), return_lse)
     return (out, lse) if return_lse else out
 
 

@@ -440,13 +440,15 @@ int cross_mask_kind(const HtrcCrossArgs* a) {
 
 bool cross_map(CUtensorMap* m, const HtrcCrossArgs* a, const void* base, const int64_t* stride, int64_t rows, int heads,
                int box_rows, int* b, int* h) {
-  *b = a->batch > 1 && stride[0] != 0;
-  *h = heads > 1 && stride[2] != 0;
+  const bool in_b = a->batch > 1 && stride[0] != 0, in_h = heads > 1 && stride[2] != 0;
+  *b = in_b;
+  *h = in_h;
   const uint64_t dims[4] = {static_cast<uint64_t>(a->dim), static_cast<uint64_t>(rows),
-                            *h ? static_cast<uint64_t>(heads) : 1, *b ? static_cast<uint64_t>(a->batch) : 1};
+                            in_h ? static_cast<uint64_t>(heads) : 1, in_b ? static_cast<uint64_t>(a->batch) : 1};
   // a dimension of one is never stepped along: any valid stride
   const uint64_t strides[3] = {rows > 1 ? static_cast<uint64_t>(stride[1]) * 2 : 256,
-                               *h ? static_cast<uint64_t>(stride[2]) * 2 : 256, *b ? static_cast<uint64_t>(stride[0]) * 2 : 256};
+                               in_h ? static_cast<uint64_t>(stride[2]) * 2 : 256,
+                               in_b ? static_cast<uint64_t>(stride[0]) * 2 : 256};
   const uint32_t box[4] = {64, static_cast<uint32_t>(box_rows), 1, 1};
   return make_tiled_map(m, a->dtype == HTRC_LAYER_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                         4, base, dims, strides, box, true);

@@ -13,7 +13,9 @@
 // Angles: an int32 position times the frequency in revolutions as a 64-bit fixed-point fraction, modulo 2^64, is the
 // exactly reduced turn for every int32 position (float32 positions: the product in two floats, its whole turns
 // dropped), so late positions lose no accuracy.
+#include <algorithm>
 #include <cmath>
+#include <cstring>
 
 #include "../../include/htrc_layer.h"
 #include "common.cuh"
@@ -461,6 +463,53 @@ bool aligned16(const void* p, const int64_t* s, int es) {
   return true;
 }
 
+// The pairs' axes and turns per position.  The last table without frequencies of the caller's own is kept per thread:
+// its 64 powers cost more host time than the rest of a small call.
+bool rotary_table(const HtrcRotaryArgs* a, RotaryParams* p) {
+  struct Kept {
+    double theta = 0.0;
+    int n_axes = 0, width[HTRC_ROTARY_MAX_AXES] = {}, npairs = 0;
+    bool floats = false;
+    uint64_t turn[kRotMaxPairs];
+    uint8_t axis[kRotMaxPairs];
+  };
+  static thread_local Kept kept;
+  bool same = a->freqs == nullptr && kept.theta == a->theta && kept.n_axes == a->n_axes && kept.floats == p->float_positions;
+  for (int x = 0; same && x < a->n_axes; ++x) same = kept.width[x] == a->axis_width[x];
+  if (!same) {
+    kept.theta = 0.0;                                               // no caller's theta: not kept until complete
+    kept.npairs = 0;
+    kept.floats = p->float_positions;
+    for (int x = 0; x < a->n_axes; ++x) {
+      kept.width[x] = a->axis_width[x];
+      for (int i = 0; i < a->axis_width[x] / 2; ++i, ++kept.npairs) {
+        const double f = (a->freqs ? a->freqs[kept.npairs] : std::pow(a->theta, -2.0 * i / a->axis_width[x])) *
+                         0.15915494309189533577;                    // 1 / (2 pi): revolutions per position
+        if (!std::isfinite(f)) return false;
+        kept.axis[kept.npairs] = static_cast<uint8_t>(x);
+        uint64_t& t = kept.turn[kept.npairs];
+        if (kept.floats) {
+          const float hi = static_cast<float>(f), lo = static_cast<float>(f - hi);
+          uint32_t h, l;
+          memcpy(&h, &hi, 4);
+          memcpy(&l, &lo, 4);
+          t = static_cast<uint64_t>(h) << 32 | l;
+        } else {
+          // the fraction of a revolution in 64 bits; whole revolutions per position turn nothing
+          const double top = (f - std::floor(f)) * 0x1p32, hi = std::floor(top);
+          t = (static_cast<uint64_t>(hi) << 32) + static_cast<uint64_t>((top - hi) * 0x1p32);
+        }
+      }
+    }
+    kept.n_axes = a->n_axes;
+    if (a->freqs == nullptr) kept.theta = a->theta;
+  }
+  p->npairs = kept.npairs;
+  memcpy(p->turn, kept.turn, kept.npairs * sizeof(kept.turn[0]));
+  memcpy(p->axis, kept.axis, kept.npairs * sizeof(kept.axis[0]));
+  return true;
+}
+
 template <typename T, int LPR, bool HALF, bool BACK>
 void run_rows(const RotaryParams& p, dim3 grid, float* partial, cudaStream_t st) {
   rotary_kernel<T, LPR, HALF, BACK><<<grid, kRotWarps * 32, 0, st>>>(p, partial);
@@ -490,24 +539,7 @@ int rotary_run(const HtrcRotaryArgs* a, cudaStream_t st) {
   p.positions = a->positions;
   p.float_positions = a->position_dtype == HTRC_LAYER_F32;
   for (int i = 0; i < 3; ++i) p.ps[i] = a->position_stride[i];
-  for (int x = 0; x < a->n_axes; ++x)
-    for (int i = 0; i < a->axis_width[x] / 2; ++i, ++p.npairs) {
-      const double f = (a->freqs ? a->freqs[p.npairs] : std::pow(a->theta, -2.0 * i / a->axis_width[x])) *
-                       0.15915494309189533577;                        // 1 / (2 pi): revolutions per position
-      if (!std::isfinite(f)) return HTRC_ERR_ARG;
-      p.axis[p.npairs] = static_cast<uint8_t>(x);
-      if (p.float_positions) {
-        const float hi = static_cast<float>(f), lo = static_cast<float>(f - hi);
-        uint32_t h, l;
-        memcpy(&h, &hi, 4);
-        memcpy(&l, &lo, 4);
-        p.turn[p.npairs] = static_cast<uint64_t>(h) << 32 | l;
-      } else {
-        // the fraction of a revolution in 64 bits; whole revolutions per position turn nothing
-        const double whole = std::floor(f), top = (f - whole) * 0x1p32, hi = std::floor(top);
-        p.turn[p.npairs] = (static_cast<uint64_t>(hi) << 32) + static_cast<uint64_t>((top - hi) * 0x1p32);
-      }
-    }
+  if (!rotary_table(a, &p)) return HTRC_ERR_ARG;
   const int es = a->dtype == HTRC_LAYER_F32 ? 4 : 2;
   const bool half = a->pairs == HTRC_ROTARY_HALF;
   bool vec = a->dim % 8 == 0 && (!half || p.npairs % 4 == 0), any_weight = false;

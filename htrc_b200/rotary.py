@@ -17,12 +17,13 @@ passes can also be called by themselves.  There is no CPU path.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
 
 from . import _lib
-from ._lib import check, lib, ptr, stream_ptr
+from ._lib import check, lib
 
 _DTYPES = {torch.float32: _lib.LAYER_F32, torch.bfloat16: _lib.LAYER_BF16, torch.float16: _lib.LAYER_F16}
 
@@ -39,17 +40,11 @@ def grid_positions(grid, *, start=None, device="cuda"):
     return torch.stack([a.reshape(-1) for a in torch.meshgrid(*at, indexing="ij")], -1)
 
 
-def _unit_rows(x):
-    """x itself when its last dimension is dense, else a copy."""
-    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
-
-
 class _Spec:
-    """The arguments that every call shares, checked."""
-    __slots__ = ("axes", "theta", "pairs", "eps", "freqs", "heads_first")
+    """The arguments that do not depend on the tensors, checked."""
+    __slots__ = ("axes", "theta", "pairs", "eps", "freqs", "heads_first", "rotated", "table")
 
     def __init__(self, axes, theta, pairs, eps, freqs, heads_first):
-        axes = tuple(int(w) for w in axes)
         if not axes or min(axes) < 0 or any(w % 2 for w in axes):
             raise ValueError("axes: an even number of rotated elements per axis")
         if len(axes) > _lib.ROTARY_MAX_AXES:
@@ -60,139 +55,171 @@ class _Spec:
             raise ValueError("theta must be positive and finite")
         if not (eps >= 0 and math.isfinite(eps)):
             raise ValueError("eps must be non-negative and finite")
+        self.table = None
         if freqs is not None:
-            freqs = tuple(float(f) for f in freqs)
             if len(freqs) != sum(axes) // 2 or not all(math.isfinite(f) for f in freqs):
                 raise ValueError("freqs: one finite frequency for each of the sum(axes) / 2 pairs")
-        self.axes, self.theta, self.pairs, self.eps = axes, float(theta), pairs, float(eps)
-        self.freqs, self.heads_first = freqs, bool(heads_first)
+            self.table = (ctypes.c_double * max(1, len(freqs)))(*freqs)
+        self.rotated = sum(axes)
+        self.axes = axes + (0,) * (_lib.ROTARY_MAX_AXES - len(axes))
+        self.theta, self.pairs, self.eps = float(theta), _lib.ROTARY_PAIRS[pairs], float(eps)
+        self.freqs = 0 if self.table is None else ctypes.addressof(self.table)
+        self.heads_first = heads_first
 
 
-def _check_rows(x, name, like=None):
+_specs = functools.lru_cache(maxsize=64)(_Spec)
+
+
+def _spec(axes, theta, pairs, eps, freqs, heads_first):
+    if type(axes) is not tuple:
+        axes = tuple(int(w) for w in axes)
+    return _specs(axes, theta, pairs, eps, None if freqs is None else tuple(float(f) for f in freqs), bool(heads_first))
+
+
+def _check_rows(x, name):
     if not isinstance(x, torch.Tensor) or x.dim() not in (3, 4):
         raise ValueError(f"{name}: [tokens, heads, dim] or [batch, tokens, heads, dim] expected")
     if x.dtype not in _DTYPES:
         raise ValueError(f"{name}: float32, bfloat16 or float16 expected, got {x.dtype}")
     if not x.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
-    if like is not None and (x.dtype != like.dtype or x.device != like.device or x.dim() != like.dim() or
-                             x.shape[:-2] != like.shape[:-2] or x.shape[-1] != like.shape[-1]):
-        raise ValueError(f"{name}: the other tensor's type, device, batch, tokens and dim expected")
 
 
 def _check(spec, tensors, weights, positions):
+    """Raises for what the kernels do not take; the positions as int32 or float32."""
     x = tensors[0]
     _check_rows(x, "x")
-    for t in tensors[1:]:
-        _check_rows(t, "k", x)
-    dim = int(x.shape[-1])
-    if dim > _lib.ROTARY_MAX_DIM or dim < 2:
+    shape, dtype, dev = x.shape, x.dtype, x.device
+    dim = shape[-1]
+    if not 2 <= dim <= _lib.ROTARY_MAX_DIM:
         raise NotImplementedError(f"heads of 2 to {_lib.ROTARY_MAX_DIM} elements are supported, got {dim}")
-    if sum(spec.axes) > dim:
-        raise ValueError(f"axes rotate {sum(spec.axes)} of {dim} elements")
+    if spec.rotated > dim:
+        raise ValueError(f"axes rotate {spec.rotated} of {dim} elements")
     for t in tensors:
-        if not 1 <= int(t.shape[-2]) <= _lib.ROTARY_MAX_HEADS:
+        if t is not x:
+            _check_rows(t, "k")
+            if t.dtype != dtype or t.device != dev or t.shape[:-2] != shape[:-2] or t.shape[-1] != dim:
+                raise ValueError("k: q's type, device, batch, tokens and dim expected")
+        if not 1 <= t.shape[-2] <= _lib.ROTARY_MAX_HEADS:
             raise NotImplementedError(f"1 to {_lib.ROTARY_MAX_HEADS} heads are supported")
     for w in weights:
-        if w is not None and (w.shape != (dim,) or w.dtype not in _DTYPES or w.device != x.device):
+        if w is not None and (w.dim() != 1 or w.shape[0] != dim or w.dtype not in _DTYPES or w.device != dev):
             raise ValueError(f"weight: [{dim}] float32, bfloat16 or float16 on the rows' device expected")
-    lead = x.shape[:-2]
-    if not isinstance(positions, torch.Tensor) or positions.device != x.device or \
-            positions.dim() not in (2, x.dim() - 1) or positions.shape[-1] != len(spec.axes) or \
-            positions.shape[-2] != lead[-1] or (positions.dim() == 3 and positions.shape[0] not in (1, lead[0])):
+    axes = sum(1 for w in spec.axes if w) if not isinstance(positions, torch.Tensor) else positions.shape[-1]
+    if not isinstance(positions, torch.Tensor) or positions.device != dev or positions.dim() not in (2, len(shape) - 1) \
+            or positions.shape[-2] != shape[-3] or (positions.dim() == 3 and positions.shape[0] not in (1, shape[0])):
         raise ValueError("positions: [tokens, axes] or [batch, tokens, axes] on the rows' device expected")
-    if positions.is_floating_point():
-        return positions if positions.dtype == torch.float32 else positions.float()
-    if positions.dtype == torch.bool or positions.is_complex():
+    if axes > _lib.ROTARY_MAX_AXES or any(spec.axes[axes:]):
+        raise ValueError("positions: one for each of the axes expected")
+    p = positions.dtype
+    if p is torch.int32 or p is torch.float32:
+        return positions
+    if p is torch.bool or p.is_complex:
         raise ValueError("positions: integers or floats expected")
-    return positions if positions.dtype == torch.int32 else positions.to(torch.int32)
+    return positions.to(torch.float32 if p.is_floating_point else torch.int32)
+
+
+def _unit_rows(x):
+    """x itself when its last dimension is dense, else a copy."""
+    return x if x.stride(-1) == 1 else x.contiguous()
 
 
 def _strides(x, heads_first=False):
     """(batch, token, head) element strides of rows [(batch,) tokens, heads, dim] (heads_first: heads, tokens)."""
     s = x.stride()
-    b = s[0] if x.dim() == 4 else 0
+    b = s[0] if len(s) == 4 else 0
     return (b, s[-2], s[-3]) if heads_first else (b, s[-3], s[-2])
 
 
-def _args(spec, like, positions):
-    a = _lib.HtrcRotaryArgs()
-    a.dtype = _DTYPES[like.dtype]
-    a.batch = int(like.shape[0]) if like.dim() == 4 else 1
-    a.tokens, a.dim = int(like.shape[-3]), int(like.shape[-1])
-    a.n_axes = len(spec.axes)
-    for i, w in enumerate(spec.axes):
-        a.axis_width[i] = w
-    a.pairs = _lib.ROTARY_PAIRS[spec.pairs]
-    a.positions = ptr(positions)
-    a.position_dtype = _lib.LAYER_F32 if positions.dtype == torch.float32 else _lib.LAYER_I32
-    batched = positions.dim() == 3 and positions.shape[0] > 1
-    a.position_stride[:] = (positions.stride(0) if batched else 0, positions.stride(-2), positions.stride(-1))
-    a.theta, a.eps = spec.theta, spec.eps
-    if spec.freqs is not None:
-        a._freqs = (ctypes.c_double * len(spec.freqs))(*spec.freqs)
-        a.freqs = ctypes.cast(a._freqs, ctypes.POINTER(ctypes.c_double))
-    return a
+def _out_shape(shape, heads_first):
+    return (*shape[:-3], shape[-2], shape[-3], shape[-1]) if heads_first else shape
 
 
-def _out_shape(x, heads_first):
-    return (*x.shape[:-3], x.shape[-2], x.shape[-3], x.shape[-1]) if heads_first else x.shape
+_NO_TENSOR = (0,) * 16
+
+
+def _pack(spec, x, positions, fields, count, ws=0, ws_bytes=0):
+    shape = x.shape
+    ps = positions.stride()
+    batched = len(ps) == 3 and positions.shape[0] > 1
+    return _lib.ROTARY_ARGS.pack(
+        *fields, *(_NO_TENSOR if count == 1 else ()), count, _DTYPES[x.dtype], shape[0] if len(shape) == 4 else 1,
+        shape[-3], shape[-1], positions.shape[-1], *spec.axes, spec.pairs, positions.data_ptr(),
+        _lib.LAYER_F32 if positions.dtype is torch.float32 else _lib.LAYER_I32, ps[0] if batched else 0, ps[-2], ps[-1],
+        spec.theta, spec.freqs, spec.eps, ws, ws_bytes)
+
+
+def _guarded(call, device):
+    """call() with the tensors' device current."""
+    if torch.cuda.current_device() == device.index:
+        return call()
+    with torch.cuda.device(device):
+        return call()
 
 
 def _forward(spec, tensors, weights, positions):
     positions = _check(spec, tensors, weights, positions)
-    a = _args(spec, tensors[0], positions)
-    a.n_tensors = len(tensors)
-    outs = []
-    keep = []
-    with torch.cuda.device(tensors[0].device):
-        for i, (x, w) in enumerate(zip(tensors, weights)):
+    x0 = tensors[0]
+    dtype, dev, hf = x0.dtype, x0.device, spec.heads_first
+
+    def call():
+        outs, fields, keep = [], [], []
+        for x, w in zip(tensors, weights):
             x = _unit_rows(x)
-            w = None if w is None else w.contiguous()
-            y = torch.empty(_out_shape(x, spec.heads_first), dtype=x.dtype, device=x.device)
-            t = a.tensor[i]
-            t.in_, t.in_stride[:], t.out, t.out_stride[:] = ptr(x), _strides(x), ptr(y), _strides(y, spec.heads_first)
-            t.heads = int(x.shape[-2])
+            y = torch.empty(_out_shape(x.shape, hf), dtype=dtype, device=dev)
+            wp = wd = 0
             if w is not None:
-                t.weight, t.weight_dtype = ptr(w), _DTYPES[w.dtype]
-            keep += [x, w]
+                w = w.contiguous()
+                wp, wd = w.data_ptr(), _DTYPES[w.dtype]
+            fields += (x.data_ptr(), *_strides(x), y.data_ptr(), *_strides(y, hf), 0, 0, 0, 0, wp, 0, wd, x.shape[-2])
+            keep += (x, w)
             outs.append(y)
-        check(lib().htrc_rotary_forward(a, stream_ptr()), "htrc_rotary_forward")
-    return outs
+        rc = lib().htrc_rotary_forward(_pack(spec, x0, positions, fields, len(outs)), _lib.raw_stream(dev.index))
+        if rc:
+            check(rc, "htrc_rotary_forward")
+        return outs
+
+    return _guarded(call, dev)
 
 
 def _backward(spec, grads, tensors, weights, positions):
     positions = _check(spec, tensors, weights, positions)
-    a = _args(spec, tensors[0], positions)
-    a.n_tensors = len(tensors)
-    outs, dws, keep = [], [], []
-    dev = tensors[0].device
-    with torch.cuda.device(dev):
-        for i, (g, x, w) in enumerate(zip(grads, tensors, weights)):
-            if not isinstance(g, torch.Tensor) or g.shape != _out_shape(x, spec.heads_first) or g.dtype != x.dtype or \
-                    g.device != dev:
-                raise ValueError(f"the output's gradient: {list(_out_shape(x, spec.heads_first))} {x.dtype} expected")
+    x0 = tensors[0]
+    dtype, dev, hf = x0.dtype, x0.device, spec.heads_first
+
+    def call():
+        outs, dws, fields, keep = [], [], [], []
+        for g, x, w in zip(grads, tensors, weights):
+            shape = _out_shape(x.shape, hf)
+            if not isinstance(g, torch.Tensor) or g.shape != shape or g.dtype != dtype or g.device != dev:
+                raise ValueError(f"the output's gradient: {list(shape)} {dtype} expected")
             g, x = _unit_rows(g), _unit_rows(x)
-            w = None if w is None else w.contiguous()
-            dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-            dw = None if w is None else torch.empty_like(w)
-            t = a.tensor[i]
-            t.in_, t.in_stride[:], t.out, t.out_stride[:] = ptr(g), _strides(g, spec.heads_first), ptr(dx), _strides(dx)
-            t.heads = int(x.shape[-2])
+            dx = torch.empty(x.shape, dtype=dtype, device=dev)
+            dw = None
+            norm = (0, 0, 0, 0, 0, 0, 0)
             if w is not None:
-                t.x, t.x_stride[:] = ptr(x), _strides(x)
-                t.weight, t.weight_dtype, t.dweight = ptr(w), _DTYPES[w.dtype], ptr(dw)
-            keep += [g, x, w]
+                w = w.contiguous()
+                dw = torch.empty_like(w)
+                norm = (x.data_ptr(), *_strides(x), w.data_ptr(), dw.data_ptr(), _DTYPES[w.dtype])
+            fields += (g.data_ptr(), *_strides(g, hf), dx.data_ptr(), *_strides(dx), *norm, x.shape[-2])
+            keep += (g, x, w)
             outs.append(dx)
             dws.append(dw)
-        ws = None
+        ws, wp, need = None, 0, 0
         if any(w is not None for w in weights):
-            need = ctypes.c_size_t()
-            check(lib().htrc_rotary_workspace_size(a, need), "htrc_rotary_workspace_size")
-            ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-            a.workspace, a.workspace_bytes = ptr(ws), need.value
-        check(lib().htrc_rotary_backward(a, stream_ptr()), "htrc_rotary_backward")
-    return outs, dws
+            size = ctypes.c_size_t()
+            check(lib().htrc_rotary_workspace_size(_pack(spec, x0, positions, fields, len(outs)), size),
+                  "htrc_rotary_workspace_size")
+            need = size.value
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            wp = ws.data_ptr()
+        rc = lib().htrc_rotary_backward(_pack(spec, x0, positions, fields, len(outs), wp, need),
+                                        _lib.raw_stream(dev.index))
+        if rc:
+            check(rc, "htrc_rotary_backward")
+        return outs, dws
+
+    return _guarded(call, dev)
 
 
 class _Rotary(torch.autograd.Function):
@@ -223,25 +250,25 @@ def rotary_axes(x, positions, *, axes, theta=10000.0, pairs="interleaved", weigh
 
     positions [(batch,) tokens, len(axes)], integers (any int32 value, its angles exactly reduced) or floats; freqs:
     the ``sum(axes) / 2`` frequencies in radians per position instead of ``theta``'s."""
-    return _apply(_Spec(axes, theta, pairs, eps, freqs, heads_first), (x,), (weight,), positions)[0]
+    return _apply(_spec(axes, theta, pairs, eps, freqs, heads_first), (x,), (weight,), positions)[0]
 
 
 def rotary_axes_backward(dy, x, positions, *, axes, theta=10000.0, pairs="interleaved", weight=None, eps=1e-6,
                          freqs=None, heads_first=False):
     """(dx, dweight) of ``rotary_axes`` for the output's gradient dy (dweight None without a weight)."""
-    dx, dw = _backward(_Spec(axes, theta, pairs, eps, freqs, heads_first), (dy,), (x,), (weight,), positions)
+    dx, dw = _backward(_spec(axes, theta, pairs, eps, freqs, heads_first), (dy,), (x,), (weight,), positions)
     return dx[0], dw[0]
 
 
 def rotary_qk(q, k, positions, *, axes, theta=10000.0, pairs="interleaved", q_weight=None, k_weight=None, eps=1e-6,
               freqs=None, heads_first=False):
     """``rotary_axes`` of q [(batch,) tokens, heads, dim] and k [(batch,) tokens, kv_heads, dim] in one launch."""
-    return _apply(_Spec(axes, theta, pairs, eps, freqs, heads_first), (q, k), (q_weight, k_weight), positions)
+    return _apply(_spec(axes, theta, pairs, eps, freqs, heads_first), (q, k), (q_weight, k_weight), positions)
 
 
 def rotary_qk_backward(dq, dk, q, k, positions, *, axes, theta=10000.0, pairs="interleaved", q_weight=None,
                        k_weight=None, eps=1e-6, freqs=None, heads_first=False):
     """(dq, dk, dq_weight, dk_weight) of ``rotary_qk`` for its outputs' gradients."""
-    dx, dw = _backward(_Spec(axes, theta, pairs, eps, freqs, heads_first), (dq, dk), (q, k), (q_weight, k_weight),
+    dx, dw = _backward(_spec(axes, theta, pairs, eps, freqs, heads_first), (dq, dk), (q, k), (q_weight, k_weight),
                        positions)
     return (*dx, *dw)

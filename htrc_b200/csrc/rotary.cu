@@ -27,7 +27,11 @@ namespace {
 
 constexpr int kRotWarps = 8;
 constexpr int kRotMaxPairs = HTRC_ROTARY_MAX_DIM / 2;
-constexpr int kRotUnroll = 4;         // row batches whose loads are in flight together
+// Row batches that a warp fetches together (one more set is in flight while they are used), and CTAs per SM the
+// registers are held to.  q and k of 129,024 tokens x 24 heads x 128, bfloat16: forward 573 us (2, 4), 601 (3, 3), 612
+// (2, 2), 654 (1, 4); backward of 32,768 tokens 251 us (3, 2), 267 (2, 2), 288 (1, 3), 362 (2, 3).
+constexpr int rot_unroll(bool back) { return back ? 3 : 2; }
+constexpr int rot_ctas(bool back, int bytes) { return back || bytes == 4 ? 2 : 4; }
 
 struct RotaryRows {
   const void* in;
@@ -136,50 +140,46 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) { ret
 template <>
 __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) { return pack_f16x2(a, b); }
 
-template <typename T>
-__device__ __forceinline__ void unpack(const Raw<T>& r, float (&v)[8]) {
+// A lane's elements as the firsts and seconds of its four pairs, two pairs per register pair: paired float32
+// instructions then do two pairs at once, whatever the pairs' layout in memory.
+struct Pairs {
+  float2 f[2], s[2];
+};
+
+template <typename T, bool HALF>
+__device__ __forceinline__ Pairs unpack(const Raw<T>& r) {
+  Pairs v;
   if constexpr (sizeof(T) == 4) {
-    v[0] = __uint_as_float(r.a.x); v[1] = __uint_as_float(r.a.y); v[2] = __uint_as_float(r.a.z);
-    v[3] = __uint_as_float(r.a.w); v[4] = __uint_as_float(r.b.x); v[5] = __uint_as_float(r.b.y);
-    v[6] = __uint_as_float(r.b.z); v[7] = __uint_as_float(r.b.w);
-  } else {
-    const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+    const float a[8] = {__uint_as_float(r.a.x), __uint_as_float(r.a.y), __uint_as_float(r.a.z), __uint_as_float(r.a.w),
+                        __uint_as_float(r.b.x), __uint_as_float(r.b.y), __uint_as_float(r.b.z), __uint_as_float(r.b.w)};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = unpack2<T>(w[i]);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
+    for (int i = 0; i < 2; ++i) {
+      v.f[i] = HALF ? make_float2(a[2 * i], a[2 * i + 1]) : make_float2(a[4 * i], a[4 * i + 2]);
+      v.s[i] = HALF ? make_float2(a[4 + 2 * i], a[5 + 2 * i]) : make_float2(a[4 * i + 1], a[4 * i + 3]);
+    }
+  } else {
+    const float2 w[4] = {unpack2<T>(r.a.x), unpack2<T>(r.a.y), unpack2<T>(r.a.z), unpack2<T>(r.a.w)};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      v.f[i] = HALF ? w[i] : make_float2(w[2 * i].x, w[2 * i + 1].x);
+      v.s[i] = HALF ? w[2 + i] : make_float2(w[2 * i].y, w[2 * i + 1].y);
     }
   }
+  return v;
 }
 template <typename T, bool HALF>
-__device__ __forceinline__ void store8(T* row, int off0, int off1, const float (&v)[8]) {
+__device__ __forceinline__ void store8(T* row, int off0, int off1, const Pairs& v) {
   if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(row + off0) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(row + off1) = make_float4(v[4], v[5], v[6], v[7]);
+    const float4 lo = HALF ? make_float4(v.f[0].x, v.f[0].y, v.f[1].x, v.f[1].y) : make_float4(v.f[0].x, v.s[0].x, v.f[0].y, v.s[0].y);
+    const float4 hi = HALF ? make_float4(v.s[0].x, v.s[0].y, v.s[1].x, v.s[1].y) : make_float4(v.f[1].x, v.s[1].x, v.f[1].y, v.s[1].y);
+    *reinterpret_cast<float4*>(row + off0) = lo;
+    *reinterpret_cast<float4*>(row + off1) = hi;
+  } else if constexpr (HALF) {
+    *reinterpret_cast<uint2*>(row + off0) = make_uint2(pack2<T>(v.f[0].x, v.f[0].y), pack2<T>(v.f[1].x, v.f[1].y));
+    *reinterpret_cast<uint2*>(row + off1) = make_uint2(pack2<T>(v.s[0].x, v.s[0].y), pack2<T>(v.s[1].x, v.s[1].y));
   } else {
-    const uint4 w = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
-    if constexpr (HALF) {
-      *reinterpret_cast<uint2*>(row + off0) = make_uint2(w.x, w.y);
-      *reinterpret_cast<uint2*>(row + off1) = make_uint2(w.z, w.w);
-    } else {
-      *reinterpret_cast<uint4*>(row + off0) = w;
-    }
-  }
-}
-
-// Rotates a lane's 8 elements in place; turned pairs only (a pair past the rotated width stays, whatever it holds).
-// HALF: pairs (v[i], v[4 + i]), all 4 turned or none; else (v[2 i], v[2 i + 1]), the first n turned.  BACK: by -angle.
-template <bool HALF, bool BACK>
-__device__ __forceinline__ void turn8(float (&v)[8], const float2 (&cs)[4], int n) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int ia = HALF ? i : 2 * i, ib = HALF ? i + 4 : 2 * i + 1;
-    const float a = v[ia], b = v[ib], c = cs[i].x, s = BACK ? -cs[i].y : cs[i].y;
-    if (i < n) {
-      v[ia] = fmaf(a, c, -b * s);
-      v[ib] = fmaf(a, s, b * c);
-    }
+    *reinterpret_cast<uint4*>(row + off0) = make_uint4(pack2<T>(v.f[0].x, v.s[0].x), pack2<T>(v.f[0].y, v.s[0].y),
+                                                       pack2<T>(v.f[1].x, v.s[1].x), pack2<T>(v.f[1].y, v.s[1].y));
   }
 }
 
@@ -190,20 +190,32 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
+// the sums of two values over the LPR lanes of a row, in one exchange more than one of them takes
+template <int LPR>
+__device__ __forceinline__ float2 row_sums(float a, float b, int lane) {
+  const bool odd = lane & 1;
+  float v = odd ? b : a;
+  v += __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
+#pragma unroll
+  for (int o = LPR / 2; o > 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const float t = __shfl_xor_sync(0xffffffffu, v, 1);
+  return odd ? make_float2(t, v) : make_float2(v, t);
+}
+
 // Rows whose pieces are 16-byte aligned, dim a multiple of 8 (HALF: the rotated width too).  blockIdx.y names the
-// tensor; a warp's task is a token and `chunk` of its heads.  BACK with a weight leaves the CTA's weight-gradient sums
-// at partial[(blockIdx.y * gridDim.x + blockIdx.x) * dim].
+// tensor; a warp's task is a token and `chunk` of its heads.  The norm's weight is folded into the token's cosines and
+// sines.  BACK with a weight leaves the CTA's weight-gradient sums at partial[(blockIdx.y * gridDim.x + blockIdx.x) * dim].
 template <typename T, int LPR, bool HALF, bool BACK>
-__global__ void __launch_bounds__(kRotWarps * 32)
+__global__ void __launch_bounds__(kRotWarps * 32, rot_ctas(BACK, sizeof(T)))
     rotary_kernel(const __grid_constant__ RotaryParams p, float* __restrict__ partial) {
   __shared__ float sums[BACK ? kRotWarps * 32 * 8 : 1];
   const RotaryRows& r = p.t[blockIdx.y];
-  constexpr int RPW = 32 / LPR;
+  constexpr int RPW = 32 / LPR, kRotUnroll = rot_unroll(BACK);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int u = lane % LPR, sub = lane / LPR;
   const int units = p.dim / 8;
   const bool on = u < units;
-  // the lane's elements and the pairs they make
+  // the lane's elements (off0 .. + 3, off1 .. + 3) and the pairs they make, the first `turned` of them rotated
   int off0 = 8 * u, off1 = 8 * u + 4, pair0 = 4 * u, turned;
   if (HALF) {
     const int rot = p.npairs / 4;
@@ -216,82 +228,172 @@ __global__ void __launch_bounds__(kRotWarps * 32)
     turned = min(4, max(0, p.npairs - pair0));
   }
   if (!on) turned = 0;
-  const bool norm = r.weight != nullptr;
-  float w[8], dw[8];
+  const bool norm = r.weight != nullptr, whole = 2 * p.npairs == p.dim;
+  // offsets of element e of the firsts (0 .. 3) and seconds
+  auto first_at = [&](int e) { return HALF ? off0 + e : off0 + 2 * e; };
+  auto second_at = [&](int e) { return HALF ? off1 + e : off0 + 2 * e + 1; };
+  auto weights = [&]() {
+    Pairs w;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    w[i] = norm && on ? load_weight(r.weight, r.weight_dtype, (i < 4 ? off0 : off1 - 4) + i) : 0.f;
-    dw[i] = 0.f;
-  }
+    for (int i = 0; i < 2; ++i) {
+      w.f[i] = w.s[i] = make_float2(1.f, 1.f);
+      if (norm && on) {
+        w.f[i] = make_float2(load_weight(r.weight, r.weight_dtype, first_at(2 * i)), load_weight(r.weight, r.weight_dtype, first_at(2 * i + 1)));
+        w.s[i] = make_float2(load_weight(r.weight, r.weight_dtype, second_at(2 * i)), load_weight(r.weight, r.weight_dtype, second_at(2 * i + 1)));
+      }
+    }
+    return w;
+  };
+  Pairs dw;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) dw.f[i] = dw.s[i] = make_float2(0.f, 0.f);
   const float inv_dim = 1.0f / static_cast<float>(p.dim);
-  const int64_t tasks = p.batch * p.tokens * r.chunks;
-  for (int64_t task = static_cast<int64_t>(blockIdx.x) * kRotWarps + warp; task < tasks;
-       task += static_cast<int64_t>(gridDim.x) * kRotWarps) {
-    const int64_t tok = task / r.chunks;
+  const uint32_t tokens = static_cast<uint32_t>(p.tokens), tasks = static_cast<uint32_t>(p.batch) * tokens * r.chunks;
+  for (uint32_t task = blockIdx.x * kRotWarps + warp; task < tasks; task += gridDim.x * kRotWarps) {
+    const uint32_t tok = task / r.chunks, b = tok / tokens, n = tok - b * tokens;
     const int h0 = static_cast<int>(task - tok * r.chunks) * r.chunk, h1 = min(r.heads, h0 + r.chunk);
-    const int64_t b = tok / p.tokens, n = tok - b * p.tokens;
-    const T* in = static_cast<const T*>(r.in) + b * r.is[0] + n * r.is[1];
-    const T* x = BACK && norm ? static_cast<const T*>(r.x) + b * r.xs[0] + n * r.xs[1] : nullptr;
-    T* out = static_cast<T*>(r.out) + b * r.os[0] + n * r.os[1];
-    float2 cs[4];
+    const T* in = static_cast<const T*>(r.in) + b * r.is[0] + n * r.is[1] + (h0 + sub) * r.is[2];
+    const T* x = BACK && norm ? static_cast<const T*>(r.x) + b * r.xs[0] + n * r.xs[1] + (h0 + sub) * r.xs[2] : nullptr;
+    T* out = static_cast<T*>(r.out) + b * r.os[0] + n * r.os[1] + (h0 + sub) * r.os[2];
+    // rows in flight: the first ones are asked for before the angles are formed, the next ones before these are used
+    Raw<T> raw[kRotUnroll], rawx[BACK ? kRotUnroll : 1];
+    auto fetch = [&](int h) {
+#pragma unroll
+      for (int k = 0; k < kRotUnroll; ++k) {
+        raw[k] = Raw<T>{};
+        if (BACK) rawx[k] = Raw<T>{};
+        if (on && h + k * RPW < h1) {
+          raw[k] = load_raw<T, HALF>(in + k * RPW * r.is[2], off0, off1);
+          if (BACK && norm) rawx[k] = load_raw<T, HALF>(x + k * RPW * r.xs[2], off0, off1);
+        }
+      }
+      in += RPW * kRotUnroll * r.is[2];
+      if (BACK && norm) x += RPW * kRotUnroll * r.xs[2];
+    };
+    fetch(h0 + sub);
+    // forward: (f, s) -> (f fc - s ss, f fs + s sc), the weight folded in; backward: (f fc + s fs, s fc - f fs)
+    float2 fc[2], fs[2], sc[2], ss[2];
+    const Pairs w = weights();
     const int64_t pos = b * p.ps[0] + n * p.ps[1];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) cs[i] = i < turned ? pair_turn(p, pos, pair0 + i) : make_float2(1.f, 0.f);
-    for (int h = h0; h < h1; h += RPW * kRotUnroll) {
-      Raw<T> raw[kRotUnroll], rawx[BACK ? kRotUnroll : 1];
-#pragma unroll
-      for (int k = 0; k < kRotUnroll; ++k) {
-        const int hh = h + k * RPW + sub;
-        if (on && hh < h1) {
-          raw[k] = load_raw<T, HALF>(in + hh * r.is[2], off0, off1);
-          if (BACK && norm) rawx[k] = load_raw<T, HALF>(x + hh * r.xs[2], off0, off1);
-        } else {
-          raw[k] = Raw<T>{};
-          if (BACK) rawx[k] = Raw<T>{};
-        }
+    for (int i = 0; i < 2; ++i) {
+      const float2 t0 = 2 * i < turned ? pair_turn(p, pos, pair0 + 2 * i) : make_float2(1.f, 0.f);
+      const float2 t1 = 2 * i + 1 < turned ? pair_turn(p, pos, pair0 + 2 * i + 1) : make_float2(1.f, 0.f);
+      fc[i] = make_float2(t0.x, t1.x);
+      fs[i] = make_float2(t0.y, t1.y);
+      if (!BACK) {
+        sc[i] = mul2(fc[i], w.s[i]);
+        ss[i] = mul2(make_float2(-t0.y, -t1.y), w.s[i]);
+        fc[i] = mul2(fc[i], w.f[i]);
+        fs[i] = mul2(fs[i], w.f[i]);
+      } else {
+        ss[i] = make_float2(-t0.y, -t1.y);
       }
+    }
+    for (int h = h0 + sub; h - sub < h1; h += RPW * kRotUnroll) {
+      Raw<T> now[kRotUnroll], nowx[BACK ? kRotUnroll : 1];
 #pragma unroll
       for (int k = 0; k < kRotUnroll; ++k) {
-        const int hh = h + k * RPW + sub;
-        float v[8];
-        unpack<T>(raw[k], v);
+        now[k] = raw[k];
+        if (BACK) nowx[k] = rawx[k];
+      }
+      if (h - sub + RPW * kRotUnroll < h1) fetch(h + RPW * kRotUnroll);
+#pragma unroll
+      for (int k = 0; k < kRotUnroll; ++k) {
+        Pairs v = unpack<T, HALF>(now[k]), y;
         if (!BACK) {
           if (norm) {
-            float ss = 0.f;
+            float2 q = mul2(v.f[0], v.f[0]);
+            q = fma2(v.f[1], v.f[1], q);
+            q = fma2(v.s[0], v.s[0], q);
+            q = fma2(v.s[1], v.s[1], q);
+            const float rs = rsqrtf(fmaf(row_sum<LPR>(q.x + q.y), inv_dim, p.eps));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
-            const float rs = rsqrtf(row_sum<LPR>(ss) * inv_dim + p.eps);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = v[i] * rs * w[i];
-          }
-          turn8<HALF, false>(v, cs, turned);
-        } else {
-          turn8<HALF, true>(v, cs, turned);
-          if (norm) {
-            float xv[8], ss = 0.f, hx = 0.f;
-            unpack<T>(rawx[k], xv);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              ss = fmaf(xv[i], xv[i], ss);
-              hx = fmaf(v[i] * w[i], xv[i], hx);
+            for (int i = 0; i < 2; ++i) {
+              v.f[i] = mul2(v.f[i], make_float2(rs, rs));
+              v.s[i] = mul2(v.s[i], make_float2(rs, rs));
             }
-            const float rs = rsqrtf(row_sum<LPR>(ss) * inv_dim + p.eps);
-            const float back = row_sum<LPR>(hx) * inv_dim * rs * rs;
+          }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              dw[i] = fmaf(v[i], xv[i] * rs, dw[i]);
-              v[i] = rs * fmaf(-xv[i], back, v[i] * w[i]);
+          for (int i = 0; i < 2; ++i) {
+            y.f[i] = fma2(v.f[i], fc[i], mul2(v.s[i], ss[i]));
+            y.s[i] = fma2(v.f[i], fs[i], mul2(v.s[i], sc[i]));
+          }
+          if (!whole) {      // a pair past the rotated width keeps its elements apart, whatever they hold
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const Pairs w = weights();
+              if (2 * i >= turned) {
+                y.f[i].x = v.f[i].x * w.f[i].x;
+                y.s[i].x = v.s[i].x * w.s[i].x;
+              }
+              if (2 * i + 1 >= turned) {
+                y.f[i].y = v.f[i].y * w.f[i].y;
+                y.s[i].y = v.s[i].y * w.s[i].y;
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            y.f[i] = fma2(v.f[i], fc[i], mul2(v.s[i], fs[i]));
+            y.s[i] = fma2(v.s[i], fc[i], mul2(v.f[i], ss[i]));
+          }
+          if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (2 * i >= turned) {
+                y.f[i].x = v.f[i].x;
+                y.s[i].x = v.s[i].x;
+              }
+              if (2 * i + 1 >= turned) {
+                y.f[i].y = v.f[i].y;
+                y.s[i].y = v.s[i].y;
+              }
+            }
+          }
+          if (norm) {
+            const Pairs xv = unpack<T, HALF>(nowx[k]);
+            float2 q = mul2(xv.f[0], xv.f[0]), hx;
+            q = fma2(xv.f[1], xv.f[1], q);
+            q = fma2(xv.s[0], xv.s[0], q);
+            q = fma2(xv.s[1], xv.s[1], q);
+            Pairs g;         // the gradient of the normalised row, times the weight
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              g.f[i] = mul2(y.f[i], w.f[i]);
+              g.s[i] = mul2(y.s[i], w.s[i]);
+            }
+            hx = mul2(g.f[0], xv.f[0]);
+            hx = fma2(g.f[1], xv.f[1], hx);
+            hx = fma2(g.s[0], xv.s[0], hx);
+            hx = fma2(g.s[1], xv.s[1], hx);
+            const float2 t = row_sums<LPR>(q.x + q.y, hx.x + hx.y, lane);
+            const float rs = rsqrtf(fmaf(t.x, inv_dim, p.eps));
+            const float back = -t.y * inv_dim * rs * rs;
+            const float2 rs2 = make_float2(rs, rs), back2 = make_float2(back, back);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 xf = mul2(xv.f[i], rs2), xs = mul2(xv.s[i], rs2);
+              dw.f[i] = fma2(y.f[i], xf, dw.f[i]);
+              dw.s[i] = fma2(y.s[i], xs, dw.s[i]);
+              y.f[i] = fma2(xf, back2, mul2(g.f[i], rs2));
+              y.s[i] = fma2(xs, back2, mul2(g.s[i], rs2));
             }
           }
         }
-        if (on && hh < h1) store8<T, HALF>(out + hh * r.os[2], off0, off1, v);
+        if (on && h + k * RPW < h1) store8<T, HALF>(out + k * RPW * r.os[2], off0, off1, y);
       }
+      out += RPW * kRotUnroll * r.os[2];
     }
   }
   if (BACK && norm) {
     // the CTA's sums, rows of a warp and then warps in order
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sums[threadIdx.x * 8 + i] = dw[i];
+    for (int i = 0; i < 2; ++i) {
+      *reinterpret_cast<float2*>(sums + threadIdx.x * 8 + 2 * i) = dw.f[i];
+      *reinterpret_cast<float2*>(sums + threadIdx.x * 8 + 4 + 2 * i) = dw.s[i];
+    }
     __syncthreads();
     float* dst = partial + (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * p.dim;
     if (threadIdx.x < LPR && on) {
@@ -299,7 +401,7 @@ __global__ void __launch_bounds__(kRotWarps * 32)
       for (int i = 0; i < 8; ++i) {
         float s = 0.f;
         for (int g = 0; g < kRotWarps * RPW; ++g) s += sums[(g * LPR + u) * 8 + i];
-        dst[(i < 4 ? off0 : off1 - 4) + i] = s;
+        dst[i < 4 ? first_at(i) : second_at(i - 4)] = s;
       }
     }
   }
@@ -431,7 +533,8 @@ int rotary_validate(const HtrcRotaryArgs* a, bool back, bool ptrs) {
   if (a == nullptr || a->n_tensors < 1 || a->n_tensors > 2) return HTRC_ERR_ARG;
   if (a->dtype < HTRC_LAYER_F32 || a->dtype > HTRC_LAYER_F16) return HTRC_ERR_ARG;
   if (a->batch < 0 || a->tokens < 0) return HTRC_ERR_ARG;
-  if (a->tokens > 0 && a->batch > (int64_t(1) << 40) / a->tokens) return HTRC_ERR_ARG;
+  constexpr int64_t kMaxRows = int64_t(1) << 32;      // of one head count's rows: a task's 32-bit index
+  if (a->tokens > 0 && a->batch > kMaxRows / a->tokens) return HTRC_ERR_UNSUPPORTED;
   if (a->dim < 2 || a->n_axes < 1) return HTRC_ERR_ARG;
   if (a->dim > HTRC_ROTARY_MAX_DIM || a->n_axes > HTRC_ROTARY_MAX_AXES) return HTRC_ERR_UNSUPPORTED;
   int64_t width = 0;
@@ -447,7 +550,7 @@ int rotary_validate(const HtrcRotaryArgs* a, bool back, bool ptrs) {
   for (int i = 0; i < a->n_tensors; ++i) {
     const HtrcRotaryTensor& t = a->tensor[i];
     if (t.heads < 1) return HTRC_ERR_ARG;
-    if (t.heads > HTRC_ROTARY_MAX_HEADS) return HTRC_ERR_UNSUPPORTED;
+    if (t.heads > HTRC_ROTARY_MAX_HEADS || a->batch * a->tokens * t.heads >= kMaxRows) return HTRC_ERR_UNSUPPORTED;
     if (t.weight_dtype < HTRC_LAYER_F32 || t.weight_dtype > HTRC_LAYER_F16) return HTRC_ERR_ARG;
     if (!ptrs || a->batch * a->tokens == 0) continue;
     if (!t.in || !t.out || !a->positions) return HTRC_ERR_ARG;

@@ -79,7 +79,7 @@ def _rotary(**kw):
 
 @pytest.mark.parametrize("kw,rc", [
     (dict(n_tensors=0), _lib.HTRC_ERR_ARG), (dict(n_tensors=3), _lib.HTRC_ERR_ARG), (dict(dtype=3), _lib.HTRC_ERR_ARG),
-    (dict(tokens=-1), _lib.HTRC_ERR_ARG), (dict(batch=1 << 39), _lib.HTRC_ERR_ARG), (dict(dim=1), _lib.HTRC_ERR_ARG),
+    (dict(tokens=-1), _lib.HTRC_ERR_ARG), (dict(batch=1 << 39), _lib.HTRC_ERR_UNSUPPORTED), (dict(dim=1), _lib.HTRC_ERR_ARG),
     (dict(dim=257), _lib.HTRC_ERR_UNSUPPORTED), (dict(n_axes=0), _lib.HTRC_ERR_ARG), (dict(n_axes=5), _lib.HTRC_ERR_UNSUPPORTED),
     (dict(axis_width=(31, 32, 0, 0)), _lib.HTRC_ERR_ARG), (dict(axis_width=(64, 2, 0, 0)), _lib.HTRC_ERR_ARG),
     (dict(pairs=2), _lib.HTRC_ERR_ARG), (dict(position_dtype=_lib.LAYER_BF16), _lib.HTRC_ERR_ARG), (dict(theta=0.0), _lib.HTRC_ERR_ARG),

@@ -156,7 +156,8 @@ SIGNATURES = {
     "htrc_rotary_workspace_size": (ctypes.c_int, [_p, ctypes.POINTER(ctypes.c_size_t)]),
     "htrc_rotary_backward": (ctypes.c_int, [_p, _p]),
     "htrc_cross_forward": (ctypes.c_int, [_p, _p]),
-    "htrc_cross_workspace_size": (ctypes.c_int, [_p, ctypes.POINTER(ctypes.c_size_t)]),
+    "htrc_cross_forward_workspace_size": (ctypes.c_int, [_p, ctypes.POINTER(ctypes.c_size_t)]),
+    "htrc_cross_backward_workspace_size": (ctypes.c_int, [_p, ctypes.POINTER(ctypes.c_size_t)]),
     "htrc_cross_backward": (ctypes.c_int, [_p, _p]),
 }
 

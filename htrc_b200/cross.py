@@ -73,7 +73,7 @@ def _mask_strides(mask, want):
 class _Call:
     """The checked arguments of one call: 4-d operands, shapes and the mask."""
     __slots__ = ("q", "k", "v", "heads_first", "lengths", "mask", "squeeze", "lse_shape", "shape_args", "mask_args",
-                 "device")
+                 "device", "few_units")
 
     def __init__(self, q, k, v, key_lengths, mask, scale, heads_first):
         for name, x in (("q", q), ("k", k), ("v", v)):
@@ -121,6 +121,8 @@ class _Call:
             self.mask_args = (mask.data_ptr(), _MASKS[mask.dtype], *_mask_strides(mask, (batch, heads, queries, keys)))
         self.q, self.k, self.v = _rows(q), _rows(k), _rows(v)
         self.lse_shape = (batch, heads, queries)
+        # enough tiles of 256 rows that the library never splits their keys (it asks for no workspace then)
+        self.few_units = batch * heads * (queries + 255) < 256 * 1024
         self.shape_args = (batch, queries, keys, heads, kv_heads, dim, _DTYPES[q.dtype], scale,
                            0 if key_lengths is None else key_lengths.data_ptr())
 
@@ -144,7 +146,14 @@ def _forward(c, want_lse):
     def call():
         out = torch.empty(c.q.shape, dtype=c.q.dtype, device=c.device)
         lse = torch.empty(c.lse_shape, dtype=torch.float32, device=c.device) if want_lse else None
-        rc = lib().htrc_cross_forward(c.pack(out, lse), _lib.raw_stream(c.device.index))
+        args = c.pack(out, lse)
+        if c.few_units:
+            need = ctypes.c_size_t()
+            check(lib().htrc_cross_forward_workspace_size(args, need), "htrc_cross_forward_workspace_size")
+            if need.value:
+                ws = torch.empty(need.value, dtype=torch.uint8, device=c.device)
+                args = c.pack(out, lse, (*(0,) * 17, ws.data_ptr(), need.value))
+        rc = lib().htrc_cross_forward(args, _lib.raw_stream(c.device.index))
         if rc:
             check(rc, "htrc_cross_forward")
         return (out[0], None if lse is None else lse[0]) if c.squeeze else (out, lse)
@@ -171,7 +180,7 @@ def _backward(c, dout, out, lse, dlse):
         back = [do.data_ptr(), *_strides(do, hf), 0 if dz is None else dz.data_ptr(), dq.data_ptr(), dk.data_ptr(),
                 dv.data_ptr(), *_strides(dq, hf), *_strides(dk, hf), *_strides(dv, hf), 0, 0]
         need = ctypes.c_size_t()
-        check(lib().htrc_cross_workspace_size(c.pack(o, z, back), need), "htrc_cross_workspace_size")
+        check(lib().htrc_cross_backward_workspace_size(c.pack(o, z, back), need), "htrc_cross_backward_workspace_size")
         ws = torch.empty(need.value, dtype=torch.uint8, device=c.device)
         back[-2:] = ws.data_ptr(), need.value
         rc = lib().htrc_cross_backward(c.pack(o, z, back), _lib.raw_stream(c.device.index))

@@ -810,7 +810,7 @@ int cross_backward(const HtrcCrossArgs* a, cudaStream_t st) {
 
 extern "C" {
 
-int htrc_cross_workspace_size(const HtrcCrossArgs* args, size_t* bytes) {
+int htrc_cross_backward_workspace_size(const HtrcCrossArgs* args, size_t* bytes) {
   if (bytes == nullptr) return HTRC_ERR_ARG;
   return htrc::cross_sizes(args, bytes);
 }

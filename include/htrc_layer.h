@@ -89,14 +89,16 @@ typedef struct {
   const float* dlse;              /* gradient of lse, laid out as lse, or NULL */
   void *dq, *dk, *dv;
   int64_t dq_stride[3], dk_stride[3], dv_stride[3];
-  void* workspace;                /* htrc_cross_workspace_size() bytes, 256-byte aligned */
+  /* both: the direction's _workspace_size() bytes (the forward's may be 0), 256-byte aligned */
+  void* workspace;
   size_t workspace_bytes;
 } HtrcCrossArgs;
 
 /* Keys and values that no query may see (past a length, or excluded by a mask that is the same for every query) are
  * never computed with, whatever they hold. */
+int htrc_cross_forward_workspace_size(const HtrcCrossArgs* args, size_t* bytes);
 int htrc_cross_forward(const HtrcCrossArgs* args, htrc_stream_t stream);
-int htrc_cross_workspace_size(const HtrcCrossArgs* args, size_t* bytes);   /* of the backward */
+int htrc_cross_backward_workspace_size(const HtrcCrossArgs* args, size_t* bytes);
 int htrc_cross_backward(const HtrcCrossArgs* args, htrc_stream_t stream);
 
 #ifdef __cplusplus

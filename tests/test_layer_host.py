@@ -142,9 +142,9 @@ def test_cross_backward_wants_its_operands(name):
 def test_cross_workspace_size():
     L = _lib.lib()
     n = ctypes.c_size_t()
-    assert L.htrc_cross_workspace_size(ctypes.byref(_cross()), ctypes.byref(n)) == _lib.HTRC_OK and n.value >= 2 * 4 * 9 * 8
-    assert L.htrc_cross_workspace_size(ctypes.byref(_cross(dim=12)), ctypes.byref(n)) == _lib.HTRC_ERR_ARG
-    assert L.htrc_cross_workspace_size(ctypes.byref(_cross()), None) == _lib.HTRC_ERR_ARG
+    assert L.htrc_cross_backward_workspace_size(ctypes.byref(_cross()), ctypes.byref(n)) == _lib.HTRC_OK and n.value >= 2 * 4 * 9 * 8
+    assert L.htrc_cross_backward_workspace_size(ctypes.byref(_cross(dim=12)), ctypes.byref(n)) == _lib.HTRC_ERR_ARG
+    assert L.htrc_cross_backward_workspace_size(ctypes.byref(_cross()), None) == _lib.HTRC_ERR_ARG
     assert L.htrc_cross_forward(None, None) == _lib.HTRC_ERR_ARG
 
 

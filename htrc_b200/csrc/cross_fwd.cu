@@ -624,7 +624,10 @@ bool rows_ok(const void* p, const int64_t* stride) {
 
 // Parts the keys are split into: the fewest rounds of CTAs times blocks (1.2 us each), with about two blocks' time for a
 // unit's ends and, for any split, four for the second launch and the time that the parts' bytes take at 5 TB/s.
+bool few_rows(const HtrcCrossArgs* a) { return a->heads / a->kv_heads * a->queries <= kCrossFewRows; }
+
 int fwd_splits(const HtrcCrossArgs* a) {
+  if (few_rows(a)) return 1;
   const int64_t units = a->batch * a->heads * ((a->queries + kXUnit - 1) / kXUnit), sms = sm_count();
   const int64_t blocks = (a->keys + kXKeys - 1) / kXKeys;
   if (units == 0 || units >= 4 * sms) return 1;
@@ -657,7 +660,7 @@ int fwd_sizes(const HtrcCrossArgs* a, int* splits, size_t* bytes) {
   *splits = fwd_splits(a);
   const int64_t units = a->batch * a->heads * ((a->queries + kXUnit - 1) / kXUnit) * *splits;
   if (units > (int64_t(1) << 31) - 1) return HTRC_ERR_UNSUPPORTED;
-  *bytes = fwd_bytes(a, *splits);
+  *bytes = few_rows(a) ? cross_few_bytes(a) : fwd_bytes(a, *splits);
   return HTRC_OK;
 }
 
@@ -672,6 +675,7 @@ int cross_forward(const HtrcCrossArgs* a, cudaStream_t st) {
   if (a->batch * a->queries == 0) return HTRC_OK;
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 256))
     return HTRC_ERR_WORKSPACE;
+  if (few_rows(a)) return cross_forward_few(a, st);
   CrossFwdParams p{};
   p.s = cross_shape(a);
   p.lse = a->lse;

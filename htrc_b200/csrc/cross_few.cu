@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2)
   copy_wait<0>();
 }
 
-// units of several segments (or none): a CTA each, a group of DP / 4 threads per segment and row
+// units of several segments (or none): a CTA per row, a group of DP / 4 threads per segment
 template <int DP, bool BF>
 __global__ void __launch_bounds__(256) cross_few_join_kernel(const __grid_constant__ CrossFewParams p, int64_t most) {
   asm volatile("griddepcontrol.wait;" ::: "memory");               // the first kernel's results
@@ -402,62 +402,60 @@ __global__ void __launch_bounds__(256) cross_few_join_kernel(const __grid_consta
     if (n == 1) return;
   }
   const int64_t slot0 = few_slot(unit, i0) * kFewRows;
-  for (int r = 0; r < kFewRows; ++r) {
-    const FewRow w(p, unit, r);
-    if (!w.live) break;
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = g; i < n; i += 4 * G) {
-      // four segments' loads together
-      float2 ml[4];
-      float4 x[4];
+  const int r = blockIdx.y;
+  const FewRow w(p, unit, r);
+  if (!w.live) return;
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = g; i < n; i += 4 * G) {
+    // four segments' loads together
+    float2 ml[4];
+    float4 x[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int64_t slot = slot0 + static_cast<int64_t>(i + k * G) * kFewRows + r;
-        const bool in = i + k * G < n;
-        ml[k] = in ? p.part_ml[slot] : make_float2(-INFINITY, 0.f);
-        x[k] = in ? *reinterpret_cast<const float4*>(p.part + slot * DP + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float mn = fmaxf(m, ml[k].x), ref = mn == -INFINITY ? 0.f : mn;
-        const float f0 = cross_ex2((m - ref) * kCrossLog2e), f1 = cross_ex2((ml[k].x - ref) * kCrossLog2e);
-        m = mn;
-        l = l * f0 + ml[k].y * f1;
-        acc.x = acc.x * f0 + x[k].x * f1;
-        acc.y = acc.y * f0 + x[k].y * f1;
-        acc.z = acc.z * f0 + x[k].z * f1;
-        acc.w = acc.w * f0 + x[k].w * f1;
-      }
+    for (int k = 0; k < 4; ++k) {
+      const int64_t slot = slot0 + static_cast<int64_t>(i + k * G) * kFewRows + r;
+      const bool in = i + k * G < n;
+      ml[k] = in ? p.part_ml[slot] : make_float2(-INFINITY, 0.f);
+      x[k] = in ? *reinterpret_cast<const float4*>(p.part + slot * DP + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    acc_s[g][c] = acc;
-    if (c == 0) {
-      ml_s[g][0] = m;
-      ml_s[g][1] = l;
-    }
-    __syncthreads();
-    if (threadIdx.x < DP) {
-      const int d = threadIdx.x;
-      float mm = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < G; ++i) mm = fmaxf(mm, ml_s[i][0]);
-      const float ref = mm == -INFINITY ? 0.f : mm;
-      float a = 0.f, ll = 0.f;
-#pragma unroll
-      for (int i = 0; i < G; ++i) {
-        const float f = cross_ex2((ml_s[i][0] - ref) * kCrossLog2e);
-        a = fmaf(reinterpret_cast<const float*>(acc_s[i])[d], f, a);
-        ll = fmaf(ml_s[i][1], f, ll);
-      }
-      if (d < p.s.dim) {
-        const float x = ll == 0.f ? 0.f : a / ll;
-        uint16_t* dst = p.out + b * p.os[0] + w.n * p.os[1] + w.h * p.os[2] + d;
-        if (BF) *reinterpret_cast<__nv_bfloat16*>(dst) = __float2bfloat16_rn(x);
-        else *reinterpret_cast<__half*>(dst) = __float2half_rn(x);
-      }
-      if (d == 0) few_lse(p, b, w, mm, ll);
+    for (int k = 0; k < 4; ++k) {
+      const float mn = fmaxf(m, ml[k].x), ref = mn == -INFINITY ? 0.f : mn;
+      const float f0 = cross_ex2((m - ref) * kCrossLog2e), f1 = cross_ex2((ml[k].x - ref) * kCrossLog2e);
+      m = mn;
+      l = l * f0 + ml[k].y * f1;
+      acc.x = acc.x * f0 + x[k].x * f1;
+      acc.y = acc.y * f0 + x[k].y * f1;
+      acc.z = acc.z * f0 + x[k].z * f1;
+      acc.w = acc.w * f0 + x[k].w * f1;
     }
-    __syncthreads();
+  }
+  acc_s[g][c] = acc;
+  if (c == 0) {
+    ml_s[g][0] = m;
+    ml_s[g][1] = l;
+  }
+  __syncthreads();
+  if (threadIdx.x < DP) {
+    const int d = threadIdx.x;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < G; ++i) mm = fmaxf(mm, ml_s[i][0]);
+    const float ref = mm == -INFINITY ? 0.f : mm;
+    float a = 0.f, ll = 0.f;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const float f = cross_ex2((ml_s[i][0] - ref) * kCrossLog2e);
+      a = fmaf(reinterpret_cast<const float*>(acc_s[i])[d], f, a);
+      ll = fmaf(ml_s[i][1], f, ll);
+    }
+    if (d < p.s.dim) {
+      const float x = ll == 0.f ? 0.f : a / ll;
+      uint16_t* dst = p.out + b * p.os[0] + w.n * p.os[1] + w.h * p.os[2] + d;
+      if (BF) *reinterpret_cast<__nv_bfloat16*>(dst) = __float2bfloat16_rn(x);
+      else *reinterpret_cast<__half*>(dst) = __float2half_rn(x);
+    }
+    if (d == 0) few_lse(p, b, w, mm, ll);
   }
 }
 
@@ -484,7 +482,7 @@ int launch_few(const CrossFewParams& p, int64_t units, int ctas, cudaStream_t st
   if (rc != HTRC_OK) return rc;
   if (!p.line) return HTRC_OK;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(units));
+  cfg.gridDim = dim3(static_cast<unsigned>(units), static_cast<unsigned>(std::min<int64_t>(kFewRows, p.s.group * p.s.queries)));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr{};

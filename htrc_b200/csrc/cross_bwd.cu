@@ -56,7 +56,7 @@ struct DqParams {
   const float* dlse;
   const uint16_t* out;
   int64_t out_stride[3];
-  float4* stat;             // [batch * heads][padded rows]: (lse in the pass's units, log2 of tied keys, delta, 0)
+  float* stat;              // [batch * heads][padded rows / 64][3][64]: lse in the pass's units, log2 of tied keys, delta
   int64_t stat_rows;
   int tiles;
   int* status;
@@ -223,7 +223,10 @@ __global__ void __launch_bounds__(kDqThreads, 2)
         if (lse == INFINITY) delta = 0.f;
       }
     }
-    p.stat[static_cast<int64_t>(bh) * p.stat_rows + row] = make_float4(lse, ties, delta, 0.f);
+    float* stat = p.stat + (static_cast<int64_t>(bh) * p.stat_rows + row / 64 * 64) * 3 + row % 64;
+    stat[0] = lse;
+    stat[64] = ties;
+    stat[128] = delta;
     for (int j = 0; ok && j < blocks; ++j) {
       const int left = count - j * kDqKeys;
       uint32_t bits[2] = {0u, 0u};
@@ -345,7 +348,7 @@ constexpr int kDkvKeys = 128, kDkvRows = 64, kDkvStages = 4;
 constexpr uint32_t kDkvColK = 0, kDkvColV = 128, kDkvColS = 256, kDkvBuf = 128, kDkvCols = 512;
 
 struct DkvBars {
-  uint64_t kv_full, full[kDkvStages], empty[kDkvStages], s_full[2], ds_full[2], acc_full;
+  uint64_t kv_full, full[kDkvStages], empty[kDkvStages], s_full[2], dp_full[2], p_full[2], ds_full[2], acc_full;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -355,7 +358,8 @@ struct DkvSmem {
   static constexpr int kChunks = DP / 64;
   static constexpr uint32_t kKeyChunk = 128 * 128, kRowChunk = 64 * 128;
   static constexpr uint32_t kTile = kChunks * kKeyChunk, kRows = kChunks * kRowChunk;
-  static constexpr uint32_t kK = 0, kV = kTile, kRing = 2 * kTile, kStage = 2 * kRows + kDkvRows * 16;
+  static constexpr uint32_t kK = 0, kV = kTile, kRing = 2 * kTile, kStat = kDkvRows * 3 * 4,
+                            kStage = 2 * kRows + 1024;
   static constexpr uint32_t kBars = kRing + kDkvStages * kStage;
   static constexpr uint32_t kUsed = kBars + 256 + 1024;
   // one CTA per SM: it takes all 512 TMEM columns
@@ -364,7 +368,7 @@ struct DkvSmem {
 
 struct DkvParams {
   CrossShape s;
-  const float4* stat;
+  const float* stat;
   int64_t stat_rows;
   int key_blocks, splits, row_blocks;
   float* partial;           // splits > 1: [2 (dk, dv)][split][batch * kv_heads][keys][DP]
@@ -402,6 +406,8 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->dp_full[i], 1);
+      mbar_init(&bars->p_full[i], 128);
       mbar_init(&bars->ds_full[i], 128);
     }
     mbar_init(&bars->acc_full, 1);
@@ -433,12 +439,12 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
         const int64_t at = first + i;
         const int h = hk * p.s.group + static_cast<int>(at / p.row_blocks), row = static_cast<int>(at % p.row_blocks) * kDkvRows;
         uint8_t* st = smem + SM::kRing + s * SM::kStage;
-        mbar_arrive_expect_tx(&bars->full[s], SM::kStage);
+        mbar_arrive_expect_tx(&bars->full[s], 2 * SM::kRows + SM::kStat);
         for (int c = 0; c < SM::kChunks; ++c) {
           tma_load_4d(st + c * SM::kRowChunk, &tm_q, &bars->full[s], 64 * c, row, h * p.s.q_h, b * p.s.q_b, pol);
           tma_load_4d(st + SM::kRows + c * SM::kRowChunk, &tm_do, &bars->full[s], 64 * c, row, h * do_h, b * do_b, pol);
         }
-        bulk_load(st + 2 * SM::kRows, p.stat + (static_cast<int64_t>(b) * p.s.heads + h) * p.stat_rows + row, kDkvRows * 16,
+        bulk_load(st + 2 * SM::kRows, p.stat + ((static_cast<int64_t>(b) * p.s.heads + h) * p.stat_rows + row) * 3, SM::kStat,
                   &bars->full[s], pol);
       }
       __syncwarp();
@@ -457,20 +463,22 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       const int s = i % kDkvStages;
       if (!mbar_wait_warp(&bars->full[s], (i / kDkvStages) & 1, status, abort_flag)) return false;
       tc_fence_after();
-      const uint64_t so = (s * SM::kStage) >> 4;
-      const uint32_t d = tmem + kDkvColS + (i & 1) * kDkvBuf;
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) {
         const uint32_t a = ((kk / 4) * SM::kKeyChunk + (kk % 4) * 32) >> 4, o = ((kk / 4) * SM::kRowChunk + (kk % 4) * 32) >> 4;
-        mma_bf16_by(leader, d, dk + a, qk0 + so + o, id_s, kk != 0);
-      }
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        const uint32_t a = ((kk / 4) * SM::kKeyChunk + (kk % 4) * 32) >> 4, o = ((kk / 4) * SM::kRowChunk + (kk % 4) * 32) >> 4;
-        mma_bf16_by(leader, d + 64, dv + a, dok0 + so + o, id_s, kk != 0);
+        mma_bf16_by(leader, tmem + kDkvColS + (i & 1) * kDkvBuf, dk + a, qk0 + ((s * SM::kStage) >> 4) + o, id_s, kk != 0);
       }
       mma_commit_by(leader, &bars->s_full[i & 1]);
       return true;
+    };
+    auto products = [&](int i) {          // dP^T, of a stage that scores() waited for
+      const int s = i % kDkvStages;
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        const uint32_t a = ((kk / 4) * SM::kKeyChunk + (kk % 4) * 32) >> 4, o = ((kk / 4) * SM::kRowChunk + (kk % 4) * 32) >> 4;
+        mma_bf16_by(leader, tmem + kDkvColS + (i & 1) * kDkvBuf + 64, dv + a, dok0 + ((s * SM::kStage) >> 4) + o, id_s, kk != 0);
+      }
+      mma_commit_by(leader, &bars->dp_full[i & 1]);
     };
     bool ok = steps == 0 || mbar_wait_warp(&bars->kv_full, 0, status, abort_flag);
     // keys past the entry's count may hold anything: their rows become zeros (with a bias the softmax threads select)
@@ -478,22 +486,31 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       zero_excluded_rows<kDkvKeys, SM::kChunks>(smem + SM::kK, SM::kKeyChunk, key0, count, p.s, 0, false, lane);
       zero_excluded_rows<kDkvKeys, SM::kChunks>(smem + SM::kV, SM::kKeyChunk, key0, count, p.s, 0, false, lane);
     }
-    for (int i = 0; ok && i < 2 && i < steps; ++i) ok = scores(i);
+    for (int i = 0; ok && i < 2 && i < steps; ++i) {
+      ok = scores(i);
+      if (ok) products(i);
+    }
     for (int i = 0; ok && i < steps; ++i) {
       const int s = i % kDkvStages;
-      if (!mbar_wait_warp(&bars->ds_full[i & 1], (i >> 1) & 1, status, abort_flag)) break;
+      // P^T first: its product and the next S^T of this buffer run while the threads form dS^T
+      ok = mbar_wait_warp(&bars->p_full[i & 1], (i >> 1) & 1, status, abort_flag);
+      if (!ok) break;
       tc_fence_after();
       const uint64_t so = (s * SM::kStage) >> 4;
       const uint32_t a = tmem + kDkvColS + (i & 1) * kDkvBuf;
 #pragma unroll
       for (int kk = 0; kk < kDkvRows / 16; ++kk)
         mma_bf16_ts_by(leader, tmem + kDkvColV, a + 8 * kk, don0 + so + ((kk * 2048) >> 4), id_g, (i | kk) != 0);
+      if (i + 2 < steps) ok = scores(i + 2);
+      ok = ok && mbar_wait_warp(&bars->ds_full[i & 1], (i >> 1) & 1, status, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
 #pragma unroll
       for (int kk = 0; kk < kDkvRows / 16; ++kk)
         mma_bf16_ts_by(leader, tmem + kDkvColK, a + 64 + 8 * kk, qn0 + so + ((kk * 2048) >> 4), id_g, (i | kk) != 0);
       mma_commit_by(leader, &bars->empty[s]);
       if (i == steps - 1) mma_commit_by(leader, &bars->acc_full);
-      if (i + 2 < steps) ok = scores(i + 2);
+      if (i + 2 < steps) products(i + 2);
     }
   } else {
     // ------------------------------------------------------------------ two warpgroups, one thread per key
@@ -518,53 +535,84 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       }
       if (!mbar_wait_warp(&bars->s_full[wg], (i >> 1) & 1, status, abort_flag)) { ok = false; break; }
       tc_fence_after();
-      const float4* st = reinterpret_cast<const float4*>(smem + SM::kRing + s * SM::kStage + 2 * SM::kRows);
+      // the queries' statistics: [lse][ties][delta], 64 each
+      const float* st = reinterpret_cast<const float*>(smem + SM::kRing + s * SM::kStage + 2 * SM::kRows);
       const uint32_t buf = tmem + lanes + kDkvColS + wg * kDkvBuf;
-#pragma unroll 1
+      float2 w[32];                         // P, kept for dS
+      uint32_t out = 0u, out_hi = 0u;       // queries this key is excluded from (with a mask per query)
+#pragma unroll
       for (int c = 0; c < 2; ++c) {
-        uint32_t x[32], y[32], pw[16], dw[16];
+        uint32_t x[32], pw[16];
         tmem_ld32(buf + 32 * c, x);
+        tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          const float4 ls = *reinterpret_cast<const float4*>(st + 32 * c + k);
+          const float4 ti = NAT ? *reinterpret_cast<const float4*>(st + 64 + 32 * c + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int h2 = 0; h2 < 2; ++h2) {
+            const float l0 = h2 ? ls.z : ls.x, l1 = h2 ? ls.w : ls.y;
+            const int kk = k + 2 * h2, q = row + 32 * c + kk;
+            float2 e = make_float2(__uint_as_float(x[kk]), __uint_as_float(x[kk + 1]));
+            if (!NAT) {
+              float2 off = make_float2(kbias - l0, kbias - l1);
+              if (KIND == CROSS_PAIRS) {
+                const uint8_t* mk = static_cast<const uint8_t*>(p.s.mask.p) + mask_at;
+                if (!(in && q < p.s.queries && __ldg(mk + q * p.s.mask.sn) != 0)) off.x = -INFINITY;
+                if (!(in && q + 1 < p.s.queries && __ldg(mk + (q + 1) * p.s.mask.sn) != 0)) off.y = -INFINITY;
+              }
+              e = fma2(e, make_float2(scale, scale), off);
+            } else {
+              float b0 = kbias, b1 = kbias;
+              if (KIND == CROSS_BIAS) {
+                b0 = in && q < p.s.queries ? mask_term(p.s.mask.p, p.s.mask.dtype, mask_at + q * p.s.mask.sn) : -INFINITY;
+                b1 = in && q + 1 < p.s.queries ? mask_term(p.s.mask.p, p.s.mask.dtype, mask_at + (q + 1) * p.s.mask.sn) : -INFINITY;
+              }
+              e = fma2(e, make_float2(scale, scale), make_float2(b0, b1));
+              e = fma2(sub2(e, make_float2(l0, l1)), make_float2(kCrossLog2e, kCrossLog2e),
+                       h2 ? make_float2(-ti.z, -ti.w) : make_float2(-ti.x, -ti.y));
+              // an excluded key's weight and gradient are zero whatever its row holds
+              if (b0 == -INFINITY) {
+                e.x = -INFINITY;
+                (c ? out_hi : out) |= 1u << kk;
+              }
+              if (b1 == -INFINITY) {
+                e.y = -INFINITY;
+                (c ? out_hi : out) |= 2u << kk;
+              }
+            }
+            e = make_float2(cross_ex2(e.x), cross_ex2(e.y));
+            w[16 * c + kk / 2] = e;
+            pw[kk / 2] = pack16x2<BF>(e.x, e.y);
+          }
+        }
+        tmem_st16(buf + 16 * c, pw);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&bars->p_full[wg]);
+      if (!mbar_wait_warp(&bars->dp_full[wg], (i >> 1) & 1, status, abort_flag)) { ok = false; break; }
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t y[32], dw[16];
         tmem_ld32(buf + 64 + 32 * c, y);
         tmem_ld_wait();
 #pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-          const float4 s0 = st[32 * c + k], s1 = st[32 * c + k + 1];     // (lse, ties, delta) of the two queries
-          float2 e = make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-          float2 g = make_float2(__uint_as_float(y[k]), __uint_as_float(y[k + 1]));
-          if (!NAT) {
-            float2 off = make_float2(kbias - s0.x, kbias - s1.x);
-            if (KIND == CROSS_PAIRS) {
-              const int q = row + 32 * c + k;
-              const uint8_t* mk = static_cast<const uint8_t*>(p.s.mask.p) + mask_at;
-              if (!(in && q < p.s.queries && __ldg(mk + q * p.s.mask.sn) != 0)) off.x = -INFINITY;
-              if (!(in && q + 1 < p.s.queries && __ldg(mk + (q + 1) * p.s.mask.sn) != 0)) off.y = -INFINITY;
+        for (int k = 0; k < 32; k += 4) {
+          const float4 de = *reinterpret_cast<const float4*>(st + 128 + 32 * c + k);
+#pragma unroll
+          for (int h2 = 0; h2 < 2; ++h2) {
+            const int kk = k + 2 * h2;
+            float2 g = make_float2(__uint_as_float(y[kk]), __uint_as_float(y[kk + 1]));
+            if (NAT) {
+              if ((c ? out_hi : out) >> kk & 1u) g.x = 0.f;
+              if ((c ? out_hi : out) >> kk & 2u) g.y = 0.f;
             }
-            e = fma2(e, make_float2(scale, scale), off);
-          } else {
-            float b0 = kbias, b1 = kbias;
-            if (KIND == CROSS_BIAS) {
-              const int q = row + 32 * c + k;
-              b0 = in && q < p.s.queries ? mask_term(p.s.mask.p, p.s.mask.dtype, mask_at + q * p.s.mask.sn) : -INFINITY;
-              b1 = in && q + 1 < p.s.queries ? mask_term(p.s.mask.p, p.s.mask.dtype, mask_at + (q + 1) * p.s.mask.sn) : -INFINITY;
-            }
-            e = fma2(e, make_float2(scale, scale), make_float2(b0, b1));
-            e = fma2(sub2(e, make_float2(s0.x, s1.x)), make_float2(kCrossLog2e, kCrossLog2e), make_float2(-s0.y, -s1.y));
-            // an excluded key's weight and gradient are zero whatever its row holds
-            if (b0 == -INFINITY) {
-              e.x = -INFINITY;
-              g.x = 0.f;
-            }
-            if (b1 == -INFINITY) {
-              e.y = -INFINITY;
-              g.y = 0.f;
-            }
+            const float2 d = mul2(w[16 * c + kk / 2], sub2(g, h2 ? make_float2(de.z, de.w) : make_float2(de.x, de.y)));
+            dw[kk / 2] = pack16x2<BF>(d.x, d.y);
           }
-          e = make_float2(cross_ex2(e.x), cross_ex2(e.y));
-          pw[k >> 1] = pack16x2<BF>(e.x, e.y);
-          const float2 d = mul2(e, sub2(g, make_float2(s0.z, s1.z)));
-          dw[k >> 1] = pack16x2<BF>(d.x, d.y);
         }
-        tmem_st16(buf + 16 * c, pw);
         tmem_st16(buf + 64 + 16 * c, dw);
       }
       tmem_st_wait();
@@ -680,7 +728,7 @@ int dkv_splits(const HtrcCrossArgs* a) {
 }
 
 int64_t stat_rows(const HtrcCrossArgs* a) { return (a->queries + kDqRows - 1) / kDqRows * kDqRows; }
-size_t stat_bytes(const HtrcCrossArgs* a) { return static_cast<size_t>(a->batch * a->heads * stat_rows(a)) * 16; }
+size_t stat_bytes(const HtrcCrossArgs* a) { return (static_cast<size_t>(a->batch * a->heads * stat_rows(a)) * 12 + 255) / 256 * 256; }
 
 template <typename K>
 bool ready(K kernel, uint32_t bytes, bool (&done)[64]) {
@@ -699,7 +747,7 @@ int launch_bwd(const HtrcCrossArgs* a, cudaStream_t st) {
   auto kkv = cross_dkv_kernel<DP, BF, KIND>;
   if (!ready(kq, DqSmem<DP>::kBytes, done_q) || !ready(kkv, DkvSmem<DP>::kBytes, done_kv)) return HTRC_ERR_CUDA;
   const CrossShape s = cross_shape(a);
-  float4* stat = static_cast<float4*>(a->workspace);
+  float* stat = static_cast<float*>(a->workspace);
   const bool keys = a->keys > 0, rows = a->queries > 0;
   // an empty side's maps are never read: the other side's rows stand in
   const void *k = keys ? a->k : a->q, *v = keys ? a->v : a->q, *q = rows ? a->q : a->k, *o = rows ? a->dout : a->k;

@@ -4,9 +4,12 @@
 //
 // Two passes, each recomputing S and dP on tcgen05, so that no gradient needs an atomic and every sum has a fixed order:
 //
-// cross_dq_kernel: a CTA owns 128 query rows and walks the keys in blocks of 64, dQ accumulating in TMEM (S 64, dP 64
-// and dQ 128 columns: two CTAs per SM, one's products under the other's exponentials).  It also forms delta from the
-// rows of dO and out that it holds and leaves (lse, delta) for the second pass.
+// cross_dq_kernel: persistent, one CTA per SM; a unit is 128 query rows of one head, walked over the keys in blocks of
+// 128, dQ accumulating in TMEM (128 columns).  S is double buffered (256 columns), so the next block's S runs under this
+// block's exponentials; dP (128 columns) is freed when the threads have read it, so its next product runs before dQ's.
+// dS overwrites S.  Two threads per row, 64 keys each: nothing passes between them (no maximum here) but delta's halves.
+// delta comes from the rows of dO and out while the unit's first weights are formed; (lse, delta) are left for the second
+// pass.  The K / V ring runs on into the next unit, and its Q and dO follow as soon as the last products have read these.
 //
 // cross_dkv_kernel: a CTA owns 128 keys of one key head (rows of S^T = K Q^T and dP^T = V dO^T) and a range of the
 // query blocks of 64 of every head that shares it; dK and dV accumulate in TMEM (256 columns), S^T and dP^T are double
@@ -28,26 +31,24 @@ namespace {
 constexpr float kHuge = 1e30f;        // a |log sum| above this is a mask's lowest value: the logits are lost in it
 
 // ------------------------------------------------------------------------------------------------ dQ
-constexpr int kDqThreads = 192;
-constexpr int kDqRows = 128, kDqKeys = 64;
-constexpr uint32_t kDqColS = 0, kDqColP = 64, kDqColQ = 128, kDqCols = 256;
+constexpr int kDqThreads = 320;
+constexpr int kDqRows = 128, kDqKeys = 128;
+constexpr uint32_t kDqColS = 0, kDqColP = 256, kDqColQ = 384, kDqCols = 512;      // S: two buffers
 
 struct DqBars {
-  uint64_t q_full, k_full[2], k_empty[2], v_full, v_empty, s_full, ds_full, dq_full;
+  uint64_t q_full, q_empty, do_full, do_empty, kv_full[5], kv_empty[5], s_full[2], ds_full[2], dp_full, dp_read, dq_full;
   uint32_t tmem_base;
   int abort_flag;
 };
 
 template <int DP>
 struct DqSmem {
-  static constexpr int kChunks = DP / 64;
-  static constexpr uint32_t kRowChunk = 128 * 128, kKeyChunk = 64 * 128;
-  static constexpr uint32_t kTile = kChunks * kRowChunk, kSlot = kChunks * kKeyChunk;
-  static constexpr uint32_t kQ = 0, kDo = kTile, kK = 2 * kTile, kV = kK + 2 * kSlot, kBias = kV + kSlot;
-  static constexpr uint32_t kBars = kBias + 2 * kDqKeys * 4, kUsed = kBars + 256;
-  static_assert(sizeof(DqBars) <= 256 && kUsed <= 115712, "two CTAs per SM");
-  // never more than two CTAs on an SM's 512 TMEM columns
-  static constexpr uint32_t kBytes = kUsed < 80 * 1024 ? 80 * 1024 : kUsed;
+  // five slots: with four, a block's K waited for the K two blocks before it to leave, a step later
+  static constexpr int kChunks = DP / 64, kSlots = 5;
+  static constexpr uint32_t kChunk = 128 * 128, kTile = kChunks * kChunk;
+  static constexpr uint32_t kQ = 0, kDo = kTile, kKV = 2 * kTile, kBias = kKV + kSlots * kTile;
+  static constexpr uint32_t kDelta = kBias + 2 * kDqKeys * 4, kBars = kDelta + 2 * kDqRows * 4, kBytes = kBars + 192;
+  static_assert(sizeof(DqBars) <= 192 && kBytes <= 232448, "shared memory of one CTA");
 };
 
 struct DqParams {
@@ -56,20 +57,48 @@ struct DqParams {
   const float* dlse;
   const uint16_t* out;
   int64_t out_stride[3];
+  uint16_t* dq;
+  int64_t dq_stride[3];
   float* stat;              // [batch * heads][padded rows / 64][3][64]: lse in the pass's units, log2 of tied keys, delta
   int64_t stat_rows;
-  int tiles;
+  uint32_t units, tiles;    // tiles of 128 rows per head
+  int do_b, do_h;
   int* status;
 };
 
+// A CTA's units, and within one its blocks of keys
+struct DqWalk {
+  uint32_t unit;
+  int b, h, row0, count, j, j1;
+  __device__ __forceinline__ void open(const DqParams& p, uint32_t u) {
+    unit = u;
+    if (u >= p.units) return;
+    const uint32_t bh = u / p.tiles;
+    b = static_cast<int>(bh / static_cast<uint32_t>(p.s.heads));
+    h = static_cast<int>(bh - b * static_cast<uint32_t>(p.s.heads));
+    row0 = static_cast<int>(u - bh * p.tiles) * kDqRows;
+    count = key_count(p.s, b);
+    j = 0;
+    j1 = (count + kDqKeys - 1) / kDqKeys;
+  }
+  __device__ __forceinline__ bool done(const DqParams& p) const { return unit >= p.units; }
+  // the first unit from u on that has a block
+  __device__ __forceinline__ void open_live(const DqParams& p, uint32_t u) {
+    for (open(p, u); !done(p) && j >= j1;) open(p, unit + gridDim.x);
+  }
+  __device__ __forceinline__ void next(const DqParams& p) {
+    if (++j >= j1) open_live(p, unit + gridDim.x);
+  }
+};
+
 template <int DP, bool BF, int KIND>
-__global__ void __launch_bounds__(kDqThreads, 2)
+__global__ void __launch_bounds__(kDqThreads, 1)
     cross_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                     const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                    const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ DqParams p, int do_b, int do_h) {
+                    const __grid_constant__ DqParams p) {
   using SM = DqSmem<DP>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  if (smem_u32(smem) & 1023) {          // the swizzled tiles need it; two CTAs leave no room to round up
+  if (smem_u32(smem) & 1023) {          // the swizzled tiles need it; there is no room to round up
     flag_status(p.status, ST_WAIT_TIMEOUT);
     return;
   }
@@ -77,269 +106,398 @@ __global__ void __launch_bounds__(kDqThreads, 2)
   volatile int* abort_flag = &bars->abort_flag;
   int* status = p.status;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tile = blockIdx.x % p.tiles;
-  const int bh = blockIdx.x / p.tiles;
-  const int h = bh % p.s.heads, b = bh / p.s.heads, hk = h / p.s.group;
-  const int row0 = tile * kDqRows;
-  const int count = key_count(p.s, b);
-  const int blocks = (count + kDqKeys - 1) / kDqKeys;
-  const int64_t mask_at = b * p.s.mask.sb + h * p.s.mask.sh;
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
+    mbar_init(&bars->q_empty, 1);
+    mbar_init(&bars->do_full, 1);
+    mbar_init(&bars->do_empty, 1 + 8);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->k_full[i], 1);
-      mbar_init(&bars->k_empty[i], 1);
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->ds_full[i], 256);
     }
-    mbar_init(&bars->v_full, 1);
-    mbar_init(&bars->v_empty, 1);
-    mbar_init(&bars->s_full, 1);
-    mbar_init(&bars->ds_full, 128);
+    for (int i = 0; i < SM::kSlots; ++i) {
+      mbar_init(&bars->kv_full[i], 1);
+      mbar_init(&bars->kv_empty[i], 1);
+    }
+    mbar_init(&bars->dp_full, 1);
+    mbar_init(&bars->dp_read, 256);
     mbar_init(&bars->dq_full, 1);
     bars->abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 5) tmem_alloc(&bars->tmem_base, kDqCols);
+  if (warp == 9) tmem_alloc(&bars->tmem_base, kDqCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
+  DqWalk w{};
 
-  if (warp == 4) {
-    // ------------------------------------------------------------------ TMA
+  if (warp == 8) {
+    // ------------------------------------------------------------------ TMA: ring slots K, V, K, V, ...
     const uint64_t pol_q = policy_evict_first(), pol_kv = policy_evict_last();
     const uint32_t leader = elect_one();
-    if (leader && blocks > 0) {
-      mbar_arrive_expect_tx(&bars->q_full, 2 * SM::kTile);
-      for (int c = 0; c < SM::kChunks; ++c) {
-        tma_load_4d(smem + SM::kQ + c * SM::kRowChunk, &tm_q, &bars->q_full, 64 * c, row0, h * p.s.q_h, b * p.s.q_b, pol_q);
-        tma_load_4d(smem + SM::kDo + c * SM::kRowChunk, &tm_do, &bars->q_full, 64 * c, row0, h * do_h, b * do_b, pol_q);
-      }
-    }
-    int j = 0;
-    for (; j < blocks; ++j) {
-      const int s = j & 1;
-      if (j > 1 && !mbar_wait_warp(&bars->k_empty[s], ((j >> 1) - 1) & 1, status, abort_flag)) break;
+    int slots = 0, units = 0;
+    auto load = [&](int j, int kv) -> bool {
+      const int s = slots % SM::kSlots, hk = w.h / p.s.group;
+      if (slots >= SM::kSlots && !mbar_wait_warp(&bars->kv_empty[s], ((slots / SM::kSlots) - 1) & 1, status, abort_flag))
+        return false;
       if (leader) {
-        mbar_arrive_expect_tx(&bars->k_full[s], SM::kSlot);
+        mbar_arrive_expect_tx(&bars->kv_full[s], SM::kTile);
         for (int c = 0; c < SM::kChunks; ++c)
-          tma_load_4d(smem + SM::kK + s * SM::kSlot + c * SM::kKeyChunk, &tm_k, &bars->k_full[s], 64 * c, j * kDqKeys,
-                      hk * p.s.k_h, b * p.s.k_b, pol_kv);
+          tma_load_4d(smem + SM::kKV + s * SM::kTile + c * SM::kChunk, kv ? &tm_v : &tm_k, &bars->kv_full[s], 64 * c,
+                      j * kDqKeys, hk * (kv ? p.s.v_h : p.s.k_h), w.b * (kv ? p.s.v_b : p.s.k_b), pol_kv);
       }
       __syncwarp();
-      if (j > 0 && !mbar_wait_warp(&bars->v_empty, (j - 1) & 1, status, abort_flag)) break;
+      ++slots;
+      return true;
+    };
+    bool ok = true;
+    auto rows = [&](const CUtensorMap* map, uint32_t at, uint64_t* full, uint64_t* empty, int in_h, int in_b) -> bool {
+      if (units > 0 && !mbar_wait_warp(empty, (units - 1) & 1, status, abort_flag)) return false;
       if (leader) {
-        mbar_arrive_expect_tx(&bars->v_full, SM::kSlot);
+        mbar_arrive_expect_tx(full, SM::kTile);
         for (int c = 0; c < SM::kChunks; ++c)
-          tma_load_4d(smem + SM::kV + c * SM::kKeyChunk, &tm_v, &bars->v_full, 64 * c, j * kDqKeys, hk * p.s.v_h,
-                      b * p.s.v_b, pol_kv);
+          tma_load_4d(smem + at + c * SM::kChunk, map, full, 64 * c, w.row0, w.h * in_h, w.b * in_b, pol_q);
       }
       __syncwarp();
+      return true;
+    };
+    for (w.open_live(p, blockIdx.x); ok && !w.done(p); w.open_live(p, w.unit + gridDim.x), ++units) {
+      ok = load(w.j, 0) && rows(&tm_q, SM::kQ, &bars->q_full, &bars->q_empty, p.s.q_h, p.s.q_b) &&
+           rows(&tm_do, SM::kDo, &bars->do_full, &bars->do_empty, p.do_h, p.do_b) && load(w.j, 1);
+      for (int j = w.j + 1; ok && j < w.j1; ++j) ok = load(j, 0) && load(j, 1);
     }
-    if (j == blocks && blocks > 0) {      // the last releases have landed before the CTA leaves
-      drain_ring<true>(bars->k_empty, 2, blocks, status, abort_flag);
-      mbar_wait_warp(&bars->v_empty, (blocks - 1) & 1, status, abort_flag);
+    if (ok && units > 0) {                // the last releases have landed before the CTA leaves
+      mbar_wait_warp(&bars->q_empty, (units - 1) & 1, status, abort_flag);
+      mbar_wait_warp(&bars->do_empty, (units - 1) & 1, status, abort_flag);
     }
-  } else if (warp == 5) {
+    if (ok) drain_ring<true>(bars->kv_empty, SM::kSlots, slots, status, abort_flag);   // before the CTA leaves
+  } else if (warp == 9) {
     // ------------------------------------------------------------------ MMA
     const uint32_t leader = elect_one();
     const uint32_t id_s = idesc16<BF>(128, kDqKeys, false, false);
     const uint32_t id_q = idesc16<BF>(128, DP, false, true);
     const uint64_t dq = desc_k(smem_u32(smem + SM::kQ)), ddo = desc_k(smem_u32(smem + SM::kDo));
-    const uint64_t dk0 = desc_k(smem_u32(smem + SM::kK)), dv = desc_k(smem_u32(smem + SM::kV));
-    const uint64_t dkn0 = desc_mn(smem_u32(smem + SM::kK), SM::kKeyChunk);
-    bool ok = blocks == 0 || mbar_wait_warp(&bars->q_full, 0, status, abort_flag);
-    for (int j = 0; ok && j < blocks; ++j) {
-      const int s = j & 1;
-      // excluded keys may hold anything: their rows of K (0 * NaN in dS K) and V become zeros
-      const bool dirty = KIND == CROSS_KEYS || (count < p.s.keys && (j + 1) * kDqKeys > count);
-      if (!mbar_wait_warp(&bars->k_full[s], (j >> 1) & 1, status, abort_flag)) break;
-      if (dirty)
-        zero_excluded_rows<kDqKeys, SM::kChunks>(smem + SM::kK + s * SM::kSlot, SM::kKeyChunk, j * kDqKeys, count, p.s,
-                                                 mask_at, KIND == CROSS_KEYS, lane);
-      if (!mbar_wait_warp(&bars->v_full, j & 1, status, abort_flag)) break;
-      if (dirty)
-        zero_excluded_rows<kDqKeys, SM::kChunks>(smem + SM::kV, SM::kKeyChunk, j * kDqKeys, count, p.s, mask_at,
-                                                 KIND == CROSS_KEYS, lane);
+    const uint64_t ring_k = desc_k(smem_u32(smem + SM::kKV)), ring_n = desc_mn(smem_u32(smem + SM::kKV), SM::kChunk);
+    DqWalk a;                             // the step whose S and dP are next
+    a.open_live(p, blockIdx.x);
+    int ahead = 0, units = 0;
+    // excluded keys may hold anything: their rows of K (0 * NaN in dS K) and V become zeros
+    auto slot = [&](int at) -> int {
+      const int s = at % SM::kSlots;
+      if (!mbar_wait_warp(&bars->kv_full[s], (at / SM::kSlots) & 1, status, abort_flag)) return -1;
+      if (KIND == CROSS_KEYS || (a.count < p.s.keys && (a.j + 1) * kDqKeys > a.count))
+        zero_excluded_rows<kDqKeys, SM::kChunks>(smem + SM::kKV + s * SM::kTile, SM::kChunk, a.j * kDqKeys, a.count, p.s,
+                                                 a.b * p.s.mask.sb + a.h * p.s.mask.sh, KIND == CROSS_KEYS, lane);
+      return s;
+    };
+    auto product = [&](uint32_t d, uint64_t rows, int s) {
       tc_fence_after();
-      const uint64_t so = (s * SM::kSlot) >> 4;
+      const uint64_t so = (s * SM::kTile) >> 4;
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) {
-        const uint32_t a = ((kk / 4) * SM::kRowChunk + (kk % 4) * 32) >> 4, o = ((kk / 4) * SM::kKeyChunk + (kk % 4) * 32) >> 4;
-        mma_bf16_by(leader, tmem + kDqColS, dq + a, dk0 + so + o, id_s, kk != 0);
+        const uint32_t o = ((kk / 4) * SM::kChunk + (kk % 4) * 32) >> 4;
+        mma_bf16_by(leader, d, rows + o, ring_k + so + o, id_s, kk != 0);
       }
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        const uint32_t a = ((kk / 4) * SM::kRowChunk + (kk % 4) * 32) >> 4, o = ((kk / 4) * SM::kKeyChunk + (kk % 4) * 32) >> 4;
-        mma_bf16_by(leader, tmem + kDqColP, ddo + a, dv + o, id_s, kk != 0);
+    };
+    auto scores = [&]() -> bool {         // S of a's step
+      if (a.j == 0 && !mbar_wait_warp(&bars->q_full, units & 1, status, abort_flag)) return false;
+      const int s = slot(2 * ahead);
+      if (s < 0) return false;
+      product(tmem + kDqColS + 128 * (ahead & 1), dq, s);
+      mma_commit_by(leader, &bars->s_full[ahead & 1]);
+      if (a.j + 1 == a.j1) mma_commit_by(leader, &bars->q_empty);
+      return true;
+    };
+    auto gradients = [&]() -> bool {      // dP of the same step, which it ends
+      if (a.j == 0 && !mbar_wait_warp(&bars->do_full, units & 1, status, abort_flag)) return false;
+      const int s = slot(2 * ahead + 1);
+      if (s < 0) return false;
+      product(tmem + kDqColP, ddo, s);
+      mma_commit_by(leader, &bars->dp_full);
+      mma_commit_by(leader, &bars->kv_empty[s]);
+      if (a.j + 1 == a.j1) {
+        mma_commit_by(leader, &bars->do_empty);
+        ++units;
       }
-      mma_commit_by(leader, &bars->s_full);
-      mma_commit_by(leader, &bars->v_empty);
-      if (!mbar_wait_warp(&bars->ds_full, j & 1, status, abort_flag)) break;
+      ++ahead;
+      a.next(p);
+      return true;
+    };
+    bool ok = true, first = true;
+    if (!a.done(p)) ok = scores() && gradients();
+    int n = 0;
+    for (w.open_live(p, blockIdx.x); ok && !w.done(p); ++n) {
+      const int s = (2 * n) % SM::kSlots;
+      const bool last = w.j + 1 == w.j1;
+      // the unit's next S and dP go before this dQ; the next unit's, whose rows come later, behind it
+      if (!last) ok = scores() && mbar_wait_warp(&bars->dp_read, n & 1, status, abort_flag) && gradients();
+      // (two barriers: the threads may finish the next step before this wait)
+      ok = ok && mbar_wait_warp(&bars->ds_full[n & 1], (n >> 1) & 1, status, abort_flag);
+      if (!ok) break;
       tc_fence_after();
+      const uint64_t ko = (s * SM::kTile) >> 4;
+      const uint32_t ds = tmem + kDqColS + 128 * (n & 1);        // keys 0-63 in columns 0-31, 64-127 in 64-95
 #pragma unroll
       for (int kk = 0; kk < kDqKeys / 16; ++kk)
-        mma_bf16_ts_by(leader, tmem + kDqColQ, tmem + kDqColS + 8 * kk, dkn0 + so + ((kk * 2048) >> 4), id_q, (j | kk) != 0);
-      mma_commit_by(leader, &bars->k_empty[s]);
-      if (j == blocks - 1) mma_commit_by(leader, &bars->dq_full);
+        mma_bf16_ts_by(leader, tmem + kDqColQ, ds + (kk / 4) * 64 + (kk % 4) * 8, ring_n + ko + ((kk * 2048) >> 4), id_q,
+                       !first || kk != 0);
+      mma_commit_by(leader, &bars->kv_empty[s]);
+      if (last) mma_commit_by(leader, &bars->dq_full);
+      if (last && !a.done(p)) ok = scores() && mbar_wait_warp(&bars->dp_read, n & 1, status, abort_flag) && gradients();
+      first = last;
+      w.next(p);
     }
   } else {
-    // ------------------------------------------------------------------ one thread per row
-    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-    const int row = row0 + threadIdx.x;
-    const bool valid = row < p.s.queries;
+    // ------------------------------------------------------------------ two threads per row, 64 keys (columns) each
+    const int half = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, key0 = 64 * half;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const float scale2 = p.s.scale * kCrossLog2e;
     constexpr bool NAT = KIND == CROSS_KEYS || KIND == CROSS_BIAS;
     float* bias = reinterpret_cast<float*>(smem + SM::kBias);
-    const int64_t at = static_cast<int64_t>(bh) * p.s.queries + row;
-    const int64_t row_mask = mask_at + (valid ? row : 0) * p.s.mask.sn;
-    // a row with nothing in it (or none): every weight exp2(-inf)
-    float lse = valid ? __ldg(p.lse + at) : -INFINITY, ties = 0.f, delta = 0.f;
-    if (NAT && fabsf(lse) > kHuge && lse != -INFINITY) {
-      // every logit of the row is a mask's lowest value and the log of their count is lost in lse: count them
-      int n = 0;
-      for (int i = 0; i < count; ++i)
-        n += mask_term(p.s.mask.p, p.s.mask.dtype, row_mask + static_cast<int64_t>(i) * p.s.mask.sm) == lse;
-      ties = n > 1 ? log2f(static_cast<float>(n)) : 0.f;
-    }
-    if (lse == -INFINITY) lse = INFINITY;
-    if (!NAT) lse *= kCrossLog2e;
+    float* delta_s = reinterpret_cast<float*>(smem + SM::kDelta);
     bool ok = true;
-    if (blocks > 0) {
-      ok = mbar_wait_warp(&bars->q_full, 0, status, abort_flag);
-      if (ok && valid) {
-        const uint16_t* o = p.out + b * p.out_stride[0] + row * p.out_stride[1] + h * p.out_stride[2];
-        float2 acc = make_float2(0.f, 0.f);
-        for (int c = 0; 8 * c < p.s.dim; ++c) {
-          const uint4 x = __ldg(reinterpret_cast<const uint4*>(o + 8 * c));
-          const uint4 y = *reinterpret_cast<const uint4*>(smem + SM::kDo + (c / 8) * SM::kRowChunk +
-                                                          sw128_off(threadIdx.x, c & 7));
-          acc = fma2(unpack16x2<BF>(x.x), unpack16x2<BF>(y.x), acc);
-          acc = fma2(unpack16x2<BF>(x.y), unpack16x2<BF>(y.y), acc);
-          acc = fma2(unpack16x2<BF>(x.z), unpack16x2<BF>(y.z), acc);
-          acc = fma2(unpack16x2<BF>(x.w), unpack16x2<BF>(y.w), acc);
+    int n = 0, units = 0;
+    // the row's lse and its gradient: loaded a unit ahead, as this half's columns of out into L2
+    float lse, dlse;
+    auto out_row = [&]() {
+      return p.out + w.b * p.out_stride[0] + static_cast<int64_t>(w.row0 + r) * p.out_stride[1] + w.h * p.out_stride[2] + half * (DP / 2);
+    };
+    auto ask = [&]() {
+      const int row = w.row0 + r;
+      const bool valid = !w.done(p) && row < p.s.queries;
+      const int64_t at = (static_cast<int64_t>(w.b) * p.s.heads + w.h) * p.s.queries + row;
+      lse = -INFINITY;
+      dlse = 0.f;
+      if (valid) {
+        lse = __ldg(p.lse + at);
+        if (p.dlse != nullptr) dlse = __ldg(p.dlse + at);
+        if (half * (DP / 2) < p.s.dim) asm volatile("prefetch.global.L2 [%0];" ::"l"(out_row()));
+      }
+    };
+    w.open(p, blockIdx.x);
+    ask();
+    while (ok && !w.done(p)) {
+      const int row = w.row0 + r;
+      const bool valid = row < p.s.queries, live = w.j1 > 0;
+      const int64_t bh = static_cast<int64_t>(w.b) * p.s.heads + w.h;
+      const int64_t mask_at = w.b * p.s.mask.sb + w.h * p.s.mask.sh;
+      const int64_t row_mask = mask_at + (valid ? row : 0) * p.s.mask.sn;
+      // a row with nothing in it (or none): every weight exp2(-inf)
+      float ties = 0.f, delta = 0.f;
+      if (NAT && fabsf(lse) > kHuge && lse != -INFINITY) {
+        // every logit of the row is a mask's lowest value and the log of their count is lost in lse: count them
+        int same = 0;
+        for (int i = 0; i < w.count; ++i)
+          same += mask_term(p.s.mask.p, p.s.mask.dtype, row_mask + static_cast<int64_t>(i) * p.s.mask.sm) == lse;
+        ties = same > 1 ? log2f(static_cast<float>(same)) : 0.f;
+      }
+      if (lse == -INFINITY) lse = INFINITY;
+      if (!NAT) lse *= kCrossLog2e;
+      for (int j = 0; j < w.j1; ++j, ++n) {
+        const int first = j * kDqKeys + key0, left = w.count - first;      // this thread's keys of the block
+        uint32_t bits[2] = {0u, 0u};
+        float* bj = bias + (n & 1) * kDqKeys + key0;
+        if (KIND == CROSS_KEYS) {
+          if (r < 64)
+            bj[r] = r < left ? mask_term(p.s.mask.p, p.s.mask.dtype, mask_at + static_cast<int64_t>(first + r) * p.s.mask.sm) : -INFINITY;
+          named_bar_sync(1 + half, 128);
         }
-        delta = acc.x + acc.y - (p.dlse != nullptr ? __ldg(p.dlse + at) : 0.f);
-        if (lse == INFINITY) delta = 0.f;
-      }
-    }
-    float* stat = p.stat + (static_cast<int64_t>(bh) * p.stat_rows + row / 64 * 64) * 3 + row % 64;
-    stat[0] = lse;
-    stat[64] = ties;
-    stat[128] = delta;
-    for (int j = 0; ok && j < blocks; ++j) {
-      const int left = count - j * kDqKeys;
-      uint32_t bits[2] = {0u, 0u};
-      float* bj = bias + (j & 1) * kDqKeys;
-      if (KIND == CROSS_KEYS) {
-        const int i = threadIdx.x;
-        if (i < kDqKeys)
-          bj[i] = i < left ? mask_term(p.s.mask.p, p.s.mask.dtype,
-                                       mask_at + static_cast<int64_t>(j * kDqKeys + i) * p.s.mask.sm) : -INFINITY;
-        named_bar_sync(1, 128);
-      }
-      if (KIND == CROSS_PAIRS) {
-        const int rows = min(32, static_cast<int>(p.s.queries) - (row0 + warp * 32));
-        const int64_t ma = mask_at + static_cast<int64_t>(row0 + warp * 32) * p.s.mask.sn +
-                           static_cast<int64_t>(j * kDqKeys) * p.s.mask.sm;
-        for (int r = 0; r < rows; ++r) {
+        if (KIND == CROSS_PAIRS) {
+          // the warp's 32 rows of mask bits: a row's 64 keys by coalesced loads, eight rows in flight, and ballots
+          const int rows = min(32, static_cast<int>(p.s.queries) - (w.row0 + quarter * 32));
+          const uint8_t* mk = static_cast<const uint8_t*>(p.s.mask.p) + mask_at +
+                              static_cast<int64_t>(w.row0 + quarter * 32) * p.s.mask.sn + static_cast<int64_t>(first + lane) * p.s.mask.sm;
+          for (int g = 0; g < rows; g += 8) {
+            uint8_t v[8][2];
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int key = 32 * q + lane;
-            const bool keep = key < left && __ldg(static_cast<const uint8_t*>(p.s.mask.p) + ma + r * p.s.mask.sn +
-                                                  key * p.s.mask.sm) != 0;
-            const uint32_t w = __ballot_sync(0xffffffffu, keep);
-            if (lane == r) bits[q] = w;
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+              for (int q = 0; q < 2; ++q)
+                v[i][q] = g + i < rows && 32 * q + lane < left ? __ldg(mk + i * p.s.mask.sn + 32 * q * p.s.mask.sm) : 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const uint32_t word = __ballot_sync(0xffffffffu, v[i][q] != 0);
+                if (lane == g + i) bits[q] = word;
+              }
+            mk += 8 * p.s.mask.sn;
           }
         }
-      }
-      if (!mbar_wait_warp(&bars->s_full, j & 1, status, abort_flag)) { ok = false; break; }
-      tc_fence_after();
-#pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
-        uint32_t s[32], g[32], w[16];
-        tmem_ld32(tmem + lanes + kDqColS + 32 * c, s);
-        tmem_ld32(tmem + lanes + kDqColP + 32 * c, g);
-        tmem_ld_wait();
-        if (KIND == CROSS_NONE) {
-          if (left < kDqKeys) {
+        // this half's columns of out, asked for before the unit's first weights are formed
+        uint4 o[DP / 16];
+        if (j == 0) {
+          const uint16_t* src = out_row();
+#pragma unroll
+          for (int c = 0; c < DP / 16; ++c) {
+            o[c] = make_uint4(0, 0, 0, 0);
+            if (valid && half * (DP / 2) + 8 * c < p.s.dim) o[c] = __ldg(reinterpret_cast<const uint4*>(src + 8 * c));
+          }
+        }
+        const uint32_t col_s = tmem + lanes + kDqColS + 128 * (n & 1) + key0, col_p = tmem + lanes + kDqColP + key0;
+        if (!mbar_wait_warp(&bars->s_full[n & 1], (n >> 1) & 1, status, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        float2 e[32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[32];
+          tmem_ld32(col_s + 32 * c, s);
+          tmem_ld_wait();
+          if (KIND == CROSS_NONE) {
+            if (left < 64) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (32 * c + i >= left) s[i] = __float_as_uint(-INFINITY);
+            }
+          } else if (KIND == CROSS_PAIRS) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (32 * c + i >= left) s[i] = __float_as_uint(-INFINITY);
+              if (!(bits[c] >> i & 1u)) s[i] = __float_as_uint(-INFINITY);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              float t;
+              if (KIND == CROSS_KEYS)
+                t = bj[32 * c + i];
+              else
+                t = 32 * c + i < left ? mask_term(p.s.mask.p, p.s.mask.dtype, row_mask + static_cast<int64_t>(first + 32 * c + i) * p.s.mask.sm)
+                                      : -INFINITY;
+              s[i] = __float_as_uint(t == -INFINITY ? t : fmaf(__uint_as_float(s[i]), p.s.scale, t));
+            }
           }
-        } else if (KIND == CROSS_PAIRS) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!(bits[c] >> i & 1u)) s[i] = __float_as_uint(-INFINITY);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float t;
-            if (KIND == CROSS_KEYS)
-              t = bj[32 * c + i];
+          for (int i = 0; i < 32; i += 2) {
+            float2 x = make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+            if (NAT)
+              x = fma2(sub2(x, make_float2(lse, lse)), make_float2(kCrossLog2e, kCrossLog2e), make_float2(-ties, -ties));
             else
-              t = 32 * c + i < left ? mask_term(p.s.mask.p, p.s.mask.dtype,
-                                                row_mask + static_cast<int64_t>(j * kDqKeys + 32 * c + i) * p.s.mask.sm)
-                                    : -INFINITY;
-            s[i] = __float_as_uint(t == -INFINITY ? t : fmaf(__uint_as_float(s[i]), p.s.scale, t));
+              x = fma2(x, make_float2(scale2, scale2), make_float2(-lse, -lse));
+            e[16 * c + i / 2] = make_float2(cross_ex2(x.x), cross_ex2(x.y));
           }
         }
+        if (j == 0) {
+          // delta: each half of the row's columns, then both
+          ok = mbar_wait_warp(&bars->do_full, units & 1, status, abort_flag);
+          if (!ok) break;
+          float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float2 e = make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-          if (NAT)
-            e = fma2(sub2(e, make_float2(lse, lse)), make_float2(kCrossLog2e, kCrossLog2e), make_float2(-ties, -ties));
-          else
-            e = fma2(e, make_float2(scale2, scale2), make_float2(-lse, -lse));
-          e = make_float2(cross_ex2(e.x), cross_ex2(e.y));
-          e = mul2(e, sub2(make_float2(__uint_as_float(g[i]), __uint_as_float(g[i + 1])), make_float2(delta, delta)));
-          w[i >> 1] = pack16x2<BF>(e.x, e.y);
+          for (int c = 0; c < DP / 16; ++c) {
+            const int piece = half * (DP / 16) + c;
+            const uint4 y = *reinterpret_cast<const uint4*>(smem + SM::kDo + (piece / 8) * SM::kChunk + sw128_off(r, piece & 7));
+            acc = fma2(unpack16x2<BF>(o[c].x), unpack16x2<BF>(y.x), acc);
+            acc = fma2(unpack16x2<BF>(o[c].y), unpack16x2<BF>(y.y), acc);
+            acc = fma2(unpack16x2<BF>(o[c].z), unpack16x2<BF>(y.z), acc);
+            acc = fma2(unpack16x2<BF>(o[c].w), unpack16x2<BF>(y.w), acc);
+          }
+          delta_s[half * kDqRows + r] = acc.x + acc.y;
+          fence_proxy_async_smem();           // generic reads of rows that TMA refills
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->do_empty);
+          named_bar_sync(3, 256);
+          delta = delta_s[r] + delta_s[kDqRows + r] - dlse;
+          if (lse == INFINITY) delta = 0.f;
+          if (half == 0) {
+            float* stat = p.stat + (bh * p.stat_rows + row / 64 * 64) * 3 + row % 64;
+            stat[0] = lse;
+            stat[64] = ties;
+            stat[128] = delta;
+          }
         }
-        tmem_st16(tmem + lanes + kDqColS + 16 * c, w);      // dS over columns of S this thread has already read
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(&bars->ds_full);
-    }
-    if (ok && blocks > 0) ok = mbar_wait_warp(&bars->dq_full, 0, status, abort_flag);
-    if (ok) {
-      tc_fence_after();
-      uint8_t* stage = smem + SM::kQ + warp * 32 * 128;
-#pragma unroll 1
-      for (int c = 0; c < DP / 32; ++c) {
-        uint32_t o[32];
-        if (blocks > 0) {
-          tmem_ld32(tmem + lanes + kDqColQ + 32 * c, o);
+        if (!mbar_wait_warp(&bars->dp_full, n & 1, status, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t g[32], x[16];
+          tmem_ld32(col_p + 32 * c, g);
           tmem_ld_wait();
-        } else {
+          if (c == 1) {
+            tc_fence_before();
+            mbar_arrive(&bars->dp_read);
+          }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0u;
+          for (int i = 0; i < 32; i += 2) {
+            const float2 d = mul2(e[16 * c + i / 2], sub2(make_float2(__uint_as_float(g[i]), __uint_as_float(g[i + 1])), make_float2(delta, delta)));
+            x[i / 2] = pack16x2<BF>(d.x, d.y);
+          }
+          tmem_st16(col_s + 16 * c, x);       // dS over columns of S this thread has read
         }
-        const uint32_t base = smem_u32(stage + (c / 2) * SM::kRowChunk);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&bars->ds_full[n & 1]);
+      }
+      if (!ok) break;
+      if (!live) {
+        // no keys at all: zeros
+        if (half == 0) {
+          float* stat = p.stat + (bh * p.stat_rows + row / 64 * 64) * 3 + row % 64;
+          stat[0] = lse;
+          stat[64] = ties;
+          stat[128] = 0.f;
+          if (valid) {
+            uint16_t* dst = p.dq + w.b * p.dq_stride[0] + row * p.dq_stride[1] + w.h * p.dq_stride[2];
+            for (int c = 0; c < p.s.dim; c += 8) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        w.open(p, w.unit + gridDim.x);
+        ask();
+        continue;
+      }
+      uint16_t* const dst0 = p.dq + w.b * p.dq_stride[0] + static_cast<int64_t>(w.row0 + quarter * 32) * p.dq_stride[1] +
+                             w.h * p.dq_stride[2] + half * (DP / 2);
+      const int rows = static_cast<int>(p.s.queries) - (w.row0 + quarter * 32);
+      w.open(p, w.unit + gridDim.x);
+      ask();
+      ok = mbar_wait_warp(&bars->dq_full, units & 1, status, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      // PIECES lanes with PIECES 16-byte pieces of a row each exchange them, so that a store instruction writes whole rows'
+      // halves: lane i then holds piece i % PIECES of the group's rows
+      constexpr int PIECES = DP / 16;
+      uint32_t x[PIECES][4];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          uint32_t w[4];
+      for (int c = 0; c < DP / 64; ++c) {
+        uint32_t a[32];
+        tmem_ld32(tmem + lanes + kDqColQ + half * (DP / 2) + 32 * c, a);
+        tmem_ld_wait();
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            w[i] = pack16x2<BF>(__uint_as_float(o[8 * g + 2 * i]) * p.s.scale, __uint_as_float(o[8 * g + 2 * i + 1]) * p.s.scale);
-          st_shared_v4(base + sw128_off(lane, (c & 1) * 4 + g), w[0], w[1], w[2], w[3]);
+            x[4 * c + g][i] = pack16x2<BF>(__uint_as_float(a[8 * g + 2 * i]) * p.s.scale, __uint_as_float(a[8 * g + 2 * i + 1]) * p.s.scale);
+      }
+      tc_fence_before();
+#pragma unroll
+      for (int d = 1; d < PIECES; d *= 2) {
+        const bool up = lane & d;
+#pragma unroll
+        for (int g = 0; g < PIECES; ++g) {
+          if (g & d) continue;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // the lower lane keeps its piece g and takes the upper's g; the upper lane keeps g + d and takes the lower's
+            const uint32_t give = up ? x[g][i] : x[g + d][i];
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, give, d);
+            if (up) x[g][i] = got;
+            else x[g + d][i] = got;
+          }
         }
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0 && row0 + warp * 32 < p.s.queries) {
-        for (int c = 0; c < SM::kChunks; ++c)
-          if (64 * c < p.s.dim) tma_store_4d(&tm_dq, stage + c * SM::kRowChunk, 64 * c, row0 + warp * 32, h, b);
-        bulk_commit_group();
-        bulk_wait_group_read0();
+      const int piece = lane % PIECES, row8 = lane / PIECES * PIECES;
+      if (half * (DP / 2) + 8 * piece < p.s.dim) {
+#pragma unroll
+        for (int g = 0; g < PIECES; ++g)
+          if (row8 + g < rows)
+            *reinterpret_cast<uint4*>(dst0 + (row8 + g) * p.dq_stride[1] + 8 * piece) = make_uint4(x[g][0], x[g][1], x[g][2], x[g][3]);
       }
-      __syncwarp();
+      ++units;
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) tmem_dealloc(tmem, kDqCols);
+  if (warp == 9) tmem_dealloc(tmem, kDqCols);
 }
 
 // ------------------------------------------------------------------------------------------------ dK, dV
@@ -757,22 +915,28 @@ int launch_bwd(const HtrcCrossArgs* a, cudaStream_t st) {
   const int hk = keys ? a->kv_heads : a->heads, hq = rows ? a->heads : a->kv_heads;
   int do_b = 0, do_h = 0, one;
   if (rows) {
-    CUtensorMap mq, mo, mk, mv, mdq;
+    CUtensorMap mq, mo, mk, mv;
     DqParams p{};
     p.s = s;
     if (!cross_map(&mq, a, q, qs, nq, hq, kDqRows, &p.s.q_b, &p.s.q_h) || !cross_map(&mo, a, o, os, nq, hq, kDqRows, &do_b, &do_h) ||
-        !cross_map(&mk, a, k, ks, nk, hk, kDqKeys, &p.s.k_b, &p.s.k_h) || !cross_map(&mv, a, v, vs, nk, hk, kDqKeys, &p.s.v_b, &p.s.v_h) ||
-        !cross_map(&mdq, a, a->dq, a->dq_stride, nq, hq, 32, &one, &one))
+        !cross_map(&mk, a, k, ks, nk, hk, kDqKeys, &p.s.k_b, &p.s.k_h) || !cross_map(&mv, a, v, vs, nk, hk, kDqKeys, &p.s.v_b, &p.s.v_h))
       return HTRC_ERR_CUDA;
     p.lse = a->lse;
     p.dlse = a->dlse;
     p.out = static_cast<const uint16_t*>(a->out);
-    for (int i = 0; i < 3; ++i) p.out_stride[i] = a->out_stride[i];
+    p.dq = static_cast<uint16_t*>(a->dq);
+    for (int i = 0; i < 3; ++i) {
+      p.out_stride[i] = a->out_stride[i];
+      p.dq_stride[i] = a->dq_stride[i];
+    }
     p.stat = stat;
     p.stat_rows = stat_rows(a);
-    p.tiles = static_cast<int>(stat_rows(a) / kDqRows);
+    p.tiles = static_cast<uint32_t>(stat_rows(a) / kDqRows);
+    p.units = static_cast<uint32_t>(p.tiles * a->batch * a->heads);
+    p.do_b = do_b;
+    p.do_h = do_h;
     p.status = a->status;
-    kq<<<static_cast<unsigned>(p.tiles * a->batch * a->heads), kDqThreads, DqSmem<DP>::kBytes, st>>>(mq, mo, mk, mv, mdq, p, do_b, do_h);
+    kq<<<std::min<uint32_t>(p.units, static_cast<uint32_t>(sm_count())), kDqThreads, DqSmem<DP>::kBytes, st>>>(mq, mo, mk, mv, p);
     if (cudaGetLastError() != cudaSuccess) return HTRC_ERR_CUDA;
   }
   if (!keys) return HTRC_OK;

@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kXThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
-  Walk w;
+  Walk w{};
 
   if (warp == 8) {
     // ------------------------------------------------------------------ TMA

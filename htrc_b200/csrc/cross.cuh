@@ -29,6 +29,31 @@ __device__ __forceinline__ float mask_term(const void* p, int dtype, int64_t i) 
   return __half2float(static_cast<const __half*>(p)[i]);
 }
 
+// N terms from element offset `at` on, `step` apart; those from n on are excluded.  The type is looked at once, so that
+// the loads are in flight together.
+template <int N>
+__device__ __forceinline__ void mask_terms(const void* p, int dtype, int64_t at, int64_t step, int n, float (&t)[N]) {
+  if (dtype == HTRC_LAYER_U8) {
+    const uint8_t* x = static_cast<const uint8_t*>(p) + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = i < n ? static_cast<float>(__ldg(x + i * step)) : 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = t[i] != 0.f ? 0.f : -INFINITY;
+  } else if (dtype == HTRC_LAYER_F32) {
+    const float* x = static_cast<const float*>(p) + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = i < n ? __ldg(x + i * step) : -INFINITY;
+  } else if (dtype == HTRC_LAYER_BF16) {
+    const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(p) + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = i < n ? __bfloat162float(x[i * step]) : -INFINITY;
+  } else {
+    const __half* x = static_cast<const __half*>(p) + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = i < n ? __half2float(x[i * step]) : -INFINITY;
+  }
+}
+
 struct CrossShape {
   int64_t batch, queries, keys;
   int heads, kv_heads, group, dim;

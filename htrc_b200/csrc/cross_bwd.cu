@@ -305,25 +305,25 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           named_bar_sync(1 + half, 128);
         }
         if (KIND == CROSS_PAIRS) {
-          // the warp's 32 rows of mask bits: a row's 64 keys by coalesced loads, eight rows in flight, and ballots
+          // the warp's 32 rows of mask bits: a row's 64 keys by coalesced loads, sixteen rows in flight, and ballots
           const int rows = min(32, static_cast<int>(p.s.queries) - (w.row0 + quarter * 32));
           const uint8_t* mk = static_cast<const uint8_t*>(p.s.mask.p) + mask_at +
                               static_cast<int64_t>(w.row0 + quarter * 32) * p.s.mask.sn + static_cast<int64_t>(first + lane) * p.s.mask.sm;
-          for (int g = 0; g < rows; g += 8) {
-            uint8_t v[8][2];
+          for (int g = 0; g < rows; g += 16) {
+            uint8_t v[16][2];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 16; ++i)
 #pragma unroll
               for (int q = 0; q < 2; ++q)
                 v[i][q] = g + i < rows && 32 * q + lane < left ? __ldg(mk + i * p.s.mask.sn + 32 * q * p.s.mask.sm) : 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 16; ++i)
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
                 const uint32_t word = __ballot_sync(0xffffffffu, v[i][q] != 0);
                 if (lane == g + i) bits[q] = word;
               }
-            mk += 8 * p.s.mask.sn;
+            mk += 16 * p.s.mask.sn;
           }
         }
         // this half's columns of out, asked for before the unit's first weights are formed
@@ -356,16 +356,17 @@ __global__ void __launch_bounds__(kDqThreads, 1)
             for (int i = 0; i < 32; ++i)
               if (!(bits[c] >> i & 1u)) s[i] = __float_as_uint(-INFINITY);
           } else {
+            float t[32];
+            if (KIND == CROSS_KEYS) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              float t;
-              if (KIND == CROSS_KEYS)
-                t = bj[32 * c + i];
-              else
-                t = 32 * c + i < left ? mask_term(p.s.mask.p, p.s.mask.dtype, row_mask + static_cast<int64_t>(first + 32 * c + i) * p.s.mask.sm)
-                                      : -INFINITY;
-              s[i] = __float_as_uint(t == -INFINITY ? t : fmaf(__uint_as_float(s[i]), p.s.scale, t));
+              for (int i = 0; i < 32; ++i) t[i] = bj[32 * c + i];
+            } else {
+              mask_terms<32>(p.s.mask.p, p.s.mask.dtype, row_mask + static_cast<int64_t>(first + 32 * c) * p.s.mask.sm, p.s.mask.sm,
+                             left - 32 * c, t);
             }
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              s[i] = __float_as_uint(t[i] == -INFINITY ? t[i] : fmaf(__uint_as_float(s[i]), p.s.scale, t[i]));
           }
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
@@ -691,18 +692,35 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
         head = hg;
         if (in) kbias = mask_term(p.s.mask.p, p.s.mask.dtype, mask_at);
       }
+      // queries this key is excluded from, with a mask per query (of a bias: found with its terms)
+      uint32_t out[2] = {0u, 0u};
+      if (KIND == CROSS_PAIRS) {
+        const uint8_t* mk = static_cast<const uint8_t*>(p.s.mask.p) + mask_at + row * p.s.mask.sn;
+        const int n = in ? static_cast<int>(p.s.queries) - row : 0;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint8_t v[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] = 32 * c + k < n ? __ldg(mk + (32 * c + k) * p.s.mask.sn) : 0;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) out[c] |= static_cast<uint32_t>(v[k] == 0) << k;
+        }
+      }
       if (!mbar_wait_warp(&bars->s_full[wg], (i >> 1) & 1, status, abort_flag)) { ok = false; break; }
       tc_fence_after();
       // the queries' statistics: [lse][ties][delta], 64 each
       const float* st = reinterpret_cast<const float*>(smem + SM::kRing + s * SM::kStage + 2 * SM::kRows);
       const uint32_t buf = tmem + lanes + kDkvColS + wg * kDkvBuf;
       float2 w[32];                         // P, kept for dS
-      uint32_t out = 0u, out_hi = 0u;       // queries this key is excluded from (with a mask per query)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t x[32], pw[16];
         tmem_ld32(buf + 32 * c, x);
         tmem_ld_wait();
+        float terms[32];
+        if (KIND == CROSS_BIAS)
+          mask_terms<32>(p.s.mask.p, p.s.mask.dtype, mask_at + (row + 32 * c) * p.s.mask.sn, p.s.mask.sn,
+                         in ? static_cast<int>(p.s.queries) - row - 32 * c : 0, terms);
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
           const float4 ls = *reinterpret_cast<const float4*>(st + 32 * c + k);
@@ -710,21 +728,20 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
 #pragma unroll
           for (int h2 = 0; h2 < 2; ++h2) {
             const float l0 = h2 ? ls.z : ls.x, l1 = h2 ? ls.w : ls.y;
-            const int kk = k + 2 * h2, q = row + 32 * c + kk;
+            const int kk = k + 2 * h2;
             float2 e = make_float2(__uint_as_float(x[kk]), __uint_as_float(x[kk + 1]));
             if (!NAT) {
               float2 off = make_float2(kbias - l0, kbias - l1);
               if (KIND == CROSS_PAIRS) {
-                const uint8_t* mk = static_cast<const uint8_t*>(p.s.mask.p) + mask_at;
-                if (!(in && q < p.s.queries && __ldg(mk + q * p.s.mask.sn) != 0)) off.x = -INFINITY;
-                if (!(in && q + 1 < p.s.queries && __ldg(mk + (q + 1) * p.s.mask.sn) != 0)) off.y = -INFINITY;
+                if (out[c] >> kk & 1u) off.x = -INFINITY;
+                if (out[c] >> kk & 2u) off.y = -INFINITY;
               }
               e = fma2(e, make_float2(scale, scale), off);
             } else {
               float b0 = kbias, b1 = kbias;
               if (KIND == CROSS_BIAS) {
-                b0 = in && q < p.s.queries ? mask_term(p.s.mask.p, p.s.mask.dtype, mask_at + q * p.s.mask.sn) : -INFINITY;
-                b1 = in && q + 1 < p.s.queries ? mask_term(p.s.mask.p, p.s.mask.dtype, mask_at + (q + 1) * p.s.mask.sn) : -INFINITY;
+                b0 = terms[kk];
+                b1 = terms[kk + 1];
               }
               e = fma2(e, make_float2(scale, scale), make_float2(b0, b1));
               e = fma2(sub2(e, make_float2(l0, l1)), make_float2(kCrossLog2e, kCrossLog2e),
@@ -732,11 +749,11 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
               // an excluded key's weight and gradient are zero whatever its row holds
               if (b0 == -INFINITY) {
                 e.x = -INFINITY;
-                (c ? out_hi : out) |= 1u << kk;
+                out[c] |= 1u << kk;
               }
               if (b1 == -INFINITY) {
                 e.y = -INFINITY;
-                (c ? out_hi : out) |= 2u << kk;
+                out[c] |= 2u << kk;
               }
             }
             e = make_float2(cross_ex2(e.x), cross_ex2(e.y));
@@ -764,8 +781,8 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
             const int kk = k + 2 * h2;
             float2 g = make_float2(__uint_as_float(y[kk]), __uint_as_float(y[kk + 1]));
             if (NAT) {
-              if ((c ? out_hi : out) >> kk & 1u) g.x = 0.f;
-              if ((c ? out_hi : out) >> kk & 2u) g.y = 0.f;
+              if (out[c] >> kk & 1u) g.x = 0.f;
+              if (out[c] >> kk & 2u) g.y = 0.f;
             }
             const float2 d = mul2(w[16 * c + kk / 2], sub2(g, h2 ? make_float2(de.z, de.w) : make_float2(de.x, de.y)));
             dw[kk / 2] = pack16x2<BF>(d.x, d.y);

@@ -371,17 +371,23 @@ __global__ void __launch_bounds__(kXThreads, 1)
 #pragma unroll
           for (int i = 0; i < kXKeys; ++i)
             if (!(bits[i / 32] >> (i % 32) & 1u)) s[i / 32][i % 32] = __float_as_uint(-INFINITY);
+        } else if (KIND == CROSS_KEYS) {
+#pragma unroll
+          for (int i = 0; i < kXKeys; ++i) {
+            uint32_t& x = s[i / 32][i % 32];
+            x = __float_as_uint(bj[i] == -INFINITY ? bj[i] : fmaf(__uint_as_float(x), p.s.scale, bj[i]));
+          }
         } else {
           const int64_t row_at = mask_at + (valid ? row : 0) * p.s.mask.sn + static_cast<int64_t>(j * kXKeys) * p.s.mask.sm;
 #pragma unroll
-          for (int i = 0; i < kXKeys; ++i) {
-            float b;
-            if (KIND == CROSS_KEYS)
-              b = bj[i];
-            else
-              b = i < left ? mask_term(p.s.mask.p, p.s.mask.dtype, row_at + static_cast<int64_t>(i) * p.s.mask.sm) : -INFINITY;
-            uint32_t& x = s[i / 32][i % 32];
-            x = __float_as_uint(b == -INFINITY ? b : fmaf(__uint_as_float(x), p.s.scale, b));
+          for (int c = 0; c < 8; ++c) {
+            float b[16];
+            mask_terms<16>(p.s.mask.p, p.s.mask.dtype, row_at + static_cast<int64_t>(16 * c) * p.s.mask.sm, p.s.mask.sm, left - 16 * c, b);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              uint32_t& x = s[c / 2][16 * (c & 1) + i];
+              x = __float_as_uint(b[i] == -INFINITY ? b[i] : fmaf(__uint_as_float(x), p.s.scale, b[i]));
+            }
           }
         }
         float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};

@@ -101,6 +101,36 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void*
                : "memory");
 }
 
+// Groups of P lanes hold P 16-byte pieces of a row each; they exchange them so that lane i holds piece i % P of the
+// group's rows, and a store instruction then writes P * 16 contiguous bytes of a few rows instead of 16 of 32 rows (which
+// takes a pass of the store path per row).
+template <int P>
+__device__ __forceinline__ void exchange_pieces(uint32_t (&x)[P][4], int lane) {
+#pragma unroll
+  for (int d = 1; d < P; d *= 2) {
+    const bool up = lane & d;
+#pragma unroll
+    for (int g = 0; g < P; ++g) {
+      if (g & d) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // the lower lane keeps its piece g and takes the upper's g; the upper lane keeps g + d and takes the lower's
+        const uint32_t give = up ? x[g][i] : x[g + d][i];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, give, d);
+        if (up) x[g][i] = got;
+        else x[g + d][i] = got;
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
+__host__ __device__ constexpr int mask_bytes(int dtype) { return dtype == HTRC_LAYER_U8 ? 1 : dtype == HTRC_LAYER_F32 ? 4 : 2; }
+// a mask's terms at element offset i and what shares their line
+__device__ __forceinline__ void prefetch_mask(const CrossMaskView& m, int64_t i) {
+  prefetch_l1(static_cast<const uint8_t*>(m.p) + i * mask_bytes(m.dtype));
+}
+
 // A descriptor's constant words: K-major operand (LBO unused) and MN-major operand with 64-element chunks lbo apart
 __device__ __forceinline__ uint64_t desc_k(uint32_t smem) { return sw128_desc(smem, 16, 1024); }
 __device__ __forceinline__ uint64_t desc_mn(uint32_t smem, uint32_t lbo) { return sw128_desc(smem, lbo, 1024); }

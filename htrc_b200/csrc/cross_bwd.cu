@@ -28,6 +28,17 @@ namespace htrc {
 
 namespace {
 
+// With a bool mask per query the first pass leaves its ballots for the second: word w of a row holds keys 32 w .. (set:
+// kept), laid out [entry][head (one where the mask has none)][word][padded row], words padded to the second pass's blocks
+struct CrossBits {
+  uint32_t* p;
+  int words;
+  bool heads;
+  __device__ __forceinline__ int64_t at(const CrossShape& s, int64_t rows, int b, int h, int word) const {
+    return ((static_cast<int64_t>(b) * (heads ? s.heads : 1) + (heads ? h : 0)) * words + word) * rows;
+  }
+};
+
 constexpr float kHuge = 1e30f;        // a |log sum| above this is a mask's lowest value: the logits are lost in it
 
 // ------------------------------------------------------------------------------------------------ dQ
@@ -61,6 +72,7 @@ struct DqParams {
   int64_t dq_stride[3];
   float* stat;              // [batch * heads][padded rows / 64][3][64]: lse in the pass's units, log2 of tied keys, delta
   int64_t stat_rows;
+  CrossBits bits;
   uint32_t units, tiles;    // tiles of 128 rows per head
   int do_b, do_h;
   int* status;
@@ -304,6 +316,8 @@ __global__ void __launch_bounds__(kDqThreads, 1)
             bj[r] = r < left ? mask_term(p.s.mask.p, p.s.mask.dtype, mask_at + static_cast<int64_t>(first + r) * p.s.mask.sm) : -INFINITY;
           named_bar_sync(1 + half, 128);
         }
+        if ((KIND == CROSS_PAIRS || KIND == CROSS_BIAS) && valid && left > kDqKeys)     // the next block's terms of this row
+          prefetch_mask(p.s.mask, row_mask + static_cast<int64_t>(first + kDqKeys) * p.s.mask.sm);
         if (KIND == CROSS_PAIRS) {
           // the warp's 32 rows of mask bits: a row's 64 keys by coalesced loads, sixteen rows in flight, and ballots
           const int rows = min(32, static_cast<int>(p.s.queries) - (w.row0 + quarter * 32));
@@ -324,6 +338,10 @@ __global__ void __launch_bounds__(kDqThreads, 1)
                 if (lane == g + i) bits[q] = word;
               }
             mk += 16 * p.s.mask.sn;
+          }
+          if (p.bits.heads || w.h == 0) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) p.bits.p[p.bits.at(p.s, p.stat_rows, w.b, w.h, first / 32 + q) + row] = bits[q];
           }
         }
         // this half's columns of out, asked for before the unit's first weights are formed
@@ -453,8 +471,6 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       ok = mbar_wait_warp(&bars->dq_full, units & 1, status, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      // PIECES lanes with PIECES 16-byte pieces of a row each exchange them, so that a store instruction writes whole rows'
-      // halves: lane i then holds piece i % PIECES of the group's rows
       constexpr int PIECES = DP / 16;
       uint32_t x[PIECES][4];
 #pragma unroll
@@ -469,22 +485,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
             x[4 * c + g][i] = pack16x2<BF>(__uint_as_float(a[8 * g + 2 * i]) * p.s.scale, __uint_as_float(a[8 * g + 2 * i + 1]) * p.s.scale);
       }
       tc_fence_before();
-#pragma unroll
-      for (int d = 1; d < PIECES; d *= 2) {
-        const bool up = lane & d;
-#pragma unroll
-        for (int g = 0; g < PIECES; ++g) {
-          if (g & d) continue;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            // the lower lane keeps its piece g and takes the upper's g; the upper lane keeps g + d and takes the lower's
-            const uint32_t give = up ? x[g][i] : x[g + d][i];
-            const uint32_t got = __shfl_xor_sync(0xffffffffu, give, d);
-            if (up) x[g][i] = got;
-            else x[g + d][i] = got;
-          }
-        }
-      }
+      exchange_pieces<PIECES>(x, lane);
       const int piece = lane % PIECES, row8 = lane / PIECES * PIECES;
       if (half * (DP / 2) + 8 * piece < p.s.dim) {
 #pragma unroll
@@ -518,7 +519,7 @@ struct DkvSmem {
   static constexpr uint32_t kKeyChunk = 128 * 128, kRowChunk = 64 * 128;
   static constexpr uint32_t kTile = kChunks * kKeyChunk, kRows = kChunks * kRowChunk;
   static constexpr uint32_t kK = 0, kV = kTile, kRing = 2 * kTile, kStat = kDkvRows * 3 * 4,
-                            kStage = 2 * kRows + 1024;
+                            kBits = 2 * kRows + 1024, kStage = kBits + 1024;      // rows, statistics, 4 words of bits per row
   static constexpr uint32_t kBars = kRing + kDkvStages * kStage;
   static constexpr uint32_t kUsed = kBars + 256 + 1024;
   // one CTA per SM: it takes all 512 TMEM columns
@@ -529,6 +530,7 @@ struct DkvParams {
   CrossShape s;
   const float* stat;
   int64_t stat_rows;
+  CrossBits bits;
   int key_blocks, splits, row_blocks;
   float* partial;           // splits > 1: [2 (dk, dv)][split][batch * kv_heads][keys][DP]
   int* status;
@@ -598,13 +600,17 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
         const int64_t at = first + i;
         const int h = hk * p.s.group + static_cast<int>(at / p.row_blocks), row = static_cast<int>(at % p.row_blocks) * kDkvRows;
         uint8_t* st = smem + SM::kRing + s * SM::kStage;
-        mbar_arrive_expect_tx(&bars->full[s], 2 * SM::kRows + SM::kStat);
+        mbar_arrive_expect_tx(&bars->full[s], 2 * SM::kRows + SM::kStat + (KIND == CROSS_PAIRS ? 4 * kDkvRows * 4 : 0));
         for (int c = 0; c < SM::kChunks; ++c) {
           tma_load_4d(st + c * SM::kRowChunk, &tm_q, &bars->full[s], 64 * c, row, h * p.s.q_h, b * p.s.q_b, pol);
           tma_load_4d(st + SM::kRows + c * SM::kRowChunk, &tm_do, &bars->full[s], 64 * c, row, h * do_h, b * do_b, pol);
         }
         bulk_load(st + 2 * SM::kRows, p.stat + ((static_cast<int64_t>(b) * p.s.heads + h) * p.stat_rows + row) * 3, SM::kStat,
                   &bars->full[s], pol);
+        if (KIND == CROSS_PAIRS)
+          for (int q = 0; q < 4; ++q)
+            bulk_load(st + SM::kBits + q * kDkvRows * 4, p.bits.p + p.bits.at(p.s, p.stat_rows, b, h, key0 / 32 + q) + row,
+                      kDkvRows * 4, &bars->full[s], pol);
       }
       __syncwarp();
     }
@@ -692,25 +698,23 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
         head = hg;
         if (in) kbias = mask_term(p.s.mask.p, p.s.mask.dtype, mask_at);
       }
-      // queries this key is excluded from, with a mask per query (of a bias: found with its terms)
-      uint32_t out[2] = {0u, 0u};
-      if (KIND == CROSS_PAIRS) {
-        const uint8_t* mk = static_cast<const uint8_t*>(p.s.mask.p) + mask_at + row * p.s.mask.sn;
-        const int n = in ? static_cast<int>(p.s.queries) - row : 0;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint8_t v[32];
-#pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = 32 * c + k < n ? __ldg(mk + (32 * c + k) * p.s.mask.sn) : 0;
-#pragma unroll
-          for (int k = 0; k < 32; ++k) out[c] |= static_cast<uint32_t>(v[k] == 0) << k;
+      if (KIND == CROSS_BIAS) {
+        // the terms of this warp's keys that its next step reads (lane: query)
+        const int64_t then = at + 2;
+        if (i + 2 < steps && key0 + quarter * 32 < count) {
+          const int row2 = static_cast<int>(then % p.row_blocks) * kDkvRows + lane, h2 = hk * p.s.group + static_cast<int>(then / p.row_blocks);
+          const int64_t m0 = b * p.s.mask.sb + h2 * p.s.mask.sh + static_cast<int64_t>(key0 + quarter * 32) * p.s.mask.sm;
+          if (row2 < p.s.queries) prefetch_mask(p.s.mask, m0 + row2 * p.s.mask.sn);
+          if (row2 + 32 < p.s.queries) prefetch_mask(p.s.mask, m0 + (row2 + 32) * p.s.mask.sn);
         }
       }
+      uint32_t out[2] = {0u, 0u};           // queries this key is excluded from (of a bias: found with its terms)
       if (!mbar_wait_warp(&bars->s_full[wg], (i >> 1) & 1, status, abort_flag)) { ok = false; break; }
       tc_fence_after();
       // the queries' statistics: [lse][ties][delta], 64 each
       const float* st = reinterpret_cast<const float*>(smem + SM::kRing + s * SM::kStage + 2 * SM::kRows);
       const uint32_t buf = tmem + lanes + kDkvColS + wg * kDkvBuf;
+      const uint4* words = reinterpret_cast<const uint4*>(smem + SM::kRing + s * SM::kStage + SM::kBits + quarter * kDkvRows * 4);
       float2 w[32];                         // P, kept for dS
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -718,6 +722,14 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
         tmem_ld32(buf + 32 * c, x);
         tmem_ld_wait();
         float terms[32];
+        if (KIND == CROSS_PAIRS) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint4 x4 = words[8 * c + k];
+            out[c] |= (~x4.x >> lane & 1u) << (4 * k) | (~x4.y >> lane & 1u) << (4 * k + 1) | (~x4.z >> lane & 1u) << (4 * k + 2) |
+                      (~x4.w >> lane & 1u) << (4 * k + 3);
+          }
+        }
         if (KIND == CROSS_BIAS)
           mask_terms<32>(p.s.mask.p, p.s.mask.dtype, mask_at + (row + 32 * c) * p.s.mask.sn, p.s.mask.sn,
                          in ? static_cast<int>(p.s.queries) - row - 32 * c : 0, terms);
@@ -803,8 +815,10 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       const float mul = wg == 0 ? 1.0f : p.s.scale;
       uint8_t* stage = smem + (wg == 0 ? SM::kV : SM::kK) + quarter * 32 * 128;
       const int64_t parts = static_cast<int64_t>(p.splits) * p.s.batch * p.s.kv_heads;
-      float* dst = p.splits > 1 ? p.partial + (((wg == 0 ? parts : 0) + (static_cast<int64_t>(split) * p.s.batch * p.s.kv_heads + bk)) *
-                                               p.s.keys + key) * DP : nullptr;
+      // splits > 1: this warp's 32 keys' rows
+      float* dst = p.partial + (((wg == 0 ? parts : 0) + (static_cast<int64_t>(split) * p.s.batch * p.s.kv_heads + bk)) * p.s.keys +
+                                key0 + quarter * 32) * DP;
+      const int rows = static_cast<int>(p.s.keys) - (key0 + quarter * 32);
 #pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
         uint32_t o[32];
@@ -816,13 +830,14 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
           for (int k = 0; k < 32; ++k) o[k] = 0u;
         }
         if (p.splits > 1) {
-          if (key < p.s.keys) {
+          uint32_t x[8][4];
 #pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              *reinterpret_cast<float4*>(dst + 32 * c + k) =
-                  make_float4(__uint_as_float(o[k]) * mul, __uint_as_float(o[k + 1]) * mul, __uint_as_float(o[k + 2]) * mul,
-                              __uint_as_float(o[k + 3]) * mul);
-          }
+          for (int k = 0; k < 32; ++k) x[k / 4][k % 4] = __float_as_uint(__uint_as_float(o[k]) * mul);
+          exchange_pieces<8>(x, lane);
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            if ((lane & ~7) + g < rows)
+              *reinterpret_cast<uint4*>(dst + ((lane & ~7) + g) * DP + 32 * c + 4 * (lane & 7)) = make_uint4(x[g][0], x[g][1], x[g][2], x[g][3]);
         } else {
           const uint32_t base = smem_u32(stage + (c / 2) * SM::kKeyChunk);
 #pragma unroll
@@ -905,6 +920,14 @@ int dkv_splits(const HtrcCrossArgs* a) {
 int64_t stat_rows(const HtrcCrossArgs* a) { return (a->queries + kDqRows - 1) / kDqRows * kDqRows; }
 size_t stat_bytes(const HtrcCrossArgs* a) { return (static_cast<size_t>(a->batch * a->heads * stat_rows(a)) * 12 + 255) / 256 * 256; }
 
+// words of a row's bits: whole blocks of either pass
+int bit_words(const HtrcCrossArgs* a) { return static_cast<int>((a->keys + 127) / 128 * 4); }
+size_t bits_bytes(const HtrcCrossArgs* a) {
+  if (cross_mask_kind(a) != CROSS_PAIRS) return 0;
+  const int64_t heads = a->mask_stride[1] != 0 ? a->heads : 1;
+  return (static_cast<size_t>(a->batch) * heads * bit_words(a) * stat_rows(a) * 4 + 255) / 256 * 256;
+}
+
 template <typename K>
 bool ready(K kernel, uint32_t bytes, bool (&done)[64]) {
   int dev = 0;
@@ -923,6 +946,7 @@ int launch_bwd(const HtrcCrossArgs* a, cudaStream_t st) {
   if (!ready(kq, DqSmem<DP>::kBytes, done_q) || !ready(kkv, DkvSmem<DP>::kBytes, done_kv)) return HTRC_ERR_CUDA;
   const CrossShape s = cross_shape(a);
   float* stat = static_cast<float*>(a->workspace);
+  const CrossBits bits{reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a->workspace) + stat_bytes(a)), bit_words(a), a->mask_stride[1] != 0};
   const bool keys = a->keys > 0, rows = a->queries > 0;
   // an empty side's maps are never read: the other side's rows stand in
   const void *k = keys ? a->k : a->q, *v = keys ? a->v : a->q, *q = rows ? a->q : a->k, *o = rows ? a->dout : a->k;
@@ -948,6 +972,7 @@ int launch_bwd(const HtrcCrossArgs* a, cudaStream_t st) {
     }
     p.stat = stat;
     p.stat_rows = stat_rows(a);
+    p.bits = bits;
     p.tiles = static_cast<uint32_t>(stat_rows(a) / kDqRows);
     p.units = static_cast<uint32_t>(p.tiles * a->batch * a->heads);
     p.do_b = do_b;
@@ -966,10 +991,11 @@ int launch_bwd(const HtrcCrossArgs* a, cudaStream_t st) {
     return HTRC_ERR_CUDA;
   p.stat = stat;
   p.stat_rows = stat_rows(a);
+  p.bits = bits;
   p.key_blocks = static_cast<int>((a->keys + kDkvKeys - 1) / kDkvKeys);
   p.row_blocks = static_cast<int>((a->queries + kDkvRows - 1) / kDkvRows);
   p.splits = dkv_splits(a);
-  p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + stat_bytes(a));
+  p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + stat_bytes(a) + bits_bytes(a));
   p.status = a->status;
   const int64_t grid = a->batch * a->kv_heads * p.splits * p.key_blocks;
   kkv<<<static_cast<unsigned>(grid), kDkvThreads, DkvSmem<DP>::kBytes, st>>>(mq, mo, mk, mv, mdk, mdv, p, do_b, do_h);
@@ -1014,7 +1040,7 @@ int cross_sizes(const HtrcCrossArgs* a, size_t* bytes) {
   if (tiles * a->batch * a->heads > limit || blocks > limit / (16 * std::max<int64_t>(1, a->batch * a->kv_heads)))
     return HTRC_ERR_UNSUPPORTED;
   const int dp = a->dim <= 64 ? 64 : 128, splits = dkv_splits(a);
-  *bytes = stat_bytes(a) + (splits > 1 ? static_cast<size_t>(2) * splits * a->batch * a->kv_heads * a->keys * dp * 4 : 0);
+  *bytes = stat_bytes(a) + bits_bytes(a) + (splits > 1 ? static_cast<size_t>(2) * splits * a->batch * a->kv_heads * a->keys * dp * 4 : 0);
   return HTRC_OK;
 }
 

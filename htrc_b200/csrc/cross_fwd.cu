@@ -325,6 +325,8 @@ __global__ void __launch_bounds__(kXThreads, 1)
                                        mask_at + static_cast<int64_t>(j * kXKeys + r) * p.s.mask.sm) : -INFINITY;
           named_bar_sync(1 + t, 128);
         }
+        if ((KIND == CROSS_PAIRS || KIND == CROSS_BIAS) && valid && left > kXKeys)      // the next block's terms of this row
+          prefetch_mask(p.s.mask, mask_at + row * p.s.mask.sn + static_cast<int64_t>((j + 1) * kXKeys) * p.s.mask.sm);
         if (KIND == CROSS_PAIRS) {
           // the warp's 32 rows of mask bits: a row's 128 keys by coalesced loads, eight rows in flight, and ballots
           const int rows = min(32, static_cast<int>(p.s.queries) - (row0 + quarter * 32));

@@ -70,7 +70,7 @@ struct DqParams {
   int64_t out_stride[3];
   uint16_t* dq;
   int64_t dq_stride[3];
-  float* stat;              // [batch * heads][padded rows / 64][3][64]: lse in the pass's units, log2 of tied keys, delta
+  float* stat;              // [batch * heads][padded rows / 64][3][64]: minus lse in the pass's units, log2 of tied keys, delta
   int64_t stat_rows;
   CrossBits bits;
   uint32_t units, tiles;    // tiles of 128 rows per head
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           if (lse == INFINITY) delta = 0.f;
           if (half == 0) {
             float* stat = p.stat + (bh * p.stat_rows + row / 64 * 64) * 3 + row % 64;
-            stat[0] = lse;
+            stat[0] = -lse;
             stat[64] = ties;
             stat[128] = delta;
           }
@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
         // no keys at all: zeros
         if (half == 0) {
           float* stat = p.stat + (bh * p.stat_rows + row / 64 * 64) * 3 + row % 64;
-          stat[0] = lse;
+          stat[0] = -lse;
           stat[64] = ties;
           stat[128] = 0.f;
           if (valid) {
@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
     const float scale = NAT ? p.s.scale : p.s.scale * kCrossLog2e;
     const bool in = key < count;
     int head = -1;
-    float kbias = in ? 0.f : -INFINITY;           // this key's term: -inf where it is excluded
+    float kbias = in ? 0.f : -INFINITY;           // with a bias: this key's term, -inf where it is excluded
     bool ok = true;
     for (int i = wg; i < steps; i += 2) {
       const int s = i % kDkvStages;
@@ -711,7 +711,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       uint32_t out[2] = {0u, 0u};           // queries this key is excluded from (of a bias: found with its terms)
       if (!mbar_wait_warp(&bars->s_full[wg], (i >> 1) & 1, status, abort_flag)) { ok = false; break; }
       tc_fence_after();
-      // the queries' statistics: [lse][ties][delta], 64 each
+      // the queries' statistics: [-lse][ties][delta], 64 each
       const float* st = reinterpret_cast<const float*>(smem + SM::kRing + s * SM::kStage + 2 * SM::kRows);
       const uint32_t buf = tmem + lanes + kDkvColS + wg * kDkvBuf;
       const uint4* words = reinterpret_cast<const uint4*>(smem + SM::kRing + s * SM::kStage + SM::kBits + quarter * kDkvRows * 4);
@@ -743,7 +743,8 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
             const int kk = k + 2 * h2;
             float2 e = make_float2(__uint_as_float(x[kk]), __uint_as_float(x[kk + 1]));
             if (!NAT) {
-              float2 off = make_float2(kbias - l0, kbias - l1);
+              // (a key past the entry's count: zero rows here, its gradients are not taken in the end)
+              float2 off = make_float2(l0, l1);
               if (KIND == CROSS_PAIRS) {
                 if (out[c] >> kk & 1u) off.x = -INFINITY;
                 if (out[c] >> kk & 2u) off.y = -INFINITY;
@@ -756,7 +757,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
                 b1 = terms[kk + 1];
               }
               e = fma2(e, make_float2(scale, scale), make_float2(b0, b1));
-              e = fma2(sub2(e, make_float2(l0, l1)), make_float2(kCrossLog2e, kCrossLog2e),
+              e = fma2(add2(e, make_float2(l0, l1)), make_float2(kCrossLog2e, kCrossLog2e),
                        h2 ? make_float2(-ti.z, -ti.w) : make_float2(-ti.x, -ti.y));
               // an excluded key's weight and gradient are zero whatever its row holds
               if (b0 == -INFINITY) {
@@ -832,7 +833,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
         if (p.splits > 1) {
           uint32_t x[8][4];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) x[k / 4][k % 4] = __float_as_uint(__uint_as_float(o[k]) * mul);
+          for (int k = 0; k < 32; ++k) x[k / 4][k % 4] = in ? __float_as_uint(__uint_as_float(o[k]) * mul) : 0u;
           exchange_pieces<8>(x, lane);
 #pragma unroll
           for (int g = 0; g < 8; ++g)
@@ -845,7 +846,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              w[k] = pack16x2<BF>(__uint_as_float(o[8 * g + 2 * k]) * mul, __uint_as_float(o[8 * g + 2 * k + 1]) * mul);
+              w[k] = in ? pack16x2<BF>(__uint_as_float(o[8 * g + 2 * k]) * mul, __uint_as_float(o[8 * g + 2 * k + 1]) * mul) : 0u;
             st_shared_v4(base + sw128_off(lane, (c & 1) * 4 + g), w[0], w[1], w[2], w[3]);
           }
         }

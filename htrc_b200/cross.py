@@ -16,6 +16,7 @@ The functions take part in autograd; the backward can also be called by itself. 
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -27,6 +28,7 @@ _DTYPES = {torch.bfloat16: _lib.LAYER_BF16, torch.float16: _lib.LAYER_F16}
 _MASKS = {torch.bool: _lib.LAYER_U8, torch.float32: _lib.LAYER_F32, torch.bfloat16: _lib.LAYER_BF16,
           torch.float16: _lib.LAYER_F16}
 _LENGTHS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+_NO_BACK = (0,) * 19
 _status = {}
 
 
@@ -126,7 +128,7 @@ class _Call:
         self.shape_args = (batch, queries, keys, heads, kv_heads, dim, _DTYPES[q.dtype], scale,
                            0 if key_lengths is None else key_lengths.data_ptr())
 
-    def pack(self, out, lse, back=(0,) * 19):
+    def pack(self, out, lse, back=_NO_BACK):
         hf, q, k, v = self.heads_first, self.q, self.k, self.v
         return _lib.CROSS_ARGS.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), *_strides(q, hf), *_strides(k, hf), *_strides(v, hf),
@@ -134,31 +136,45 @@ class _Call:
             _status_word(self.device).data_ptr(), *back)
 
 
-def _guarded(call, device):
-    """call() with the tensors' device current."""
-    if torch.cuda.current_device() == device.index:
-        return call()
-    with torch.cuda.device(device):
-        return call()
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(entry, device_index, args):
+    """What ``entry`` asks for with these packed arguments, whose pointers are blanked: it goes by shapes alone."""
+    need = ctypes.c_size_t()
+    check(getattr(lib(), entry)(args, need), entry)
+    return need.value
+
+
+def _workspace(c, entry):
+    """A fresh workspace for the call (or None): (tensor, pointer, bytes)."""
+    blank = _lib.CROSS_ARGS.pack(*(0,) * 17, *c.shape_args[:-1], 0, c.mask_args[0] and 1, *c.mask_args[1:], 0, *(0,) * 19)
+    need = _workspace_bytes(entry, c.device.index, blank)
+    if need == 0:
+        return None, 0, 0
+    ws = torch.empty(need, dtype=torch.uint8, device=c.device)
+    return ws, ws.data_ptr(), need
+
+
+def _on(device):
+    """A context with the tensors' device current (None where it is)."""
+    return None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _forward(c, want_lse):
-    def call():
-        out = torch.empty(c.q.shape, dtype=c.q.dtype, device=c.device)
-        lse = torch.empty(c.lse_shape, dtype=torch.float32, device=c.device) if want_lse else None
+    guard = _on(c.device)
+    if guard is not None:
+        with guard:
+            return _forward(c, want_lse)
+    out = torch.empty_like(c.q, memory_format=torch.contiguous_format)
+    lse = c.q.new_empty(c.lse_shape, dtype=torch.float32) if want_lse else None
+    if c.few_units:
+        ws, ptr, need = _workspace(c, "htrc_cross_forward_workspace_size")
+        args = c.pack(out, lse, (*_NO_BACK[:17], ptr, need))
+    else:
         args = c.pack(out, lse)
-        if c.few_units:
-            need = ctypes.c_size_t()
-            check(lib().htrc_cross_forward_workspace_size(args, need), "htrc_cross_forward_workspace_size")
-            if need.value:
-                ws = torch.empty(need.value, dtype=torch.uint8, device=c.device)
-                args = c.pack(out, lse, (*(0,) * 17, ws.data_ptr(), need.value))
-        rc = lib().htrc_cross_forward(args, _lib.raw_stream(c.device.index))
-        if rc:
-            check(rc, "htrc_cross_forward")
-        return (out[0], None if lse is None else lse[0]) if c.squeeze else (out, lse)
-
-    return _guarded(call, c.device)
+    rc = lib().htrc_cross_forward(args, _lib.raw_stream(c.device.index))
+    if rc:
+        check(rc, "htrc_cross_forward")
+    return (out[0], None if lse is None else lse[0]) if c.squeeze else (out, lse)
 
 
 def _backward(c, dout, out, lse, dlse):
@@ -172,23 +188,25 @@ def _backward(c, dout, out, lse, dlse):
     for name, x in (("lse", lse), ("dlse", dlse)):
         if x is not None and (x.shape != c.lse_shape or x.dtype != torch.float32 or x.device != c.device):
             raise ValueError(f"{name}: [batch, heads, queries] float32 on q's device expected")
+    guard = _on(c.device)
+    if guard is not None:
+        with guard:
+            return _launch_backward(c, dout, out, lse, dlse)
+    return _launch_backward(c, dout, out, lse, dlse)
 
-    def call():
-        do, o, z = _rows(dout), _rows(out), lse.contiguous()
-        dz = None if dlse is None else dlse.contiguous()
-        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=c.device) for x in (q, c.k, c.v))
-        back = [do.data_ptr(), *_strides(do, hf), 0 if dz is None else dz.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-                dv.data_ptr(), *_strides(dq, hf), *_strides(dk, hf), *_strides(dv, hf), 0, 0]
-        need = ctypes.c_size_t()
-        check(lib().htrc_cross_backward_workspace_size(c.pack(o, z, back), need), "htrc_cross_backward_workspace_size")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=c.device)
-        back[-2:] = ws.data_ptr(), need.value
-        rc = lib().htrc_cross_backward(c.pack(o, z, back), _lib.raw_stream(c.device.index))
-        if rc:
-            check(rc, "htrc_cross_backward")
-        return (dq[0], dk[0], dv[0]) if c.squeeze else (dq, dk, dv)
 
-    return _guarded(call, c.device)
+def _launch_backward(c, dout, out, lse, dlse):
+    hf = c.heads_first
+    do, o, z = _rows(dout), _rows(out), lse.contiguous()
+    dz = None if dlse is None else dlse.contiguous()
+    dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (c.q, c.k, c.v))
+    ws, ptr, need = _workspace(c, "htrc_cross_backward_workspace_size")
+    args = c.pack(o, z, (do.data_ptr(), *_strides(do, hf), 0 if dz is None else dz.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                         dv.data_ptr(), *_strides(dq, hf), *_strides(dk, hf), *_strides(dv, hf), ptr, need))
+    rc = lib().htrc_cross_backward(args, _lib.raw_stream(c.device.index))
+    if rc:
+        check(rc, "htrc_cross_backward")
+    return (dq[0], dk[0], dv[0]) if c.squeeze else (dq, dk, dv)
 
 
 class _Cross(torch.autograd.Function):

@@ -42,7 +42,7 @@ def grid_positions(grid, *, start=None, device="cuda"):
 
 class _Spec:
     """The arguments that do not depend on the tensors, checked."""
-    __slots__ = ("axes", "theta", "pairs", "eps", "freqs", "heads_first", "rotated", "table")
+    __slots__ = ("axes", "theta", "pairs", "eps", "freqs", "heads_first", "rotated", "table", "n_axes")
 
     def __init__(self, axes, theta, pairs, eps, freqs, heads_first):
         if not axes or min(axes) < 0 or any(w % 2 for w in axes):
@@ -60,7 +60,7 @@ class _Spec:
             if len(freqs) != sum(axes) // 2 or not all(math.isfinite(f) for f in freqs):
                 raise ValueError("freqs: one finite frequency for each of the sum(axes) / 2 pairs")
             self.table = (ctypes.c_double * max(1, len(freqs)))(*freqs)
-        self.rotated = sum(axes)
+        self.rotated, self.n_axes = sum(axes), len(axes)
         self.axes = axes + (0,) * (_lib.ROTARY_MAX_AXES - len(axes))
         self.theta, self.pairs, self.eps = float(theta), _lib.ROTARY_PAIRS[pairs], float(eps)
         self.freqs = 0 if self.table is None else ctypes.addressof(self.table)
@@ -105,11 +105,10 @@ def _check(spec, tensors, weights, positions):
     for w in weights:
         if w is not None and (w.dim() != 1 or w.shape[0] != dim or w.dtype not in _DTYPES or w.device != dev):
             raise ValueError(f"weight: [{dim}] float32, bfloat16 or float16 on the rows' device expected")
-    axes = sum(1 for w in spec.axes if w) if not isinstance(positions, torch.Tensor) else positions.shape[-1]
-    if not isinstance(positions, torch.Tensor) or positions.device != dev or positions.dim() not in (2, len(shape) - 1) \
-            or positions.shape[-2] != shape[-3] or (positions.dim() == 3 and positions.shape[0] not in (1, shape[0])):
+    at = positions.shape if isinstance(positions, torch.Tensor) and positions.device == dev else ()
+    if len(at) not in (2, len(shape) - 1) or at[-2] != shape[-3] or (len(at) == 3 and at[0] not in (1, shape[0])):
         raise ValueError("positions: [tokens, axes] or [batch, tokens, axes] on the rows' device expected")
-    if axes > _lib.ROTARY_MAX_AXES or any(spec.axes[axes:]):
+    if at[-1] != spec.n_axes:
         raise ValueError("positions: one for each of the axes expected")
     p = positions.dtype
     if p is torch.int32 or p is torch.float32:
@@ -149,77 +148,80 @@ def _pack(spec, x, positions, fields, count, ws=0, ws_bytes=0):
         spec.theta, spec.freqs, spec.eps, ws, ws_bytes)
 
 
-def _guarded(call, device):
-    """call() with the tensors' device current."""
-    if torch.cuda.current_device() == device.index:
-        return call()
-    with torch.cuda.device(device):
-        return call()
+def _empty(x, heads_first):
+    """A contiguous output for rows x in either order."""
+    return torch.empty_like(x.transpose(-3, -2) if heads_first else x, memory_format=torch.contiguous_format)
+
+
+def _on(device):
+    """A context with the tensors' device current (None where it is)."""
+    return None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _forward(spec, tensors, weights, positions):
     positions = _check(spec, tensors, weights, positions)
     x0 = tensors[0]
-    dtype, dev, hf = x0.dtype, x0.device, spec.heads_first
-
-    def call():
-        outs, fields, keep = [], [], []
-        for x, w in zip(tensors, weights):
-            x = _unit_rows(x)
-            y = torch.empty(_out_shape(x.shape, hf), dtype=dtype, device=dev)
-            wp = wd = 0
-            if w is not None:
-                w = w.contiguous()
-                wp, wd = w.data_ptr(), _DTYPES[w.dtype]
-            fields += (x.data_ptr(), *_strides(x), y.data_ptr(), *_strides(y, hf), 0, 0, 0, 0, wp, 0, wd, x.shape[-2])
-            keep += (x, w)
-            outs.append(y)
-        rc = lib().htrc_rotary_forward(_pack(spec, x0, positions, fields, len(outs)), _lib.raw_stream(dev.index))
-        if rc:
-            check(rc, "htrc_rotary_forward")
-        return outs
-
-    return _guarded(call, dev)
+    dev, hf = x0.device, spec.heads_first
+    guard = _on(dev)
+    if guard is not None:
+        with guard:
+            return _forward(spec, tensors, weights, positions)
+    outs, fields, keep = [], [], []
+    for x, w in zip(tensors, weights):
+        if x.stride(-1) != 1:
+            x = x.contiguous()
+        y = _empty(x, hf)
+        wp = wd = 0
+        if w is not None:
+            w = w.contiguous()
+            wp, wd = w.data_ptr(), _DTYPES[w.dtype]
+        fields += (x.data_ptr(), *_strides(x), y.data_ptr(), *_strides(y, hf), 0, 0, 0, 0, wp, 0, wd, x.shape[-2])
+        keep += (x, w)
+        outs.append(y)
+    rc = lib().htrc_rotary_forward(_pack(spec, x0, positions, fields, len(outs)), _lib.raw_stream(dev.index))
+    if rc:
+        check(rc, "htrc_rotary_forward")
+    return outs
 
 
 def _backward(spec, grads, tensors, weights, positions):
     positions = _check(spec, tensors, weights, positions)
     x0 = tensors[0]
     dtype, dev, hf = x0.dtype, x0.device, spec.heads_first
-
-    def call():
-        outs, dws, fields, keep = [], [], [], []
-        for g, x, w in zip(grads, tensors, weights):
-            shape = _out_shape(x.shape, hf)
-            if not isinstance(g, torch.Tensor) or g.shape != shape or g.dtype != dtype or g.device != dev:
-                raise ValueError(f"the output's gradient: {list(shape)} {dtype} expected")
-            g, x = _unit_rows(g), _unit_rows(x)
-            dx = torch.empty(x.shape, dtype=dtype, device=dev)
-            dw = None
-            norm = (0, 0, 0, 0, 0, 0, 0)
-            if w is not None:
-                w = w.contiguous()
-                dw = torch.empty_like(w)
-                norm = (x.data_ptr(), *_strides(x), w.data_ptr(), dw.data_ptr(), _DTYPES[w.dtype])
-            fields += (g.data_ptr(), *_strides(g, hf), dx.data_ptr(), *_strides(dx), *norm, x.shape[-2])
-            keep += (g, x, w)
-            outs.append(dx)
-            dws.append(dw)
-        ws, wp, need = None, 0, 0
-        if any(w is not None for w in weights):
-            size = ctypes.c_size_t()
-            check(lib().htrc_rotary_workspace_size(_pack(spec, x0, positions, fields, len(outs)), size),
-                  "htrc_rotary_workspace_size")
-            need = size.value
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            wp = ws.data_ptr()
-        rc = lib().htrc_rotary_backward(_pack(spec, x0, positions, fields, len(outs), wp, need),
-                                        _lib.raw_stream(dev.index))
-        if rc:
-            check(rc, "htrc_rotary_backward")
-        return outs, dws
-
-    return _guarded(call, dev)
+    for g, x in zip(grads, tensors):
+        shape = _out_shape(x.shape, hf)
+        if not isinstance(g, torch.Tensor) or g.shape != shape or g.dtype != dtype or g.device != dev:
+            raise ValueError(f"the output's gradient: {list(shape)} {dtype} expected")
+    guard = _on(dev)
+    if guard is not None:
+        with guard:
+            return _backward(spec, grads, tensors, weights, positions)
+    outs, dws, fields, keep = [], [], [], []
+    for g, x, w in zip(grads, tensors, weights):
+        g, x = _unit_rows(g), _unit_rows(x)
+        dx = _empty(x, False)
+        dw = None
+        norm = (0, 0, 0, 0, 0, 0, 0)
+        if w is not None:
+            w = w.contiguous()
+            dw = torch.empty_like(w)
+            norm = (x.data_ptr(), *_strides(x), w.data_ptr(), dw.data_ptr(), _DTYPES[w.dtype])
+        fields += (g.data_ptr(), *_strides(g, hf), dx.data_ptr(), *_strides(dx), *norm, x.shape[-2])
+        keep += (g, x, w)
+        outs.append(dx)
+        dws.append(dw)
+    ws, wp, need = None, 0, 0
+    if any(w is not None for w in weights):
+        size = ctypes.c_size_t()
+        check(lib().htrc_rotary_workspace_size(_pack(spec, x0, positions, fields, len(outs)), size),
+              "htrc_rotary_workspace_size")
+        need = size.value
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        wp = ws.data_ptr()
+    rc = lib().htrc_rotary_backward(_pack(spec, x0, positions, fields, len(outs), wp, need), _lib.raw_stream(dev.index))
+    if rc:
+        check(rc, "htrc_rotary_backward")
+    return outs, dws
 
 
 class _Rotary(torch.autograd.Function):
@@ -238,8 +240,10 @@ class _Rotary(torch.autograd.Function):
 
 
 def _apply(spec, tensors, weights, positions):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*tensors, *weights)):
-        return _Rotary.apply(spec, positions, len(tensors), *tensors, *weights)
+    if torch.is_grad_enabled():
+        for t in (*tensors, *weights):
+            if t is not None and t.requires_grad:
+                return _Rotary.apply(spec, positions, len(tensors), *tensors, *weights)
     return tuple(_forward(spec, tensors, weights, positions))
 
 

@@ -28,8 +28,9 @@ namespace {
 constexpr int kRotWarps = 8;
 constexpr int kRotMaxPairs = HTRC_ROTARY_MAX_DIM / 2;
 // Row batches that a warp fetches together (one more set is in flight while they are used), and CTAs per SM the
-// registers are held to.  q and k of 129,024 tokens x 24 heads x 128, bfloat16: forward 573 us (2, 4), 601 (3, 3), 612
-// (2, 2), 654 (1, 4); backward of 32,768 tokens 251 us (3, 2), 267 (2, 2), 288 (1, 3), 362 (2, 3).
+// registers are held to.  q and k of 129,024 tokens x 24 heads x 128, bfloat16, before the tables were in shared memory:
+// forward 573 us (2, 4), 601 (3, 3), 612 (2, 2), 654 (1, 4); backward of 32,768 tokens 251 us (3, 2), 267 (2, 2), 288
+// (1, 3), 362 (2, 3).
 constexpr int rot_unroll(bool back) { return back ? 3 : 2; }
 constexpr int rot_ctas(bool back, int bytes) { return back || bytes == 4 ? 2 : 4; }
 
@@ -78,10 +79,28 @@ __device__ __forceinline__ float load_weight(const void* w, int dtype, int i) {
   return __half2float(static_cast<const __half*>(w)[i]);
 }
 
-// cosine and sine of pair i of a token whose positions start at pos
-__device__ __forceinline__ float2 pair_turn(const RotaryParams& p, int64_t pos, int i) {
-  const int64_t at = pos + p.axis[i] * p.ps[2];
-  const uint64_t f = p.turn[i];
+// A CTA's copies of what its lanes index: a kernel parameter read at an index that differs by lane takes a pass for each
+// (32,768 tokens x 24 heads: 154 us with the parameters themselves, 136 so)
+struct RotaryShared {
+  uint64_t turn[kRotMaxPairs];
+  int64_t axis[kRotMaxPairs];           // element offset of the pair's position
+  float weight[2 * kRotMaxPairs];       // 1 without a norm
+  __device__ __forceinline__ void fill(const RotaryParams& p, const RotaryRows& r) {
+    for (int i = threadIdx.x; i < p.npairs; i += blockDim.x) {
+      turn[i] = p.turn[i];
+      axis[i] = p.axis[i] * p.ps[2];
+    }
+    for (int i = threadIdx.x; i < p.dim; i += blockDim.x) weight[i] = r.weight ? load_weight(r.weight, r.weight_dtype, i) : 1.f;
+    __syncthreads();
+  }
+};
+
+// cosine and sine of pair i of a token whose positions start at pos.  QUICK (16-bit rows): by the special function units,
+// absolute error 2^-21 on the reduced angle, against a rounding of 2^-9 or 2^-12; float32 rows take the 2-ulp functions.
+template <bool QUICK>
+__device__ __forceinline__ float2 pair_turn(const RotaryParams& p, const RotaryShared& sh, int64_t pos, int i) {
+  const int64_t at = pos + sh.axis[i];
+  const uint64_t f = sh.turn[i];
   float turns;
   if (!p.float_positions) {
     const int32_t n = __ldg(static_cast<const int32_t*>(p.positions) + at);
@@ -94,7 +113,8 @@ __device__ __forceinline__ float2 pair_turn(const RotaryParams& p, int64_t pos, 
     turns = (t - rintf(t)) + fmaf(n, lo, fmaf(n, hi, -t));
   }
   float s, c;
-  sincospif(2.0f * turns, &s, &c);
+  if constexpr (QUICK) __sincosf(6.283185307179586f * turns, &s, &c);
+  else sincospif(2.0f * turns, &s, &c);
   return make_float2(c, s);
 }
 
@@ -203,13 +223,15 @@ __device__ __forceinline__ float2 row_sums(float a, float b, int lane) {
 }
 
 // Rows whose pieces are 16-byte aligned, dim a multiple of 8 (HALF: the rotated width too).  blockIdx.y names the
-// tensor; a warp's task is a token and `chunk` of its heads.  The norm's weight is folded into the token's cosines and
-// sines.  BACK with a weight leaves the CTA's weight-gradient sums at partial[(blockIdx.y * gridDim.x + blockIdx.x) * dim].
-template <typename T, int LPR, bool HALF, bool BACK>
+// tensor; a warp's task is a token and `chunk` of its heads or, FLAT, rows of any tokens.  The norm's weight is folded
+// into the cosines and sines.  BACK with a weight leaves the CTA's weight-gradient sums at partial[(blockIdx.y * gridDim.x + blockIdx.x) * dim].
+template <typename T, int LPR, bool HALF, bool BACK, bool FLAT>
 __global__ void __launch_bounds__(kRotWarps * 32, rot_ctas(BACK, sizeof(T)))
     rotary_kernel(const __grid_constant__ RotaryParams p, float* __restrict__ partial) {
   __shared__ float sums[BACK ? kRotWarps * 32 * 8 : 1];
+  __shared__ RotaryShared sh;
   const RotaryRows& r = p.t[blockIdx.y];
+  sh.fill(p, r);
   constexpr int RPW = 32 / LPR, kRotUnroll = rot_unroll(BACK);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int u = lane % LPR, sub = lane / LPR;
@@ -237,9 +259,9 @@ __global__ void __launch_bounds__(kRotWarps * 32, rot_ctas(BACK, sizeof(T)))
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       w.f[i] = w.s[i] = make_float2(1.f, 1.f);
-      if (norm && on) {
-        w.f[i] = make_float2(load_weight(r.weight, r.weight_dtype, first_at(2 * i)), load_weight(r.weight, r.weight_dtype, first_at(2 * i + 1)));
-        w.s[i] = make_float2(load_weight(r.weight, r.weight_dtype, second_at(2 * i)), load_weight(r.weight, r.weight_dtype, second_at(2 * i + 1)));
+      if (on) {
+        w.f[i] = make_float2(sh.weight[first_at(2 * i)], sh.weight[first_at(2 * i + 1)]);
+        w.s[i] = make_float2(sh.weight[second_at(2 * i)], sh.weight[second_at(2 * i + 1)]);
       }
     }
     return w;
@@ -248,37 +270,14 @@ __global__ void __launch_bounds__(kRotWarps * 32, rot_ctas(BACK, sizeof(T)))
 #pragma unroll
   for (int i = 0; i < 2; ++i) dw.f[i] = dw.s[i] = make_float2(0.f, 0.f);
   const float inv_dim = 1.0f / static_cast<float>(p.dim);
-  const uint32_t tokens = static_cast<uint32_t>(p.tokens), tasks = static_cast<uint32_t>(p.batch) * tokens * r.chunks;
-  for (uint32_t task = blockIdx.x * kRotWarps + warp; task < tasks; task += gridDim.x * kRotWarps) {
-    const uint32_t tok = task / r.chunks, b = tok / tokens, n = tok - b * tokens;
-    const int h0 = static_cast<int>(task - tok * r.chunks) * r.chunk, h1 = min(r.heads, h0 + r.chunk);
-    const T* in = static_cast<const T*>(r.in) + b * r.is[0] + n * r.is[1] + (h0 + sub) * r.is[2];
-    const T* x = BACK && norm ? static_cast<const T*>(r.x) + b * r.xs[0] + n * r.xs[1] + (h0 + sub) * r.xs[2] : nullptr;
-    T* out = static_cast<T*>(r.out) + b * r.os[0] + n * r.os[1] + (h0 + sub) * r.os[2];
-    // rows in flight: the first ones are asked for before the angles are formed, the next ones before these are used
-    Raw<T> raw[kRotUnroll], rawx[BACK ? kRotUnroll : 1];
-    auto fetch = [&](int h) {
-#pragma unroll
-      for (int k = 0; k < kRotUnroll; ++k) {
-        raw[k] = Raw<T>{};
-        if (BACK) rawx[k] = Raw<T>{};
-        if (on && h + k * RPW < h1) {
-          raw[k] = load_raw<T, HALF>(in + k * RPW * r.is[2], off0, off1);
-          if (BACK && norm) rawx[k] = load_raw<T, HALF>(x + k * RPW * r.xs[2], off0, off1);
-        }
-      }
-      in += RPW * kRotUnroll * r.is[2];
-      if (BACK && norm) x += RPW * kRotUnroll * r.xs[2];
-    };
-    fetch(h0 + sub);
-    // forward: (f, s) -> (f fc - s ss, f fs + s sc), the weight folded in; backward: (f fc + s fs, s fc - f fs)
-    float2 fc[2], fs[2], sc[2], ss[2];
+  // forward: (f, s) -> (f fc - s ss, f fs + s sc), the weight folded in; backward: (f fc + s fs, s fc - f fs)
+  float2 fc[2], fs[2], sc[2], ss[2];
+  auto angles = [&](int64_t pos) {
     const Pairs w = weights();
-    const int64_t pos = b * p.ps[0] + n * p.ps[1];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float2 t0 = 2 * i < turned ? pair_turn(p, pos, pair0 + 2 * i) : make_float2(1.f, 0.f);
-      const float2 t1 = 2 * i + 1 < turned ? pair_turn(p, pos, pair0 + 2 * i + 1) : make_float2(1.f, 0.f);
+      const float2 t0 = 2 * i < turned ? pair_turn<sizeof(T) == 2>(p, sh, pos, pair0 + 2 * i) : make_float2(1.f, 0.f);
+      const float2 t1 = 2 * i + 1 < turned ? pair_turn<sizeof(T) == 2>(p, sh, pos, pair0 + 2 * i + 1) : make_float2(1.f, 0.f);
       fc[i] = make_float2(t0.x, t1.x);
       fs[i] = make_float2(t0.y, t1.y);
       if (!BACK) {
@@ -290,101 +289,162 @@ __global__ void __launch_bounds__(kRotWarps * 32, rot_ctas(BACK, sizeof(T)))
         ss[i] = make_float2(-t0.y, -t1.y);
       }
     }
-    for (int h = h0 + sub; h - sub < h1; h += RPW * kRotUnroll) {
-      Raw<T> now[kRotUnroll], nowx[BACK ? kRotUnroll : 1];
+  };
+  // one row's elements of this lane: what was read (backward: the gradient, and x with a norm) to what is written
+  auto turn = [&](const Raw<T>& now, const Raw<T>& nowx) {
+    Pairs v = unpack<T, HALF>(now), y;
+    if (!BACK) {
+      if (norm) {
+        float2 q = mul2(v.f[0], v.f[0]);
+        q = fma2(v.f[1], v.f[1], q);
+        q = fma2(v.s[0], v.s[0], q);
+        q = fma2(v.s[1], v.s[1], q);
+        const float rs = rsqrtf(fmaf(row_sum<LPR>(q.x + q.y), inv_dim, p.eps));
 #pragma unroll
-      for (int k = 0; k < kRotUnroll; ++k) {
-        now[k] = raw[k];
-        if (BACK) nowx[k] = rawx[k];
+        for (int i = 0; i < 2; ++i) {
+          v.f[i] = mul2(v.f[i], make_float2(rs, rs));
+          v.s[i] = mul2(v.s[i], make_float2(rs, rs));
+        }
       }
-      if (h - sub + RPW * kRotUnroll < h1) fetch(h + RPW * kRotUnroll);
 #pragma unroll
-      for (int k = 0; k < kRotUnroll; ++k) {
-        Pairs v = unpack<T, HALF>(now[k]), y;
-        if (!BACK) {
-          if (norm) {
-            float2 q = mul2(v.f[0], v.f[0]);
-            q = fma2(v.f[1], v.f[1], q);
-            q = fma2(v.s[0], v.s[0], q);
-            q = fma2(v.s[1], v.s[1], q);
-            const float rs = rsqrtf(fmaf(row_sum<LPR>(q.x + q.y), inv_dim, p.eps));
+      for (int i = 0; i < 2; ++i) {
+        y.f[i] = fma2(v.f[i], fc[i], mul2(v.s[i], ss[i]));
+        y.s[i] = fma2(v.f[i], fs[i], mul2(v.s[i], sc[i]));
+      }
+      if (!whole) {      // a pair past the rotated width keeps its elements apart, whatever they hold
+        const Pairs w = weights();
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              v.f[i] = mul2(v.f[i], make_float2(rs, rs));
-              v.s[i] = mul2(v.s[i], make_float2(rs, rs));
-            }
+        for (int i = 0; i < 2; ++i) {
+          if (2 * i >= turned) {
+            y.f[i].x = v.f[i].x * w.f[i].x;
+            y.s[i].x = v.s[i].x * w.s[i].x;
           }
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            y.f[i] = fma2(v.f[i], fc[i], mul2(v.s[i], ss[i]));
-            y.s[i] = fma2(v.f[i], fs[i], mul2(v.s[i], sc[i]));
-          }
-          if (!whole) {      // a pair past the rotated width keeps its elements apart, whatever they hold
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const Pairs w = weights();
-              if (2 * i >= turned) {
-                y.f[i].x = v.f[i].x * w.f[i].x;
-                y.s[i].x = v.s[i].x * w.s[i].x;
-              }
-              if (2 * i + 1 >= turned) {
-                y.f[i].y = v.f[i].y * w.f[i].y;
-                y.s[i].y = v.s[i].y * w.s[i].y;
-              }
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            y.f[i] = fma2(v.f[i], fc[i], mul2(v.s[i], fs[i]));
-            y.s[i] = fma2(v.s[i], fc[i], mul2(v.f[i], ss[i]));
-          }
-          if (!whole) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              if (2 * i >= turned) {
-                y.f[i].x = v.f[i].x;
-                y.s[i].x = v.s[i].x;
-              }
-              if (2 * i + 1 >= turned) {
-                y.f[i].y = v.f[i].y;
-                y.s[i].y = v.s[i].y;
-              }
-            }
-          }
-          if (norm) {
-            const Pairs xv = unpack<T, HALF>(nowx[k]);
-            float2 q = mul2(xv.f[0], xv.f[0]), hx;
-            q = fma2(xv.f[1], xv.f[1], q);
-            q = fma2(xv.s[0], xv.s[0], q);
-            q = fma2(xv.s[1], xv.s[1], q);
-            Pairs g;         // the gradient of the normalised row, times the weight
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              g.f[i] = mul2(y.f[i], w.f[i]);
-              g.s[i] = mul2(y.s[i], w.s[i]);
-            }
-            hx = mul2(g.f[0], xv.f[0]);
-            hx = fma2(g.f[1], xv.f[1], hx);
-            hx = fma2(g.s[0], xv.s[0], hx);
-            hx = fma2(g.s[1], xv.s[1], hx);
-            const float2 t = row_sums<LPR>(q.x + q.y, hx.x + hx.y, lane);
-            const float rs = rsqrtf(fmaf(t.x, inv_dim, p.eps));
-            const float back = -t.y * inv_dim * rs * rs;
-            const float2 rs2 = make_float2(rs, rs), back2 = make_float2(back, back);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float2 xf = mul2(xv.f[i], rs2), xs = mul2(xv.s[i], rs2);
-              dw.f[i] = fma2(y.f[i], xf, dw.f[i]);
-              dw.s[i] = fma2(y.s[i], xs, dw.s[i]);
-              y.f[i] = fma2(xf, back2, mul2(g.f[i], rs2));
-              y.s[i] = fma2(xs, back2, mul2(g.s[i], rs2));
-            }
+          if (2 * i + 1 >= turned) {
+            y.f[i].y = v.f[i].y * w.f[i].y;
+            y.s[i].y = v.s[i].y * w.s[i].y;
           }
         }
-        if (on && h + k * RPW < h1) store8<T, HALF>(out + k * RPW * r.os[2], off0, off1, y);
       }
-      out += RPW * kRotUnroll * r.os[2];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        y.f[i] = fma2(v.f[i], fc[i], mul2(v.s[i], fs[i]));
+        y.s[i] = fma2(v.s[i], fc[i], mul2(v.f[i], ss[i]));
+      }
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (2 * i >= turned) {
+            y.f[i].x = v.f[i].x;
+            y.s[i].x = v.s[i].x;
+          }
+          if (2 * i + 1 >= turned) {
+            y.f[i].y = v.f[i].y;
+            y.s[i].y = v.s[i].y;
+          }
+        }
+      }
+      if (norm) {
+        const Pairs w = weights(), xv = unpack<T, HALF>(nowx);
+        float2 q = mul2(xv.f[0], xv.f[0]), hx;
+        q = fma2(xv.f[1], xv.f[1], q);
+        q = fma2(xv.s[0], xv.s[0], q);
+        q = fma2(xv.s[1], xv.s[1], q);
+        Pairs g;         // the gradient of the normalised row, times the weight
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          g.f[i] = mul2(y.f[i], w.f[i]);
+          g.s[i] = mul2(y.s[i], w.s[i]);
+        }
+        hx = mul2(g.f[0], xv.f[0]);
+        hx = fma2(g.f[1], xv.f[1], hx);
+        hx = fma2(g.s[0], xv.s[0], hx);
+        hx = fma2(g.s[1], xv.s[1], hx);
+        const float2 t = row_sums<LPR>(q.x + q.y, hx.x + hx.y, lane);
+        const float rs = rsqrtf(fmaf(t.x, inv_dim, p.eps));
+        const float back = -t.y * inv_dim * rs * rs;
+        const float2 rs2 = make_float2(rs, rs), back2 = make_float2(back, back);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 xf = mul2(xv.f[i], rs2), xs = mul2(xv.s[i], rs2);
+          dw.f[i] = fma2(y.f[i], xf, dw.f[i]);
+          dw.s[i] = fma2(y.s[i], xs, dw.s[i]);
+          y.f[i] = fma2(xf, back2, mul2(g.f[i], rs2));
+          y.s[i] = fma2(xs, back2, mul2(g.s[i], rs2));
+        }
+      }
+    }
+    return y;
+  };
+  const uint32_t tokens = static_cast<uint32_t>(p.tokens);
+  if constexpr (FLAT) {
+    // a task is RPW * kRotUnroll rows, each with a token of its own
+    const uint32_t rows = static_cast<uint32_t>(p.batch) * tokens * r.heads, per = RPW * kRotUnroll;
+    for (uint32_t task = blockIdx.x * kRotWarps + warp; task * static_cast<uint64_t>(per) < rows; task += gridDim.x * kRotWarps) {
+      Raw<T> raw[kRotUnroll], rawx[BACK ? kRotUnroll : 1];
+      T* out[kRotUnroll];
+      int64_t pos[kRotUnroll];
+#pragma unroll
+      for (int k = 0; k < kRotUnroll; ++k) {
+        const uint32_t row = task * per + k * RPW + sub;
+        const bool in_k = row < rows;
+        const uint32_t at = in_k ? row : 0, tok = at / r.heads, h = at - tok * r.heads, b = tok / tokens, n = tok - b * tokens;
+        raw[k] = Raw<T>{};
+        if (BACK) rawx[k] = Raw<T>{};
+        if (on && in_k) {
+          raw[k] = load_raw<T, HALF>(static_cast<const T*>(r.in) + b * r.is[0] + n * r.is[1] + h * r.is[2], off0, off1);
+          if (BACK && norm) rawx[k] = load_raw<T, HALF>(static_cast<const T*>(r.x) + b * r.xs[0] + n * r.xs[1] + h * r.xs[2], off0, off1);
+        }
+        out[k] = on && in_k ? static_cast<T*>(r.out) + b * r.os[0] + n * r.os[1] + h * r.os[2] : nullptr;
+        pos[k] = b * p.ps[0] + n * p.ps[1];
+      }
+#pragma unroll
+      for (int k = 0; k < kRotUnroll; ++k) {
+        angles(pos[k]);
+        const Pairs y = turn(raw[k], rawx[BACK ? k : 0]);
+        if (out[k] != nullptr) store8<T, HALF>(out[k], off0, off1, y);
+      }
+    }
+  } else {
+    const uint32_t tasks = static_cast<uint32_t>(p.batch) * tokens * r.chunks;
+    for (uint32_t task = blockIdx.x * kRotWarps + warp; task < tasks; task += gridDim.x * kRotWarps) {
+      const uint32_t tok = task / r.chunks, b = tok / tokens, n = tok - b * tokens;
+      const int h0 = static_cast<int>(task - tok * r.chunks) * r.chunk, h1 = min(r.heads, h0 + r.chunk);
+      const T* in = static_cast<const T*>(r.in) + b * r.is[0] + n * r.is[1] + (h0 + sub) * r.is[2];
+      const T* x = BACK && norm ? static_cast<const T*>(r.x) + b * r.xs[0] + n * r.xs[1] + (h0 + sub) * r.xs[2] : nullptr;
+      T* out = static_cast<T*>(r.out) + b * r.os[0] + n * r.os[1] + (h0 + sub) * r.os[2];
+      // rows in flight: the first ones are asked for before the angles are formed, the next ones before these are used
+      Raw<T> raw[kRotUnroll], rawx[BACK ? kRotUnroll : 1];
+      auto fetch = [&](int h) {
+#pragma unroll
+        for (int k = 0; k < kRotUnroll; ++k) {
+          raw[k] = Raw<T>{};
+          if (BACK) rawx[k] = Raw<T>{};
+          if (on && h + k * RPW < h1) {
+            raw[k] = load_raw<T, HALF>(in + k * RPW * r.is[2], off0, off1);
+            if (BACK && norm) rawx[k] = load_raw<T, HALF>(x + k * RPW * r.xs[2], off0, off1);
+          }
+        }
+        in += RPW * kRotUnroll * r.is[2];
+        if (BACK && norm) x += RPW * kRotUnroll * r.xs[2];
+      };
+      fetch(h0 + sub);
+      angles(b * p.ps[0] + n * p.ps[1]);
+      for (int h = h0 + sub; h - sub < h1; h += RPW * kRotUnroll) {
+        Raw<T> now[kRotUnroll], nowx[BACK ? kRotUnroll : 1];
+#pragma unroll
+        for (int k = 0; k < kRotUnroll; ++k) {
+          now[k] = raw[k];
+          if (BACK) nowx[k] = rawx[k];
+        }
+        if (h - sub + RPW * kRotUnroll < h1) fetch(h + RPW * kRotUnroll);
+#pragma unroll
+        for (int k = 0; k < kRotUnroll; ++k) {
+          const Pairs y = turn(now[k], nowx[BACK ? k : 0]);
+          if (on && h + k * RPW < h1) store8<T, HALF>(out + k * RPW * r.os[2], off0, off1, y);
+        }
+        out += RPW * kRotUnroll * r.os[2];
+      }
     }
   }
   if (BACK && norm) {
@@ -414,7 +474,9 @@ __global__ void __launch_bounds__(kRotWarps * 32)
     rotary_any_kernel(const __grid_constant__ RotaryParams p, bool half, float* __restrict__ partial) {
   constexpr int kMax = HTRC_ROTARY_MAX_DIM, kEl = kMax / 32;
   __shared__ float rows[kRotWarps][kMax];
+  __shared__ RotaryShared sh;
   const RotaryRows& r = p.t[blockIdx.y];
+  sh.fill(p, r);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool norm = r.weight != nullptr;
   float dw[kEl];
@@ -440,7 +502,7 @@ __global__ void __launch_bounds__(kRotWarps * 32)
 #pragma unroll
       for (int k = 0; k < kEl; ++k) {
         const int e = lane + 32 * k;
-        if (e < p.dim) v[k] *= rs * load_weight(r.weight, r.weight_dtype, e);
+        if (e < p.dim) v[k] *= rs * sh.weight[e];
       }
     }
     __syncwarp();
@@ -454,7 +516,7 @@ __global__ void __launch_bounds__(kRotWarps * 32)
         const int i = half ? (e < p.npairs ? e : e - p.npairs) : e >> 1;
         const bool second = half ? e >= p.npairs : (e & 1);
         const float other = rows[warp][half ? (second ? i : i + p.npairs) : e ^ 1];
-        const float2 cs = pair_turn(p, pos, i);
+        const float2 cs = pair_turn<sizeof(T) == 2>(p, sh, pos, i);
         const float s = (BACK != second) ? cs.y : -cs.y;     // forward: a c - b s and b c + a s
         v[k] = fmaf(v[k], cs.x, other * s);
       }
@@ -468,7 +530,7 @@ __global__ void __launch_bounds__(kRotWarps * 32)
         const int e = lane + 32 * k;
         xv[k] = e < p.dim ? to_f<T>(x[e]) : 0.f;
         ss = fmaf(xv[k], xv[k], ss);
-        if (e < p.dim) hx = fmaf(v[k] * load_weight(r.weight, r.weight_dtype, e), xv[k], hx);
+        if (e < p.dim) hx = fmaf(v[k] * sh.weight[e], xv[k], hx);
       }
       const float rs = rsqrtf(row_sum<32>(ss) * inv_dim + p.eps);
       const float back = row_sum<32>(hx) * inv_dim * rs * rs;
@@ -477,7 +539,7 @@ __global__ void __launch_bounds__(kRotWarps * 32)
         const int e = lane + 32 * k;
         if (e < p.dim) {
           dw[k] = fmaf(v[k], xv[k] * rs, dw[k]);
-          v[k] = rs * fmaf(-xv[k], back, v[k] * load_weight(r.weight, r.weight_dtype, e));
+          v[k] = rs * fmaf(-xv[k], back, v[k] * sh.weight[e]);
         }
       }
     }
@@ -525,6 +587,7 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
+constexpr int kRotFlatHeads = 2;       // FLAT: see rotary_run
 constexpr int kRotBlocksPerSm = 8;      // 256-thread CTAs per SM the grids are sized for
 
 int rotary_max_blocks() { return sm_count() * kRotBlocksPerSm; }
@@ -613,20 +676,17 @@ bool rotary_table(const HtrcRotaryArgs* a, RotaryParams* p) {
   return true;
 }
 
-template <typename T, int LPR, bool HALF, bool BACK>
-void run_rows(const RotaryParams& p, dim3 grid, float* partial, cudaStream_t st) {
-  rotary_kernel<T, LPR, HALF, BACK><<<grid, kRotWarps * 32, 0, st>>>(p, partial);
+template <typename T, int LPR, bool BACK, bool FLAT>
+void run_rows(const RotaryParams& p, bool half, dim3 grid, float* partial, cudaStream_t st) {
+  if (half) rotary_kernel<T, LPR, true, BACK, FLAT><<<grid, kRotWarps * 32, 0, st>>>(p, partial);
+  else rotary_kernel<T, LPR, false, BACK, FLAT><<<grid, kRotWarps * 32, 0, st>>>(p, partial);
 }
 
-template <typename T, bool BACK>
+template <typename T, bool BACK, bool FLAT>
 void run_dim(const RotaryParams& p, bool half, dim3 grid, float* partial, cudaStream_t st) {
-  if (p.dim <= 64) {
-    half ? run_rows<T, 8, true, BACK>(p, grid, partial, st) : run_rows<T, 8, false, BACK>(p, grid, partial, st);
-  } else if (p.dim <= 128) {
-    half ? run_rows<T, 16, true, BACK>(p, grid, partial, st) : run_rows<T, 16, false, BACK>(p, grid, partial, st);
-  } else {
-    half ? run_rows<T, 32, true, BACK>(p, grid, partial, st) : run_rows<T, 32, false, BACK>(p, grid, partial, st);
-  }
+  if (p.dim <= 64) run_rows<T, 8, BACK, FLAT>(p, half, grid, partial, st);
+  else if (p.dim <= 128) run_rows<T, 16, BACK, FLAT>(p, half, grid, partial, st);
+  else run_rows<T, 32, BACK, FLAT>(p, half, grid, partial, st);
 }
 
 template <bool BACK>
@@ -673,15 +733,27 @@ int rotary_run(const HtrcRotaryArgs* a, cudaStream_t st) {
       return HTRC_ERR_WORKSPACE;
   }
   const int lpr = a->dim <= 64 ? 8 : a->dim <= 128 ? 16 : 32;
+  // few heads: a warp's rows come from several tokens, each with angles of its own, rather than leave lanes idle.
+  // q and k of 32,768 tokens x 128, bfloat16: 1 head 17.9 us against 40.3, 4 heads 58.1 against 44.3; of 16,384 tokens
+  // x 2 heads 17.9 against 22.6, backward of 32,768 x 2 58.9 against 89.1
+  bool flat = true;
+  for (int i = 0; i < a->n_tensors; ++i) {
+    flat = flat && a->tensor[i].heads <= kRotFlatHeads;
+    vec = vec && rows * a->tensor[i].heads < int64_t{1} << 31;      // its task numbers are 32-bit
+  }
   int64_t blocks = 1;
   for (int i = 0; i < a->n_tensors; ++i) {
     RotaryRows& r = p.t[i];
-    // heads per warp: all of a token's, whose angles are then computed once, where the tokens alone fill the
-    // device; else one batch of rows, for the shortest chain
+    // heads per warp: all of a token's, whose angles are then formed once, where the tokens alone give every SM 8
+    // warps; else the token's heads are shared out until they do.  1,024 tokens x 24 heads: 7.8 us shared out, 31.5 not;
+    // 16,384 tokens: 83 us shared out twice as far, 72 not
     const int batch_rows = 32 / lpr;
-    r.chunk = rows >= 2 * sm_count() * kRotWarps ? r.heads : std::min<int>(r.heads, batch_rows);
+    const int64_t most = (r.heads + batch_rows - 1) / batch_rows, want = 8 * sm_count();
+    const int64_t parts = rows > 0 ? std::min(most, (want + rows - 1) / rows) : 1;
+    r.chunk = static_cast<int>((most + parts - 1) / parts) * batch_rows;
     r.chunks = (r.heads + r.chunk - 1) / r.chunk;
-    const int64_t tasks = rows * (vec ? r.chunks : r.heads);
+    const int64_t per = 32 / lpr * rot_unroll(BACK);
+    const int64_t tasks = !vec ? rows * r.heads : flat ? (rows * r.heads + per - 1) / per : rows * r.chunks;
     blocks = std::max(blocks, (tasks + kRotWarps - 1) / kRotWarps);
   }
   blocks = std::min<int64_t>(blocks, rotary_max_blocks());
@@ -690,7 +762,8 @@ int rotary_run(const HtrcRotaryArgs* a, cudaStream_t st) {
   if (rows > 0 || partials) {
     auto go = [&](auto tag) {
       using T = decltype(tag);
-      if (vec) run_dim<T, BACK>(p, half, grid, partial, st);
+      if (vec && flat) run_dim<T, BACK, true>(p, half, grid, partial, st);
+      else if (vec) run_dim<T, BACK, false>(p, half, grid, partial, st);
       else rotary_any_kernel<T, BACK><<<grid, kRotWarps * 32, 0, st>>>(p, half, partial);
     };
     if (a->dtype == HTRC_LAYER_F32) go(float{});

@@ -127,6 +127,30 @@ def test_forward_and_backward_match_float64(dev, dtype, pairs, dim, axes):
                 assert dw is None
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("b,n,hq,hk", [(2, 137, 2, 1), (3, 61, 1, 1), (1, 20011, 2, 2), (1, 20011, 3, 1), (5, 4001, 6, 2)])
+def test_few_heads_and_many_tokens(dev, dtype, b, n, hq, hk):
+    """Rows of several tokens per warp, and more rows than one pass over the grid takes."""
+    import htrc_b200
+    gen = torch.Generator(device=dev).manual_seed(n + hq)
+    for dim, axes, pairs in [(64, (20, 22, 22), "half"), (72, (8, 16, 24), "interleaved"), (128, (44, 42, 42), "interleaved")]:
+        q = torch.randn((b, n, hq, dim), generator=gen, device=dev).to(dtype)
+        k = torch.randn((b, n, hk, dim), generator=gen, device=dev).to(dtype)
+        pos = torch.randint(0, 3000, (b, n, 3), generator=gen, device=dev, dtype=torch.int32)
+        wq = 1 + 0.3 * torch.randn(dim, generator=gen, device=dev)
+        wk = 1 + 0.3 * torch.randn(dim, generator=gen, device=dev)
+        kw = dict(axes=axes, pairs=pairs, q_weight=wq, k_weight=wk, heads_first=True)
+        got = htrc_b200.rotary_qk(q, k, pos, **kw)
+        for x, w, y in zip((q, k), (wq, wk), got):
+            _close(_major(y, True), *_plain(x, pos, axes, pairs, w))
+        dy = [torch.randn(y.shape, generator=gen, device=dev).to(dtype) for y in got]
+        dq, dk, dwq, dwk = htrc_b200.rotary_qk_backward(*dy, q, k, pos, **kw)
+        for x, w, g, dx, dw in zip((q, k), (wq, wk), dy, (dq, dk), (dwq, dwk)):
+            want, size, want_w, size_w = _plain_backward(_major(g, True), x, pos, axes, pairs, w)
+            _close(dx, want, size)
+            _close(dw, want_w, size_w)
+
+
 @pytest.mark.parametrize("pairs", ["interleaved", "half"])
 def test_late_positions_keep_their_accuracy(dev, pairs):
     """int32 positions are reduced exactly: the last ones rotate as accurately as the first."""

@@ -22,7 +22,6 @@
 // the zeroing of excluded keys' values.
 #include <algorithm>
 #include <cmath>
-#include <type_traits>
 
 #include "cross.cuh"
 
@@ -35,10 +34,6 @@ constexpr int kXRows = 128, kXUnit = 256, kXKeys = 128;
 constexpr uint32_t kXChunk = 128 * 128;            // 128 rows of 64 16-bit elements
 constexpr uint32_t kXColS = 0, kXColO = 256, kXCols = 512;   // tile t: S at 128 t, O at 256 + 128 t
 constexpr float kXRescale = 8.0f;
-#ifndef XPOLY
-#define XPOLY 0
-#endif
-constexpr int kXPoly = XPOLY;                      // pairs of 16: of 32 exponentials, 2 kXPoly
 
 template <int DP>
 struct CrossFwdSmem {
@@ -102,22 +97,6 @@ struct Walk {
     if (++j >= j1) open_live(p, unit + gridDim.x);
   }
 };
-
-// 2^x of two values by Cody-Waite reduction to [-1/2, 1/2] and a degree-4 minimax polynomial (relative error 2.7e-6,
-// of mean 4e-8), float32 throughout; values below 2^-126 give 2^-126
-__device__ __forceinline__ float2 poly_ex2(float2 x) {
-  constexpr float kMagic = 12582912.0f;             // 1.5 * 2^23: the sum's low bits are the nearest integer
-  x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
-  const float2 t = add2(x, make_float2(kMagic, kMagic));
-  const float2 f = sub2(x, sub2(t, make_float2(kMagic, kMagic)));
-  float2 y = make_float2(0.009570102207362652f, 0.009570102207362652f);
-  y = fma2(y, f, make_float2(0.05591785907745361f, 0.05591785907745361f));
-  y = fma2(y, f, make_float2(0.240247443318367f, 0.240247443318367f));
-  y = fma2(y, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
-  y = fma2(y, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
-}
 
 template <int DP, bool BF, int KIND>
 __global__ void __launch_bounds__(kXThreads, 1)
@@ -428,7 +407,7 @@ __global__ void __launch_bounds__(kXThreads, 1)
         }
         const float mref = m == -INFINITY ? 0.f : m;      // nothing seen yet: every term is exp2(-inf) = 0
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        auto weights = [&](auto mixed) {
+        auto weights = [&]() {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t pw[16];
@@ -439,10 +418,7 @@ __global__ void __launch_bounds__(kXThreads, 1)
                 e = mul2(sub2(e, make_float2(mref, mref)), make_float2(kCrossLog2e, kCrossLog2e));
               else
                 e = fma2(e, make_float2(scale2, scale2), make_float2(-mref, -mref));
-              if (decltype(mixed)::value && (i * kXPoly) / 16 != ((i + 1) * kXPoly) / 16)
-                e = poly_ex2(e);
-              else
-                e = make_float2(cross_ex2(e.x), cross_ex2(e.y));
+              e = make_float2(cross_ex2(e.x), cross_ex2(e.y));
               sum[i & 1] = add2(sum[i & 1], e);
               pw[i] = pack16x2<BF>(e.x, e.y);
             }
@@ -452,11 +428,12 @@ __global__ void __launch_bounds__(kXThreads, 1)
             mbar_arrive(&bars->p_full[t][c]);
           }
         };
-        // the polynomial cannot tell an excluded key's -inf: full blocks only
+        // without a mask whole blocks have a copy of their own: one copy for these and the ragged last ones spills twice
+        // as much (129,024 queries x 512 keys x 24 heads: 922 us, 834 with two)
         if (KIND == CROSS_NONE && left >= kXKeys)
-          weights(std::true_type{});
+          weights();
         else
-          weights(std::false_type{});
+          weights();
         if (two) {
           if (lane == 0) mbar_arrive(&bars->turn[t ^ 1]);
           ++turns;

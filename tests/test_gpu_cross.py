@@ -143,6 +143,31 @@ def test_sizes_match_float64(dev, dtype, size):
     _check(q, k, v, heads_first=size[1] % 2 == 0, with_dlse=size[2] % 2 == 0)
 
 
+# more units than SMs (each CTA walks several), keys split over CTAs, more entries than one pass of the lengths' sums
+MANY = [(40, 300, 150, 6, 3, 64), (7, 700, 390, 16, 16, 128), (230, 1, 70, 4, 2, 64), (260, 3, 130, 2, 1, 128),
+        (2, 40, 9000, 2, 1, 64), (1, 130, 12000, 1, 1, 128), (2, 1, 30000, 4, 1, 128), (5, 4, 2000, 24, 8, 64)]
+
+
+@pytest.mark.parametrize("kind", ["none", "lengths", "pairs", "bias"])
+@pytest.mark.parametrize("size", MANY)
+def test_many_units_and_dead_ones(dev, size, kind):
+    b, n, m, h, hk, d = size
+    q, k, v = _rows(dev, *size, torch.bfloat16, seed=sum(size))
+    gen = torch.Generator(device=dev).manual_seed(b + m)
+    lengths = mask = None
+    if kind != "none":
+        lengths = torch.randint(0, m + 1, (b,), generator=gen, device=dev, dtype=torch.int32)
+        lengths[b // 3] = 0                       # entries without a key, at the start, in the middle and at the end
+        if b > 4:
+            lengths[0] = lengths[b // 2] = lengths[b // 2 + 1] = lengths[-1] = 0
+    if kind == "pairs":
+        mask = torch.rand((b, 1, n, m), generator=gen, device=dev) < 0.5
+        mask[:, :, ::5] = False
+    elif kind == "bias":
+        mask = torch.randn((1, h, n, m), generator=gen, device=dev)
+    _check(q, k, v, lengths=lengths, mask=mask)
+
+
 def _mask(kind, b, h, n, m, dtype, dev, seed=3):
     gen = torch.Generator(device=dev).manual_seed(seed)
     keys = torch.rand((b, 1, 1, m), generator=gen, device=dev) < 0.6

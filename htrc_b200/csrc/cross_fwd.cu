@@ -399,7 +399,8 @@ __global__ void __launch_bounds__(kXThreads, 1)
           }
         }
         // The two tiles' exponentials take turns: each then has the special function units to itself, and the other's
-        // loads, maxima and products run meanwhile (together, both would wait for the units and then both leave them)
+        // loads, maxima and products run meanwhile (together, both would wait for the units and then both leave them:
+        // 4,115 clocks a pair of steps, 3,900 in turns).  The turn passes on before the last quarter has landed
         const bool two = w.row0 + kXRows < p.s.queries;
         if (two && (t == 1 || turns > 0)) {
           ok = mbar_wait_warp(&bars->turn[t], (turns - (t == 0)) & 1, status, abort_flag);
@@ -423,6 +424,7 @@ __global__ void __launch_bounds__(kXThreads, 1)
               pw[i] = pack16x2<BF>(e.x, e.y);
             }
             tmem_st16(col_s + 16 * c, pw);
+            if (two && c == 3 && lane == 0) mbar_arrive(&bars->turn[t ^ 1]);
             tmem_st_wait();
             tc_fence_before();
             mbar_arrive(&bars->p_full[t][c]);
@@ -434,10 +436,7 @@ __global__ void __launch_bounds__(kXThreads, 1)
           weights();
         else
           weights();
-        if (two) {
-          if (lane == 0) mbar_arrive(&bars->turn[t ^ 1]);
-          ++turns;
-        }
+        turns += two;
         sum[0] = add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
       }

@@ -124,7 +124,7 @@ class _Call:
         self.q, self.k, self.v = _rows(q), _rows(k), _rows(v)
         self.lse_shape = (batch, heads, queries)
         # beyond this many tiles of 256 rows the library never splits their keys (it asks for no workspace then)
-        self.few_units = batch * heads * (queries + 255) < 256 * 1024 or heads // kv_heads * queries <= 16
+        self.few_units = batch * heads * (queries + 255) < 256 * 1024 or heads // kv_heads * queries <= 32
         self.shape_args = (batch, queries, keys, heads, kv_heads, dim, _DTYPES[q.dtype], scale,
                            0 if key_lengths is None else key_lengths.data_ptr())
 

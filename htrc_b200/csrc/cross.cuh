@@ -177,9 +177,9 @@ int cross_mask_kind(const HtrcCrossArgs* a);
 bool cross_map(CUtensorMap* m, const HtrcCrossArgs* a, const void* base, const int64_t* stride, int64_t rows, int heads,
                int box_rows, int* b, int* h);
 
-// rows that share a key head, below which they are computed without matrix tiles (cross_few.cu)
+// few rows that share a key head, computed without matrix tiles (cross_few.cu)
 int cross_forward_few(const HtrcCrossArgs* a, cudaStream_t st);
 size_t cross_few_bytes(const HtrcCrossArgs* a);              // its workspace
-constexpr int kCrossFewRows = 16;
+constexpr int kCrossFewRows = 16;                            // a chunk of them
 
 }  // namespace htrc

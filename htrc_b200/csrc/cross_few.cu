@@ -7,8 +7,8 @@
 // All units' tiles of 32 keys (a unit: one entry, key head and up to 16 rows) form one line that the warps share evenly,
 // 12 per SM, whatever the entries' lengths; what a warp has of a unit is a segment, and cross_few_join_kernel joins the
 // units' segments.  (A cluster of up to 8 CTAs per unit, joined in place, took 28 us for the case above: the longest
-// entry's clusters ran on while the others' SMs were idle.)  Units of two tiles or less get a warp each and no second
-// launch.
+// entry's clusters ran on while the others' SMs were idle.)  Units of two tiles or less, or as many units as half the
+// warps, get a warp each and no second launch.
 //
 // A warp has buffers of its own in shared memory (16-byte asynchronous copies: the next tile's keys land while this
 // tile's values are used, its values while its scores are formed; 192 KB per SM) and waits on no other.  S = Q K^T has the
@@ -505,8 +505,10 @@ FewPlan few_plan(const HtrcCrossArgs* a) {
   const int64_t rows = a->heads / a->kv_heads * a->queries, tiles = (a->keys + 31) / 32;
   f.chunks = static_cast<int>((rows + kFewRows - 1) / kFewRows);
   f.units = a->batch * a->kv_heads * f.chunks;
-  // (the line's starts are found by one CTA: batches beyond that are many units anyway)
-  f.line = tiles > kFewAlone && a->batch <= kFewBatch;
+  // The line evens out the entries' lengths for the price of the segments' rows and the join.  Ragged entries, 8 key heads
+  // of up to 1,000 keys: 512 units of 3 rows 36.5 us in line and 52.2 apart, of 15 rows 62.7 and 59.1; 1,024 units of 3
+  // rows 64.7 either way, of 15 rows 107 and 71.  (Its starts are found by one CTA: kFewBatch entries.)
+  f.line = tiles > kFewAlone && a->batch <= kFewBatch && f.units < int64_t(sm_count()) * kFewWarps;
   const int64_t most = f.line ? std::min(f.units * std::min<int64_t>(tiles, kFewSegments), int64_t(2) * sm_count() * kFewWarps) : f.units;
   f.ctas = static_cast<int>((most + kFewWarps - 1) / kFewWarps);
   if (!f.line) return f;

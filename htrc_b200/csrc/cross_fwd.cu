@@ -606,9 +606,17 @@ bool rows_ok(const void* p, const int64_t* stride) {
   return true;
 }
 
+// Whether the rows that share a key head go without matrix tiles (cross_few.cu): 16 at most, a chunk of its products, or
+// two chunks where this file's units alone fill the SMs, so that it would not split their keys.  4 entries x 24 heads x
+// 1,000 keys: 16 rows 22.4 us there and 20.2 here, 24 rows 29.3 and 20.3; 16 x 24 heads on 8 key heads of 1,000 keys: 24
+// rows 35.9 and 53.9; 64 x 24 x 500: 16 rows 67 and 112, 32 rows 87 and 112, 64 rows 155 and 112.
+bool few_rows(const HtrcCrossArgs* a) {
+  const int64_t rows = a->heads / a->kv_heads * a->queries;
+  return rows <= kCrossFewRows || (rows <= 2 * kCrossFewRows && a->batch * a->heads >= sm_count());
+}
+
 // Parts the keys are split into: the fewest rounds of CTAs times blocks (1.2 us each), with about two blocks' time for a
 // unit's ends and, for any split, four for the second launch and the time that the parts' bytes take at 5 TB/s.
-bool few_rows(const HtrcCrossArgs* a) { return a->heads / a->kv_heads * a->queries <= kCrossFewRows; }
 
 int fwd_splits(const HtrcCrossArgs* a) {
   if (few_rows(a)) return 1;

@@ -145,6 +145,7 @@ def test_sizes_match_float64(dev, dtype, size):
 
 # more units than SMs (each CTA walks several), keys split over CTAs, more entries than one pass of the lengths' sums
 MANY = [(40, 300, 150, 6, 3, 64), (7, 700, 390, 16, 16, 128), (230, 1, 70, 4, 2, 64), (260, 3, 130, 2, 1, 128),
+        (300, 5, 90, 4, 4, 64), (100, 2, 200, 24, 12, 64), (30, 24, 150, 6, 6, 128), (20, 9, 333, 24, 8, 128),
         (2, 40, 9000, 2, 1, 64), (1, 130, 12000, 1, 1, 128), (2, 1, 30000, 4, 1, 128), (5, 4, 2000, 24, 8, 64)]
 
 

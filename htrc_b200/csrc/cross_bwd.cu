@@ -18,7 +18,9 @@
 // Where the key blocks alone do not fill the device evenly, the query range is split and the float32 partial sums are
 // added by cross_dkv_sum_kernel in order.
 //
-// Rounding: P and dS enter their products in the operands' 16-bit type, the gradients are rounded once from float32.
+// Rounding: P and dS enter their products in the operands' 16-bit type (a relative 2^-9 for bfloat16, about what the
+// result's own rounding adds; carrying the rest would take a second product each), the gradients are rounded once from
+// float32.
 #include <algorithm>
 #include <cmath>
 

@@ -78,7 +78,7 @@ bool make_map(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base
 }  // namespace
 
 namespace htrc {
-bool device_ok() { return device_info().ok; }
+bool device_is_b200() { return device_info().ok; }
 int sm_count() { return device_info().sms; }
 bool make_tiled_map(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
                     const uint64_t* strides, const uint32_t* box, bool swizzle128) {

@@ -663,7 +663,7 @@ int cross_forward(const HtrcCrossArgs* a, cudaStream_t st) {
   size_t need = 0;
   rc = fwd_sizes(a, &splits, &need);
   if (rc != HTRC_OK) return rc;
-  if (!device_ok()) return HTRC_ERR_DEVICE;
+  if (!device_is_b200()) return HTRC_ERR_DEVICE;
   if (a->batch * a->queries == 0) return HTRC_OK;
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 256))
     return HTRC_ERR_WORKSPACE;

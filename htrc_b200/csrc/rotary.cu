@@ -693,7 +693,7 @@ template <bool BACK>
 int rotary_run(const HtrcRotaryArgs* a, cudaStream_t st) {
   int rc = rotary_validate(a, BACK, true);
   if (rc != HTRC_OK) return rc;
-  if (!device_ok()) return HTRC_ERR_DEVICE;
+  if (!device_is_b200()) return HTRC_ERR_DEVICE;
   RotaryParams p{};
   p.batch = a->batch;
   p.tokens = a->tokens;

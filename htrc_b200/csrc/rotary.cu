@@ -596,7 +596,7 @@ int rotary_validate(const HtrcRotaryArgs* a, bool back, bool ptrs) {
   if (a == nullptr || a->n_tensors < 1 || a->n_tensors > 2) return HTRC_ERR_ARG;
   if (a->dtype < HTRC_LAYER_F32 || a->dtype > HTRC_LAYER_F16) return HTRC_ERR_ARG;
   if (a->batch < 0 || a->tokens < 0) return HTRC_ERR_ARG;
-  constexpr int64_t kMaxRows = int64_t(1) << 32;      // of one head count's rows: a task's 32-bit index
+  constexpr int64_t kMaxRows = int64_t(1) << 32;      // more would not fit the device: the products below cannot overflow
   if (a->tokens > 0 && a->batch > kMaxRows / a->tokens) return HTRC_ERR_UNSUPPORTED;
   if (a->dim < 2 || a->n_axes < 1) return HTRC_ERR_ARG;
   if (a->dim > HTRC_ROTARY_MAX_DIM || a->n_axes > HTRC_ROTARY_MAX_AXES) return HTRC_ERR_UNSUPPORTED;

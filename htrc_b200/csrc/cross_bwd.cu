@@ -8,6 +8,7 @@
 // 128, dQ accumulating in TMEM (128 columns).  S is double buffered (256 columns), so the next block's S runs under this
 // block's exponentials; dP (128 columns) is freed when the threads have read it, so its next product runs before dQ's.
 // dS overwrites S.  Two threads per row, 64 keys each: nothing passes between them (no maximum here) but delta's halves.
+// Where there are few units the keys are split and cross_grad_sum_kernel adds the parts' float32 dQ in order.
 // delta comes from the rows of dO and out while the unit's first weights are formed; (lse, delta) are left for the second
 // pass.  The K / V ring runs on into the next unit, and its Q and dO follow as soon as the last products have read these.
 //
@@ -16,7 +17,7 @@
 // buffered beside them, and two softmax warpgroups take alternate steps, so a step's exponentials run under the
 // neighbouring steps' products.  P^T and dS^T never leave TMEM: they are the A operands of the products with dO and Q.
 // Where the key blocks alone do not fill the device evenly, the query range is split and the float32 partial sums are
-// added by cross_dkv_sum_kernel in order.
+// added by cross_grad_sum_kernel in order.
 //
 // Rounding: P and dS enter their products in the operands' 16-bit type (a relative 2^-9 for bfloat16, about what the
 // result's own rounding adds; carrying the rest would take a second product each), the gradients are rounded once from
@@ -76,25 +77,43 @@ struct DqParams {
   int64_t stat_rows;
   CrossBits bits;
   uint32_t units, tiles;    // tiles of 128 rows per head
+  int splits;               // parts of the keys
+  float* part;              // splits > 1: [split][batch * heads][queries][DP]
   int do_b, do_h;
   int* status;
 };
 
-// A CTA's units, and within one its blocks of keys
+// A CTA's units, and within one its blocks of keys.  SPLIT: its part of them (a kernel of its own: with both in one, the
+// unsplit pass of 74,344 x 50 keys x 16 heads took 509 us instead of 437)
+template <bool SPLIT>
 struct DqWalk {
   uint32_t unit;
-  int b, h, row0, count, j, j1;
+  int b, h, row0, split, count, j, j0, j1;
   __device__ __forceinline__ void open(const DqParams& p, uint32_t u) {
     unit = u;
     if (u >= p.units) return;
-    const uint32_t bh = u / p.tiles;
+    const uint32_t rest = u / p.tiles;
+    uint32_t bh = rest;
+    split = 0;
+    if (SPLIT) {
+      bh = rest / p.splits;
+      split = static_cast<int>(rest - bh * p.splits);
+    }
     b = static_cast<int>(bh / static_cast<uint32_t>(p.s.heads));
     h = static_cast<int>(bh - b * static_cast<uint32_t>(p.s.heads));
-    row0 = static_cast<int>(u - bh * p.tiles) * kDqRows;
+    row0 = static_cast<int>(u - rest * p.tiles) * kDqRows;
     count = key_count(p.s, b);
-    j = 0;
     j1 = (count + kDqKeys - 1) / kDqKeys;
+    if (SPLIT) {
+      const int64_t nb = j1;
+      j0 = static_cast<int>(nb * split / p.splits);
+      j1 = static_cast<int>(nb * (split + 1) / p.splits);
+    }
+    j = from();
   }
+  // the part that leaves the rows' statistics: the last, which has a block wherever the entry has a key
+  __device__ __forceinline__ bool leaves_stat(const DqParams& p) const { return !SPLIT || split == p.splits - 1; }
+  __device__ __forceinline__ int from() const { return SPLIT ? j0 : 0; }
   __device__ __forceinline__ bool done(const DqParams& p) const { return unit >= p.units; }
   // the first unit from u on that has a block
   __device__ __forceinline__ void open_live(const DqParams& p, uint32_t u) {
@@ -105,7 +124,7 @@ struct DqWalk {
   }
 };
 
-template <int DP, bool BF, int KIND>
+template <int DP, bool BF, int KIND, bool SPLIT>
 __global__ void __launch_bounds__(kDqThreads, 1)
     cross_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                     const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -145,7 +164,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
-  DqWalk w{};
+  DqWalk<SPLIT> w{};
 
   if (warp == 8) {
     // ------------------------------------------------------------------ TMA: ring slots K, V, K, V, ...
@@ -194,7 +213,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
     const uint32_t id_q = idesc16<BF>(128, DP, false, true);
     const uint64_t dq = desc_k(smem_u32(smem + SM::kQ)), ddo = desc_k(smem_u32(smem + SM::kDo));
     const uint64_t ring_k = desc_k(smem_u32(smem + SM::kKV)), ring_n = desc_mn(smem_u32(smem + SM::kKV), SM::kChunk);
-    DqWalk a;                             // the step whose S and dP are next
+    DqWalk<SPLIT> a;                           // the step whose S and dP are next
     a.open_live(p, blockIdx.x);
     int ahead = 0, units = 0;
     // excluded keys may hold anything: their rows of K (0 * NaN in dS K) and V become zeros
@@ -216,7 +235,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       }
     };
     auto scores = [&]() -> bool {         // S of a's step
-      if (a.j == 0 && !mbar_wait_warp(&bars->q_full, units & 1, status, abort_flag)) return false;
+      if (a.j == a.from() && !mbar_wait_warp(&bars->q_full, units & 1, status, abort_flag)) return false;
       const int s = slot(2 * ahead);
       if (s < 0) return false;
       product(tmem + kDqColS + 128 * (ahead & 1), dq, s);
@@ -225,7 +244,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       return true;
     };
     auto gradients = [&]() -> bool {      // dP of the same step, which it ends
-      if (a.j == 0 && !mbar_wait_warp(&bars->do_full, units & 1, status, abort_flag)) return false;
+      if (a.j == a.from() && !mbar_wait_warp(&bars->do_full, units & 1, status, abort_flag)) return false;
       const int s = slot(2 * ahead + 1);
       if (s < 0) return false;
       product(tmem + kDqColP, ddo, s);
@@ -294,7 +313,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
     ask();
     while (ok && !w.done(p)) {
       const int row = w.row0 + r;
-      const bool valid = row < p.s.queries, live = w.j1 > 0;
+      const bool valid = row < p.s.queries, live = w.from() < w.j1;
       const int64_t bh = static_cast<int64_t>(w.b) * p.s.heads + w.h;
       const int64_t mask_at = w.b * p.s.mask.sb + w.h * p.s.mask.sh;
       const int64_t row_mask = mask_at + (valid ? row : 0) * p.s.mask.sn;
@@ -309,7 +328,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       }
       if (lse == -INFINITY) lse = INFINITY;
       if (!NAT) lse *= kCrossLog2e;
-      for (int j = 0; j < w.j1; ++j, ++n) {
+      for (int j = w.from(); j < w.j1; ++j, ++n) {
         const int first = j * kDqKeys + key0, left = w.count - first;      // this thread's keys of the block
         uint32_t bits[2] = {0u, 0u};
         float* bj = bias + (n & 1) * kDqKeys + key0;
@@ -348,7 +367,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
         }
         // this half's columns of out, asked for before the unit's first weights are formed
         uint4 o[DP / 16];
-        if (j == 0) {
+        if (j == w.from()) {
           const uint16_t* src = out_row();
 #pragma unroll
           for (int c = 0; c < DP / 16; ++c) {
@@ -398,7 +417,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
             e[16 * c + i / 2] = make_float2(cross_ex2(x.x), cross_ex2(x.y));
           }
         }
-        if (j == 0) {
+        if (j == w.from()) {
           // delta: each half of the row's columns, then both
           ok = mbar_wait_warp(&bars->do_full, units & 1, status, abort_flag);
           if (!ok) break;
@@ -419,7 +438,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           named_bar_sync(3, 256);
           delta = delta_s[r] + delta_s[kDqRows + r] - dlse;
           if (lse == INFINITY) delta = 0.f;
-          if (half == 0) {
+          if (half == 0 && w.leaves_stat(p)) {
             float* stat = p.stat + (bh * p.stat_rows + row / 64 * 64) * 3 + row % 64;
             stat[0] = -lse;
             stat[64] = ties;
@@ -450,13 +469,18 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       }
       if (!ok) break;
       if (!live) {
-        // no keys at all: zeros
+        // no keys at all, or none for this part: zeros
         if (half == 0) {
-          float* stat = p.stat + (bh * p.stat_rows + row / 64 * 64) * 3 + row % 64;
-          stat[0] = -lse;
-          stat[64] = ties;
-          stat[128] = 0.f;
-          if (valid) {
+          if (w.leaves_stat(p)) {
+            float* stat = p.stat + (bh * p.stat_rows + row / 64 * 64) * 3 + row % 64;
+            stat[0] = -lse;
+            stat[64] = ties;
+            stat[128] = 0.f;
+          }
+          if (SPLIT && valid) {
+            float* dst = p.part + ((w.split * p.s.batch * p.s.heads + bh) * p.s.queries + row) * DP;
+            for (int c = 0; c < DP; c += 4) *reinterpret_cast<float4*>(dst + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+          } else if (valid) {
             uint16_t* dst = p.dq + w.b * p.dq_stride[0] + row * p.dq_stride[1] + w.h * p.dq_stride[2];
             for (int c = 0; c < p.s.dim; c += 8) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0, 0, 0, 0);
           }
@@ -467,12 +491,31 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       }
       uint16_t* const dst0 = p.dq + w.b * p.dq_stride[0] + static_cast<int64_t>(w.row0 + quarter * 32) * p.dq_stride[1] +
                              w.h * p.dq_stride[2] + half * (DP / 2);
+      float* const part = SPLIT ? p.part + ((w.split * p.s.batch * p.s.heads + bh) * p.s.queries + row) * DP + half * (DP / 2) : nullptr;
       const int rows = static_cast<int>(p.s.queries) - (w.row0 + quarter * 32);
       w.open(p, w.unit + gridDim.x);
       ask();
       ok = mbar_wait_warp(&bars->dq_full, units & 1, status, abort_flag);
       if (!ok) break;
       tc_fence_after();
+      if constexpr (SPLIT) {
+#pragma unroll 1
+        for (int c = 0; c < DP / 64; ++c) {
+          uint32_t a[32];
+          tmem_ld32(tmem + lanes + kDqColQ + half * (DP / 2) + 32 * c, a);
+          tmem_ld_wait();
+          if (valid) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(part + 32 * c + i) =
+                  make_float4(__uint_as_float(a[i]) * p.s.scale, __uint_as_float(a[i + 1]) * p.s.scale,
+                              __uint_as_float(a[i + 2]) * p.s.scale, __uint_as_float(a[i + 3]) * p.s.scale);
+          }
+        }
+        tc_fence_before();
+        ++units;
+        continue;
+      }
       constexpr int PIECES = DP / 16;
       uint32_t x[PIECES][4];
 #pragma unroll
@@ -873,17 +916,17 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
   if (warp == 9) tmem_dealloc(tmem, kDkvCols);
 }
 
-struct DkvSumParams {
-  const float* partial;
-  uint16_t *dk, *dv;
-  int64_t dk_stride[3], dv_stride[3];
-  int64_t keys, rows;               // rows = batch * kv_heads * keys
-  int kv_heads, dim, splits;
+struct GradSumParams {
+  const float* partial;             // [tensor][split][batch * heads][tokens][DP]
+  uint16_t* out[2];
+  int64_t stride[2][3];
+  int64_t tokens, rows;             // rows = batch * heads * tokens
+  int heads, dim, splits;
 };
 
-// the splits' partial sums added in order; 8 elements per thread, blockIdx.y: dK, dV
+// the splits' partial sums added in order; 8 elements per thread, blockIdx.y: the tensor (dQ; dK, dV)
 template <int DP, bool BF>
-__global__ void __launch_bounds__(256) cross_dkv_sum_kernel(const __grid_constant__ DkvSumParams p) {
+__global__ void __launch_bounds__(256) cross_grad_sum_kernel(const __grid_constant__ GradSumParams p) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t row = i / (DP / 8);
   const int e = static_cast<int>(i % (DP / 8)) * 8;
@@ -895,11 +938,43 @@ __global__ void __launch_bounds__(256) cross_dkv_sum_kernel(const __grid_constan
     a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
     c.x += y.x; c.y += y.y; c.z += y.z; c.w += y.w;
   }
-  const int64_t key = row % p.keys, bk = row / p.keys, hk = bk % p.kv_heads, b = bk / p.kv_heads;
-  const int64_t* st = blockIdx.y ? p.dv_stride : p.dk_stride;
-  uint16_t* dst = (blockIdx.y ? p.dv : p.dk) + b * st[0] + key * st[1] + hk * st[2] + e;
+  const int64_t token = row % p.tokens, bh = row / p.tokens, h = bh % p.heads, b = bh / p.heads;
+  const int64_t* st = p.stride[blockIdx.y];
+  uint16_t* dst = p.out[blockIdx.y] + b * st[0] + token * st[1] + h * st[2] + e;
   *reinterpret_cast<uint4*>(dst) = make_uint4(pack16x2<BF>(a.x, a.y), pack16x2<BF>(a.z, a.w), pack16x2<BF>(c.x, c.y),
                                               pack16x2<BF>(c.z, c.w));
+}
+
+template <int DP, bool BF>
+int launch_sum(GradSumParams r, const float* partial, int tensors, int64_t batch, int heads, int64_t tokens, int dim, int splits,
+               cudaStream_t st) {
+  r.partial = partial;
+  r.tokens = tokens;
+  r.rows = batch * heads * tokens;
+  r.heads = heads;
+  r.dim = dim;
+  r.splits = splits;
+  const int64_t blocks = (r.rows * (DP / 8) + 255) / 256;
+  cross_grad_sum_kernel<DP, BF><<<dim3(static_cast<unsigned>(blocks), tensors), 256, 0, st>>>(r);
+  return cudaGetLastError() == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
+}
+
+// Parts of the keys in the dQ pass: the fewest rounds of CTAs times blocks (about 1.7 us each), with three blocks' time
+// for a unit's ends and, for any split, three for the sum's launch and the time the parts' bytes take at 5 TB/s.
+int dq_splits(const HtrcCrossArgs* a) {
+  const int64_t units = a->batch * a->heads * ((a->queries + kDqRows - 1) / kDqRows);
+  const int64_t steps = (a->keys + kDqKeys - 1) / kDqKeys, sms = sm_count();
+  const double part_steps = static_cast<double>(a->batch) * a->heads * a->queries * (a->dim <= 64 ? 64 : 128) * 8 / 5e12 / 1.7e-6;
+  int best = 1;
+  double cost = 1e300;
+  for (int s = 1; s <= 64 && s <= std::max<int64_t>(steps, 1); ++s) {
+    const double c = static_cast<double>((units * s + sms - 1) / sms) * ((steps + s - 1) / s + 3) + (s > 1 ? 3 + s * part_steps : 0);
+    if (c < cost) {
+      cost = c;
+      best = s;
+    }
+  }
+  return best;
 }
 
 // Query-range splits of the dK / dV pass: the fewest rounds of CTAs times steps, each CTA's prologue and epilogue
@@ -943,13 +1018,16 @@ bool ready(K kernel, uint32_t bytes, bool (&done)[64]) {
 
 template <int DP, bool BF, int KIND>
 int launch_bwd(const HtrcCrossArgs* a, cudaStream_t st) {
-  static bool done_q[64] = {}, done_kv[64] = {};
-  auto kq = cross_dq_kernel<DP, BF, KIND>;
+  static bool done_q[64] = {}, done_qs[64] = {}, done_kv[64] = {};
+  auto kq = cross_dq_kernel<DP, BF, KIND, false>;
+  auto kqs = cross_dq_kernel<DP, BF, KIND, true>;
   auto kkv = cross_dkv_kernel<DP, BF, KIND>;
-  if (!ready(kq, DqSmem<DP>::kBytes, done_q) || !ready(kkv, DkvSmem<DP>::kBytes, done_kv)) return HTRC_ERR_CUDA;
+  if (!ready(kq, DqSmem<DP>::kBytes, done_q) || !ready(kqs, DqSmem<DP>::kBytes, done_qs) || !ready(kkv, DkvSmem<DP>::kBytes, done_kv)) return HTRC_ERR_CUDA;
   const CrossShape s = cross_shape(a);
   float* stat = static_cast<float*>(a->workspace);
   const CrossBits bits{reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a->workspace) + stat_bytes(a)), bit_words(a), a->mask_stride[1] != 0};
+  // the two passes' partial sums, one after the other
+  float* partial = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + stat_bytes(a) + bits_bytes(a));
   const bool keys = a->keys > 0, rows = a->queries > 0;
   // an empty side's maps are never read: the other side's rows stand in
   const void *k = keys ? a->k : a->q, *v = keys ? a->v : a->q, *q = rows ? a->q : a->k, *o = rows ? a->dout : a->k;
@@ -977,12 +1055,21 @@ int launch_bwd(const HtrcCrossArgs* a, cudaStream_t st) {
     p.stat_rows = stat_rows(a);
     p.bits = bits;
     p.tiles = static_cast<uint32_t>(stat_rows(a) / kDqRows);
-    p.units = static_cast<uint32_t>(p.tiles * a->batch * a->heads);
+    p.splits = dq_splits(a);
+    p.part = partial;
+    p.units = static_cast<uint32_t>(p.tiles * a->batch * a->heads * p.splits);
     p.do_b = do_b;
     p.do_h = do_h;
     p.status = a->status;
-    kq<<<std::min<uint32_t>(p.units, static_cast<uint32_t>(sm_count())), kDqThreads, DqSmem<DP>::kBytes, st>>>(mq, mo, mk, mv, p);
+    (p.splits > 1 ? kqs : kq)<<<std::min<uint32_t>(p.units, static_cast<uint32_t>(sm_count())), kDqThreads, DqSmem<DP>::kBytes, st>>>(mq, mo, mk, mv, p);
     if (cudaGetLastError() != cudaSuccess) return HTRC_ERR_CUDA;
+    if (p.splits > 1) {
+      GradSumParams r{};
+      r.out[0] = p.dq;
+      for (int i = 0; i < 3; ++i) r.stride[0][i] = a->dq_stride[i];
+      const int rc = launch_sum<DP, BF>(r, partial, 1, a->batch, a->heads, a->queries, a->dim, p.splits, st);
+      if (rc != HTRC_OK) return rc;
+    }
   }
   if (!keys) return HTRC_OK;
   CUtensorMap mq, mo, mk, mv, mdk, mdv;
@@ -998,28 +1085,20 @@ int launch_bwd(const HtrcCrossArgs* a, cudaStream_t st) {
   p.key_blocks = static_cast<int>((a->keys + kDkvKeys - 1) / kDkvKeys);
   p.row_blocks = static_cast<int>((a->queries + kDkvRows - 1) / kDkvRows);
   p.splits = dkv_splits(a);
-  p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + stat_bytes(a) + bits_bytes(a));
+  p.partial = partial;
   p.status = a->status;
   const int64_t grid = a->batch * a->kv_heads * p.splits * p.key_blocks;
   kkv<<<static_cast<unsigned>(grid), kDkvThreads, DkvSmem<DP>::kBytes, st>>>(mq, mo, mk, mv, mdk, mdv, p, do_b, do_h);
   if (cudaGetLastError() != cudaSuccess) return HTRC_ERR_CUDA;
   if (p.splits > 1) {
-    DkvSumParams r{};
-    r.partial = p.partial;
-    r.dk = static_cast<uint16_t*>(a->dk);
-    r.dv = static_cast<uint16_t*>(a->dv);
+    GradSumParams r{};
+    r.out[0] = static_cast<uint16_t*>(a->dk);
+    r.out[1] = static_cast<uint16_t*>(a->dv);
     for (int i = 0; i < 3; ++i) {
-      r.dk_stride[i] = a->dk_stride[i];
-      r.dv_stride[i] = a->dv_stride[i];
+      r.stride[0][i] = a->dk_stride[i];
+      r.stride[1][i] = a->dv_stride[i];
     }
-    r.keys = a->keys;
-    r.rows = a->batch * a->kv_heads * a->keys;
-    r.kv_heads = a->kv_heads;
-    r.dim = a->dim;
-    r.splits = p.splits;
-    const int64_t blocks = (r.rows * (DP / 8) + 255) / 256;
-    cross_dkv_sum_kernel<DP, BF><<<dim3(static_cast<unsigned>(blocks), 2), 256, 0, st>>>(r);
-    if (cudaGetLastError() != cudaSuccess) return HTRC_ERR_CUDA;
+    return launch_sum<DP, BF>(r, p.partial, 2, a->batch, a->kv_heads, a->keys, a->dim, p.splits, st);
   }
   return HTRC_OK;
 }
@@ -1040,10 +1119,12 @@ int cross_sizes(const HtrcCrossArgs* a, size_t* bytes) {
   // the grids, and the workspace as a whole
   const int64_t limit = (int64_t(1) << 31) - 1;
   const int64_t tiles = stat_rows(a) / kDqRows, blocks = (a->keys + kDkvKeys - 1) / kDkvKeys;
-  if (tiles * a->batch * a->heads > limit || blocks > limit / (16 * std::max<int64_t>(1, a->batch * a->kv_heads)))
+  if (tiles * a->batch * a->heads > limit || tiles * a->batch * a->heads * dq_splits(a) > limit || blocks > limit / (16 * std::max<int64_t>(1, a->batch * a->kv_heads)))
     return HTRC_ERR_UNSUPPORTED;
-  const int dp = a->dim <= 64 ? 64 : 128, splits = dkv_splits(a);
-  *bytes = stat_bytes(a) + bits_bytes(a) + (splits > 1 ? static_cast<size_t>(2) * splits * a->batch * a->kv_heads * a->keys * dp * 4 : 0);
+  const int dp = a->dim <= 64 ? 64 : 128, sq = dq_splits(a), sk = dkv_splits(a);
+  const size_t of_dq = sq > 1 ? static_cast<size_t>(sq) * a->batch * a->heads * a->queries : 0;
+  const size_t of_dkv = sk > 1 ? static_cast<size_t>(2) * sk * a->batch * a->kv_heads * a->keys : 0;
+  *bytes = stat_bytes(a) + bits_bytes(a) + std::max(of_dq, of_dkv) * dp * 4;
   return HTRC_OK;
 }
 

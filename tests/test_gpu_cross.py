@@ -146,6 +146,7 @@ def test_sizes_match_float64(dev, dtype, size):
 # more units than SMs (each CTA walks several), keys split over CTAs, more entries than one pass of the lengths' sums
 MANY = [(40, 300, 150, 6, 3, 64), (7, 700, 390, 16, 16, 128), (230, 1, 70, 4, 2, 64), (260, 3, 130, 2, 1, 128),
         (300, 5, 90, 4, 4, 64), (100, 2, 200, 24, 12, 64), (30, 24, 150, 6, 6, 128), (20, 9, 333, 24, 8, 128),
+        (3, 32, 4243, 1, 1, 72), (2, 200, 1500, 4, 2, 128), (1, 300, 400, 2, 2, 64),
         (2, 40, 9000, 2, 1, 64), (1, 130, 12000, 1, 1, 128), (2, 1, 30000, 4, 1, 128), (5, 4, 2000, 24, 8, 64)]
 
 
@@ -340,7 +341,8 @@ def test_no_batch_dimension_and_order(dev):
     assert all(torch.equal(x, y) for x, y in zip(torch.autograd.grad(out, (q, k, v), do), ga))
 
 
-@pytest.mark.parametrize("size", [(2, 500, 300, 4, 2, 128), (3, 1, 3000, 4, 2, 128), (1, 3000, 200, 2, 2, 64)])
+@pytest.mark.parametrize("size", [(2, 500, 300, 4, 2, 128), (3, 1, 3000, 4, 2, 128), (1, 3000, 200, 2, 2, 64),
+                                  (2, 40, 5000, 2, 1, 128)])
 def test_one_result_whatever_the_stream_or_the_run(dev, size):
     import htrc_b200
     q, k, v = _rows(dev, *size, torch.bfloat16)

@@ -307,25 +307,46 @@ __global__ void __launch_bounds__(kXThreads, 1)
         if ((KIND == CROSS_PAIRS || KIND == CROSS_BIAS) && valid && left > kXKeys)      // the next block's terms of this row
           prefetch_mask(p.s.mask, mask_at + row * p.s.mask.sn + static_cast<int64_t>((j + 1) * kXKeys) * p.s.mask.sm);
         if (KIND == CROSS_PAIRS) {
-          // the warp's 32 rows of mask bits: a row's 128 keys by coalesced loads, eight rows in flight, and ballots
-          const int rows = min(32, static_cast<int>(p.s.queries) - (row0 + quarter * 32));
+          // the warp's 32 rows of mask bits: a lane's four keys of each row, by one load where all rows are aligned
+          // to it, else a byte each, and ballots: bit k of word q is key 4 k + q.  (5 x 52 queries x 260 keys x 6 heads: 15.6
+          // us, consecutive bytes 22.1; 2 x 29,540 x 1,151 x 2, by bytes: 302 us, 284 with a word of consecutive keys; two
+          // aligned words shifted together: 437)
+          const int rows = min(32, static_cast<int>(p.s.queries) - (row0 + quarter * 32)), mine4 = left - 4 * lane;
+          const uint32_t keep = mine4 >= 4 ? 0xffffffffu : mine4 <= 0 ? 0u : (1u << 8 * mine4) - 1u;
           const uint8_t* mk = static_cast<const uint8_t*>(p.s.mask.p) + mask_at + static_cast<int64_t>(row0 + quarter * 32) * p.s.mask.sn +
-                              static_cast<int64_t>(j * kXKeys + lane) * p.s.mask.sm;
-          for (int g = 0; g < rows; g += 8) {
-            uint8_t v[8][4];
+                              static_cast<int64_t>(j * kXKeys + 4 * lane) * p.s.mask.sm;
+          auto vote = [&](int row, uint32_t v) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t word = __ballot_sync(0xffffffffu, (v >> 8 * q & 0xffu) != 0);
+              if (lane == row) bits[q] = word;
+            }
+          };
+          if (p.s.mask.sm == 1 && !((reinterpret_cast<uintptr_t>(p.s.mask.p) + mask_at) & 3) && !(p.s.mask.sn & 3)) {
+            // (a word with one of the row's keys in it lies in the mask's allocation as a whole)
+            for (int g = 0; g < rows; g += 16) {
+              uint32_t v[16];
 #pragma unroll
-              for (int q = 0; q < 4; ++q)
-                v[i][q] = g + i < rows && 32 * q + lane < left ? __ldg(mk + i * p.s.mask.sn + 32 * q * p.s.mask.sm) : 0;
+              for (int i = 0; i < 16; ++i)
+                v[i] = g + i < rows && keep ? __ldg(reinterpret_cast<const uint32_t*>(mk + i * p.s.mask.sn)) & keep : 0u;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+              for (int i = 0; i < 16; ++i) vote(g + i, v[i]);
+              mk += 16 * p.s.mask.sn;
+            }
+          } else {
+            for (int g = 0; g < rows; g += 8) {
+              uint32_t v[8];
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const uint32_t word = __ballot_sync(0xffffffffu, v[i][q] != 0);
-                if (lane == g + i) bits[q] = word;
+              for (int i = 0; i < 8; ++i) {
+                v[i] = 0;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  if (g + i < rows && q < mine4) v[i] |= static_cast<uint32_t>(__ldg(mk + i * p.s.mask.sn + q * p.s.mask.sm)) << 8 * q;
               }
-            mk += 8 * p.s.mask.sn;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) vote(g + i, v[i]);
+              mk += 8 * p.s.mask.sn;
+            }
           }
         }
         // the block's logits: times scale2 in the exponent for NONE / PAIRS, natural units with a bias
@@ -351,7 +372,7 @@ __global__ void __launch_bounds__(kXThreads, 1)
         } else if (KIND == CROSS_PAIRS) {
 #pragma unroll
           for (int i = 0; i < kXKeys; ++i)
-            if (!(bits[i / 32] >> (i % 32) & 1u)) s[i / 32][i % 32] = __float_as_uint(-INFINITY);
+            if (!(bits[i % 4] >> (i / 4) & 1u)) s[i / 32][i % 32] = __float_as_uint(-INFINITY);
         } else if (KIND == CROSS_KEYS) {
 #pragma unroll
           for (int i = 0; i < kXKeys; ++i) {

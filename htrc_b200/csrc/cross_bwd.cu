@@ -19,6 +19,9 @@
 // Where the key blocks alone do not fill the device evenly, the query range is split and the float32 partial sums are
 // added by cross_grad_sum_kernel in order.
 //
+// Measured: 16,384 queries x 512 keys x 24 heads of 128, bfloat16, 368 us, of which the dQ pass a little over half; the chain
+// S, dP -> threads -> dS -> product bounds both (tensor pipe 39 % and 60 % busy).
+//
 // Rounding: P and dS enter their products in the operands' 16-bit type (a relative 2^-9 for bfloat16, about what the
 // result's own rounding adds; carrying the rest would take a second product each), the gradients are rounded once from
 // float32.

@@ -1,6 +1,6 @@
 // Cross attention of few rows (single tokens): the query rows that share a key head, up to 16 at a time, against that
 // head's keys and values.  The keys and values are read once and nothing else matters: a tcgen05 tile of 128 rows would
-// load the same bytes behind a much longer chain of steps (87 us where this takes 22 for the 65 MB of 16 tokens,
+// load the same bytes behind a much longer chain of steps (87 us where this takes 19 for the 65 MB of 16 tokens,
 // 24 heads on 8 key heads of 1,000 keys on average), so the products run on warp-level m16n8k16 instructions, whose rate
 // is far above what the bytes ask for.
 //

@@ -18,6 +18,10 @@
 // Rounding: P is rounded to the operands' 16-bit type for the second product (a relative 2^-9 for bfloat16, of
 // weights whose errors average out over the row); out is rounded once from float32.
 //
+// Measured, bfloat16, 24 heads of 128: 129,024 queries x 512 keys 807-834 us (1,000 TFLOP/s), 4,096 x 16,384 750-870 us by
+// the clock.  The exponentials' turns bound it: 1,700 clocks for a tile's block, of which the special function units need
+// 1,024 and the products, under the other tile's turn, 1,280.
+//
 // Warps 0-3 and 4-7: softmax of tile A and B, rows 32 w ..; warp 8: TMA; warps 9 and 10: MMA issue of tile A and B, and
 // the zeroing of excluded keys' values.
 #include <algorithm>

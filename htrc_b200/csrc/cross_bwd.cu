@@ -25,6 +25,12 @@
 // Rounding: P and dS enter their products in the operands' 16-bit type (a relative 2^-9 for bfloat16, about what the
 // result's own rounding adds; carrying the rest would take a second product each), the gradients are rounded once from
 // float32.
+//
+// With an added mask lse is no full account of a row's sum: float32 near a mask of -1e9 is spaced 64 apart, so the log of
+// the sum is lost in it (a row of 256 such keys: exp(x - lse) = 1 for each instead of 1 / 256), and from -1e4 on it costs
+// more than the gradients' rounding.  x - lse itself is exact there.  So the first pass adds the row's weights up as lse
+// gives them, divides dQ by the sum, and leaves its log2 for the second pass.  (They are at most 1: lse, the rounding
+// of something no less than the row's maximum, is no less than that either.)
 #include <algorithm>
 #include <cmath>
 
@@ -44,8 +50,6 @@ struct CrossBits {
     return ((static_cast<int64_t>(b) * (heads ? s.heads : 1) + (heads ? h : 0)) * words + word) * rows;
   }
 };
-
-constexpr float kHuge = 1e30f;        // a |log sum| above this is a mask's lowest value: the logits are lost in it
 
 // ------------------------------------------------------------------------------------------------ dQ
 constexpr int kDqThreads = 320;
@@ -76,12 +80,14 @@ struct DqParams {
   int64_t out_stride[3];
   uint16_t* dq;
   int64_t dq_stride[3];
-  float* stat;              // [batch * heads][padded rows / 64][3][64]: minus lse in the pass's units, log2 of tied keys, delta
+  // [batch * heads][padded rows / 64][3][64]: minus lse in the pass's units, log2 of the weights' sum by it, delta
+  float* stat;
   int64_t stat_rows;
   CrossBits bits;
   uint32_t units, tiles;    // tiles of 128 rows per head
   int splits;               // parts of the keys
-  float* part;              // splits > 1: [split][batch * heads][queries][DP]
+  float* part;              // splits > 1: [split][batch * heads][queries][DP], not divided by the weights' sums
+  float* part_sum;          // with an added mask: [split][batch * heads][queries]
   int do_b, do_h;
   int* status;
 };
@@ -320,16 +326,9 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       const int64_t bh = static_cast<int64_t>(w.b) * p.s.heads + w.h;
       const int64_t mask_at = w.b * p.s.mask.sb + w.h * p.s.mask.sh;
       const int64_t row_mask = mask_at + (valid ? row : 0) * p.s.mask.sn;
-      // a row with nothing in it (or none): every weight exp2(-inf)
-      float ties = 0.f, delta = 0.f;
-      if (NAT && fabsf(lse) > kHuge && lse != -INFINITY) {
-        // every logit of the row is a mask's lowest value and the log of their count is lost in lse: count them
-        int same = 0;
-        for (int i = 0; i < w.count; ++i)
-          same += mask_term(p.s.mask.p, p.s.mask.dtype, row_mask + static_cast<int64_t>(i) * p.s.mask.sm) == lse;
-        ties = same > 1 ? log2f(static_cast<float>(same)) : 0.f;
-      }
-      if (lse == -INFINITY) lse = INFINITY;
+      float delta = 0.f;
+      float2 sum = make_float2(0.f, 0.f);
+      if (lse == -INFINITY) lse = INFINITY;     // a row with nothing in it (or none): every weight exp2(-inf)
       if (!NAT) lse *= kCrossLog2e;
       for (int j = w.from(); j < w.j1; ++j, ++n) {
         const int first = j * kDqKeys + key0, left = w.count - first;      // this thread's keys of the block
@@ -414,10 +413,12 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           for (int i = 0; i < 32; i += 2) {
             float2 x = make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
             if (NAT)
-              x = fma2(sub2(x, make_float2(lse, lse)), make_float2(kCrossLog2e, kCrossLog2e), make_float2(-ties, -ties));
+              x = mul2(sub2(x, make_float2(lse, lse)), make_float2(kCrossLog2e, kCrossLog2e));
             else
               x = fma2(x, make_float2(scale2, scale2), make_float2(-lse, -lse));
-            e[16 * c + i / 2] = make_float2(cross_ex2(x.x), cross_ex2(x.y));
+            x = make_float2(cross_ex2(x.x), cross_ex2(x.y));
+            if (NAT) sum = add2(sum, x);
+            e[16 * c + i / 2] = x;
           }
         }
         if (j == w.from()) {
@@ -444,7 +445,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           if (half == 0 && w.leaves_stat(p)) {
             float* stat = p.stat + (bh * p.stat_rows + row / 64 * 64) * 3 + row % 64;
             stat[0] = -lse;
-            stat[64] = ties;
+            if (!NAT || SPLIT) stat[64] = 0.f;
             stat[128] = delta;
           }
         }
@@ -477,12 +478,13 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           if (w.leaves_stat(p)) {
             float* stat = p.stat + (bh * p.stat_rows + row / 64 * 64) * 3 + row % 64;
             stat[0] = -lse;
-            stat[64] = ties;
+            stat[64] = 0.f;
             stat[128] = 0.f;
           }
           if (SPLIT && valid) {
             float* dst = p.part + ((w.split * p.s.batch * p.s.heads + bh) * p.s.queries + row) * DP;
             for (int c = 0; c < DP; c += 4) *reinterpret_cast<float4*>(dst + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (NAT) p.part_sum[(w.split * p.s.batch * p.s.heads + bh) * p.s.queries + row] = 0.f;
           } else if (valid) {
             uint16_t* dst = p.dq + w.b * p.dq_stride[0] + row * p.dq_stride[1] + w.h * p.dq_stride[2];
             for (int c = 0; c < p.s.dim; c += 8) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0, 0, 0, 0);
@@ -496,11 +498,28 @@ __global__ void __launch_bounds__(kDqThreads, 1)
                              w.h * p.dq_stride[2] + half * (DP / 2);
       float* const part = SPLIT ? p.part + ((w.split * p.s.batch * p.s.heads + bh) * p.s.queries + row) * DP + half * (DP / 2) : nullptr;
       const int rows = static_cast<int>(p.s.queries) - (w.row0 + quarter * 32);
+      const int64_t sum_at = SPLIT ? (w.split * p.s.batch * p.s.heads + bh) * p.s.queries + row : 0;
+      float* const stat = p.stat + (bh * p.stat_rows + row / 64 * 64) * 3 + row % 64;
       w.open(p, w.unit + gridDim.x);
       ask();
       ok = mbar_wait_warp(&bars->dq_full, units & 1, status, abort_flag);
       if (!ok) break;
       tc_fence_after();
+      float mul = p.s.scale;
+      if (NAT) {
+        // the weights' sum, of both halves of the row: by way of delta_s, which every thread has read before its last dS
+        delta_s[half * kDqRows + r] = sum.x + sum.y;
+        named_bar_sync(3, 256);
+        const float total = delta_s[r] + delta_s[kDqRows + r];
+        named_bar_sync(3, 256);               // before the next unit's delta is written there
+        if constexpr (SPLIT) {
+          if (half == 0 && valid) p.part_sum[sum_at] = total;
+        } else {
+          // (none: a row with nothing in it, whose dQ is zero)
+          if (half == 0) stat[64] = total == 0.f ? 0.f : log2f(total);
+          if (total != 0.f) mul /= total;
+        }
+      }
       if constexpr (SPLIT) {
 #pragma unroll 1
         for (int c = 0; c < DP / 64; ++c) {
@@ -511,8 +530,8 @@ __global__ void __launch_bounds__(kDqThreads, 1)
 #pragma unroll
             for (int i = 0; i < 32; i += 4)
               *reinterpret_cast<float4*>(part + 32 * c + i) =
-                  make_float4(__uint_as_float(a[i]) * p.s.scale, __uint_as_float(a[i + 1]) * p.s.scale,
-                              __uint_as_float(a[i + 2]) * p.s.scale, __uint_as_float(a[i + 3]) * p.s.scale);
+                  make_float4(__uint_as_float(a[i]) * mul, __uint_as_float(a[i + 1]) * mul, __uint_as_float(a[i + 2]) * mul,
+                              __uint_as_float(a[i + 3]) * mul);
           }
         }
         tc_fence_before();
@@ -530,7 +549,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
         for (int g = 0; g < 4; ++g)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            x[4 * c + g][i] = pack16x2<BF>(__uint_as_float(a[8 * g + 2 * i]) * p.s.scale, __uint_as_float(a[8 * g + 2 * i + 1]) * p.s.scale);
+            x[4 * c + g][i] = pack16x2<BF>(__uint_as_float(a[8 * g + 2 * i]) * mul, __uint_as_float(a[8 * g + 2 * i + 1]) * mul);
       }
       tc_fence_before();
       exchange_pieces<PIECES>(x, lane);
@@ -759,7 +778,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       uint32_t out[2] = {0u, 0u};           // queries this key is excluded from (of a bias: found with its terms)
       if (!mbar_wait_warp(&bars->s_full[wg], (i >> 1) & 1, status, abort_flag)) { ok = false; break; }
       tc_fence_after();
-      // the queries' statistics: [-lse][ties][delta], 64 each
+      // the queries' statistics: [-lse][log2 of the weights' sum by it][delta], 64 each
       const float* st = reinterpret_cast<const float*>(smem + SM::kRing + s * SM::kStage + 2 * SM::kRows);
       const uint32_t buf = tmem + lanes + kDkvColS + wg * kDkvBuf;
       const uint4* words = reinterpret_cast<const uint4*>(smem + SM::kRing + s * SM::kStage + SM::kBits + quarter * kDkvRows * 4);
@@ -784,7 +803,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
           const float4 ls = *reinterpret_cast<const float4*>(st + 32 * c + k);
-          const float4 ti = NAT ? *reinterpret_cast<const float4*>(st + 64 + 32 * c + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 ls2 = NAT ? *reinterpret_cast<const float4*>(st + 64 + 32 * c + k) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int h2 = 0; h2 < 2; ++h2) {
             const float l0 = h2 ? ls.z : ls.x, l1 = h2 ? ls.w : ls.y;
@@ -806,7 +825,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
               }
               e = fma2(e, make_float2(scale, scale), make_float2(b0, b1));
               e = fma2(add2(e, make_float2(l0, l1)), make_float2(kCrossLog2e, kCrossLog2e),
-                       h2 ? make_float2(-ti.z, -ti.w) : make_float2(-ti.x, -ti.y));
+                       h2 ? make_float2(-ls2.z, -ls2.w) : make_float2(-ls2.x, -ls2.y));
               // an excluded key's weight and gradient are zero whatever its row holds
               if (b0 == -INFINITY) {
                 e.x = -INFINITY;
@@ -925,10 +944,14 @@ struct GradSumParams {
   int64_t stride[2][3];
   int64_t tokens, rows;             // rows = batch * heads * tokens
   int heads, dim, splits;
+  // SUMS (dQ with an added mask): the parts' sums of weights, which dQ is divided by, and the statistics their log2 goes to
+  const float* sums;
+  float* stat;
+  int64_t stat_rows;
 };
 
 // the splits' partial sums added in order; 8 elements per thread, blockIdx.y: the tensor (dQ; dK, dV)
-template <int DP, bool BF>
+template <int DP, bool BF, bool SUMS>
 __global__ void __launch_bounds__(256) cross_grad_sum_kernel(const __grid_constant__ GradSumParams p) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t row = i / (DP / 8);
@@ -936,12 +959,20 @@ __global__ void __launch_bounds__(256) cross_grad_sum_kernel(const __grid_consta
   if (row >= p.rows || e >= p.dim) return;
   const float* src = p.partial + (blockIdx.y * p.splits * p.rows + row) * DP + e;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f), c = a;
+  float total = 0.f;
   for (int s = 0; s < p.splits; ++s, src += p.rows * DP) {
+    if (SUMS) total += __ldg(p.sums + s * p.rows + row);
     const float4 x = __ldcs(reinterpret_cast<const float4*>(src)), y = __ldcs(reinterpret_cast<const float4*>(src + 4));
     a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
     c.x += y.x; c.y += y.y; c.z += y.z; c.w += y.w;
   }
   const int64_t token = row % p.tokens, bh = row / p.tokens, h = bh % p.heads, b = bh / p.heads;
+  if (SUMS) {
+    if (e == 0) p.stat[(bh * p.stat_rows + token / 64 * 64) * 3 + 64 + token % 64] = total == 0.f ? 0.f : log2f(total);
+    const float inv = total == 0.f ? 1.f : 1.f / total;
+    a.x *= inv; a.y *= inv; a.z *= inv; a.w *= inv;
+    c.x *= inv; c.y *= inv; c.z *= inv; c.w *= inv;
+  }
   const int64_t* st = p.stride[blockIdx.y];
   uint16_t* dst = p.out[blockIdx.y] + b * st[0] + token * st[1] + h * st[2] + e;
   *reinterpret_cast<uint4*>(dst) = make_uint4(pack16x2<BF>(a.x, a.y), pack16x2<BF>(a.z, a.w), pack16x2<BF>(c.x, c.y),
@@ -958,7 +989,9 @@ int launch_sum(GradSumParams r, const float* partial, int tensors, int64_t batch
   r.dim = dim;
   r.splits = splits;
   const int64_t blocks = (r.rows * (DP / 8) + 255) / 256;
-  cross_grad_sum_kernel<DP, BF><<<dim3(static_cast<unsigned>(blocks), tensors), 256, 0, st>>>(r);
+  const dim3 grid(static_cast<unsigned>(blocks), tensors);
+  if (r.sums != nullptr) cross_grad_sum_kernel<DP, BF, true><<<grid, 256, 0, st>>>(r);
+  else cross_grad_sum_kernel<DP, BF, false><<<grid, 256, 0, st>>>(r);
   return cudaGetLastError() == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
 }
 
@@ -1060,6 +1093,8 @@ int launch_bwd(const HtrcCrossArgs* a, cudaStream_t st) {
     p.tiles = static_cast<uint32_t>(stat_rows(a) / kDqRows);
     p.splits = dq_splits(a);
     p.part = partial;
+    constexpr bool natural = KIND == CROSS_KEYS || KIND == CROSS_BIAS;
+    if (natural && p.splits > 1) p.part_sum = partial + static_cast<int64_t>(p.splits) * a->batch * a->heads * a->queries * DP;
     p.units = static_cast<uint32_t>(p.tiles * a->batch * a->heads * p.splits);
     p.do_b = do_b;
     p.do_h = do_h;
@@ -1070,6 +1105,9 @@ int launch_bwd(const HtrcCrossArgs* a, cudaStream_t st) {
       GradSumParams r{};
       r.out[0] = p.dq;
       for (int i = 0; i < 3; ++i) r.stride[0][i] = a->dq_stride[i];
+      r.sums = p.part_sum;
+      r.stat = stat;
+      r.stat_rows = p.stat_rows;
       const int rc = launch_sum<DP, BF>(r, partial, 1, a->batch, a->heads, a->queries, a->dim, p.splits, st);
       if (rc != HTRC_OK) return rc;
     }
@@ -1127,7 +1165,8 @@ int cross_sizes(const HtrcCrossArgs* a, size_t* bytes) {
   const int dp = a->dim <= 64 ? 64 : 128, sq = dq_splits(a), sk = dkv_splits(a);
   const size_t of_dq = sq > 1 ? static_cast<size_t>(sq) * a->batch * a->heads * a->queries : 0;
   const size_t of_dkv = sk > 1 ? static_cast<size_t>(2) * sk * a->batch * a->kv_heads * a->keys : 0;
-  *bytes = stat_bytes(a) + bits_bytes(a) + std::max(of_dq, of_dkv) * dp * 4;
+  // (a part's row of dQ: its elements and its sum of weights)
+  *bytes = stat_bytes(a) + bits_bytes(a) + std::max(of_dq * (dp + 1), of_dkv * dp) * 4;
   return HTRC_OK;
 }
 

@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <limits>
 
 #include "../../include/htrc_layer.h"
 #include "common.cuh"
@@ -698,7 +699,10 @@ int rotary_run(const HtrcRotaryArgs* a, cudaStream_t st) {
   p.batch = a->batch;
   p.tokens = a->tokens;
   p.dim = a->dim;
-  p.eps = a->eps;
+  // The backward's warps are filled up with rows of zeros, which must add nothing to the weight's gradient: with eps = 0
+  // their rsqrt(0) would make 0 * inf of it.  The smallest float instead, which changes no mean square that is a normal
+  // number, costs nothing; leaving such rows out by a select in the loop took 237.6 us for 232.6 (32,768 tokens x 24 heads).
+  p.eps = BACK ? std::max(a->eps, std::numeric_limits<float>::denorm_min()) : a->eps;
   p.positions = a->positions;
   p.float_positions = a->position_dtype == HTRC_LAYER_F32;
   for (int i = 0; i < 3; ++i) p.ps[i] = a->position_stride[i];

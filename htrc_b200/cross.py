@@ -28,7 +28,7 @@ _DTYPES = {torch.bfloat16: _lib.LAYER_BF16, torch.float16: _lib.LAYER_F16}
 _MASKS = {torch.bool: _lib.LAYER_U8, torch.float32: _lib.LAYER_F32, torch.bfloat16: _lib.LAYER_BF16,
           torch.float16: _lib.LAYER_F16}
 _LENGTHS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
-_NO_BACK = (0,) * 19
+_NO_BACK = (0,) * 17
 _status = {}
 
 
@@ -75,7 +75,7 @@ def _mask_strides(mask, want):
 class _Call:
     """The checked arguments of one call: 4-d operands, shapes and the mask."""
     __slots__ = ("q", "k", "v", "heads_first", "lengths", "mask", "squeeze", "lse_shape", "shape_args", "mask_args",
-                 "device", "few_units")
+                 "device")
 
     def __init__(self, q, k, v, key_lengths, mask, scale, heads_first):
         for name, x in (("q", q), ("k", k), ("v", v)):
@@ -123,12 +123,10 @@ class _Call:
             self.mask_args = (mask.data_ptr(), _MASKS[mask.dtype], *_mask_strides(mask, (batch, heads, queries, keys)))
         self.q, self.k, self.v = _rows(q), _rows(k), _rows(v)
         self.lse_shape = (batch, heads, queries)
-        # beyond this many tiles of 256 rows the library never splits their keys (it asks for no workspace then)
-        self.few_units = batch * heads * (queries + 255) < 256 * 1024 or heads // kv_heads * queries <= 32
         self.shape_args = (batch, queries, keys, heads, kv_heads, dim, _DTYPES[q.dtype], scale,
                            0 if key_lengths is None else key_lengths.data_ptr())
 
-    def pack(self, out, lse, back=_NO_BACK):
+    def pack(self, out, lse, back):
         hf, q, k, v = self.heads_first, self.q, self.k, self.v
         return _lib.CROSS_ARGS.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), *_strides(q, hf), *_strides(k, hf), *_strides(v, hf),
@@ -166,11 +164,8 @@ def _forward(c, want_lse):
             return _forward(c, want_lse)
     out = torch.empty_like(c.q, memory_format=torch.contiguous_format)
     lse = c.q.new_empty(c.lse_shape, dtype=torch.float32) if want_lse else None
-    if c.few_units:
-        ws, ptr, need = _workspace(c, "htrc_cross_forward_workspace_size")
-        args = c.pack(out, lse, (*_NO_BACK[:17], ptr, need))
-    else:
-        args = c.pack(out, lse)
+    ws, ptr, need = _workspace(c, "htrc_cross_forward_workspace_size")
+    args = c.pack(out, lse, (*_NO_BACK, ptr, need))
     rc = lib().htrc_cross_forward(args, _lib.raw_stream(c.device.index))
     if rc:
         check(rc, "htrc_cross_forward")

@@ -14,6 +14,10 @@
 // tile's values are used, its values while its scores are formed; 192 KB per SM) and waits on no other.  S = Q K^T has the
 // layout of the second product's left operand, so P stays in registers; running maximum and sum in float32; P enters P V
 // in the operands' 16-bit type as on the larger path.  Every sum has a fixed order.
+//
+// With a key mask per query head a unit has one head's rows: a key that this head excludes and another one sees may hold
+// anything (0 * NaN in P V), and its values become zeros only where no row of the unit sees it.  (Three heads to a key
+// head then read it three times: 16 tokens x 24 heads on 8 key heads of 2,000 keys 70 us, 36 with one mask for all.)
 #include <algorithm>
 
 #include "cross.cuh"
@@ -65,6 +69,7 @@ struct CrossFewParams {
   float* lse;
   int64_t qs[3], ks[3], vs[3], os[3];
   int chunks;               // of 16 rows of (head in the group, query)
+  int span;                 // rows of a head: its queries, or whole chunks of them
   bool line;                // the warps share the line of all units' tiles (else a warp has a unit)
   int64_t units;
   // line: the entries' starts (in tiles of one key head and chunk) [batch + 1], then each segment's rows
@@ -76,15 +81,15 @@ struct CrossFewParams {
 // Segment of unit u in warp i: segments in order step i, u or both, so the sum numbers them
 __device__ __forceinline__ int64_t few_slot(int64_t u, int64_t i) { return u + i; }
 
-// a row's place: index = head in the group * queries + query
+// a row's place: index = head in the group * span + query; n and h mean something where it is live
 struct FewRow {
   int n, h;
   bool live;
   __device__ __forceinline__ FewRow(const CrossFewParams& p, int unit, int r) {
     const int queries = static_cast<int>(p.s.queries), at = unit % p.chunks * kFewRows + r;
-    live = at < p.s.group * queries;
-    const int g = live ? at / queries : 0;
-    n = live ? at - g * queries : 0;
+    const int g = at / p.span;
+    n = at - g * p.span;
+    live = g < p.s.group && n < queries;
     h = unit / p.chunks % p.s.kv_heads * p.s.group + g;
   }
 };
@@ -474,15 +479,22 @@ int launch_few_main(const CrossFewParams& p, int ctas, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
 }
 
+struct FewPlan {
+  int64_t units;
+  int rows, span, chunks, ctas;   // rows: of a unit, at most
+  bool line;
+  size_t starts, ml, bytes;       // workspace: where the segments' parts begin, and its size
+};
+
 template <int DP, bool BF>
-int launch_few(const CrossFewParams& p, int64_t units, int ctas, cudaStream_t st) {
-  const bool wide = p.s.group * p.s.queries > 8;
-  const int rc = p.s.mask.p ? (wide ? launch_few_main<DP, BF, true, true>(p, ctas, st) : launch_few_main<DP, BF, true, false>(p, ctas, st))
-                            : (wide ? launch_few_main<DP, BF, false, true>(p, ctas, st) : launch_few_main<DP, BF, false, false>(p, ctas, st));
+int launch_few(const CrossFewParams& p, const FewPlan& f, cudaStream_t st) {
+  const bool wide = f.rows > 8;
+  const int rc = p.s.mask.p ? (wide ? launch_few_main<DP, BF, true, true>(p, f.ctas, st) : launch_few_main<DP, BF, true, false>(p, f.ctas, st))
+                            : (wide ? launch_few_main<DP, BF, false, true>(p, f.ctas, st) : launch_few_main<DP, BF, false, false>(p, f.ctas, st));
   if (rc != HTRC_OK) return rc;
   if (!p.line) return HTRC_OK;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(units), static_cast<unsigned>(std::min<int64_t>(kFewRows, p.s.group * p.s.queries)));
+  cfg.gridDim = dim3(static_cast<unsigned>(f.units), static_cast<unsigned>(f.rows));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
@@ -490,20 +502,16 @@ int launch_few(const CrossFewParams& p, int64_t units, int ctas, cudaStream_t st
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, cross_few_join_kernel<DP, BF>, p, static_cast<int64_t>(ctas) * kFewWarps) == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, cross_few_join_kernel<DP, BF>, p, static_cast<int64_t>(f.ctas) * kFewWarps) == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
 }
-
-struct FewPlan {
-  int64_t units;
-  int chunks, ctas;
-  bool line;
-  size_t starts, ml, bytes;       // workspace: where the segments' parts begin, and its size
-};
 
 FewPlan few_plan(const HtrcCrossArgs* a) {
   FewPlan f{};
-  const int64_t rows = a->heads / a->kv_heads * a->queries, tiles = (a->keys + 31) / 32;
-  f.chunks = static_cast<int>((rows + kFewRows - 1) / kFewRows);
+  const int64_t group = a->heads / a->kv_heads, tiles = (a->keys + 31) / 32;
+  const bool apart = group > 1 && cross_mask_kind(a) == CROSS_KEYS && a->mask_stride[1] != 0;      // a key mask per head
+  f.span = static_cast<int>(apart ? (a->queries + kFewRows - 1) / kFewRows * kFewRows : a->queries);
+  f.rows = static_cast<int>(std::min<int64_t>(kFewRows, apart ? a->queries : group * a->queries));
+  f.chunks = static_cast<int>((group * f.span + kFewRows - 1) / kFewRows);
   f.units = a->batch * a->kv_heads * f.chunks;
   // The line evens out the entries' lengths for the price of the segments' rows and the join.  Ragged entries, 8 key heads
   // of up to 1,000 keys: 512 units of 3 rows 36.5 us in line and 52.2 apart, of 15 rows 62.7 and 59.1; 1,024 units of 3
@@ -541,6 +549,7 @@ int cross_forward_few(const HtrcCrossArgs* a, cudaStream_t st) {
     p.os[i] = a->out_stride[i];
   }
   p.chunks = f.chunks;
+  p.span = f.span;
   p.line = f.line;
   p.units = f.units;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
@@ -550,8 +559,8 @@ int cross_forward_few(const HtrcCrossArgs* a, cudaStream_t st) {
     p.part = reinterpret_cast<float*>(ws + f.ml);
   }
   const bool bf = a->dtype == HTRC_LAYER_BF16;
-  if (a->dim <= 64) return bf ? launch_few<64, true>(p, f.units, f.ctas, st) : launch_few<64, false>(p, f.units, f.ctas, st);
-  return bf ? launch_few<128, true>(p, f.units, f.ctas, st) : launch_few<128, false>(p, f.units, f.ctas, st);
+  if (a->dim <= 64) return bf ? launch_few<64, true>(p, f, st) : launch_few<64, false>(p, f, st);
+  return bf ? launch_few<128, true>(p, f, st) : launch_few<128, false>(p, f, st);
 }
 
 }  // namespace htrc

@@ -11,7 +11,8 @@ exclude are never computed with, whatever their rows hold; a mask with one expec
 
 q, k, v: bfloat16 or float16, dim a multiple of 8 up to 128, any strides that keep rows 16-byte aligned (others are
 copied).  Logits, softmax and sums are float32; the softmax weights enter the second product in the operands' type.
-The functions take part in autograd; the backward can also be called by itself.  There is no CPU path.
+The functions take part in autograd (first derivatives, reverse mode); the backward can also be called by itself.  There is
+no CPU path.
 """
 from __future__ import annotations
 
@@ -22,6 +23,7 @@ import math
 import torch
 
 from . import _lib
+from ._autograd import first_order, recorded
 from ._lib import check, lib
 
 _DTYPES = {torch.bfloat16: _lib.LAYER_BF16, torch.float16: _lib.LAYER_F16}
@@ -221,14 +223,14 @@ class _Cross(torch.autograd.Function):
             return (None,) * 7
         dout = torch.zeros_like(out) if dout is None else dout
         grads = _backward(_Call(q, k, v, key_lengths, mask, *ctx.more), dout, out, lse, dlse)
-        return (*grads, None, None, None, None)
+        return (*first_order("cross_attention", grads, (q, k, v, dout, dlse)), None, None, None, None)
 
 
 def cross_attention(q, k, v, *, key_lengths=None, mask=None, scale=None, heads_first=False, return_lse=False):
     """q [batch, queries, heads, dim], k / v [batch, keys, kv_heads, dim] (heads_first: heads before tokens; batch may
     be left out) -> out in q's shape, type and order, and with return_lse the float32 log-sum-exp of the logits
     [batch, heads, queries].  scale: of the logits, 1 / sqrt(dim) by default; a mask gets no gradient."""
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if recorded(q, k, v):
         out, lse = _Cross.apply(q, k, v, key_lengths, mask, scale, heads_first)
     else:
         out, lse = _forward(_Call(q, k, v, key_lengths, mask, scale, heads_first), return_lse)

@@ -11,8 +11,8 @@ of an axis of width ``w`` turns by ``position * theta ** (-2 i / w)`` (or ``posi
 as it is.  With a weight, the row is first normalised: ``x * rsqrt(mean(x ** 2) + eps) * weight``.
 
 Inputs are float32, bfloat16 or float16 with any strides but a unit last one (slices of a joint projection are read in
-place); arithmetic is float32, rounded once to the input's type.  The functions take part in autograd; the backward
-passes can also be called by themselves.  There is no CPU path.
+place); arithmetic is float32, rounded once to the input's type.  The functions take part in autograd (first derivatives, reverse
+mode); the backward passes can also be called by themselves.  There is no CPU path.
 """
 from __future__ import annotations
 
@@ -23,6 +23,7 @@ import math
 import torch
 
 from . import _lib
+from ._autograd import first_order, recorded
 from ._lib import check, lib
 
 _DTYPES = {torch.float32: _lib.LAYER_F32, torch.bfloat16: _lib.LAYER_BF16, torch.float16: _lib.LAYER_F16}
@@ -236,14 +237,12 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, *grads):
         positions, *args = ctx.saved_tensors
         dx, dw = _backward(ctx.spec, grads, args[:ctx.count], args[ctx.count:], positions)
-        return (None, None, None, *dx, *dw)
+        return (None, None, None, *first_order("rotary_axes", (*dx, *dw), (*args, *grads)))
 
 
 def _apply(spec, tensors, weights, positions):
-    if torch.is_grad_enabled():
-        for t in (*tensors, *weights):
-            if t is not None and t.requires_grad:
-                return _Rotary.apply(spec, positions, len(tensors), *tensors, *weights)
+    if recorded(*tensors, *weights):
+        return _Rotary.apply(spec, positions, len(tensors), *tensors, *weights)
     return tuple(_forward(spec, tensors, weights, positions))
 
 

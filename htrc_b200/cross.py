@@ -114,8 +114,8 @@ class _Call:
                     key_lengths.dtype not in _LENGTHS or key_lengths.device != dev:
                 raise ValueError("key_lengths: [batch] integers on q's device expected")
             if key_lengths.dtype is not torch.int32 or not key_lengths.is_contiguous():
-                # more keys than there are is all of them, whatever the wider type held
-                key_lengths = key_lengths.clamp(0, keys).to(torch.int32).contiguous()
+                # more keys than there are is all of them, whatever a wider type held (a narrower one may not hold `keys`)
+                key_lengths = key_lengths.long().clamp(0, keys).to(torch.int32).contiguous()
         self.lengths = key_lengths
         self.mask = mask
         self.mask_args = (0, 0, 0, 0, 0, 0)

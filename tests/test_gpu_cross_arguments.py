@@ -1,0 +1,27 @@
+"""Arguments that cross attention takes in every form its documentation names."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return torch.device("cuda:0")
+
+
+@pytest.mark.parametrize("dtype,keys", [(torch.uint8, 300), (torch.int8, 200), (torch.int16, 33000), (torch.int64, 300)])
+def test_lengths_of_narrow_types(dev, dtype, keys):
+    """A type that cannot hold the number of keys still says how many of them an entry has."""
+    import htrc_b200
+    gen = torch.Generator(device=dev).manual_seed(3)
+    q = torch.randn((4, 3, 2, 64), generator=gen, device=dev).bfloat16()
+    k, v = (torch.randn((4, keys, 2, 64), generator=gen, device=dev).bfloat16() for _ in range(2))
+    lengths = torch.tensor([100, 0, 127, 7], device=dev)
+    want = htrc_b200.cross_attention(q, k, v, key_lengths=lengths.int(), return_lse=True)
+    got = htrc_b200.cross_attention(q, k, v, key_lengths=lengths.to(dtype), return_lse=True)
+    assert all(torch.equal(x, y) for x, y in zip(want, got))

@@ -45,7 +45,9 @@ def _status_word(device):
 def cross_status(device=None):
     """Raise if a cross-attention kernel on the device reported a failed guard since the last check (synchronises)."""
     from .flat import device_status
-    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    dev = torch.device("cuda" if device is None else device)
+    if dev.index is None:                 # the words are kept by index
+        dev = torch.device(dev.type, torch.cuda.current_device())
     with torch.cuda.device(dev):
         return device_status(_status_word(dev))
 

@@ -25,3 +25,15 @@ def test_lengths_of_narrow_types(dev, dtype, keys):
     want = htrc_b200.cross_attention(q, k, v, key_lengths=lengths.int(), return_lse=True)
     got = htrc_b200.cross_attention(q, k, v, key_lengths=lengths.to(dtype), return_lse=True)
     assert all(torch.equal(x, y) for x, y in zip(want, got))
+
+
+@pytest.mark.parametrize("name", ["cuda", "cuda:0", 0, None])
+def test_status_of_a_device_by_any_name(dev, name):
+    """A bit in the device's status word is reported, and cleared, whatever the device is called."""
+    import htrc_b200
+    from htrc_b200 import _lib, cross
+    htrc_b200.cross_status(dev)
+    cross._status_word(dev)[0] = 1
+    with pytest.raises(_lib.HtrcError, match="bounded wait"):
+        htrc_b200.cross_status(name)
+    htrc_b200.cross_status(dev)

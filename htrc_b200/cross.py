@@ -35,15 +35,19 @@ _status = {}
 
 
 def _status_word(device):
-    """The device word that the kernels' guards write (one per device, zeroed when it is made)."""
+    """The device word that the kernels' guards write (one per device, zeroed before any stream sees it).  None while a
+    graph is captured before the first call: its zero fill would become part of the graph."""
     w = _status.get(device)
-    if w is None:
-        w = _status[device] = torch.zeros(64, dtype=torch.int32, device=device)
+    if w is None and not torch.cuda.is_current_stream_capturing():
+        w = torch.zeros(64, dtype=torch.int32, device=device)
+        torch.cuda.current_stream(device).synchronize()
+        _status[device] = w
     return w
 
 
 def cross_status(device=None):
-    """Raise if a cross-attention kernel on the device reported a failed guard since the last check (synchronises)."""
+    """Raise if a cross-attention kernel on the device reported a failed guard since the last check (synchronises).  The
+    calls of a graph report where the device had a call before the capture."""
     from .flat import device_status
     dev = torch.device("cuda" if device is None else device)
     if dev.index is None:                 # the words are kept by index
@@ -132,10 +136,11 @@ class _Call:
 
     def pack(self, out, lse, back):
         hf, q, k, v = self.heads_first, self.q, self.k, self.v
+        status = _status_word(self.device)
         return _lib.CROSS_ARGS.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), *_strides(q, hf), *_strides(k, hf), *_strides(v, hf),
             out.data_ptr(), *_strides(out, hf), 0 if lse is None else lse.data_ptr(), *self.shape_args, *self.mask_args,
-            _status_word(self.device).data_ptr(), *back)
+            0 if status is None else status.data_ptr(), *back)
 
 
 @functools.lru_cache(maxsize=256)

@@ -37,3 +37,49 @@ def test_status_of_a_device_by_any_name(dev, name):
     with pytest.raises(_lib.HtrcError, match="bounded wait"):
         htrc_b200.cross_status(name)
     htrc_b200.cross_status(dev)
+
+
+def _operands(dev):
+    gen = torch.Generator(device=dev).manual_seed(4)
+    return [torch.randn((2, 40, 2, 64), generator=gen, device=dev).bfloat16() for _ in range(3)]
+
+
+def test_status_word_is_zeroed_before_any_stream_sees_it(dev):
+    """The word is made by the first call; a bit that another stream sets right after it is not lost under the zero fill."""
+    import htrc_b200
+    from htrc_b200 import _lib, cross
+    args = _operands(dev)
+    htrc_b200.cross_attention(*args)
+    torch.cuda.synchronize()
+    cross._status.clear()
+    busy, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(busy):
+        torch.cuda._sleep(50_000_000)               # some 30 ms before anything else of this stream runs
+        htrc_b200.cross_attention(*args)
+    with torch.cuda.stream(other):
+        cross._status_word(dev)[0] = 1
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.HtrcError, match="bounded wait"):
+        htrc_b200.cross_status(dev)
+    htrc_b200.cross_status(dev)
+
+
+def test_first_call_in_a_graph(dev):
+    """A capture does not make the word: no replay then clears what other calls reported."""
+    import htrc_b200
+    from htrc_b200 import _lib, cross
+    args = _operands(dev)
+    want = htrc_b200.cross_attention(*args)
+    torch.cuda.synchronize()
+    cross._status.clear()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = htrc_b200.cross_attention(*args)
+    htrc_b200.cross_status(dev)
+    cross._status_word(dev)[0] = 1
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(want, got)
+    with pytest.raises(_lib.HtrcError, match="bounded wait"):
+        htrc_b200.cross_status(dev)
+    htrc_b200.cross_status(dev)

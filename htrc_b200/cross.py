@@ -62,7 +62,11 @@ def _rows(x):
     if s3 == 1 and s1 > 0 and s2 > 0 and not (s0 | s1 | s2) & 7 and not x.data_ptr() & 15:
         return x
     x = x.contiguous()
-    return x if not x.data_ptr() & 15 else x.clone()
+    if x.data_ptr() & 15:
+        x = x.clone()
+    # a dense tensor may still hold any stride for a dimension of one
+    _, n1, n2, n3 = x.shape
+    return x.as_strided(x.shape, (n1 * n2 * n3, n2 * n3, n3, 1))
 
 
 def _strides(x, heads_first):

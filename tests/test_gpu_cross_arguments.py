@@ -83,3 +83,23 @@ def test_first_call_in_a_graph(dev):
     with pytest.raises(_lib.HtrcError, match="bounded wait"):
         htrc_b200.cross_status(dev)
     htrc_b200.cross_status(dev)
+
+
+def test_odd_strides_of_single_rows(dev):
+    """A dimension of one is never stepped along: its stride may be anything (a token cut from a wider buffer)."""
+    import htrc_b200
+    gen = torch.Generator(device=dev).manual_seed(5)
+    wide = torch.randn((4, 1, 1, 1, 67), generator=gen, device=dev).bfloat16()
+    q, k, v, do = (x[..., :64] for x in wide.unbind())
+    assert q.stride(1) % 8 and q.is_contiguous()
+    for heads_first in (False, True):
+        out, lse = htrc_b200.cross_attention(q, k, v, heads_first=heads_first, return_lse=True)
+        assert torch.equal(out, v) and (lse.double() - (q.double() * k.double()).sum() * 0.125).abs().max() < 1e-5
+        dq, dk, dv = htrc_b200.cross_attention_backward(do, q, k, v, out, lse, heads_first=heads_first)
+        assert torch.equal(dv, do) and dq.abs().max() < 1e-2 and dk.abs().max() < 1e-2
+    x = torch.randn((1, 9 * 64 + 1), generator=gen, device=dev).bfloat16()[:, :9 * 64]
+    rows = x.as_strided((1, 9, 1, 64), (9 * 64 + 1, 64, 3, 1))          # one entry, one head, by any stride
+    dense = x.reshape(1, 9, 1, 64).clone()
+    for a, b in zip(htrc_b200.cross_attention(rows, rows, rows, return_lse=True),
+                    htrc_b200.cross_attention(dense, dense, dense, return_lse=True)):
+        assert torch.equal(a, b)

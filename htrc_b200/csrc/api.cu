@@ -56,12 +56,12 @@ DeviceInfo device_info() {
   return cache[dev];
 }
 
-// rank-2..5 tiled map; dims innermost first, strides in bytes for dims 1..rank-1
+// rank-2..4 tiled map; dims innermost first, strides in bytes for dims 1..rank-1
 bool make_map(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
               const uint64_t* strides, const uint32_t* box, bool swizzle128) {
-  if (!encoder() || base == nullptr || rank < 2 || rank > 5) return false;
-  cuuint64_t gd[5], gs[4];
-  cuuint32_t bx[5], es[5] = {1, 1, 1, 1, 1};
+  if (!encoder() || base == nullptr || rank < 2 || rank > 4) return false;
+  cuuint64_t gd[4], gs[3];
+  cuuint32_t bx[4], es[4] = {1, 1, 1, 1};
   for (int i = 0; i < rank; ++i) {
     gd[i] = dims[i];
     bx[i] = box[i];

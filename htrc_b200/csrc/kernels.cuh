@@ -9,7 +9,7 @@ namespace htrc {
 // the current device, and the tensor-map encoder, for the C entries outside api.cu (defined there)
 bool device_is_b200();
 int sm_count();
-// rank-2..5 tiled map; dims innermost first, strides in bytes for dims 1..rank-1
+// rank-2..4 tiled map; dims innermost first, strides in bytes for dims 1..rank-1
 bool make_tiled_map(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
                     const uint64_t* strides, const uint32_t* box, bool swizzle128);
 

@@ -31,6 +31,14 @@
 // more than the gradients' rounding.  x - lse itself is exact there.  So the first pass adds the row's weights up as lse
 // gives them, divides dQ by the sum, and leaves its log2 for the second pass.  (They are at most 1: lse, the rounding
 // of something no less than the row's maximum, is no less than that either.)
+//
+// float16 has no room below: with an upstream gradient of 1e-5 dS would be among its subnormals, and so are the weights of
+// many keys.  There P enters its product times 2^12 and dS times 2^t, both taken out of the float32 results.  t goes by
+// |dS| <= 2 max|dP| + max|dlse| <= 2 dim max|dO| max|v| + max|dlse|, of a tile of rows in the first pass and of all rows
+// that share a key head in the second: 2^t times that stays below 2^15, half of what float16 holds.  It only ever
+// enlarges.  cross_vmax_kernel finds max|v| ahead; the first pass has dO at hand.  (4,096 x 512 x 2 heads of 128, upstream
+// 1e-5: dK's relative error 0.0017, the rounding of the result itself, in place of 0.0157.  16,384 x 512 x 24 heads 425 ->
+// 440 us, 3 x 777 x 130 x 12 heads 42.9 -> 44.7.)
 #include <algorithm>
 #include <cmath>
 
@@ -51,6 +59,67 @@ struct CrossBits {
   }
 };
 
+// ------------------------------------------------------------------------------------------------ float16's room
+constexpr int kVmaxParts = 32;        // CTAs per entry and key head, at most
+template <bool BF>
+__host__ __device__ constexpr float p_room() { return BF ? 0.f : 12.f; }     // P enters its product times 2^this
+__device__ __forceinline__ float two_to(int t) { return __int_as_float((127 + t) << 23); }
+// t for a bound on |dS|: bound < 2^(e + 1)
+__device__ __forceinline__ int room(float bound) {
+  const int e = static_cast<int>(__float_as_uint(bound) >> 23) - 127;
+  return max(0, min(40, 14 - e));
+}
+// two float16 magnitudes of each word, those that are not finite as 0 (they make the results they reach not finite
+// whatever t is)
+__device__ __forceinline__ uint32_t magnitudes(uint32_t x) {
+  x &= 0x7fff7fffu;
+  return x & ~__vcmpgeu2(x, 0x7c007c00u);
+}
+__device__ __forceinline__ uint32_t most(uint32_t to, const uint4& x) {
+  return __vmaxu2(__vmaxu2(to, __vmaxu2(magnitudes(x.x), magnitudes(x.y))), __vmaxu2(magnitudes(x.z), magnitudes(x.w)));
+}
+// the larger of two float16 magnitudes, as the bits of a float32 (which compare as they do)
+__device__ __forceinline__ uint32_t wide(uint32_t x) {
+  return __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(max(x & 0xffffu, x >> 16)))));
+}
+
+struct VmaxParams {
+  CrossShape s;
+  const uint16_t* v;
+  int64_t vs[3];
+  uint32_t* vmax;             // [batch * kv_heads][parts], float32 bits
+  int parts;
+};
+
+// max|v| of the keys that a query may see; 8 or 16 lanes per row
+template <int DP, bool KEYED>
+__global__ void __launch_bounds__(256) cross_vmax_kernel(const __grid_constant__ VmaxParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");          // the dQ pass waits for this kernel's end itself
+  constexpr int LPR = DP / 8, RPC = 256 / LPR;
+  __shared__ uint32_t part[8];
+  const int bk = blockIdx.x / p.parts, first = (blockIdx.x - bk * p.parts) * RPC + threadIdx.x / LPR, step = p.parts * RPC;
+  const int b = bk / p.s.kv_heads, hk = bk - b * p.s.kv_heads, e = threadIdx.x % LPR * 8;
+  const int count = key_count(p.s, b);
+  const uint16_t* src = p.v + b * p.vs[0] + hk * p.vs[2] + e;
+  uint32_t m = 0;
+#pragma unroll 4
+  for (int64_t key = first; key < count; key += step) {
+    const uint4 x = e < p.s.dim ? __ldg(reinterpret_cast<const uint4*>(src + key * p.vs[1])) : make_uint4(0, 0, 0, 0);
+    bool seen = !KEYED;
+    if (KEYED)
+      for (int g = 0; g < (p.s.mask.sh != 0 ? p.s.group : 1) && !seen; ++g)
+        seen = mask_term(p.s.mask.p, p.s.mask.dtype, b * p.s.mask.sb + (hk * p.s.group + g) * p.s.mask.sh + key * p.s.mask.sm) != -INFINITY;
+    if (seen) m = most(m, x);
+  }
+  m = __reduce_max_sync(0xffffffffu, wide(m));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) m = max(m, part[w]);
+    p.vmax[blockIdx.x] = m;
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ dQ
 constexpr int kDqThreads = 320;
 constexpr int kDqRows = 128, kDqKeys = 128;
@@ -68,7 +137,7 @@ struct DqSmem {
   static constexpr int kChunks = DP / 64, kSlots = 5;
   static constexpr uint32_t kChunk = 128 * 128, kTile = kChunks * kChunk;
   static constexpr uint32_t kQ = 0, kDo = kTile, kKV = 2 * kTile, kBias = kKV + kSlots * kTile;
-  static constexpr uint32_t kDelta = kBias + 2 * kDqKeys * 4, kBars = kDelta + 2 * kDqRows * 4, kBytes = kBars + 192;
+  static constexpr uint32_t kDelta = kBias + 2 * kDqKeys * 4, kMax = kDelta + 2 * kDqRows * 4, kBars = kMax + 64, kBytes = kBars + 192;
   static_assert(sizeof(DqBars) <= 192 && kBytes <= 232448, "shared memory of one CTA");
 };
 
@@ -80,10 +149,14 @@ struct DqParams {
   int64_t out_stride[3];
   uint16_t* dq;
   int64_t dq_stride[3];
-  // [batch * heads][padded rows / 64][3][64]: minus lse in the pass's units, log2 of the weights' sum by it, delta
+  // [batch * heads][padded rows / 64][3][64]: minus lse in the pass's units, log2 of the weights' sum by it, delta.  (p_room
+  // is in the second with an added mask, else in the first)
   float* stat;
   int64_t stat_rows;
   CrossBits bits;
+  const uint32_t* vmax;     // float16: [batch * kv_heads][vmax_parts]
+  float* bounds;            // float16, left for the second pass: the bound on |dS| of each tile [batch * heads][tiles]
+  int vmax_parts;
   uint32_t units, tiles;    // tiles of 128 rows per head
   int splits;               // parts of the keys
   float* part;              // splits > 1: [split][batch * heads][queries][DP], not divided by the weights' sums
@@ -299,14 +372,20 @@ __global__ void __launch_bounds__(kDqThreads, 1)
     constexpr bool NAT = KIND == CROSS_KEYS || KIND == CROSS_BIAS;
     float* bias = reinterpret_cast<float*>(smem + SM::kBias);
     float* delta_s = reinterpret_cast<float*>(smem + SM::kDelta);
+    uint2* max_s = reinterpret_cast<uint2*>(smem + SM::kMax);
     bool ok = true;
     int n = 0, units = 0;
-    // the row's lse and its gradient: loaded a unit ahead, as this half's columns of out into L2
+    // the row's lse and its gradient: loaded a unit ahead, as this half's columns of out into L2 (float16: and vmax's parts,
+    // once the first unit with a block has waited for cross_vmax_kernel)
     float lse, dlse;
+    uint32_t vmax = 0;
+    auto ask_vmax = [&]() {
+      if (lane < p.vmax_parts) vmax = p.vmax[(static_cast<int64_t>(w.b) * p.s.kv_heads + w.h / p.s.group) * p.vmax_parts + lane];
+    };
     auto out_row = [&]() {
       return p.out + w.b * p.out_stride[0] + static_cast<int64_t>(w.row0 + r) * p.out_stride[1] + w.h * p.out_stride[2] + half * (DP / 2);
     };
-    auto ask = [&]() {
+    auto ask = [&](bool waited) {
       const int row = w.row0 + r;
       const bool valid = !w.done(p) && row < p.s.queries;
       const int64_t at = (static_cast<int64_t>(w.b) * p.s.heads + w.h) * p.s.queries + row;
@@ -317,16 +396,17 @@ __global__ void __launch_bounds__(kDqThreads, 1)
         if (p.dlse != nullptr) dlse = __ldg(p.dlse + at);
         if (half * (DP / 2) < p.s.dim) asm volatile("prefetch.global.L2 [%0];" ::"l"(out_row()));
       }
+      if (!BF && waited && !w.done(p)) ask_vmax();
     };
     w.open(p, blockIdx.x);
-    ask();
+    ask(false);
     while (ok && !w.done(p)) {
       const int row = w.row0 + r;
       const bool valid = row < p.s.queries, live = w.from() < w.j1;
       const int64_t bh = static_cast<int64_t>(w.b) * p.s.heads + w.h;
       const int64_t mask_at = w.b * p.s.mask.sb + w.h * p.s.mask.sh;
       const int64_t row_mask = mask_at + (valid ? row : 0) * p.s.mask.sn;
-      float delta = 0.f;
+      float delta = 0.f, shift = 0.f;         // shift: t, once it is known
       float2 sum = make_float2(0.f, 0.f);
       if (lse == -INFINITY) lse = INFINITY;     // a row with nothing in it (or none): every weight exp2(-inf)
       if (!NAT) lse *= kCrossLog2e;
@@ -413,7 +493,8 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           for (int i = 0; i < 32; i += 2) {
             float2 x = make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
             if (NAT)
-              x = mul2(sub2(x, make_float2(lse, lse)), make_float2(kCrossLog2e, kCrossLog2e));
+              x = BF ? mul2(sub2(x, make_float2(lse, lse)), make_float2(kCrossLog2e, kCrossLog2e))
+                     : fma2(sub2(x, make_float2(lse, lse)), make_float2(kCrossLog2e, kCrossLog2e), make_float2(shift, shift));
             else
               x = fma2(x, make_float2(scale2, scale2), make_float2(-lse, -lse));
             x = make_float2(cross_ex2(x.x), cross_ex2(x.y));
@@ -422,10 +503,15 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           }
         }
         if (j == w.from()) {
+          if (!BF && units == 0) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            ask_vmax();
+          }
           // delta: each half of the row's columns, then both
           ok = mbar_wait_warp(&bars->do_full, units & 1, status, abort_flag);
           if (!ok) break;
           float2 acc = make_float2(0.f, 0.f);
+          __half2 top = __float2half2_rn(0.f);
 #pragma unroll
           for (int c = 0; c < DP / 16; ++c) {
             const int piece = half * (DP / 16) + c;
@@ -434,8 +520,21 @@ __global__ void __launch_bounds__(kDqThreads, 1)
             acc = fma2(unpack16x2<BF>(o[c].y), unpack16x2<BF>(y.y), acc);
             acc = fma2(unpack16x2<BF>(o[c].z), unpack16x2<BF>(y.z), acc);
             acc = fma2(unpack16x2<BF>(o[c].w), unpack16x2<BF>(y.w), acc);
+            if (!BF) {
+              // (a gradient that is not finite: NaN is passed over, an infinity makes t 0)
+              const uint32_t words[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) top = __hmax2(top, __habs2(*reinterpret_cast<const __half2*>(&words[i])));
+            }
           }
           delta_s[half * kDqRows + r] = acc.x + acc.y;
+          if (!BF) {
+            // max|dO| and max|dlse| of the warp's rows that see a key
+            const uint32_t z = __float_as_uint(dlse) & 0x7fffffffu;
+            const uint32_t most_do = __reduce_max_sync(0xffffffffu, lse == INFINITY ? 0u : wide(*reinterpret_cast<const uint32_t*>(&top)));
+            const uint32_t most_z = __reduce_max_sync(0xffffffffu, lse == INFINITY || z >= 0x7f800000u ? 0u : z);
+            if (lane == 0) max_s[warp] = make_uint2(most_do, most_z);
+          }
           fence_proxy_async_smem();           // generic reads of rows that TMA refills
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars->do_empty);
@@ -444,9 +543,24 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           if (lse == INFINITY) delta = 0.f;
           if (half == 0 && w.leaves_stat(p)) {
             float* stat = p.stat + (bh * p.stat_rows + row / 64 * 64) * 3 + row % 64;
-            stat[0] = -lse;
-            if (!NAT || SPLIT) stat[64] = 0.f;
+            stat[0] = NAT ? -lse : p_room<BF>() - lse;
+            if (!NAT || SPLIT) stat[64] = NAT ? -p_room<BF>() : 0.f;
             stat[128] = delta;
+          }
+          if (!BF) {
+            uint2 m = max_s[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) m = make_uint2(max(m.x, max_s[i].x), max(m.y, max_s[i].y));
+            const float bound = 2.f * p.s.dim * __uint_as_float(m.x) * __uint_as_float(__reduce_max_sync(0xffffffffu, vmax)) + __uint_as_float(m.y);
+            if (threadIdx.x == 0 && w.leaves_stat(p)) p.bounds[bh * p.tiles + w.row0 / kDqRows] = bound;
+            // the weights of this first block are there already
+            const int t = room(bound);
+            shift = static_cast<float>(t);
+            const float2 up = make_float2(two_to(t), two_to(t));
+#pragma unroll
+            for (int i = 0; i < 32; ++i) e[i] = mul2(e[i], up);
+            sum = mul2(sum, up);
+            if (!NAT) lse -= shift;
           }
         }
         if (!mbar_wait_warp(&bars->dp_full, n & 1, status, abort_flag)) { ok = false; break; }
@@ -491,7 +605,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           }
         }
         w.open(p, w.unit + gridDim.x);
-        ask();
+        ask(units > 0);
         continue;
       }
       uint16_t* const dst0 = p.dq + w.b * p.dq_stride[0] + static_cast<int64_t>(w.row0 + quarter * 32) * p.dq_stride[1] +
@@ -501,11 +615,12 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       const int64_t sum_at = SPLIT ? (w.split * p.s.batch * p.s.heads + bh) * p.s.queries + row : 0;
       float* const stat = p.stat + (bh * p.stat_rows + row / 64 * 64) * 3 + row % 64;
       w.open(p, w.unit + gridDim.x);
-      ask();
+      ask(true);
       ok = mbar_wait_warp(&bars->dq_full, units & 1, status, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      float mul = p.s.scale;
+      const float down = BF ? 1.f : two_to(-static_cast<int>(shift));
+      float mul = p.s.scale * down;
       if (NAT) {
         // the weights' sum, of both halves of the row: by way of delta_s, which every thread has read before its last dS
         delta_s[half * kDqRows + r] = sum.x + sum.y;
@@ -513,11 +628,11 @@ __global__ void __launch_bounds__(kDqThreads, 1)
         const float total = delta_s[r] + delta_s[kDqRows + r];
         named_bar_sync(3, 256);               // before the next unit's delta is written there
         if constexpr (SPLIT) {
-          if (half == 0 && valid) p.part_sum[sum_at] = total;
+          if (half == 0 && valid) p.part_sum[sum_at] = total * down;
         } else {
           // (none: a row with nothing in it, whose dQ is zero)
-          if (half == 0) stat[64] = total == 0.f ? 0.f : log2f(total);
-          if (total != 0.f) mul /= total;
+          if (half == 0) stat[64] = total == 0.f ? 0.f : log2f(total) - shift - p_room<BF>();
+          if (total != 0.f) mul = p.s.scale / total;
         }
       }
       if constexpr (SPLIT) {
@@ -562,6 +677,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       }
       ++units;
     }
+    if (!BF && units == 0) asm volatile("griddepcontrol.wait;" ::: "memory");        // this kernel's end is that one's too
   }
   tc_fence_before();
   __syncthreads();
@@ -598,6 +714,8 @@ struct DkvParams {
   const float* stat;
   int64_t stat_rows;
   CrossBits bits;
+  const float* bounds;      // float16: [batch * heads][tiles]
+  int tiles;
   int key_blocks, splits, row_blocks;
   float* partial;           // splits > 1: [2 (dk, dv)][split][batch * kv_heads][keys][DP]
   int* status;
@@ -752,6 +870,15 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
     constexpr bool NAT = KIND == CROSS_KEYS || KIND == CROSS_BIAS;
     const float scale = NAT ? p.s.scale : p.s.scale * kCrossLog2e;
     const bool in = key < count;
+    int t = 0;
+    if (!BF && steps > 0) {
+      const float* bound = p.bounds + (static_cast<int64_t>(b) * p.s.heads + hk * p.s.group) * p.tiles;
+      uint32_t m = 0;
+#pragma unroll 4
+      for (int64_t i = lane; i < static_cast<int64_t>(p.s.group) * p.tiles; i += 32) m = max(m, __float_as_uint(__ldg(bound + i)));
+      t = room(__uint_as_float(__reduce_max_sync(0xffffffffu, m)));
+    }
+    const float2 up = make_float2(two_to(t - static_cast<int>(p_room<BF>())), two_to(t - static_cast<int>(p_room<BF>())));
     int head = -1;
     float kbias = in ? 0.f : -INFINITY;           // with a bias: this key's term, -inf where it is excluded
     bool ok = true;
@@ -864,7 +991,8 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
               if (out[c] >> kk & 1u) g.x = 0.f;
               if (out[c] >> kk & 2u) g.y = 0.f;
             }
-            const float2 d = mul2(w[16 * c + kk / 2], sub2(g, h2 ? make_float2(de.z, de.w) : make_float2(de.x, de.y)));
+            float2 d = mul2(w[16 * c + kk / 2], sub2(g, h2 ? make_float2(de.z, de.w) : make_float2(de.x, de.y)));
+            if (!BF) d = mul2(d, up);
             dw[kk / 2] = pack16x2<BF>(d.x, d.y);
           }
         }
@@ -880,7 +1008,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       // warpgroup 0 writes dV, 1 dK
       tc_fence_after();
       const uint32_t acc = tmem + lanes + (wg == 0 ? kDkvColV : kDkvColK);
-      const float mul = wg == 0 ? 1.0f : p.s.scale;
+      const float mul = wg == 0 ? two_to(-static_cast<int>(p_room<BF>())) : p.s.scale * two_to(-t);
       uint8_t* stage = smem + (wg == 0 ? SM::kV : SM::kK) + quarter * 32 * 128;
       const int64_t parts = static_cast<int64_t>(p.splits) * p.s.batch * p.s.kv_heads;
       // splits > 1: this warp's 32 keys' rows
@@ -968,7 +1096,7 @@ __global__ void __launch_bounds__(256) cross_grad_sum_kernel(const __grid_consta
   }
   const int64_t token = row % p.tokens, bh = row / p.tokens, h = bh % p.heads, b = bh / p.heads;
   if (SUMS) {
-    if (e == 0) p.stat[(bh * p.stat_rows + token / 64 * 64) * 3 + 64 + token % 64] = total == 0.f ? 0.f : log2f(total);
+    if (e == 0 && total != 0.f) p.stat[(bh * p.stat_rows + token / 64 * 64) * 3 + 64 + token % 64] += log2f(total);    // to -p_room
     const float inv = total == 0.f ? 1.f : 1.f / total;
     a.x *= inv; a.y *= inv; a.z *= inv; a.w *= inv;
     c.x *= inv; c.y *= inv; c.z *= inv; c.w *= inv;
@@ -1042,6 +1170,30 @@ size_t bits_bytes(const HtrcCrossArgs* a) {
   return (static_cast<size_t>(a->batch) * heads * bit_words(a) * stat_rows(a) * 4 + 255) / 256 * 256;
 }
 
+// float16: CTAs per entry and key head that look for max|v|, and the bytes of their finds and the tiles' bounds
+int vmax_parts(const HtrcCrossArgs* a) {
+  const int64_t units = std::max<int64_t>(1, a->batch * a->kv_heads);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kVmaxParts, (4 * sm_count() + units - 1) / units, (a->keys + 63) / 64})));
+}
+size_t vmax_bytes(const HtrcCrossArgs* a) {
+  return a->dtype == HTRC_LAYER_F16 ? (static_cast<size_t>(a->batch) * a->kv_heads * vmax_parts(a) * 4 + 255) / 256 * 256 : 0;
+}
+size_t bounds_bytes(const HtrcCrossArgs* a) {
+  return a->dtype == HTRC_LAYER_F16 ? (static_cast<size_t>(a->batch) * a->heads * (stat_rows(a) / kDqRows) * 4 + 255) / 256 * 256 : 0;
+}
+
+template <int DP, bool KEYED>
+int launch_vmax(const HtrcCrossArgs* a, const CrossShape& s, uint32_t* vmax, cudaStream_t st) {
+  VmaxParams m{};
+  m.s = s;
+  m.v = static_cast<const uint16_t*>(a->v);
+  for (int i = 0; i < 3; ++i) m.vs[i] = a->v_stride[i];
+  m.vmax = vmax;
+  m.parts = vmax_parts(a);
+  cross_vmax_kernel<DP, KEYED><<<static_cast<unsigned>(a->batch * a->kv_heads * m.parts), 256, 0, st>>>(m);
+  return cudaGetLastError() == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
+}
+
 template <typename K>
 bool ready(K kernel, uint32_t bytes, bool (&done)[64]) {
   int dev = 0;
@@ -1062,8 +1214,11 @@ int launch_bwd(const HtrcCrossArgs* a, cudaStream_t st) {
   const CrossShape s = cross_shape(a);
   float* stat = static_cast<float*>(a->workspace);
   const CrossBits bits{reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a->workspace) + stat_bytes(a)), bit_words(a), a->mask_stride[1] != 0};
+  uint8_t* rest = static_cast<uint8_t*>(a->workspace) + stat_bytes(a) + bits_bytes(a);
+  uint32_t* vmax = reinterpret_cast<uint32_t*>(rest);
+  float* bounds = reinterpret_cast<float*>(rest + vmax_bytes(a));
   // the two passes' partial sums, one after the other
-  float* partial = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + stat_bytes(a) + bits_bytes(a));
+  float* partial = reinterpret_cast<float*>(rest + vmax_bytes(a) + bounds_bytes(a));
   const bool keys = a->keys > 0, rows = a->queries > 0;
   // an empty side's maps are never read: the other side's rows stand in
   const void *k = keys ? a->k : a->q, *v = keys ? a->v : a->q, *q = rows ? a->q : a->k, *o = rows ? a->dout : a->k;
@@ -1099,8 +1254,25 @@ int launch_bwd(const HtrcCrossArgs* a, cudaStream_t st) {
     p.do_b = do_b;
     p.do_h = do_h;
     p.status = a->status;
-    (p.splits > 1 ? kqs : kq)<<<std::min<uint32_t>(p.units, static_cast<uint32_t>(sm_count())), kDqThreads, DqSmem<DP>::kBytes, st>>>(mq, mo, mk, mv, p);
-    if (cudaGetLastError() != cudaSuccess) return HTRC_ERR_CUDA;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(std::min<uint32_t>(p.units, static_cast<uint32_t>(sm_count())));
+    cfg.blockDim = dim3(kDqThreads);
+    cfg.dynamicSmemBytes = DqSmem<DP>::kBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    if (!BF) {
+      p.vmax = vmax;
+      p.vmax_parts = vmax_parts(a);
+      p.bounds = bounds;
+      const int rc = launch_vmax<DP, KIND == CROSS_KEYS>(a, s, vmax, st);
+      if (rc != HTRC_OK) return rc;
+      // the launch, the first tiles and the first scores under that kernel, which itself started after all before it
+      attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr.val.programmaticStreamSerializationAllowed = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+    }
+    if (cudaLaunchKernelEx(&cfg, p.splits > 1 ? kqs : kq, mq, mo, mk, mv, p) != cudaSuccess) return HTRC_ERR_CUDA;
     if (p.splits > 1) {
       GradSumParams r{};
       r.out[0] = p.dq;
@@ -1123,6 +1295,8 @@ int launch_bwd(const HtrcCrossArgs* a, cudaStream_t st) {
   p.stat = stat;
   p.stat_rows = stat_rows(a);
   p.bits = bits;
+  p.bounds = bounds;
+  p.tiles = static_cast<int>(stat_rows(a) / kDqRows);
   p.key_blocks = static_cast<int>((a->keys + kDkvKeys - 1) / kDkvKeys);
   p.row_blocks = static_cast<int>((a->queries + kDkvRows - 1) / kDkvRows);
   p.splits = dkv_splits(a);
@@ -1166,7 +1340,7 @@ int cross_sizes(const HtrcCrossArgs* a, size_t* bytes) {
   const size_t of_dq = sq > 1 ? static_cast<size_t>(sq) * a->batch * a->heads * a->queries : 0;
   const size_t of_dkv = sk > 1 ? static_cast<size_t>(2) * sk * a->batch * a->kv_heads * a->keys : 0;
   // (a part's row of dQ: its elements and its sum of weights)
-  *bytes = stat_bytes(a) + bits_bytes(a) + std::max(of_dq * (dp + 1), of_dkv * dp) * 4;
+  *bytes = stat_bytes(a) + bits_bytes(a) + vmax_bytes(a) + bounds_bytes(a) + std::max(of_dq * (dp + 1), of_dkv * dp) * 4;
   return HTRC_OK;
 }
 

@@ -126,9 +126,9 @@ constexpr int kDqRows = 128, kDqKeys = 128;
 constexpr uint32_t kDqColS = 0, kDqColP = 256, kDqColQ = 384, kDqCols = 512;      // S: two buffers
 
 struct DqBars {
-  uint64_t q_full, q_empty, do_full, do_empty, kv_full[5], kv_empty[5], s_full[2], ds_full[2], dp_full, dp_read, dq_full;
+  uint64_t q_full, q_empty, do_full, do_empty, kv_full[5], kv_empty[5], s_full[2], ds_full[2], dp_full, dp_read, dq_full, idle;
   uint32_t tmem_base;
-  int abort_flag;
+  int abort_flag, loads[3];           // of the TMA warp in all: K / V, Q, dO
 };
 
 template <int DP>
@@ -137,8 +137,8 @@ struct DqSmem {
   static constexpr int kChunks = DP / 64, kSlots = 5;
   static constexpr uint32_t kChunk = 128 * 128, kTile = kChunks * kChunk;
   static constexpr uint32_t kQ = 0, kDo = kTile, kKV = 2 * kTile, kBias = kKV + kSlots * kTile;
-  static constexpr uint32_t kDelta = kBias + 2 * kDqKeys * 4, kMax = kDelta + 2 * kDqRows * 4, kBars = kMax + 64, kBytes = kBars + 192;
-  static_assert(sizeof(DqBars) <= 192 && kBytes <= 232448, "shared memory of one CTA");
+  static constexpr uint32_t kDelta = kBias + 2 * kDqKeys * 4, kMax = kDelta + 2 * kDqRows * 4, kBars = kMax + 64, kBytes = kBars + 224;
+  static_assert(sizeof(DqBars) <= 224 && kBytes <= 232448, "shared memory of one CTA");
 };
 
 struct DqParams {
@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->ds_full[i], 256);
     }
+    mbar_init(&bars->idle, 1);
     for (int i = 0; i < SM::kSlots; ++i) {
       mbar_init(&bars->kv_full[i], 1);
       mbar_init(&bars->kv_empty[i], 1);
@@ -238,7 +239,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
     mbar_init(&bars->dp_full, 1);
     mbar_init(&bars->dp_read, 256);
     mbar_init(&bars->dq_full, 1);
-    bars->abort_flag = 0;
+    bars->abort_flag = bars->loads[0] = bars->loads[1] = bars->loads[2] = 0;
     fence_barrier_init();
   }
   if (warp == 9) tmem_alloc(&bars->tmem_base, kDqCols);
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
     // ------------------------------------------------------------------ TMA: ring slots K, V, K, V, ...
     const uint64_t pol_q = policy_evict_first(), pol_kv = policy_evict_last();
     const uint32_t leader = elect_one();
-    int slots = 0, units = 0;
+    int slots = 0, units = 0, q_loads = 0, do_loads = 0;
     auto load = [&](int j, int kv) -> bool {
       const int s = slots % SM::kSlots, hk = w.h / p.s.group;
       if (slots >= SM::kSlots && !mbar_wait_warp(&bars->kv_empty[s], ((slots / SM::kSlots) - 1) & 1, status, abort_flag))
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       return true;
     };
     bool ok = true;
-    auto rows = [&](const CUtensorMap* map, uint32_t at, uint64_t* full, uint64_t* empty, int in_h, int in_b) -> bool {
+    auto rows = [&](const CUtensorMap* map, uint32_t at, uint64_t* full, uint64_t* empty, int in_h, int in_b, int& loads) -> bool {
       if (units > 0 && !mbar_wait_warp(empty, (units - 1) & 1, status, abort_flag)) return false;
       if (leader) {
         mbar_arrive_expect_tx(full, SM::kTile);
@@ -276,11 +277,12 @@ __global__ void __launch_bounds__(kDqThreads, 1)
           tma_load_4d(smem + at + c * SM::kChunk, map, full, 64 * c, w.row0, w.h * in_h, w.b * in_b, pol_q);
       }
       __syncwarp();
+      ++loads;
       return true;
     };
     for (w.open_live(p, blockIdx.x); ok && !w.done(p); w.open_live(p, w.unit + gridDim.x), ++units) {
-      ok = load(w.j, 0) && rows(&tm_q, SM::kQ, &bars->q_full, &bars->q_empty, p.s.q_h, p.s.q_b) &&
-           rows(&tm_do, SM::kDo, &bars->do_full, &bars->do_empty, p.do_h, p.do_b) && load(w.j, 1);
+      ok = load(w.j, 0) && rows(&tm_q, SM::kQ, &bars->q_full, &bars->q_empty, p.s.q_h, p.s.q_b, q_loads) &&
+           rows(&tm_do, SM::kDo, &bars->do_full, &bars->do_empty, p.do_h, p.do_b, do_loads) && load(w.j, 1);
       for (int j = w.j + 1; ok && j < w.j1; ++j) ok = load(j, 0) && load(j, 1);
     }
     if (ok && units > 0) {                // the last releases have landed before the CTA leaves
@@ -288,6 +290,11 @@ __global__ void __launch_bounds__(kDqThreads, 1)
       mbar_wait_warp(&bars->do_empty, (units - 1) & 1, status, abort_flag);
     }
     if (ok) drain_ring<true>(bars->kv_empty, SM::kSlots, slots, status, abort_flag);   // before the CTA leaves
+    if (lane == 0) {
+      bars->loads[0] = slots;
+      bars->loads[1] = q_loads;
+      bars->loads[2] = do_loads;
+    }
   } else if (warp == 9) {
     // ------------------------------------------------------------------ MMA
     const uint32_t leader = elect_one();
@@ -681,6 +688,16 @@ __global__ void __launch_bounds__(kDqThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {
+    if (warp == 8) {
+      settle_loads(bars->kv_full, SM::kSlots, bars->loads[0], status);
+      settle_loads(&bars->q_full, 1, bars->loads[1], status);
+      settle_loads(&bars->do_full, 1, bars->loads[2], status);
+    } else if (warp == 9) {
+      settle_products(&bars->idle, status);
+    }
+    __syncthreads();
+  }
   tc_fence_after();
   if (warp == 9) tmem_dealloc(tmem, kDqCols);
 }
@@ -691,9 +708,9 @@ constexpr int kDkvKeys = 128, kDkvRows = 64, kDkvStages = 4;
 constexpr uint32_t kDkvColK = 0, kDkvColV = 128, kDkvColS = 256, kDkvBuf = 128, kDkvCols = 512;
 
 struct DkvBars {
-  uint64_t kv_full, full[kDkvStages], empty[kDkvStages], s_full[2], dp_full[2], p_full[2], ds_full[2], acc_full;
+  uint64_t kv_full, full[kDkvStages], empty[kDkvStages], s_full[2], dp_full[2], p_full[2], ds_full[2], acc_full, idle;
   uint32_t tmem_base;
-  int abort_flag;
+  int abort_flag, loads;              // of the TMA warp in all: stages
 };
 
 template <int DP>
@@ -757,7 +774,8 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       mbar_init(&bars->ds_full[i], 128);
     }
     mbar_init(&bars->acc_full, 1);
-    bars->abort_flag = 0;
+    mbar_init(&bars->idle, 1);
+    bars->abort_flag = bars->loads = 0;
     fence_barrier_init();
   }
   if (warp == 9) tmem_alloc(&bars->tmem_base, kDkvCols);
@@ -800,6 +818,7 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
       __syncwarp();
     }
     if (i == steps) drain_ring<true>(bars->empty, kDkvStages, steps, status, abort_flag);
+    if (lane == 0) bars->loads = i;
   } else if (warp == 9) {
     // ------------------------------------------------------------------ MMA
     const uint32_t leader = elect_one();
@@ -1062,6 +1081,15 @@ __global__ void __launch_bounds__(kDkvThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {
+    if (warp == 8) {
+      settle_loads(bars->full, kDkvStages, bars->loads, status);
+      settle_loads(&bars->kv_full, 1, steps > 0, status);
+    } else if (warp == 9) {
+      settle_products(&bars->idle, status);
+    }
+    __syncthreads();
+  }
   tc_fence_after();
   if (warp == 9) tmem_dealloc(tmem, kDkvCols);
 }

@@ -48,9 +48,9 @@ struct CrossFwdSmem {
 };
 
 struct CrossBars {
-  uint64_t q_full[2], q_empty[2], kv_full[4], kv_empty[4], s_full[2][2], s_read[2], p_full[2][4], o_full[2], turn[2];
+  uint64_t q_full[2], q_empty[2], kv_full[4], kv_empty[4], s_full[2][2], s_read[2], p_full[2][4], o_full[2], turn[2], idle[2];
   uint32_t tmem_base;
-  int abort_flag;
+  int abort_flag, loads[3];           // of the TMA warp in all: K / V, Q of either tile
 };
 static_assert(sizeof(CrossBars) <= 320, "barriers");
 
@@ -128,12 +128,13 @@ __global__ void __launch_bounds__(kXThreads, 1)
       for (int c = 0; c < 4; ++c) mbar_init(&bars->p_full[t][c], 128);
       mbar_init(&bars->o_full[t], 1);
       mbar_init(&bars->turn[t], 4);
+      mbar_init(&bars->idle[t], 1);
     }
     for (int i = 0; i < SM::kSlots; ++i) {
       mbar_init(&bars->kv_full[i], 1);
       mbar_init(&bars->kv_empty[i], 2);
     }
-    bars->abort_flag = 0;
+    bars->abort_flag = bars->loads[0] = bars->loads[1] = bars->loads[2] = 0;
     fence_barrier_init();
   }
   if (warp == 9) tmem_alloc(&bars->tmem_base, kXCols);
@@ -185,6 +186,11 @@ __global__ void __launch_bounds__(kXThreads, 1)
       drain_ring<true>(bars->kv_empty, SM::kSlots, slots, status, abort_flag);
       for (int t = 0; t < 2; ++t)
         if (units[t] > 0) mbar_wait_warp(&bars->q_empty[t], (units[t] - 1) & 1, status, abort_flag);
+    }
+    if (lane == 0) {
+      bars->loads[0] = slots;
+      bars->loads[1] = units[0];
+      bars->loads[2] = units[1];
     }
   } else if (warp >= 9) {
     // ------------------------------------------------------------------ MMA of tile t
@@ -534,6 +540,16 @@ __global__ void __launch_bounds__(kXThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {
+    if (warp == 8) {
+      settle_loads(bars->kv_full, SM::kSlots, bars->loads[0], status);
+      settle_loads(&bars->q_full[0], 1, bars->loads[1], status);
+      settle_loads(&bars->q_full[1], 1, bars->loads[2], status);
+    } else if (warp >= 9) {
+      settle_products(&bars->idle[warp - 9], status);
+    }
+    __syncthreads();
+  }
   tc_fence_after();
   if (warp == 9) tmem_dealloc(tmem, kXCols);
 }

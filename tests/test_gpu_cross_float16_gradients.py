@@ -113,3 +113,35 @@ def test_excluded_keys_and_empty_rows_do_not_count(dev, kind, bad):
     dirty = (~keep[:, 0, 0, :, None])[:, None].expand(k.shape)
     got = htrc_b200.cross_attention_backward(do, q, k.masked_fill(dirty, bad), v.masked_fill(dirty, bad), out, lse, **kw)
     assert all(torch.equal(x, y) for x, y in zip(want, got))
+
+
+@pytest.mark.parametrize("size", [(2, 500, 300, 4, 2, 128), (1, 23, 3287, 3, 3, 128), (3, 777, 130, 12, 4, 64)])
+def test_one_result_whatever_the_stream_or_the_run(dev, size):
+    """Under a graph, on a side stream and right behind another call that reuses its workspace."""
+    import htrc_b200
+    q, k, v = _rows(dev, *size, F16)
+    gen = torch.Generator(device=dev).manual_seed(9)
+    do = (torch.randn(q.shape, generator=gen, device=dev) * 1e-4).half()
+    mask = torch.randn((size[0], 1, 1, size[2]), generator=gen, device=dev).half()
+    out, lse = htrc_b200.cross_attention(q, k, v, mask=mask, heads_first=True, return_lse=True)
+
+    def grads():
+        return htrc_b200.cross_attention_backward(do, q, k, v, out, lse, mask=mask, heads_first=True)
+
+    first = grads()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = grads()
+    torch.cuda.current_stream().wait_stream(side)
+    htrc_b200.cross_attention_backward(do * 100, q, k, v * 50, out, lse, mask=mask, heads_first=True)
+    third = grads()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        fourth = grads()
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    for other in (second, third, fourth):
+        assert all(torch.equal(x, y) for x, y in zip(first, other))
+    htrc_b200.cross_status()

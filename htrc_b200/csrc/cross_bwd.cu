@@ -19,7 +19,8 @@
 // Where the key blocks alone do not fill the device evenly, the query range is split and the float32 partial sums are
 // added by cross_grad_sum_kernel in order.
 //
-// Measured: 16,384 queries x 512 keys x 24 heads of 128, bfloat16, 368 us, of which the dQ pass a little over half; the chain
+// Measured: 16,384 queries x 512 keys x 24 heads of 128, bfloat16, device time of 20 passes: 376 us after a second's rest, 435
+// once the power cap holds the SM clock (1,635 MHz), of which the dQ pass a little over half; the chain
 // S, dP -> threads -> dS -> product bounds both (tensor pipe 39 % and 60 % busy).
 //
 // Rounding: P and dS enter their products in the operands' 16-bit type (a relative 2^-9 for bfloat16, about what the
@@ -37,8 +38,8 @@
 // |dS| <= 2 max|dP| + max|dlse| <= 2 dim max|dO| max|v| + max|dlse|, of a tile of rows in the first pass and of all rows
 // that share a key head in the second: 2^t times that stays below 2^15, half of what float16 holds.  It only ever
 // enlarges.  cross_vmax_kernel finds max|v| ahead; the first pass has dO at hand.  (4,096 x 512 x 2 heads of 128, upstream
-// 1e-5: dK's relative error 0.0017, the rounding of the result itself, in place of 0.0157.  16,384 x 512 x 24 heads 425 ->
-// 440 us, 3 x 777 x 130 x 12 heads 42.9 -> 44.7.)
+// 1e-5: dK's relative error 0.0017, the rounding of the result itself, in place of 0.0157.  In a row, 16,384 x 512 x 24
+// heads 425 -> 440 us, 3 x 777 x 130 x 12 heads 42.9 -> 44.7.)
 #include <algorithm>
 #include <cmath>
 
@@ -166,7 +167,7 @@ struct DqParams {
 };
 
 // A CTA's units, and within one its blocks of keys.  SPLIT: its part of them (a kernel of its own: with both in one, the
-// unsplit pass of 74,344 x 50 keys x 16 heads took 509 us instead of 437)
+// unsplit pass lost 6 to 16 %)
 template <bool SPLIT>
 struct DqWalk {
   uint32_t unit;

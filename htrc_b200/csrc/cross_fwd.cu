@@ -18,8 +18,9 @@
 // Rounding: P is rounded to the operands' 16-bit type for the second product (a relative 2^-9 for bfloat16, of
 // weights whose errors average out over the row); out is rounded once from float32.
 //
-// Measured, bfloat16, 24 heads of 128: 129,024 queries x 512 keys 807-834 us (1,000 TFLOP/s), 4,096 x 16,384 750-870 us by
-// the clock.  The exponentials' turns bound it: 1,700 clocks for a tile's block, of which the special function units need
+// Measured, bfloat16, 24 heads of 128, device time of 20 passes: 129,024 queries x 512 keys 839 us after a second's rest (968
+// TFLOP/s) and 972 once the power cap holds the SM clock, at 1,605 MHz (836); 4,096 x 16,384 761 and 851 (1,725 MHz).  Times
+// beside variants below are after a rest.  The exponentials' turns bound it: 1,700 clocks for a tile's block, of which the special function units need
 // 1,024 and the products, under the other tile's turn, 1,280.
 //
 // Warps 0-3 and 4-7: softmax of tile A and B, rows 32 w ..; warp 8: TMA; warps 9 and 10: MMA issue of tile A and B, and
@@ -461,8 +462,8 @@ __global__ void __launch_bounds__(kXThreads, 1)
             mbar_arrive(&bars->p_full[t][c]);
           }
         };
-        // without a mask whole blocks have a copy of their own: one copy for these and the ragged last ones spills twice
-        // as much (129,024 queries x 512 keys x 24 heads: 922 us, 834 with two)
+        // without a mask whole blocks have a copy of their own: one copy for these and the ragged last ones spills more
+        // (129,024 queries x 512 keys x 24 heads: 840 us, 837 with two; 4,096 x 16,384: 763 and 758)
         if (KIND == CROSS_NONE && left >= kXKeys)
           weights();
         else

@@ -29,9 +29,9 @@ namespace {
 constexpr int kRotWarps = 8;
 constexpr int kRotMaxPairs = HTRC_ROTARY_MAX_DIM / 2;
 // Row batches that a warp fetches together (one more set is in flight while they are used), and CTAs per SM the
-// registers are held to.  q and k of 129,024 tokens x 24 heads x 128, bfloat16, before the tables were in shared memory:
-// forward 573 us (2, 4), 601 (3, 3), 612 (2, 2), 654 (1, 4); backward of 32,768 tokens 251 us (3, 2), 267 (2, 2), 288
-// (1, 3), 362 (2, 3).
+// registers are held to.  q and k of 129,024 tokens x 24 heads x 128, bfloat16, after a rest: forward 504 us (2, 4), 529
+// (3, 3), 571 (2, 2), 576 (2, 3), 618 (1, 4); backward of 32,768 tokens 233 us (3, 2), 239 (4, 2), 247 (2, 2), 266 (1, 3), 320
+// (2, 3).
 constexpr int rot_unroll(bool back) { return back ? 3 : 2; }
 constexpr int rot_ctas(bool back, int bytes) { return back || bytes == 4 ? 2 : 4; }
 

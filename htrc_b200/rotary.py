@@ -251,7 +251,8 @@ def rotary_axes(x, positions, *, axes, theta=10000.0, pairs="interleaved", weigh
     """x [(batch,) tokens, heads, dim] normalised (with ``weight`` [dim]) and rotated, in x's type and order
     (heads_first: [(batch,) heads, tokens, dim], contiguous).
 
-    positions [(batch,) tokens, len(axes)], integers (any int32 value, its angles exactly reduced) or floats; freqs:
+    positions [(batch,) tokens, len(axes)], integers (any int32 value, its angles exactly reduced) or floats (taken as
+    float32); freqs:
     the ``sum(axes) / 2`` frequencies in radians per position instead of ``theta``'s."""
     return _apply(_spec(axes, theta, pairs, eps, freqs, heads_first), (x,), (weight,), positions)[0]
 

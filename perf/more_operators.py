@@ -176,7 +176,9 @@ def x_type(s):
 def _quantise(x):
     """int8 codes [.., w] and float32 scales [..] of float32 rows."""
     top = x.abs().amax(-1).clamp_min(LEAST)
-    return (x * (127.0 / top)[..., None]).round().to(torch.int8), top / 127.0
+    # one division (a number over a tensor is a reciprocal and a product): elements of half the largest stand on a border
+    by = torch.full_like(top, 127.0) / top
+    return (x * by[..., None]).round().to(torch.int8), top / 127.0
 
 
 def _product(s, codes, scales):

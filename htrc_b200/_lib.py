@@ -56,10 +56,12 @@ TREE_MAX_LEVELS, TREE_MAX_CENTRES, TREE_KMEANS_CENTRES = 16, 256, 32
 TREE_STAGE_ACCEPT, TREE_STAGE_LEAVES, TREE_STAGE_FINAL, TREE_STAGE_ALL = 1, 2, 4, 7
 
 # element types of include/htrc_layer.h
-LAYER_F32, LAYER_BF16, LAYER_F16, LAYER_I32, LAYER_U8 = range(5)
+LAYER_F32, LAYER_BF16, LAYER_F16, LAYER_I32, LAYER_U8, LAYER_I8 = range(6)
+NORM_MAX_WIDTH, LINEAR8_MAX_WIDTH = 16384, 65536
 CROSS_MAX_DIM = 128
 ROTARY_MAX_AXES, ROTARY_MAX_DIM, ROTARY_MAX_HEADS = 4, 256, 1024
 ROTARY_PAIRS = {"interleaved": 0, "half": 1}
+_i64x2 = _i64 * 2
 _i64x3 = _i64 * 3
 _i64x4 = _i64 * 4
 
@@ -90,11 +92,31 @@ class HtrcCrossArgs(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_size_t)]
 
 
+class HtrcNormArgs(ctypes.Structure):
+    """Mirror of include/htrc_layer.h HtrcNormArgs."""
+    _fields_ = [("x", _p), ("x_stride", _i64x2), ("batch", _i64), ("tokens", _i64), ("width", _i32), ("dtype", _i32),
+                ("weight", _p), ("bias", _p), ("scale", _p), ("shift", _p), ("scale_stride", _i64), ("shift_stride", _i64),
+                ("weight_dtype", _i32), ("bias_dtype", _i32), ("scale_dtype", _i32), ("shift_dtype", _i32), ("eps", _f32),
+                ("out", _p), ("out_stride", _i64x2), ("codes", _p), ("codes_pitch", _i64), ("scales", _p), ("mean", _p),
+                ("rstd", _p), ("dy", _p), ("dy_stride", _i64x2), ("dx", _p), ("dx_stride", _i64x2), ("dweight", _p),
+                ("dbias", _p), ("dscale", _p), ("dshift", _p), ("workspace", _p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class HtrcLinear8Args(ctypes.Structure):
+    """Mirror of include/htrc_layer.h HtrcLinear8Args."""
+    _fields_ = [("x", _p), ("x_stride", _i64x2), ("x_scales", _p), ("batch", _i64), ("tokens", _i64), ("width", _i32),
+                ("channels", _i32), ("dtype", _i32), ("w", _p), ("w_pitch", _i64), ("w_scales", _p), ("bias", _p),
+                ("bias_dtype", _i32), ("out_dtype", _i32), ("out", _p), ("status", _p), ("workspace", _p),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
 # The same structs as one native-aligned pack of their fields in order: filling a ctypes structure field by field costs
 # several microseconds of the small calls.
 _ROTARY_TENSOR = "P3qP3qP3qPPii"
 ROTARY_ARGS = struct.Struct("@" + 2 * _ROTARY_TENSOR + "iiqqii4iiPi3qdPfPN0q")
 CROSS_ARGS = struct.Struct("@PPP3q3q3qP3qPqqqiiiifPPi4qPP3qPPPP3q3q3qPN0q")
+NORM_ARGS = struct.Struct("@P2qqqiiPPPPqqiiiifP2qPqPPPP2qP2qPPPPPN0q")
+LINEAR8_ARGS = struct.Struct("@P2qPqqiiiPqPPiiPPPN0q")
 
 
 # name -> (restype, argtypes); every symbol include/htrc_flat.h, include/htrc_tree.h and include/htrc_layer.h
@@ -151,7 +173,7 @@ SIGNATURES = {
     "htrc_tree_centres_scratch_size": (ctypes.c_int, [_i64, ctypes.POINTER(ctypes.c_size_t)]),
     "htrc_tree_centres": (ctypes.c_int, [_p, _i32, _i64, _f32, _p, _p, _p, ctypes.c_size_t, _p]),
     # operators around the flat attention (include/htrc_layer.h)
-    # (their structs are passed as packed bytes, ROTARY_ARGS / CROSS_ARGS, or by reference)
+    # (their structs are passed as packed bytes, ROTARY_ARGS and its like, or by reference)
     "htrc_rotary_forward": (ctypes.c_int, [_p, _p]),
     "htrc_rotary_workspace_size": (ctypes.c_int, [_p, ctypes.POINTER(ctypes.c_size_t)]),
     "htrc_rotary_backward": (ctypes.c_int, [_p, _p]),
@@ -159,6 +181,12 @@ SIGNATURES = {
     "htrc_cross_forward_workspace_size": (ctypes.c_int, [_p, ctypes.POINTER(ctypes.c_size_t)]),
     "htrc_cross_backward_workspace_size": (ctypes.c_int, [_p, ctypes.POINTER(ctypes.c_size_t)]),
     "htrc_cross_backward": (ctypes.c_int, [_p, _p]),
+    "htrc_norm_forward": (ctypes.c_int, [_p, _p]),
+    "htrc_norm_workspace_size": (ctypes.c_int, [_p, ctypes.POINTER(ctypes.c_size_t)]),
+    "htrc_norm_backward": (ctypes.c_int, [_p, _p]),
+    "htrc_quantize_rows": (ctypes.c_int, [_p, _i32, _i64, _i64, _i32, _p, _p, _i64, _p, _p]),
+    "htrc_linear8_workspace_size": (ctypes.c_int, [_p, ctypes.POINTER(ctypes.c_size_t)]),
+    "htrc_linear8_forward": (ctypes.c_int, [_p, _p]),
 }
 
 _lib = None

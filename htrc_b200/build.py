@@ -18,7 +18,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libhtrc_flat.so"
 SOURCES = ["api.cu", "prep.cu", "stats.cu", "rowmax.cu", "route.cu", "tile.cu", "kmeans.cu", "quant.cu", "static_ws.cu", "fp8.cu", "tree.cu",
-           "rotary.cu", "cross_fwd.cu", "cross_few.cu", "cross_bwd.cu"]
+           "rotary.cu", "cross_fwd.cu", "cross_few.cu", "cross_bwd.cu", "norm.cu", "linear8.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -1,0 +1,213 @@
+"""The matrix product in 8-bit integers with a scale for each token and each channel (``csrc/linear8.cu``, tcgen05), as a
+layer's projections use it, and the 8-bit rows that it reads.
+
+    w = quantize_rows(weight)                                 # once: [channels, width] -> codes and a scale per channel
+    y = int8_linear(x, w, bias=bias)                          # rows quantised on the way: [.., width] -> [.., channels]
+    y = int8_linear(layer_norm_int8(x, scale=s, shift=t), w)  # rows that a norm wrote in 8 bits
+
+A row's codes are the integers nearest ``x * (127 / top)``, ties to even, and its scale is ``top / 127``, with ``top`` its
+largest magnitude (at least 1e-30), all in float32; a row with a NaN or an infinity has the scale NaN, and so do its
+products.  The product's sums are exact 32-bit integers; scales and bias are applied in float32 and rounded once.
+
+These functions are for inference: they have no gradients and refuse inputs that record them.  There is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from ._autograd import recorded
+from ._lib import check, lib
+from .cross import _on, _status_word, cross_status
+
+_DTYPES = {torch.float32: _lib.LAYER_F32, torch.bfloat16: _lib.LAYER_BF16, torch.float16: _lib.LAYER_F16}
+
+
+class Int8Rows(NamedTuple):
+    """Rows in 8-bit integers: ``codes`` [.., width] int8 and ``scales`` [..] float32, a row's values codes * scale."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def _check_codes(rows, name):
+    if not (isinstance(rows, tuple) and len(rows) == 2 and all(isinstance(t, torch.Tensor) for t in rows)):
+        raise ValueError(f"{name}: Int8Rows (codes, scales) expected")
+    codes, scales = rows
+    if codes.dtype is not torch.int8 or codes.dim() < 1 or scales.dtype is not torch.float32 or \
+            scales.shape != codes.shape[:-1]:
+        raise ValueError(f"{name}: int8 codes [.., width] and float32 scales [..] expected")
+    if not codes.is_cuda or scales.device != codes.device:
+        raise ValueError(f"{name} must be on one CUDA device (there is no CPU path)")
+    return codes, scales
+
+
+def _pitch(codes):
+    """The even distance between the rows of codes [.., width] as the kernels read them, or None."""
+    shape, stride = codes.shape, codes.stride()
+    if codes.data_ptr() & 15 or (stride[-1] != 1 and shape[-1] != 1):
+        return None
+    pitch = covered = None
+    for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+        if n == 1:
+            continue
+        if pitch is None:
+            pitch = s
+        elif s != covered:
+            return None
+        covered = s * n
+    if pitch is None:
+        return (shape[-1] + 15) // 16 * 16
+    return pitch if pitch >= shape[-1] and not pitch & 15 else None
+
+
+def _new_codes(shape, device):
+    """Codes [.., width] whose rows start at multiples of 16 bytes: (codes, pitch)."""
+    width = shape[-1]
+    pitch = (width + 15) // 16 * 16
+    codes = torch.empty((*shape[:-1], pitch), dtype=torch.int8, device=device)
+    return (codes if pitch == width else codes[..., :width]), pitch
+
+
+def int8_rows(codes, scales):
+    """``Int8Rows`` laid out as the kernels read them (codes whose rows start at even multiples of 16 bytes are taken as
+    they are), so that no product has to."""
+    codes, scales = _check_codes((codes, scales), "rows")
+    if _pitch(codes) is None:
+        laid, _ = _new_codes(codes.shape, codes.device)
+        codes = laid.copy_(codes)
+    return Int8Rows(codes, scales.contiguous())
+
+
+def _two_strides(x):
+    """x [.., width] as (tensor, batch, tokens, width, batch stride, token stride); a copy only where its strides need one."""
+    if x.dim() == 0 or x.shape[-1] < 1:
+        raise ValueError("rows of at least one element expected")
+    if x.stride(-1) != 1 and x.shape[-1] != 1:
+        x = x.contiguous()
+    d = x.dim()
+    if d == 3:
+        (b, n, w), (sb, sn, _) = x.shape, x.stride()
+    elif d == 2:
+        (n, w), (sn, _) = x.shape, x.stride()
+        b, sb = 1, 0
+    elif d == 1:
+        b, n, w, sb, sn = 1, 1, x.shape[0], 0, 0
+    else:
+        x = x.reshape(-1, x.shape[-2], x.shape[-1]) if x.numel() else x.new_empty((0, 1, x.shape[-1]))
+        if x.stride(-1) != 1 and x.shape[-1] != 1:
+            x = x.contiguous()
+        (b, n, w), (sb, sn, _) = x.shape, x.stride()
+    return x, b, n, w, sb, sn
+
+
+def _check_float_rows(x):
+    if not isinstance(x, torch.Tensor) or x.dtype not in _DTYPES or x.dim() < 1:
+        raise ValueError("x: float32, bfloat16 or float16 rows [.., width] expected")
+    if not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor (there is no CPU path)")
+
+
+def _refuse_gradients(what, *tensors):
+    if recorded(*tensors):
+        raise NotImplementedError(f"{what} has no gradients: call it under torch.no_grad() or with detached tensors")
+
+
+def quantize_rows(x):
+    """``Int8Rows`` of float32, bfloat16 or float16 rows x [.., width] (any strides), a scale per row."""
+    _check_float_rows(x)
+    _refuse_gradients("quantize_rows", x)
+    guard = _on(x.device)
+    if guard is not None:
+        with guard:
+            return quantize_rows(x)
+    shape = x.shape
+    kept, b, n, w, sb, sn = _two_strides(x)
+    if w > _lib.NORM_MAX_WIDTH:
+        raise NotImplementedError(f"rows of up to {_lib.NORM_MAX_WIDTH} elements are supported, got {w}")
+    codes, pitch = _new_codes(shape, x.device)
+    scales = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    check(lib().htrc_quantize_rows(kept.data_ptr(), _DTYPES[x.dtype], b, n, w, (ctypes.c_int64 * 2)(sb, sn),
+                                   codes.data_ptr(), pitch, scales.data_ptr(), _lib.raw_stream(x.device.index)),
+          "htrc_quantize_rows")
+    return Int8Rows(codes, scales)
+
+
+def int8_linear_status(device=None):
+    """Raise if a kernel of this library's layer operators on the device reported a failed guard since the last check
+    (synchronises); the same word as ``cross_status``."""
+    return cross_status(device)
+
+
+def int8_linear(x, weight, *, bias=None, dtype=None):
+    """x [.., width], as float rows (quantised on the way) or ``Int8Rows``, times weight (``Int8Rows`` of
+    [channels, width]) -> [.., channels] in ``dtype``: x's by default, bfloat16 for ``Int8Rows``.
+
+    bias: [channels] float32, bfloat16 or float16."""
+    wc, ws = _check_codes(weight, "weight")
+    if wc.dim() != 2 or wc.shape[0] < 1 or wc.shape[1] < 1:
+        raise ValueError("weight: Int8Rows of [channels, width] expected")
+    floats = isinstance(x, torch.Tensor)
+    if floats:
+        _check_float_rows(x)
+        codes, xs = x, None
+        _refuse_gradients("int8_linear", x, ws, bias)
+    else:
+        codes, xs = _check_codes(x, "x")
+        _refuse_gradients("int8_linear", xs, ws, bias)
+    dev = codes.device
+    channels, width = wc.shape
+    if codes.shape[-1] != width:
+        raise ValueError(f"x: rows of {width} elements expected, got {codes.shape[-1]}")
+    most = _lib.NORM_MAX_WIDTH if floats else _lib.LINEAR8_MAX_WIDTH
+    if width > most:
+        raise NotImplementedError(f"rows of up to {most} elements are supported, got {width}")
+    if wc.device != dev:
+        raise ValueError("weight: x's device expected")
+    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.shape != (channels,) or bias.dtype not in _DTYPES or
+                             bias.device != dev):
+        raise ValueError(f"bias: [{channels}] float32, bfloat16 or float16 on x's device expected")
+    if dtype is None:
+        dtype = x.dtype if floats else torch.bfloat16
+    elif dtype not in _DTYPES:
+        raise ValueError("dtype: float32, bfloat16 or float16 expected")
+    guard = _on(dev)
+    if guard is not None:
+        with guard:
+            return int8_linear(x, weight, bias=bias, dtype=dtype)
+    lead = codes.shape[:-1]
+    wpitch = _pitch(wc)
+    if wpitch is None:
+        wc, ws = int8_rows(wc, ws)
+        wpitch = _pitch(wc)
+    elif not ws.is_contiguous():
+        ws = ws.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    out = torch.empty((*lead, channels), dtype=dtype, device=dev)
+    if floats:
+        kept, b, n, _, sb, sn = _two_strides(x)
+        kind, scales, rows = _DTYPES[x.dtype], 0, b * n
+        room = (rows * ((width + 15) // 16 * 16) + 255) // 256 * 256
+        need = room + 4 * rows
+        ws8 = torch.empty(need, dtype=torch.uint8, device=dev)
+        wp = ws8.data_ptr()
+    else:
+        pitch = _pitch(codes)
+        if pitch is None:
+            codes, xs = int8_rows(codes, xs)
+            pitch = _pitch(codes)
+        xs = xs.contiguous()
+        kept, kind, scales = codes, _lib.LAYER_I8, xs.data_ptr()
+        b, n, sb, sn, wp, need = 1, xs.numel(), 0, pitch, 0, 0
+    status = _status_word(dev)
+    args = _lib.LINEAR8_ARGS.pack(
+        kept.data_ptr(), sb, sn, scales, b, n, width, channels, kind, wc.data_ptr(), wpitch, ws.data_ptr(),
+        0 if bias is None else bias.data_ptr(), 0 if bias is None else _DTYPES[bias.dtype], _DTYPES[dtype], out.data_ptr(),
+        0 if status is None else status.data_ptr(), wp, need)
+    rc = lib().htrc_linear8_forward(args, _lib.raw_stream(dev.index))
+    if rc:
+        check(rc, "htrc_linear8_forward")
+    return out

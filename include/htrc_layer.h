@@ -1,7 +1,9 @@
 /* C ABI of the operators around the flat attention in a video transformer's layer (libhtrc_flat.so, sm_100a):
  *   rotary positions over several axes (time, height, width), with the per-head RMS norm before them and the
  *   token-major -> head-major reorder in the same pass, forward and backward;
- *   cross attention of the tokens to an encoder's states of another length, forward and backward.
+ *   cross attention of the tokens to an encoder's states of another length, forward and backward;
+ *   layer norm with a learned affine and a modulation per batch entry, forward and backward;
+ *   the matrix product in 8-bit integers with a scale per token and channel, and the rows it reads.
  *
  * Pointers are device pointers on the current CUDA device unless stated otherwise; the caller owns all memory;
  * no entry point allocates or synchronises, so every call can be captured in a CUDA graph after the first one
@@ -15,7 +17,8 @@
 extern "C" {
 #endif
 
-enum { HTRC_LAYER_F32 = 0, HTRC_LAYER_BF16 = 1, HTRC_LAYER_F16 = 2, HTRC_LAYER_I32 = 3, HTRC_LAYER_U8 = 4 }; /* types */
+enum { HTRC_LAYER_F32 = 0, HTRC_LAYER_BF16 = 1, HTRC_LAYER_F16 = 2, HTRC_LAYER_I32 = 3, HTRC_LAYER_U8 = 4,
+       HTRC_LAYER_I8 = 5 }; /* types */
 
 enum { HTRC_ROTARY_MAX_AXES = 4, HTRC_ROTARY_MAX_DIM = 256, HTRC_ROTARY_MAX_HEADS = 1024 };
 /* pairs of a head's rotated width R: (2 i, 2 i + 1), or (i, i + R / 2) */
@@ -100,6 +103,75 @@ int htrc_cross_forward_workspace_size(const HtrcCrossArgs* args, size_t* bytes);
 int htrc_cross_forward(const HtrcCrossArgs* args, htrc_stream_t stream);
 int htrc_cross_backward_workspace_size(const HtrcCrossArgs* args, size_t* bytes);
 int htrc_cross_backward(const HtrcCrossArgs* args, htrc_stream_t stream);
+
+/* Layer norm: u = (x - mean) rstd over the width, y = (u weight + bias) (1 + scale) + shift, rstd = 1 / sqrt(variance +
+ * eps).  Rows are [batch][token][width] through their strides (batch, token; the width's is 1). */
+enum { HTRC_NORM_MAX_WIDTH = 16384 };
+
+typedef struct {
+  const void* x;
+  int64_t x_stride[2];
+  int64_t batch, tokens;        /* >= 0, fewer than 2^31 rows */
+  int32_t width;                /* 1 .. HTRC_NORM_MAX_WIDTH */
+  int32_t dtype;                /* HTRC_LAYER_F32 / BF16 / F16, of x, out, dy and dx */
+  const void *weight, *bias;    /* [width], or NULL for 1 and 0 */
+  const void *scale, *shift;    /* [batch][width], batch entries scale_stride / shift_stride apart, or NULL for 0 */
+  int64_t scale_stride, shift_stride;
+  int32_t weight_dtype, bias_dtype, scale_dtype, shift_dtype;   /* HTRC_LAYER_F32 / BF16 / F16 */
+  float eps;                    /* >= 0 */
+  /* forward: rows of dtype in out, or with codes 8-bit rows (see htrc_quantize_rows) */
+  void* out;
+  int64_t out_stride[2];
+  int8_t* codes;                /* [batch * tokens][codes_pitch] */
+  int64_t codes_pitch;
+  float* scales;                /* [batch * tokens] */
+  float *mean, *rstd;           /* [batch * tokens]; forward: written unless NULL; backward: the forward's */
+  /* backward only */
+  const void* dy;
+  int64_t dy_stride[2];
+  void* dx;
+  int64_t dx_stride[2];
+  void *dweight, *dbias;        /* [width], each in its parameter's type, or NULL */
+  void *dscale, *dshift;        /* [batch][width] */
+  void* workspace;              /* htrc_norm_workspace_size() bytes */
+  size_t workspace_bytes;
+} HtrcNormArgs;
+
+int htrc_norm_forward(const HtrcNormArgs* args, htrc_stream_t stream);
+/* of the backward; every sum in a fixed order */
+int htrc_norm_workspace_size(const HtrcNormArgs* args, size_t* bytes);
+int htrc_norm_backward(const HtrcNormArgs* args, htrc_stream_t stream);
+
+/* 8-bit rows of x [batch][token][width] (strides: batch, token): codes[row][i] = the integer nearest x 127 / top, ties to
+ * even, scales[row] = top / 127, top = the row's largest magnitude, 10^-30 at least.  A row with a NaN or an infinity
+ * gets a scale of NaN.  pitch: bytes between rows of codes, a multiple of 16 (codes 16-byte aligned). */
+int htrc_quantize_rows(const void* x, int32_t dtype, int64_t batch, int64_t tokens, int32_t width, const int64_t* stride,
+                       int8_t* codes, int64_t pitch, float* scales, htrc_stream_t stream);
+
+/* Product in 8-bit integers: out[row][n] = (sum over k of x[row][k] w[n][k]) x_scales[row] w_scales[n] + bias[n], the sum
+ * an exact 32-bit integer, the rest float32, rounded once.  Rows that are not 8-bit yet are quantised into the workspace. */
+enum { HTRC_LINEAR8_MAX_WIDTH = 65536 };
+
+typedef struct {
+  const void* x;                /* [batch][token][width]; HTRC_LAYER_I8: 16-byte aligned, batch stride = tokens * token stride */
+  int64_t x_stride[2];          /* HTRC_LAYER_I8: multiples of 16 */
+  const float* x_scales;        /* HTRC_LAYER_I8: [batch * tokens] */
+  int64_t batch, tokens;        /* >= 0, fewer than 2^31 - 1024 rows */
+  int32_t width, channels;      /* >= 1; HTRC_LINEAR8_MAX_WIDTH at most (HTRC_NORM_MAX_WIDTH where x is quantised here) */
+  int32_t dtype;                /* of x: HTRC_LAYER_F32 / BF16 / F16 / I8 */
+  const int8_t* w;              /* [channels][width], 16-byte aligned, rows w_pitch apart, a multiple of 16 */
+  int64_t w_pitch;
+  const float* w_scales;        /* [channels] */
+  const void* bias;             /* [channels] or NULL */
+  int32_t bias_dtype, out_dtype;   /* HTRC_LAYER_F32 / BF16 / F16 */
+  void* out;                    /* [batch * tokens][channels], dense */
+  int32_t* status;              /* as in HtrcCrossArgs */
+  void* workspace;              /* htrc_linear8_workspace_size() bytes (0 for 8-bit rows), 256-byte aligned */
+  size_t workspace_bytes;
+} HtrcLinear8Args;
+
+int htrc_linear8_workspace_size(const HtrcLinear8Args* args, size_t* bytes);
+int htrc_linear8_forward(const HtrcLinear8Args* args, htrc_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -11,6 +11,7 @@
 // products.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "../../include/htrc_layer.h"
 #include "common.cuh"
@@ -249,6 +250,294 @@ int small_launch(const CUtensorMap& mx, const CUtensorMap& mw, const Linear8Para
   return cudaLaunchKernelEx(&cfg, kernel, mx, mw, p) == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
 }
 
+// ------------------------------------------------------------------------------------------------ many tokens
+// Of the pair's 256 x 256 tile each CTA holds the sums of its own 128 tokens (TMEM lanes) and all 256 channels (columns),
+// twice.  Warps 0-7: the way out, 32 tokens x 128 channels each; 8: TMA; 9: MMA issue (the leader's, rank 0).
+constexpr int kPairThreads = 320, kPairStages = 6;
+constexpr int kPairRows = 256, kPairChannels = 256;         // of the pair
+constexpr uint32_t kPairTile = 128 * 128, kPairStage = 2 * kPairTile;
+constexpr uint32_t kPairOut = kPairStages * kPairStage, kPairTable = kPairOut + 8 * 4096, kPairBars = kPairTable + 2 * kPairChannels * 4;
+constexpr uint32_t kPairBytes = kPairBars + 192;
+constexpr int kPairGroup = 8;                               // row tiles that are walked together: their operands stay in L2
+
+struct PairBars {
+  uint64_t full[kPairStages], empty[kPairStages], sums_full[2], sums_empty[2], idle;
+  uint32_t tmem;
+  int abort_flag;
+};
+static_assert(sizeof(PairBars) <= 192 && kPairBytes <= 232448, "shared memory");
+
+// mbarrier waits on arrivals from the other CTA
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int* status, volatile int* abort_flag) {
+  bool ok = try_wait_cluster(bar, parity);
+  if (!ok) {
+    const long long t0 = clock64();
+    while (!(ok = try_wait_cluster(bar, parity))) {
+      if (*abort_flag) break;
+      if (clock64() - t0 > kWaitCycles) {
+        *abort_flag = 1;
+        flag_status(status, ST_WAIT_TIMEOUT);
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ void arrive_in(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+// a load into this CTA whose bytes are counted by a barrier of the pair's leader
+__device__ __forceinline__ void pair_load(void* dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(cluster_bar), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ void pair_mma(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(leader)
+      : "memory");
+}
+// an arrival on the barrier of either CTA once the products issued so far are done
+__device__ __forceinline__ void pair_commit(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}" ::"r"(
+          smem_u32(bar)),
+      "r"(leader), "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+__device__ __forceinline__ void store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
+}
+
+// the pair's tile t: groups of kPairGroup row tiles, within one its row tiles first
+__device__ __forceinline__ void pair_tile(const Linear8Params& p, int t, int& row, int& channel) {
+  const int size = kPairGroup * p.tiles_n, group = t / size, first = group * kPairGroup;
+  const int high = min(kPairGroup, p.tiles_m - first), rest = t - group * size;
+  row = (first + rest % high) * kPairRows;
+  channel = rest / high * kPairChannels;
+}
+
+template <typename O>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    linear8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                        const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ Linear8Params p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  PairBars* bars = reinterpret_cast<PairBars*>(smem + kPairBars);
+  volatile int* abort_flag = &bars->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool aligned = (smem_u32(smem) & 1023) == 0;        // the same in either CTA
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kPairStages; ++i) {
+      mbar_init(&bars->full[i], 1);
+      mbar_init(&bars->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->sums_full[i], 1);
+      mbar_init(&bars->sums_empty[i], 16);
+    }
+    mbar_init(&bars->idle, 1);
+    bars->abort_flag = !aligned;
+    if (!aligned) flag_status(p.status, ST_WAIT_TIMEOUT);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&bars->tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem;
+  const int pairs = gridDim.x / 2, first = blockIdx.x / 2, tiles = p.tiles_m * p.tiles_n;
+
+  if (warp == 8) {
+    int issued = 0;
+    if (lane == 0 && aligned) {
+      const uint64_t keep = policy_evict_last(), normal = policy_evict_normal();
+      bool ok = true;
+      for (int t = first; ok && t < tiles; t += pairs) {
+        int row, channel;
+        pair_tile(p, t, row, channel);
+        row += 128 * rank;
+        channel += 128 * rank;
+        for (int b = 0; b < p.blocks; ++b) {
+          const int s = issued % kPairStages;
+          if (issued >= kPairStages && !mbar_wait(&bars->empty[s], (issued / kPairStages - 1) & 1, p.status, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) expect_tx(&bars->full[s], 2 * kPairStage);
+          const uint32_t bar = in_cta(smem_u32(&bars->full[s]), 0);
+          pair_load(smem + s * kPairStage, &tm_x, bar, b * 128, row, normal);
+          pair_load(smem + s * kPairStage + kPairTile, &tm_w, bar, b * 128, channel, keep);
+          ++issued;
+        }
+      }
+      // every load of the pair has landed and every stage has been read, before either CTA leaves (again with a limit)
+      int gave_up = 0;
+      if (rank == 0) drain_ring<false>(bars->full, kPairStages, issued, p.status, &gave_up);
+      if (ok) drain_ring<false>(bars->empty, kPairStages, issued, p.status, &gave_up);
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (rank == 0) {
+      const uint32_t leader = elect_one();
+      constexpr uint32_t idesc = idesc_i8(256, 256);
+      bool ok = aligned;
+      int step = 0, turn = 0;
+      for (int t = first; ok && t < tiles; t += pairs, ++turn) {
+        const int half = turn & 1;
+        if (turn >= 2) ok = wait_cluster(&bars->sums_empty[half], (turn / 2 - 1) & 1, p.status, abort_flag);
+        tc_fence_after();
+        for (int b = 0; ok && b < p.blocks; ++b, ++step) {
+          const int s = step % kPairStages;
+          ok = wait_cluster(&bars->full[s], (step / kPairStages) & 1, p.status, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t a = sw128_desc(smem_u32(smem + s * kPairStage), 16, 1024);
+          const uint64_t w = sw128_desc(smem_u32(smem + s * kPairStage + kPairTile), 16, 1024);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            pair_mma(leader, tmem + 256 * half, a + 2 * k, w + 2 * k, idesc, b > 0 || k > 0);
+          pair_commit(leader, &bars->empty[s]);
+        }
+        if (ok) pair_commit(leader, &bars->sums_full[half]);
+      }
+      // the products are done before the CTAs leave, those of an aborted launch too
+      int gave_up = 0;
+      asm volatile(
+          "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+          "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(&bars->idle)),
+          "r"(leader)
+          : "memory");
+      mbar_wait_warp(&bars->idle, 0, p.status, &gave_up);
+    }
+  } else {
+    constexpr int kCols = 128 / sizeof(O);                  // of a staged 128-byte row
+    float* table = reinterpret_cast<float*>(smem + kPairTable);
+    uint8_t* stage = smem + kPairOut + warp * 4096;
+    const int quarter = warp & 3, side = warp >> 2;
+    const uint32_t at = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + 128 * side;
+    const uint32_t leaders[2] = {in_cta(smem_u32(&bars->sums_empty[0]), 0), in_cta(smem_u32(&bars->sums_empty[1]), 0)};
+    bool ok = aligned;
+    int turn = 0;
+    // (a warp whose wait ran out goes on to the barriers that the others stand at, without work)
+    for (int t = first; t < tiles; t += pairs, ++turn) {
+      int row, channel;
+      pair_tile(p, t, row, channel);
+      row += 128 * rank + 32 * quarter;
+      const int half = turn & 1;
+      // the tile's scales and biases, a thread a channel
+      const int n = channel + threadIdx.x;
+      const float2 term = n < p.channels ? make_float2(__ldg(p.ws + n), bias_at(p, n)) : make_float2(0.f, 0.f);
+      const float xs = row + lane < p.rows ? __ldg(p.xs + row + lane) : 0.f;
+      named_bar_sync(1, 256);
+      table[threadIdx.x] = term.x;
+      table[kPairChannels + threadIdx.x] = term.y;
+      named_bar_sync(1, 256);
+      ok = ok && wait_cluster(&bars->sums_full[half], (turn / 2) & 1, p.status, abort_flag);
+      if (!ok) continue;
+      tc_fence_after();
+      channel += 128 * side;
+      const float* ws = table + 128 * side;
+#pragma unroll 1
+      for (int c = 0; c < 128; c += kCols) {
+        bulk_wait_group_read0();                            // lane 0's: the stage has left
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kCols; i += 32) {
+          uint32_t v[32];
+          tmem_ld32(at + 256 * half + c + i, v);
+          tmem_ld_wait();
+          if (c + kCols == 128 && i + 32 == kCols) {        // the last read of these sums
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_in(leaders[half]);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 s4 = *reinterpret_cast<const float4*>(ws + c + i + j);
+            const float4 b4 = *reinterpret_cast<const float4*>(ws + kPairChannels + c + i + j);
+            const float y0 = scaled(static_cast<int>(v[j]), xs, s4.x, b4.x), y1 = scaled(static_cast<int>(v[j + 1]), xs, s4.y, b4.y);
+            const float y2 = scaled(static_cast<int>(v[j + 2]), xs, s4.z, b4.z), y3 = scaled(static_cast<int>(v[j + 3]), xs, s4.w, b4.w);
+            if constexpr (sizeof(O) == 4) {
+              v[j] = __float_as_uint(y0);
+              v[j + 1] = __float_as_uint(y1);
+              v[j + 2] = __float_as_uint(y2);
+              v[j + 3] = __float_as_uint(y3);
+            } else if constexpr (std::is_same<O, __nv_bfloat16>::value) {
+              v[j / 2] = pack_bf16x2(y0, y1);
+              v[j / 2 + 1] = pack_bf16x2(y2, y3);
+            } else {
+              v[j / 2] = pack_f16x2(y0, y1);
+              v[j / 2 + 1] = pack_f16x2(y2, y3);
+            }
+          }
+          constexpr int kPieces = 32 * sizeof(O) / 16;      // 16-byte pieces of these columns
+#pragma unroll
+          for (int q = 0; q < kPieces; ++q)
+            st_shared_v4(smem_u32(stage) + sw128_off(lane, i * sizeof(O) / 16 + q), v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        }
+        if (!p.direct) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (row < p.rows && channel + c < p.channels) store_2d(&tm_o, stage, channel + c, row);
+            bulk_commit_group();
+          }
+        } else {
+          // rows of any alignment: element by element, a row's neighbours together
+          __syncwarp();
+          O* out = static_cast<O*>(p.out) + static_cast<int64_t>(row) * p.channels + channel + c;
+          for (int r = 0; r < 32 && row + r < p.rows; ++r)
+            for (int e = lane; e < kCols && channel + c + e < p.channels; e += 32)
+              out[static_cast<int64_t>(r) * p.channels + e] =
+                  *reinterpret_cast<const O*>(stage + sw128_off(r, e * sizeof(O) / 16) + e * sizeof(O) % 16);
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_group0();
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();                          // neither CTA leaves while the other may still signal it
+  tc_fence_after();
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <typename O>
+int pair_launch(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mo, const Linear8Params& p, cudaStream_t st) {
+  auto kernel = linear8_pair_kernel<O>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairBytes) != cudaSuccess) return HTRC_ERR_CUDA;
+  const int pairs = std::min(sm_count() / 2, p.tiles_m * p.tiles_n);
+  kernel<<<2 * pairs, kPairThreads, kPairBytes, st>>>(mx, mw, mo, p);
+  return cudaGetLastError() == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
+}
+
 // ------------------------------------------------------------------------------------------------ host
 bool float_type(int t) { return t == HTRC_LAYER_F32 || t == HTRC_LAYER_BF16 || t == HTRC_LAYER_F16; }
 
@@ -280,6 +569,27 @@ int linear8_validate(const HtrcLinear8Args* a) {
 
 template <typename O>
 int linear8_launch(Linear8Params& p, const int8_t* x, int64_t pitch, const HtrcLinear8Args* a, cudaStream_t st) {
+  const int64_t pairs = (static_cast<int64_t>(p.rows) + 255) / 256 * ((static_cast<int64_t>(p.channels) + 255) / 256);
+  if (pairs >= sm_count() / 2) {
+    CUtensorMap mx, mw, mo;
+    constexpr int es = sizeof(O);
+    p.direct = p.channels * es % 16 != 0 || reinterpret_cast<uintptr_t>(p.out) % 16 != 0;
+    if (!code_map(&mx, x, p.rows, a->width, pitch, 128) || !code_map(&mw, a->w, p.channels, a->width, a->w_pitch, 128))
+      return HTRC_ERR_CUDA;
+    mo = mx;
+    if (!p.direct) {
+      const uint64_t dims[2] = {static_cast<uint64_t>(p.channels), static_cast<uint64_t>(p.rows)};
+      const uint64_t strides[1] = {static_cast<uint64_t>(p.channels) * es};
+      const uint32_t box[2] = {128 / es, 32};
+      const CUtensorMapDataType type = es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                       : std::is_same<O, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+      if (!make_tiled_map(&mo, type, 2, p.out, dims, strides, box, true)) return HTRC_ERR_CUDA;
+    }
+    p.tiles_m = (p.rows + kPairRows - 1) / kPairRows;
+    p.tiles_n = (p.channels + kPairChannels - 1) / kPairChannels;
+    return pair_launch<O>(mx, mw, mo, p, st);
+  }
   const int tile = p.rows <= 16 ? 16 : p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : 128;
   CUtensorMap mx, mw;
   if (!code_map(&mx, x, p.rows, a->width, pitch, tile) || !code_map(&mw, a->w, p.channels, a->width, a->w_pitch, kSmallChannels))

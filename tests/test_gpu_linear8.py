@@ -45,7 +45,9 @@ def _check(got, x, w, bias, dtype):
 # bytes, tiles that are split over the width, several tiles
 SIZES = [(1, 1, 1), (1, 2048, 515), (2, 16, 128), (15, 17, 127), (16, 128, 129), (17, 129, 300), (32, 4100, 64), (33, 255, 2),
          (64, 1000, 1000), (65, 777, 515), (128, 512, 256), (129, 130, 130), (255, 384, 1023), (256, 64, 256), (300, 2048, 2048),
-         (1001, 777, 515), (513, 4096, 384), (2049, 96, 1025), (7, 16384, 40), (5, 65536, 33)]
+         (1001, 777, 515), (513, 4096, 384), (2049, 96, 1025), (7, 16384, 40), (5, 65536, 33),
+         # pairs of SMs: several tiles each, ends in every direction, rows that are not 16-byte aligned
+         (5000, 384, 1100), (2049, 96, 2308), (3001, 777, 2051), (19000, 130, 304), (300, 1000, 20000), (4096, 2048, 4096)]
 
 
 @pytest.mark.parametrize("size", SIZES)
@@ -110,7 +112,8 @@ def test_shapes_and_strides(dev):
     assert htrc_b200.int8_rows(*laid).codes.data_ptr() == laid.codes.data_ptr()
 
 
-@pytest.mark.parametrize("tokens,channels", [(1, 1), (3, 77), (130, 130), (300, 520), (2100, 1030), (700, 2048)])
+@pytest.mark.parametrize("tokens,channels", [(1, 1), (3, 77), (130, 130), (300, 520), (2100, 1030), (700, 2048),
+                                             (5000, 1032), (9000, 515)])
 def test_what_lies_around_the_result_is_left_alone(dev, tokens, channels):
     """Through the C entry, into the middle of a larger buffer."""
     gen = torch.Generator(device=dev).manual_seed(5)
@@ -125,6 +128,22 @@ def test_what_lies_around_the_result_is_left_alone(dev, tokens, channels):
         assert _lib.lib().htrc_linear8_forward(args, _lib.stream_ptr()) == _lib.HTRC_OK
         _check(out.view(tokens, channels), x, w, None, dtype)
         assert (buf[:4096] == 7).all() and (buf[4096 + tokens * channels:] == 7).all() and status[0] == 0
+
+
+def test_offsets_past_32_bits(dev):
+    gen = torch.Generator(device=dev).manual_seed(11)
+    x, w = _rows(gen, dev, 70000, 64), _rows(gen, dev, 32768, 64)
+    got = htrc_b200.int8_linear(x, w)
+    for a in (0, 35000, 65500, 69990):
+        some = slice(a, a + 10)
+        _check(got[some], Int8Rows(x.codes[some], x.scales[some]), w, None, torch.bfloat16)
+    x = torch.randn((140000, 16384), generator=gen, device=dev, dtype=torch.bfloat16)
+    rows = htrc_b200.quantize_rows(x)
+    w = htrc_b200.quantize_rows(x[:40])
+    got = htrc_b200.int8_linear(x, w)
+    for a in (0, 131060, 139990):
+        some = slice(a, a + 10)
+        _check(got[some], Int8Rows(rows.codes[some], rows.scales[some]), w, None, torch.bfloat16)
 
 
 def test_bad_rows_stay_by_themselves(dev):

@@ -99,7 +99,7 @@ class HtrcNormArgs(ctypes.Structure):
                 ("weight_dtype", _i32), ("bias_dtype", _i32), ("scale_dtype", _i32), ("shift_dtype", _i32), ("eps", _f32),
                 ("out", _p), ("out_stride", _i64x2), ("codes", _p), ("codes_pitch", _i64), ("scales", _p), ("mean", _p),
                 ("rstd", _p), ("dy", _p), ("dy_stride", _i64x2), ("dx", _p), ("dx_stride", _i64x2), ("dweight", _p),
-                ("dbias", _p), ("dscale", _p), ("dshift", _p), ("workspace", _p), ("workspace_bytes", ctypes.c_size_t)]
+                ("dbias", _p), ("dscale", _p), ("dshift", _p), ("status", _p), ("workspace", _p), ("workspace_bytes", ctypes.c_size_t)]
 
 
 class HtrcLinear8Args(ctypes.Structure):
@@ -115,7 +115,7 @@ class HtrcLinear8Args(ctypes.Structure):
 _ROTARY_TENSOR = "P3qP3qP3qPPii"
 ROTARY_ARGS = struct.Struct("@" + 2 * _ROTARY_TENSOR + "iiqqii4iiPi3qdPfPN0q")
 CROSS_ARGS = struct.Struct("@PPP3q3q3qP3qPqqqiiiifPPi4qPP3qPPPP3q3q3qPN0q")
-NORM_ARGS = struct.Struct("@P2qqqiiPPPPqqiiiifP2qPqPPPP2qP2qPPPPPN0q")
+NORM_ARGS = struct.Struct("@P2qqqiiPPPPqqiiiifP2qPqPPPP2qP2qPPPPPPN0q")
 LINEAR8_ARGS = struct.Struct("@P2qPqqiiiPqPPiiPPPN0q")
 
 

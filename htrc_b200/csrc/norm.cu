@@ -4,9 +4,10 @@
 //   u = (x - mean) rstd,   y = (u weight + bias) (1 + scale) + shift = u A + B
 //   codes = rint(y (127 / top)), scales = top / 127, top = max |y| of the row
 //
-// Forward: a row is read once and stays in registers as it was read, W warps to a row and rows to the CTA's warps; mean,
-// then the squared deviations from it (no cancellation under a large mean), then the result, all float32.  A and B are
-// formed once per batch entry in shared memory.  HBM bounds it: 4 bytes per 16-bit element, 3 to 8-bit rows.
+// Forward: a row is read once and stays in registers as it was read, 8 lanes to 16 warps to a row, several rows to a lane's
+// eight pieces, and the next rows are fetched before these are used.  The mean, then the squared deviations from it (no
+// cancellation under a large mean), then the result, all float32.  A and B are formed once per batch entry in shared memory.
+// HBM bounds it: 4 bytes per 16-bit element, 3 to 8-bit rows.
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
@@ -20,8 +21,9 @@ namespace htrc {
 
 namespace {
 
-constexpr int kNormThreads = 256;           // of a CTA with a warp per row; wider rows: 32 W
+constexpr int kNormThreads = 256;           // of a CTA whose rows take a warp or less; wider rows: one row's lanes
 constexpr int kNormMaxWarps = 16;           // per row
+constexpr int kNormSms = 228 * 1024;        // shared memory of an SM
 constexpr float kRoundMagic = 12582912.f;   // 1.5 * 2^23: adding it rounds to the nearest integer, ties to even
 constexpr float kLeastTop = 1e-30f;         // of a quantised row: 127 / top stays finite
 
@@ -43,8 +45,9 @@ struct NormParams {
   float* scales;
   float *mean, *rstd;
   int64_t entries, rows;                    // rows per entry
-  int width, nvec, warps;                   // vectors per row, warps per row
-  int64_t chunk, chunks;                    // rows of a task, tasks per entry
+  int width, nvec, lanes;                   // pieces per row, lanes per row (a power of two)
+  bool pairs;                               // unaligned rows: two elements stand at multiples of their size
+  int64_t chunks;                           // CTAs that share an entry
   float eps, inv_width;
   bool affine, modulated;
   TermView weight, bias, scale, shift;
@@ -71,7 +74,20 @@ struct Piece {
 #pragma unroll
     for (int i = 0; i < W; ++i) asm volatile("" : "+r"(w[i]));
   }
-  __device__ __forceinline__ void load(const T* p, bool both) {
+  // pairs: the two elements in one load
+  __device__ __forceinline__ void load(const T* p, bool both, bool pairs) {
+    if (!VEC && pairs && both) {
+      if constexpr (sizeof(T) == 4) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        w[0] = v.x;
+        w[1] = v.y;
+      } else {
+        const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(p));
+        w[0] = v & 0xFFFFu;
+        w[1] = v >> 16;
+      }
+      return;
+    }
     if constexpr (VEC) {
       const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
       w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
@@ -112,7 +128,12 @@ struct Piece {
       }
     }
   }
-  __device__ __forceinline__ void store(T* p, bool both) const {
+  __device__ __forceinline__ void store(T* p, bool both, bool pairs) const {
+    if (!VEC && pairs && both) {
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(p) = w[0] | w[1] << 16;
+      return;
+    }
     if constexpr (VEC) {
       __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
     } else if constexpr (sizeof(T) == 4) {
@@ -152,36 +173,51 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// the row's sum / maximum over its W warps (W > 1: the CTA is one row's; slots alternate, so one barrier each)
-__device__ __forceinline__ float row_add(float v, int warps, float* slots, int& turn) {
-  v = warp_sum(v);
-  if (warps == 1) return v;
-  float* s = slots + (turn ^= 1) * kNormMaxWarps;
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = s[0];
-  for (int i = 1; i < warps; ++i) v += s[i];
-  return v;
+__device__ __forceinline__ float larger(float a, float b) {      // NaN if either is
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
 }
-__device__ __forceinline__ uint32_t row_most(uint32_t v, int warps, float* slots, int& turn) {
-  v = __reduce_max_sync(0xffffffffu, v);
-  if (warps == 1) return v;
-  uint32_t* s = reinterpret_cast<uint32_t*>(slots + (turn ^= 1) * kNormMaxWarps);
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+
+// R rows' sums (or maxima) over their L lanes.  L > 32: the CTA is one row's; slots alternate, so one barrier each.
+template <int R, bool MOST>
+__device__ __forceinline__ void over_lanes(float (&v)[R], int L, float (*slots)[kNormMaxWarps][8], int& turn) {
+  auto step = [&](int d) {
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const float o = __shfl_xor_sync(0xffffffffu, v[k], d);
+      v[k] = MOST ? larger(v[k], o) : v[k] + o;
+    }
+  };
+  if (L >= 32) step(16);
+  if (L >= 16) step(8);
+  step(4);
+  step(2);
+  step(1);
+  if (L <= 32) return;
+  turn ^= 1;
+  if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+    for (int k = 0; k < R; ++k) slots[turn][threadIdx.x >> 5][k] = v[k];
+  }
   __syncthreads();
-  v = s[0];
-  for (int i = 1; i < warps; ++i) v = max(v, s[i]);
-  return v;
+  const int warps = L >> 5;
+#pragma unroll
+  for (int k = 0; k < R; ++k) v[k] = slots[turn][0][k];
+  for (int i = 1; i < warps; ++i) {
+#pragma unroll
+    for (int k = 0; k < R; ++k) v[k] = MOST ? larger(v[k], slots[turn][i][k]) : v[k] + slots[turn][i][k];
+  }
 }
 
 template <typename T, bool VEC, int V, int MODE>
-__global__ void __launch_bounds__(kNormMaxWarps * 32) norm_rows_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(kNormMaxWarps * 32) __maxnreg__(MODE == NORM_CODES ? 128 : MODE == NORM_ROWS ? 80 : 64)
+    norm_rows_kernel(const __grid_constant__ NormParams p) {
   using P = Piece<T, VEC>;
-  constexpr int N = P::N, H = N / 2;
+  constexpr int N = P::N, H = N / 2, R = V >= 8 ? 1 : V == 1 ? 4 : 8 / V;
   extern __shared__ __align__(16) float terms[];
-  __shared__ float slots[2 * kNormMaxWarps];
-  const int W = p.warps, L = 32 * W;
-  const int group = threadIdx.x / L, at = threadIdx.x % L, groups = blockDim.x / L;
+  __shared__ float slots[2][kNormMaxWarps][8];
+  const int L = p.lanes, at = threadIdx.x & (L - 1), G = blockDim.x / L, group = threadIdx.x / L;
   const int room = p.nvec * N;
   const float *sa = terms, *sb = terms + room;
   int turn = 0;
@@ -189,7 +225,23 @@ __global__ void __launch_bounds__(kNormMaxWarps * 32) norm_rows_kernel(const __g
   const int64_t tasks = p.entries * p.chunks;
   if (MODE != NORM_ROWS) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // a product waits for this kernel's end itself
   for (int64_t task = blockIdx.x; task < tasks; task += gridDim.x) {
-    const int64_t e = task / p.chunks, r0 = (task - e * p.chunks) * p.chunk, r1 = min(r0 + p.chunk, p.rows);
+    // an entry's CTAs sweep its rows together: neighbouring CTAs at neighbouring rows
+    const int64_t e = task / p.chunks, r0 = (task - e * p.chunks) * G * R, r1 = p.rows, step = p.chunks * G * R;
+    const T* x = static_cast<const T*>(p.x) + e * p.xs[0] + at * N;
+    auto fetch = [&](P (&v)[R][V], int64_t r) {
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const int64_t row = r + k * G + group;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int vec = at + i * L;
+          if (row < r1 && vec < p.nvec) v[k][i].load(x + row * p.xs[1] + i * L * N, N > 2 || 2 * vec + 1 < p.width, p.pairs);
+          else v[k][i].clear();
+        }
+      }
+    };
+    P v[R][V];
+    fetch(v, r0);
     if (MODE != QUANT_CODES && p.affine && held != (p.modulated ? e : 0)) {
       if (held >= 0) __syncthreads();
       held = p.modulated ? e : 0;
@@ -198,137 +250,176 @@ __global__ void __launch_bounds__(kNormMaxWarps * 32) norm_rows_kernel(const __g
         if (i < p.width) {
           a = p.weight.p ? term_at(p.weight.p, p.weight.dtype, i) : 1.f;
           b = p.bias.p ? term_at(p.bias.p, p.bias.dtype, i) : 0.f;
+          if (p.scale.p) {
+            const float s = 1.f + term_at(p.scale.p, p.scale.dtype, e * p.scale.stride + i);
+            a *= s;
+            b *= s;
+          }
+          if (p.shift.p) b += term_at(p.shift.p, p.shift.dtype, e * p.shift.stride + i);
         }
-        if (i < p.width && p.scale.p) {
-          const float s = 1.f + term_at(p.scale.p, p.scale.dtype, e * p.scale.stride + i);
-          a *= s;
-          b *= s;
-        }
-        if (i < p.width && p.shift.p) b += term_at(p.shift.p, p.shift.dtype, e * p.shift.stride + i);
         const int slot = term_slot<N>(i, p.nvec);
         terms[slot] = a;
         terms[room + slot] = b;
       }
       __syncthreads();
     }
-    for (int64_t r = r0 + group; r < r1; r += groups) {
-      const T* x = static_cast<const T*>(p.x) + e * p.xs[0] + r * p.xs[1];
-      P v[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int vec = at + i * L;
-        if (vec < p.nvec) v[i].load(x + vec * N, N > 2 || 2 * vec + 1 < p.width);
-        else v[i].clear();
-      }
-      const int64_t row = e * p.rows + r;
-      float mean = 0.f, rstd = 1.f;
+    for (int64_t r = r0; r < r1; r += step) {
+      if (MODE != NORM_CODES && r > r0) fetch(v, r);
+      float mean[R], rstd[R];
       if (MODE != QUANT_CODES) {
-        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < V; ++i)
+        for (int k = 0; k < R; ++k) {
+          float2 sum = make_float2(0.f, 0.f);
+          if (r + k * G < r1) {                             // the same for all of the CTA
 #pragma unroll
-          for (int h = 0; h < H; ++h) sum = add2(sum, v[i].pair(h));
-        mean = row_add(sum.x + sum.y, W, slots, turn) * p.inv_width;
+            for (int i = 0; i < V; ++i)
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i].packed();
-        float2 ss = make_float2(0.f, 0.f);
-        const float2 m2 = make_float2(mean, mean);
+              for (int h = 0; h < H; ++h) sum = add2(sum, v[k][i].pair(h));
+          }
+          mean[k] = sum.x + sum.y;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if (at + i * L < p.nvec) {
+          for (int i = 0; i < V; ++i) v[k][i].packed();
+        }
+        over_lanes<R, false>(mean, L, slots, turn);
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-              float2 d = sub2(v[i].pair(h), m2);
-              if (N == 2 && 2 * (at + i * L) + 1 >= p.width) d.y = 0.f;
-              ss = fma2(d, d, ss);
+        for (int k = 0; k < R; ++k) {
+          mean[k] *= p.inv_width;
+          float2 ss = make_float2(0.f, 0.f);
+          const float2 m2 = make_float2(mean[k], mean[k]);
+          if (r + k * G < r1) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              if (at + i * L < p.nvec) {
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                  float2 d = sub2(v[k][i].pair(h), m2);
+                  if (N == 2 && 2 * (at + i * L) + 1 >= p.width) d.y = 0.f;
+                  ss = fma2(d, d, ss);
+                }
+              }
             }
           }
-        }
-        rstd = rsqrtf(row_add(ss.x + ss.y, W, slots, turn) * p.inv_width + p.eps);
+          rstd[k] = ss.x + ss.y;
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i].packed();
-        if (at == 0) {
-          if (p.mean) p.mean[row] = mean;
-          if (p.rstd) p.rstd[row] = rstd;
+          for (int i = 0; i < V; ++i) v[k][i].packed();
+        }
+        over_lanes<R, false>(rstd, L, slots, turn);
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          rstd[k] = rsqrtf(rstd[k] * p.inv_width + p.eps);
+          const int64_t row = r + k * G + group;
+          if (at == 0 && row < r1) {
+            if (p.mean) p.mean[e * p.rows + row] = mean[k];
+            if (p.rstd) p.rstd[e * p.rows + row] = rstd[k];
+          }
         }
       }
-      const float2 m2 = make_float2(mean, mean), r2 = make_float2(rstd, rstd);
-      auto result = [&](int i, int vec, float2 (&y)[H]) {
+      // the results of piece i of every row, which share its A and B
+      auto results = [&](int i, int vec, auto use) {
         float2 a[H], b[H];
         if (p.affine) {
           term_load<N>(sa, vec, p.nvec, a);
           term_load<N>(sb, vec, p.nvec, b);
         }
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-          y[h] = mul2(sub2(v[i].pair(h), m2), r2);
-          if (p.affine) y[h] = fma2(y[h], a[h], b[h]);
+        for (int k = 0; k < R; ++k) {
+          if (r + k * G >= r1) break;
+          const float2 m2 = make_float2(mean[k], mean[k]), r2 = make_float2(rstd[k], rstd[k]);
+          float2 y[H];
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            y[h] = mul2(sub2(v[k][i].pair(h), m2), r2);
+            if (p.affine) y[h] = fma2(y[h], a[h], b[h]);
+          }
+          use(k, y);
         }
       };
-      if (MODE == NORM_ROWS) {
-        T* out = static_cast<T*>(p.out) + e * p.os[0] + r * p.os[1];
+      if constexpr (MODE == NORM_ROWS) {
+        T* out = static_cast<T*>(p.out) + e * p.os[0] + at * N;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const int vec = at + i * L;
           if (vec < p.nvec) {
-            float2 y[H];
-            result(i, vec, y);
+            results(i, vec, [&](int k, float2 (&y)[H]) {
+              const int64_t row = r + k * G + group;
+              P o;
 #pragma unroll
-            for (int h = 0; h < H; ++h) v[i].set(h, y[h]);
-            v[i].store(out + vec * N, N > 2 || 2 * vec + 1 < p.width);
+              for (int h = 0; h < H; ++h) o.set(h, y[h]);
+              if (row < r1) o.store(out + row * p.os[1] + i * L * N, N > 2 || 2 * vec + 1 < p.width, p.pairs);
+            });
           }
         }
       } else {
         // a norm's results stay in float32 until the row's largest is known
-        float2 y[MODE == NORM_CODES ? V : 1][H];
-        uint32_t top = 0;             // as bits: of magnitudes they are ordered, NaN above infinity
+        float2 y[MODE == NORM_CODES ? R : 1][MODE == NORM_CODES ? V : 1][H];
+        float top[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) top[k] = 0.f;
+        auto most = [&](int k, float2 t, bool both) {
+          top[k] = larger(top[k], fabsf(t.x));
+          if (both) top[k] = larger(top[k], fabsf(t.y));
+        };
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const int vec = at + i * L;
+          const bool both = N > 2 || 2 * vec + 1 < p.width;
           if (vec < p.nvec) {
-            if (MODE == NORM_CODES) result(i, vec, y[MODE == NORM_CODES ? i : 0]);
+            if constexpr (MODE == NORM_CODES) {
+              results(i, vec, [&](int k, float2 (&t)[H]) {
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-              const float2 t = MODE == NORM_CODES ? y[MODE == NORM_CODES ? i : 0][h] : v[i].pair(h);
-              top = max(top, __float_as_uint(t.x) & 0x7FFFFFFFu);
-              if (N > 2 || 2 * vec + 1 < p.width) top = max(top, __float_as_uint(t.y) & 0x7FFFFFFFu);
+                for (int h = 0; h < H; ++h) {
+                  y[k][i][h] = t[h];
+                  most(k, t[h], both);
+                }
+              });
+            } else {
+#pragma unroll
+              for (int k = 0; k < R; ++k)
+#pragma unroll
+                for (int h = 0; h < H; ++h) most(k, v[k][i].pair(h), both);
             }
           }
         }
-        top = row_most(top, W, slots, turn);
-        if (MODE == QUANT_CODES) {
+        // the rows as they were read are done with: the next ones arrive while these are quantised
+        if (MODE == NORM_CODES) fetch(v, r + step);
+        over_lanes<R, true>(top, L, slots, turn);
 #pragma unroll
-          for (int i = 0; i < V; ++i) v[i].packed();
-        }
-        // a row with a NaN or an infinity has no codes: its scale is NaN, and with it what is made of it
-        const float most = top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : fmaxf(__uint_as_float(top), kLeastTop);
-        const float by = __fdiv_rn(127.f, most);
-        if (at == 0) p.scales[row] = __fdiv_rn(most, 127.f);
-        int8_t* codes = p.codes + row * p.pitch;
-        const float2 by2 = make_float2(by, by);
+        for (int k = 0; k < R; ++k) {
+          const int64_t row = r + k * G + group;
+          if (r + k * G >= r1) break;
+          // a row with a NaN or an infinity has no codes: its scale is NaN, and with it what is made of it
+          const float full = top[k] <= 3.4028235e38f ? fmaxf(top[k], kLeastTop) : __uint_as_float(0x7FC00000u);
+          const float by = __fdiv_rn(127.f, full);
+          if (at == 0 && row < r1) p.scales[e * p.rows + row] = __fdiv_rn(full, 127.f);
+          const float2 by2 = make_float2(by, by);
+          int8_t* codes = p.codes + (e * p.rows + row) * p.pitch;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int vec = at + i * L;
-          if (vec < p.nvec) {
-            uint32_t c[2 * H];
+          for (int i = 0; i < V; ++i) {
+            const int vec = at + i * L;
+            if (MODE == QUANT_CODES) v[k][i].packed();
+            if (vec < p.nvec && row < r1) {
+              uint32_t c[2 * H];
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-              // rounded to float32 by the product and to an integer by the sum: two roundings, as the definition has them
-              // (elements of half the largest stand on a border; a paired sum would be fused with the paired product)
-              const float2 z = mul2(MODE == NORM_CODES ? y[MODE == NORM_CODES ? i : 0][h] : v[i].pair(h), by2);
-              c[2 * h] = __float_as_uint(__fadd_rn(z.x, kRoundMagic));
-              c[2 * h + 1] = __float_as_uint(__fadd_rn(z.y, kRoundMagic));
-            }
-            if constexpr (N == 2) {             // an odd row's last store reaches into the pitch
-              *reinterpret_cast<unsigned short*>(codes + 2 * vec) = static_cast<unsigned short>(__byte_perm(c[0], c[1], 0x0040));
-            } else {
-              uint32_t w[N / 4];
+              for (int h = 0; h < H; ++h) {
+                // rounded to float32 by the product and to an integer by the sum: two roundings, as the definition has
+                // them (elements of half the largest stand on a border; a paired sum would be fused with the product)
+                float2 z;
+                if constexpr (MODE == NORM_CODES) z = mul2(y[k][i][h], by2);
+                else z = mul2(v[k][i].pair(h), by2);
+                c[2 * h] = __float_as_uint(__fadd_rn(z.x, kRoundMagic));
+                c[2 * h + 1] = __float_as_uint(__fadd_rn(z.y, kRoundMagic));
+              }
+              if constexpr (N == 2) {             // an odd row's last store reaches into the pitch
+                *reinterpret_cast<unsigned short*>(codes + 2 * vec) = static_cast<unsigned short>(__byte_perm(c[0], c[1], 0x0040));
+              } else {
+                uint32_t w[N / 4];
 #pragma unroll
-              for (int k = 0; k < N / 4; ++k)
-                w[k] = __byte_perm(__byte_perm(c[4 * k], c[4 * k + 1], 0x0040), __byte_perm(c[4 * k + 2], c[4 * k + 3], 0x0040),
-                                   0x5410);
-              if constexpr (N == 8) *reinterpret_cast<uint2*>(codes + vec * 8) = make_uint2(w[0], w[1]);
-              else *reinterpret_cast<uint32_t*>(codes + vec * 4) = w[0];
+                for (int q = 0; q < N / 4; ++q)
+                  w[q] = __byte_perm(__byte_perm(c[4 * q], c[4 * q + 1], 0x0040), __byte_perm(c[4 * q + 2], c[4 * q + 3], 0x0040),
+                                     0x5410);
+                if constexpr (N == 8) *reinterpret_cast<uint2*>(codes + vec * 8) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<uint32_t*>(codes + vec * 4) = w[0];
+              }
             }
           }
         }
@@ -338,10 +429,12 @@ __global__ void __launch_bounds__(kNormMaxWarps * 32) norm_rows_kernel(const __g
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// A thread keeps its columns: C vectors of them, over R rows at a time, so that the columns' sums P = sum dy u and
-// Q = sum dy stay in registers over all of the CTA's rows; the rows' two sums go over the CTA.
-//   g = dy A,  dx = rstd (g - mean(g) - u mean(g u))
-// The parts' P and Q are added in order by norm_terms_kernel.  HBM bounds it: 6 bytes per 16-bit element.
+//   g = dy A,  dx = rstd (g - mean(g) - u mean(g u)),  P = sum over rows of dy u,  Q = sum over rows of dy
+// A thread keeps its columns over all of the CTA's rows, so that their P and Q stay in registers; the rows' two sums go over
+// the lanes.  Rows of half a warp to a warp's pieces (norm_back_narrow_kernel) need no barrier.  A wider row is the whole
+// CTA's (norm_back_ring_kernel): rows arrive in shared memory by bulk copies several stages ahead, since a barrier per
+// four rows leaves loads by the threads themselves no time in flight.  norm_back_any_kernel: rows that are not 16-byte aligned, and float32 rows too wide for
+// the registers.  The parts' P and Q are added in order by norm_terms_kernel.  HBM bounds it: 6 bytes per 16-bit element.
 struct NormBackParams {
   const void *dy, *x;
   int64_t gs[2], xs[2];
@@ -350,24 +443,25 @@ struct NormBackParams {
   const float *mean, *rstd;
   int64_t entries, rows;
   int width, nvec;
-  int64_t chunk, chunks;
+  int64_t chunks;                           // CTAs that share an entry
   float inv_width;
-  bool sums, affine;                        // sums: P and Q are wanted
+  bool sums, affine, pairs;                 // sums: P and Q are wanted
+  int lanes, stages;
+  int* status;
   TermView weight, scale;
   float* part;                              // [entry * chunks][2][width]
 };
 
 // RELOAD: rows too wide for the registers are read again (from L2) once their sums are known.
 template <typename T, bool VEC, int C, int R, bool RELOAD>
-__global__ void __launch_bounds__(512) norm_back_kernel(const __grid_constant__ NormBackParams p) {
+__global__ void __launch_bounds__(512, 1) norm_back_any_kernel(const __grid_constant__ NormBackParams p) {
   using P = Piece<T, VEC>;
   constexpr int N = P::N, H = N / 2, HELD = RELOAD ? 1 : C;
   __shared__ float slots[2][16][2 * R];
   extern __shared__ __align__(16) float gain[];          // A, as term_slot() has it
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, L = blockDim.x;
   int turn = 0;
-  const int64_t e = blockIdx.x / p.chunks, c0 = blockIdx.x - e * p.chunks;
-  const int64_t r0 = c0 * p.chunk, r1 = min(r0 + p.chunk, p.rows);
+  const int64_t e = blockIdx.x / p.chunks, r1 = p.rows, r0 = (blockIdx.x - e * p.chunks) * R, step = p.chunks * R;
   if (p.affine) {
     for (int i = threadIdx.x; i < p.nvec * N; i += L) {
       float t = i >= p.width ? 0.f : p.weight.p ? term_at(p.weight.p, p.weight.dtype, i) : 1.f;
@@ -389,15 +483,15 @@ __global__ void __launch_bounds__(512) norm_back_kernel(const __grid_constant__ 
   const T* dy = static_cast<const T*>(p.dy) + e * p.gs[0];
   const T* x = static_cast<const T*>(p.x) + e * p.xs[0];
   T* dx = static_cast<T*>(p.dx) + e * p.os[0];
-  for (int64_t r = r0; r < r1; r += R) {
+  for (int64_t r = r0; r < r1; r += step) {
     P vg[R][HELD], vx[R][HELD];
     float mean[R], rstd[R];
     auto fetch = [&](int k, int c, int to) {
       const int vec = threadIdx.x + c * L;
       if (r + k < r1 && vec < p.nvec) {
         const bool both = N > 2 || 2 * vec + 1 < p.width;
-        vg[k][to].load(dy + (r + k) * p.gs[1] + vec * N, both);
-        vx[k][to].load(x + (r + k) * p.xs[1] + vec * N, both);
+        vg[k][to].load(dy + (r + k) * p.gs[1] + vec * N, both, p.pairs);
+        vx[k][to].load(x + (r + k) * p.xs[1] + vec * N, both, p.pairs);
       } else {
         vg[k][to].clear();
         vx[k][to].clear();
@@ -474,7 +568,7 @@ __global__ void __launch_bounds__(512) norm_back_kernel(const __grid_constant__ 
           const float2 u = mul2(sub2(vx[k][at].pair(h), m2), r2), g = mul2(vg[k][at].pair(h), a[h]);
           o.set(h, mul2(fma2(u, g1, sub2(g, g0)), r2));
         }
-        o.store(dx + (r + k) * p.os[1] + vec * N, N > 2 || 2 * vec + 1 < p.width);
+        o.store(dx + (r + k) * p.os[1] + vec * N, N > 2 || 2 * vec + 1 < p.width, p.pairs);
       }
     }
   }
@@ -494,6 +588,317 @@ __global__ void __launch_bounds__(512) norm_back_kernel(const __grid_constant__ 
           }
         }
       }
+  }
+}
+
+// 8 values over a warp: afterwards lane 4 i' holds one of them, value_of(lane)
+__device__ __forceinline__ float warp_sum8(float (&v)[8], int lane) {
+#pragma unroll
+  for (int n = 4; n; n >>= 1) {
+    const bool up = lane & (4 * n);
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float give = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, 4 * n);
+    }
+  }
+  float t = v[0];
+  t += __shfl_xor_sync(0xffffffffu, t, 2);
+  return t + __shfl_xor_sync(0xffffffffu, t, 1);
+}
+__device__ __forceinline__ int value_of(int lane) { return lane >> 2; }
+
+// C pieces of R = 4 / C rows to a thread, the CTA one row wide
+template <typename T, int C>
+__global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_constant__ NormBackParams p) {
+  using P = Piece<T, true>;
+  constexpr int N = P::N, H = N / 2, R = 4 / C, kStages = 4;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ __align__(8) uint64_t full[kStages];
+  __shared__ float slots[2][8][16];
+  __shared__ int abort_flag;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, L = blockDim.x;
+  const uint32_t row_bytes = p.width * sizeof(T), stage_bytes = 2 * R * row_bytes;
+  float* gain = reinterpret_cast<float*>(ring + p.stages * stage_bytes);       // C > 1: A, as term_slot() has it
+  int turn = 0;
+  const int64_t e = blockIdx.x / p.chunks, r1 = p.rows, r0 = (blockIdx.x - e * p.chunks) * R, step = p.chunks * R;
+  const T* dy = static_cast<const T*>(p.dy) + e * p.gs[0];
+  const T* x = static_cast<const T*>(p.x) + e * p.xs[0];
+  T* dx = static_cast<T*>(p.dx) + e * p.os[0];
+  const uint64_t policy = policy_evict_first();
+  auto fill = [&](int s, int64_t r) {
+    const int n = static_cast<int>(min(static_cast<int64_t>(R), r1 - r));
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&full[s])), "r"(2 * n * row_bytes) : "memory");
+    for (int k = 0; k < n; ++k) {
+      uint8_t* to = ring + s * stage_bytes + 2 * k * row_bytes;
+      bulk_load(to, dy + (r + k) * p.gs[1], row_bytes, &full[s], policy);
+      bulk_load(to + row_bytes, x + (r + k) * p.xs[1], row_bytes, &full[s], policy);
+    }
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+    abort_flag = 0;
+    fence_barrier_init();
+    for (int s = 0; s < p.stages && r0 + s * step < r1; ++s) fill(s, r0 + s * step);
+  }
+  auto gain_of = [&](int i) {
+    float t = i >= p.width ? 0.f : p.weight.p ? term_at(p.weight.p, p.weight.dtype, i) : 1.f;
+    if (i < p.width && p.scale.p) t *= 1.f + term_at(p.scale.p, p.scale.dtype, e * p.scale.stride + i);
+    return t;
+  };
+  float2 own[H];
+  if (C == 1) {
+#pragma unroll
+    for (int h = 0; h < H; ++h) own[h] = make_float2(gain_of(threadIdx.x * N + 2 * h), gain_of(threadIdx.x * N + 2 * h + 1));
+  } else if (p.affine) {
+    for (int i = threadIdx.x; i < p.nvec * N; i += L) gain[term_slot<N>(i, p.nvec)] = gain_of(i);
+  }
+  float2 sp[C][H], sq[C][H];
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int h = 0; h < H; ++h) sp[c][h] = sq[c][h] = make_float2(0.f, 0.f);
+  auto gains = [&](int vec, float2 (&a)[H]) {
+    if (C == 1) {
+#pragma unroll
+      for (int h = 0; h < H; ++h) a[h] = own[h];
+    } else if (p.affine) {
+      term_load<N>(gain, vec, p.nvec, a);
+    } else {
+#pragma unroll
+      for (int h = 0; h < H; ++h) a[h] = make_float2(1.f, 1.f);
+    }
+  };
+  __syncthreads();
+  bool ok = true;
+  int it = 0;
+  for (int64_t r = r0; r < r1; r += step, ++it) {
+    const int s = it % p.stages;
+    // (a wait that ran out: the launch ends without further waits, its status says so)
+    ok = ok && mbar_wait(&full[s], (it / p.stages) & 1, p.status, &abort_flag);
+    const uint8_t* from = ring + s * stage_bytes;
+    P vg[R][C], vx[R][C];
+    float mean[R], rstd[R], sum[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum[k] = 0.f;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const bool in = r + k < r1;
+      mean[k] = in ? __ldg(p.mean + e * p.rows + r + k) : 0.f;
+      rstd[k] = in ? __ldg(p.rstd + e * p.rows + r + k) : 0.f;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int vec = threadIdx.x + c * L;
+        vg[k][c].clear();
+        vx[k][c].clear();
+        if (in && vec < p.nvec) {
+          const uint4 g = *reinterpret_cast<const uint4*>(from + 2 * k * row_bytes + vec * 16);
+          const uint4 v = *reinterpret_cast<const uint4*>(from + (2 * k + 1) * row_bytes + vec * 16);
+          vg[k][c].w[0] = g.x; vg[k][c].w[1] = g.y; vg[k][c].w[2] = g.z; vg[k][c].w[3] = g.w;
+          vx[k][c].w[0] = v.x; vx[k][c].w[1] = v.y; vx[k][c].w[2] = v.z; vx[k][c].w[3] = v.w;
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int vec = threadIdx.x + c * L;
+      if (vec >= p.nvec) break;
+      float2 a[H];
+      gains(vec, a);
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const float2 r2 = make_float2(rstd[k], rstd[k]), m2 = make_float2(mean[k], mean[k]);
+        float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const float2 d = vg[k][c].pair(h), u = mul2(sub2(vx[k][c].pair(h), m2), r2), g = mul2(d, a[h]);
+          sq[c][h] = add2(sq[c][h], d);
+          sp[c][h] = fma2(d, u, sp[c][h]);
+          s0 = add2(s0, g);
+          s1 = fma2(g, u, s1);
+        }
+        sum[2 * k] += s0.x + s0.y;
+        sum[2 * k + 1] += s1.x + s1.y;
+        vg[k][c].packed();
+        vx[k][c].packed();
+      }
+    }
+    turn ^= 1;
+    const float mine = warp_sum8(sum, lane);
+    if ((lane & 3) == 0) slots[turn][value_of(lane)][warp] = mine;
+    __syncthreads();
+    // the stage has been read: its next rows
+    if (threadIdx.x == 0 && ok && r + p.stages * step < r1) fill(s, r + p.stages * step);
+    // lane 4 i + j adds warps j, j + 4, .. of value i
+    float t = 0.f;
+    for (int w = lane & 3; w < warps; w += 4) t += slots[turn][lane >> 2][w];
+    t += __shfl_xor_sync(0xffffffffu, t, 1);
+    t += __shfl_xor_sync(0xffffffffu, t, 2);
+    t *= p.inv_width;
+#pragma unroll
+    for (int k = 0; k < 2 * R; ++k) sum[k] = __shfl_sync(0xffffffffu, t, 4 * k);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int vec = threadIdx.x + c * L;
+      if (vec >= p.nvec) break;
+      float2 a[H];
+      gains(vec, a);
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        if (r + k >= r1) break;
+        const float2 r2 = make_float2(rstd[k], rstd[k]), m2 = make_float2(mean[k], mean[k]);
+        const float2 g0 = make_float2(sum[2 * k], sum[2 * k]), g1 = make_float2(-sum[2 * k + 1], -sum[2 * k + 1]);
+        P o;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const float2 u = mul2(sub2(vx[k][c].pair(h), m2), r2), g = mul2(vg[k][c].pair(h), a[h]);
+          o.set(h, mul2(fma2(u, g1, sub2(g, g0)), r2));
+        }
+        o.store(dx + (r + k) * p.os[1] + vec * N, true, true);
+      }
+    }
+  }
+  if (!ok && threadIdx.x == 0) {          // the copies in flight have landed before the CTA leaves (again with a limit)
+    int gave_up = 0;
+    drain_ring<false>(full, p.stages, it, p.status, &gave_up);
+  }
+  if (p.sums) {
+    float* part = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.width;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int vec = threadIdx.x + c * L;
+      if (vec >= p.nvec) break;
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        *reinterpret_cast<float2*>(part + vec * N + 2 * h) = sp[c][h];
+        *reinterpret_cast<float2*>(part + p.width + vec * N + 2 * h) = sq[c][h];
+      }
+    }
+  }
+}
+
+// 8 to 32 lanes to a row, V pieces of R = 2 / V rows to a lane, the next rows fetched before these are used
+template <typename T, int V>
+__global__ void __launch_bounds__(kNormThreads, 2) norm_back_narrow_kernel(const __grid_constant__ NormBackParams p) {
+  using P = Piece<T, true>;
+  constexpr int N = P::N, H = N / 2, R = 2 / V;
+  extern __shared__ __align__(16) float sums[];             // [group][2][nvec * N]
+  const int L = p.lanes, at = threadIdx.x & (L - 1), G = kNormThreads / L, group = threadIdx.x / L;
+  const int64_t e = blockIdx.x / p.chunks, r1 = p.rows, r0 = (blockIdx.x - e * p.chunks) * G * R, step = p.chunks * G * R;
+  float2 a[V][H], sp[V][H], sq[V][H];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      float t[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int n = (at + i * L) * N + 2 * h + j;
+        t[j] = n >= p.width ? 0.f : p.weight.p ? term_at(p.weight.p, p.weight.dtype, n) : 1.f;
+        if (n < p.width && p.scale.p) t[j] *= 1.f + term_at(p.scale.p, p.scale.dtype, e * p.scale.stride + n);
+      }
+      a[i][h] = make_float2(t[0], t[1]);
+      sp[i][h] = sq[i][h] = make_float2(0.f, 0.f);
+    }
+  const T* dy = static_cast<const T*>(p.dy) + e * p.gs[0] + at * N;
+  const T* x = static_cast<const T*>(p.x) + e * p.xs[0] + at * N;
+  T* dx = static_cast<T*>(p.dx) + e * p.os[0] + at * N;
+  struct Rows {
+    P g[R][V], x[R][V];
+    float mean[R], rstd[R];
+  };
+  auto fetch = [&](Rows& v, int64_t r) {
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const int64_t row = r + k * G + group;
+      const bool in = row < r1;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        v.g[k][i].clear();
+        v.x[k][i].clear();
+        if (in && at + i * L < p.nvec) {
+          v.g[k][i].load(dy + row * p.gs[1] + i * L * N, true, true);
+          v.x[k][i].load(x + row * p.xs[1] + i * L * N, true, true);
+        }
+      }
+      v.mean[k] = in ? __ldg(p.mean + e * p.rows + row) : 0.f;
+      v.rstd[k] = in ? __ldg(p.rstd + e * p.rows + row) : 0.f;
+    }
+  };
+  Rows v;
+  fetch(v, r0);
+  for (int64_t r = r0; r < r1; r += step) {
+    Rows next;
+    fetch(next, r + step);
+    float s0[R], s1[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const float2 r2 = make_float2(v.rstd[k], v.rstd[k]), m2 = make_float2(v.mean[k], v.mean[k]);
+      float2 t0 = make_float2(0.f, 0.f), t1 = t0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const float2 d = v.g[k][i].pair(h), u = mul2(sub2(v.x[k][i].pair(h), m2), r2), g = mul2(d, a[i][h]);
+          sq[i][h] = add2(sq[i][h], d);
+          sp[i][h] = fma2(d, u, sp[i][h]);
+          t0 = add2(t0, g);
+          t1 = fma2(g, u, t1);
+        }
+        v.g[k][i].packed();
+        v.x[k][i].packed();
+      }
+      s0[k] = t0.x + t0.y;
+      s1[k] = t1.x + t1.y;
+    }
+    auto step = [&](int d) {
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        s0[k] += __shfl_xor_sync(0xffffffffu, s0[k], d);
+        s1[k] += __shfl_xor_sync(0xffffffffu, s1[k], d);
+      }
+    };
+    if (L >= 32) step(16);
+    if (L >= 16) step(8);
+    step(4);
+    step(2);
+    step(1);
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const int64_t row = r + k * G + group;
+      const float2 r2 = make_float2(v.rstd[k], v.rstd[k]), m2 = make_float2(v.mean[k], v.mean[k]);
+      const float m0 = s0[k] * p.inv_width, m1 = -s1[k] * p.inv_width;
+      const float2 g0 = make_float2(m0, m0), g1 = make_float2(m1, m1);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        P o;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          const float2 u = mul2(sub2(v.x[k][i].pair(h), m2), r2), g = mul2(v.g[k][i].pair(h), a[i][h]);
+          o.set(h, mul2(fma2(u, g1, sub2(g, g0)), r2));
+        }
+        if (row < r1 && at + i * L < p.nvec) o.store(dx + row * p.os[1] + i * L * N, true, true);
+      }
+    }
+    v = next;
+  }
+  if (!p.sums) return;
+  const int room = p.nvec * N;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+      if (at + i * L < p.nvec) {
+        float* to = sums + group * 2 * room + (at + i * L) * N + 2 * h;
+        *reinterpret_cast<float2*>(to) = sp[i][h];
+        *reinterpret_cast<float2*>(to + room) = sq[i][h];
+      }
+  __syncthreads();
+  float* part = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.width;
+  for (int n = threadIdx.x; n < 2 * p.width; n += kNormThreads) {
+    float t = 0.f;
+    for (int g = 0; g < G; ++g) t += sums[g * 2 * room + (n < p.width ? n : room + n - p.width)];
+    part[n] = t;
   }
 }
 
@@ -576,6 +981,10 @@ int norm_validate(const HtrcNormArgs* a) {
   return HTRC_OK;
 }
 
+bool rows_even(const void* p, const int64_t* s, int es) {
+  return reinterpret_cast<uintptr_t>(p) % (2 * es) == 0 && s[0] % 2 == 0 && s[1] % 2 == 0;
+}
+
 bool rows16(const void* p, const int64_t* s, int es) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] * es % 16 == 0 && s[1] * es % 16 == 0;
 }
@@ -598,41 +1007,56 @@ struct RowShape {
   }
 };
 
+// CTAs of a kernel that an SM holds at once
+template <typename K>
+int resident_ctas(K kernel, int threads, size_t smem, int* registers) {
+  if (*registers == 0) {
+    cudaFuncAttributes attr{};
+    if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess) return 0;
+    *registers = attr.numRegs;
+  }
+  const int by_registers = 65536 / ((*registers + 7) / 8 * 8 * threads), by_smem = static_cast<int>(kNormSms / (smem + 3 * 1024));
+  return std::max(1, std::min({by_registers, by_smem, 2048 / threads, 32}));
+}
+
+bool allow_smem(const void* kernel, size_t smem) {
+  return smem <= 40 * 1024 ||
+         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) == cudaSuccess;
+}
+
+template <typename T, bool VEC, int MODE, int V>
+int norm_run(NormParams& p, cudaStream_t st) {
+  constexpr int N = Piece<T, VEC>::N, R = V >= 8 ? 1 : V == 1 ? 4 : 8 / V;
+  auto kernel = norm_rows_kernel<T, VEC, V, MODE>;
+  const int threads = p.lanes > 32 ? p.lanes : kNormThreads, groups = threads / p.lanes;
+  const size_t smem = MODE != QUANT_CODES && p.affine ? static_cast<size_t>(p.nvec) * N * 2 * sizeof(float) : 0;
+  static int registers = 0;
+  const int resident = resident_ctas(kernel, threads, smem, &registers);
+  if (resident == 0 || !allow_smem(reinterpret_cast<const void*>(kernel), smem)) return HTRC_ERR_CUDA;
+  const int64_t ctas = static_cast<int64_t>(sm_count()) * resident;
+  p.chunks = std::min(std::max<int64_t>(1, ctas / p.entries), (p.rows + groups * R - 1) / (groups * R));
+  kernel<<<static_cast<unsigned>(std::min(p.entries * p.chunks, ctas)), threads, smem, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
+}
+
 template <typename T, bool VEC, int MODE>
 int norm_launch(NormParams& p, cudaStream_t st) {
   constexpr int N = Piece<T, VEC>::N;
   p.nvec = (p.width + N - 1) / N;
   const int64_t rows = p.entries * p.rows;
-  int w = 1;
-  while (w < kNormMaxWarps && p.nvec > 32 * w * (VEC ? 8 : 4)) w *= 2;
-  // few rows: more warps to each, as long as a lane has more than two pieces
-  while (w < kNormMaxWarps && p.nvec > 32 * w * 2 && rows * w * 2 <= 4 * sm_count()) w *= 2;
-  p.warps = w;
-  const int threads = w > 1 ? 32 * w : kNormThreads, groups = threads / (32 * w);
-  const size_t smem = MODE != QUANT_CODES && p.affine ? static_cast<size_t>(p.nvec) * N * 2 * sizeof(float) : 0;
-  const int resident = std::max<int>(1, std::min<int64_t>(MODE == NORM_CODES ? 512 / threads : 1024 / threads,
-                                                          smem > 0 ? 220 * 1024 / (smem + 1024) : 32));
-  const int64_t ctas = static_cast<int64_t>(sm_count()) * resident;
-  p.chunks = std::max<int64_t>(1, std::min((p.rows + groups - 1) / groups, ctas / std::max<int64_t>(1, p.entries)));
-  p.chunk = (p.rows + p.chunks - 1) / p.chunks;
-  p.chunks = (p.rows + p.chunk - 1) / p.chunk;
-  const unsigned grid = static_cast<unsigned>(std::min(p.entries * p.chunks, ctas));
-  const int per = (p.nvec + 32 * w - 1) / (32 * w);
-  auto go = [&](auto kernel) {
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
-      return HTRC_ERR_CUDA;
-    kernel<<<grid, threads, smem, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
-  };
-  if constexpr (VEC) {
-    if (per <= 2) return go(norm_rows_kernel<T, VEC, 2, MODE>);
-    if (per <= 4) return go(norm_rows_kernel<T, VEC, 4, MODE>);
-    return go(norm_rows_kernel<T, VEC, 8, MODE>);
-  } else {
-    if (per <= 4) return go(norm_rows_kernel<T, VEC, 4, MODE>);
-    return go(norm_rows_kernel<T, VEC, 16, MODE>);
-  }
+  // lanes to a row: four pieces each; a warp takes eight before a row takes several
+  int lanes = 8;
+  while (lanes < 32 * kNormMaxWarps && p.nvec > lanes * (lanes == 32 ? 8 : 4)) lanes *= 2;
+  // few rows: more lanes to each
+  while (lanes < 32 * kNormMaxWarps && p.nvec > lanes && rows * lanes * 2 <= 128 * sm_count()) lanes *= 2;
+  p.lanes = lanes;
+  const int per = (p.nvec + lanes - 1) / lanes;
+  if (per <= 1) return norm_run<T, VEC, MODE, 1>(p, st);
+  if (per <= 2) return norm_run<T, VEC, MODE, 2>(p, st);
+  if (per <= 4) return norm_run<T, VEC, MODE, 4>(p, st);
+  if (VEC || per <= 8) return norm_run<T, VEC, MODE, 8>(p, st);
+  if constexpr (!VEC) return norm_run<T, VEC, MODE, 16>(p, st);
+  return HTRC_ERR_UNSUPPORTED;
 }
 
 template <int MODE>
@@ -671,7 +1095,11 @@ int norm_forward(const HtrcNormArgs* a, cudaStream_t st) {
   p.affine = p.modulated || a->weight || a->bias;
   const int es = type_size(a->dtype);
   bool vec = a->width * es % 16 == 0 && rows16(a->x, a->x_stride, es);
-  if (!codes) vec = vec && rows16(a->out, a->out_stride, es);
+  p.pairs = rows_even(a->x, a->x_stride, es);
+  if (!codes) {
+    vec = vec && rows16(a->out, a->out_stride, es);
+    p.pairs = p.pairs && rows_even(a->out, a->out_stride, es);
+  }
   const RowShape shape = codes ? RowShape(a->batch, a->tokens, p.modulated, {a->x_stride})
                                : RowShape(a->batch, a->tokens, p.modulated, {a->x_stride, a->out_stride});
   p.entries = shape.entries;
@@ -681,13 +1109,47 @@ int norm_forward(const HtrcNormArgs* a, cudaStream_t st) {
   return codes ? norm_types<NORM_CODES>(p, a->dtype, vec, st) : norm_types<NORM_ROWS>(p, a->dtype, vec, st);
 }
 
-int64_t norm_back_chunks(int64_t entries, int64_t rows, int64_t* chunk) {
-  // two CTAs per SM, and no chunk of less than four rows
-  const int64_t want = std::max<int64_t>(1, 2 * sm_count() / std::max<int64_t>(1, entries));
-  const int64_t chunks = std::max<int64_t>(1, std::min(want, (rows + 3) / 4));
-  *chunk = std::max<int64_t>(1, (rows + chunks - 1) / chunks);
-  return std::max<int64_t>(1, (rows + *chunk - 1) / *chunk);
-}
+// How the backward's rows are shared out: the kernel, its CTAs' threads, shared memory and rows
+struct NormBackPlan {
+  enum { NARROW, RING, ANY } kind;
+  int per, lanes, threads, stages;          // per: pieces of a row to a thread
+  size_t smem;
+  int64_t chunks;                           // CTAs of an entry
+  NormBackPlan(int width, int es, bool vec, bool affine, int64_t entries, int64_t rows) {
+    const int n = vec ? 16 / es : 2, nvec = (width + n - 1) / n;
+    int resident;
+    lanes = stages = 0;
+    int least;                              // rows that a CTA takes at a time
+    if (vec && nvec <= 64) {
+      kind = NARROW;
+      lanes = nvec <= 8 ? 8 : nvec <= 16 ? 16 : 32;
+      per = nvec <= lanes ? 1 : 2;
+      threads = kNormThreads;
+      smem = static_cast<size_t>(threads / lanes) * 2 * nvec * n * sizeof(float);
+      resident = 2;
+      least = threads / lanes * (2 / per);
+    } else if (vec && nvec <= 2048) {
+      kind = RING;
+      per = nvec <= 512 ? 1 : nvec <= 1024 ? 2 : 4;
+      threads = ((nvec + per - 1) / per + 31) / 32 * 32;
+      least = 4 / per;
+      resident = std::max(1, 512 / threads);
+      const size_t stage = static_cast<size_t>(8 / per) * width * es, gain = per > 1 && affine ? static_cast<size_t>(nvec) * n * 4 : 0;
+      stages = static_cast<int>(std::max<size_t>(2, std::min<size_t>(4, (200 * 1024 / resident - gain) / stage)));
+      smem = stages * stage + gain;
+    } else {
+      kind = ANY;
+      const int wide = (nvec + 511) / 512;
+      per = vec ? 8 : wide <= 2 ? 2 : wide <= 4 ? 4 : 16;
+      least = per == 2 ? 4 : per == 4 ? 2 : 1;
+      threads = ((nvec + per - 1) / per + 31) / 32 * 32;
+      smem = affine ? static_cast<size_t>(nvec) * n * sizeof(float) : 0;
+      resident = std::max(1, 512 / threads);
+    }
+    const int64_t share = std::max<int64_t>(1, static_cast<int64_t>(resident) * sm_count() / std::max<int64_t>(1, entries));
+    chunks = std::max<int64_t>(1, std::min(share, (rows + least - 1) / least));
+  }
+};
 
 bool norm_sums(const HtrcNormArgs* a) { return a->dweight || a->dbias || a->dscale || a->dshift; }
 
@@ -695,39 +1157,45 @@ RowShape norm_back_shape(const HtrcNormArgs* a) {
   return RowShape(a->batch, a->tokens, a->scale || a->shift, {a->dy_stride, a->x_stride, a->dx_stride});
 }
 
-template <typename T, bool VEC>
-int norm_back_launch(NormBackParams& p, unsigned grid, cudaStream_t st) {
-  constexpr int N = Piece<T, VEC>::N;
-  p.nvec = (p.width + N - 1) / N;
-  const int per = (p.nvec + 511) / 512;
-  const size_t smem = p.affine ? static_cast<size_t>(p.nvec) * N * sizeof(float) : 0;
-  auto go = [&](auto kernel, int c) {
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
-      return HTRC_ERR_CUDA;
-    kernel<<<grid, ((p.nvec + c - 1) / c + 31) / 32 * 32, smem, st>>>(p);
+template <typename T>
+int norm_back_launch(NormBackParams& p, const NormBackPlan& plan, bool vec, cudaStream_t st) {
+  const int n = vec ? static_cast<int>(16 / sizeof(T)) : 2;
+  p.nvec = (p.width + n - 1) / n;
+  p.lanes = plan.lanes;
+  p.stages = plan.stages;
+  p.chunks = plan.chunks;
+  const unsigned grid = static_cast<unsigned>(p.entries * p.chunks);
+  if (grid == 0) return HTRC_OK;
+  auto go = [&](auto kernel) {
+    if (!allow_smem(reinterpret_cast<const void*>(kernel), plan.smem)) return HTRC_ERR_CUDA;
+    kernel<<<grid, plan.threads, plan.smem, st>>>(p);
     return cudaGetLastError() == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
   };
-  if constexpr (VEC) {
-    if (per <= 1) return go(norm_back_kernel<T, VEC, 1, 4, false>, 1);
-    if (per <= 2) return go(norm_back_kernel<T, VEC, 2, 2, false>, 2);
-    if constexpr (N == 8) return go(norm_back_kernel<T, VEC, 4, 1, true>, 4);
-    else return per <= 4 ? go(norm_back_kernel<T, VEC, 4, 1, true>, 4) : go(norm_back_kernel<T, VEC, 8, 1, true>, 8);
-  } else {
-    if (per <= 2) return go(norm_back_kernel<T, VEC, 2, 4, false>, 2);
-    if (per <= 4) return go(norm_back_kernel<T, VEC, 4, 2, false>, 4);
-    return go(norm_back_kernel<T, VEC, 16, 1, true>, 16);
-  }
+  if (plan.kind == NormBackPlan::NARROW)
+    return plan.per == 1 ? go(norm_back_narrow_kernel<T, 1>) : go(norm_back_narrow_kernel<T, 2>);
+  if (plan.kind == NormBackPlan::RING)
+    return plan.per == 1 ? go(norm_back_ring_kernel<T, 1>)
+                         : plan.per == 2 ? go(norm_back_ring_kernel<T, 2>) : go(norm_back_ring_kernel<T, 4>);
+  if (vec) return go(norm_back_any_kernel<T, true, 8, 1, true>);
+  if (plan.per == 2) return go(norm_back_any_kernel<T, false, 2, 4, false>);
+  if (plan.per == 4) return go(norm_back_any_kernel<T, false, 4, 2, false>);
+  return go(norm_back_any_kernel<T, false, 16, 1, true>);
+}
+
+// whether a tensor's rows allow 16-byte pieces, and pairs of elements
+bool back_vec(const HtrcNormArgs* a) {
+  const int es = type_size(a->dtype);
+  return a->width * es % 16 == 0 && rows16(a->x, a->x_stride, es) && rows16(a->dy, a->dy_stride, es) &&
+         rows16(a->dx, a->dx_stride, es);
 }
 
 int norm_back_size(const HtrcNormArgs* a, size_t* bytes) {
   if (bytes == nullptr) return HTRC_ERR_ARG;
   const int rc = norm_validate(a);
   if (rc != HTRC_OK) return rc;
-  int64_t chunk;
   const RowShape shape = norm_back_shape(a);
-  const int64_t chunks = norm_back_chunks(shape.entries, shape.rows, &chunk);
-  *bytes = norm_sums(a) ? static_cast<size_t>(shape.entries) * chunks * 2 * a->width * sizeof(float) : 0;
+  const NormBackPlan plan(a->width, type_size(a->dtype), back_vec(a), a->weight || a->scale, shape.entries, shape.rows);
+  *bytes = norm_sums(a) ? static_cast<size_t>(shape.entries) * plan.chunks * 2 * a->width * sizeof(float) : 0;
   return HTRC_OK;
 }
 
@@ -762,21 +1230,16 @@ int norm_backward(const HtrcNormArgs* a, cudaStream_t st) {
   p.sums = norm_sums(a);
   p.affine = a->weight || a->scale;
   p.part = static_cast<float*>(a->workspace);
-  p.chunks = norm_back_chunks(p.entries, p.rows, &p.chunk);
-  if (p.entries * p.chunks >= kMaxRows) return HTRC_ERR_UNSUPPORTED;
-  const unsigned grid = static_cast<unsigned>(p.entries * p.chunks);
+  const bool vec = back_vec(a);
   const int es = type_size(a->dtype);
-  const bool vec = a->width * es % 16 == 0 && rows16(a->x, a->x_stride, es) && rows16(a->dy, a->dy_stride, es) &&
-                   rows16(a->dx, a->dx_stride, es);
-  if (grid > 0) {
-    if (a->dtype == HTRC_LAYER_F32)
-      rc = vec ? norm_back_launch<float, true>(p, grid, st) : norm_back_launch<float, false>(p, grid, st);
-    else if (a->dtype == HTRC_LAYER_BF16)
-      rc = vec ? norm_back_launch<__nv_bfloat16, true>(p, grid, st) : norm_back_launch<__nv_bfloat16, false>(p, grid, st);
-    else
-      rc = vec ? norm_back_launch<__half, true>(p, grid, st) : norm_back_launch<__half, false>(p, grid, st);
-    if (rc != HTRC_OK) return rc;
-  }
+  p.pairs = rows_even(a->x, a->x_stride, es) && rows_even(a->dy, a->dy_stride, es) && rows_even(a->dx, a->dx_stride, es);
+  p.status = a->status;
+  const NormBackPlan plan(a->width, es, vec, p.affine, p.entries, p.rows);
+  if (p.entries * plan.chunks >= kMaxRows) return HTRC_ERR_UNSUPPORTED;
+  rc = a->dtype == HTRC_LAYER_F32    ? norm_back_launch<float>(p, plan, vec, st)
+       : a->dtype == HTRC_LAYER_BF16 ? norm_back_launch<__nv_bfloat16>(p, plan, vec, st)
+                                     : norm_back_launch<__half>(p, plan, vec, st);
+  if (rc != HTRC_OK) return rc;
   if (p.sums) {
     NormTermsParams t{};
     t.part = p.part;
@@ -817,7 +1280,8 @@ int quantize_rows(const void* x, int dtype, int64_t batch, int64_t tokens, int w
   p.scales = scales;
   p.width = width;
   const int es = type_size(dtype);
-  const bool vec = static_cast<int64_t>(width) * es % 16 == 0 && rows16(x, stride, es);
+  const bool vec = width * es % 16 == 0 && rows16(x, stride, es);
+  p.pairs = rows_even(x, stride, es);
   const RowShape shape(batch, tokens, false, {stride});
   p.entries = shape.entries;
   p.rows = shape.rows;

@@ -20,7 +20,7 @@ import torch
 from . import _lib
 from ._autograd import first_order, recorded
 from ._lib import check, lib
-from .cross import _on
+from .cross import _on, _status_word
 from .linear8 import Int8Rows, _check_float_rows, _DTYPES, _new_codes, _refuse_gradients, _two_strides
 
 
@@ -82,7 +82,7 @@ class _Call:
         return (torch.empty(self.shape[:-1], dtype=torch.float32, device=self.device) for _ in range(2))
 
 
-_NO_BACK = (0,) * 12
+_NO_BACK = (0,) * 13
 
 
 def _forward(c, stats):
@@ -118,7 +118,9 @@ def _backward(c, dy, mean, rstd, wanted=(True,) * 4):
     dx = torch.empty(c.shape, dtype=c.dtype, device=c.device)
     grads = [torch.empty(t.shape, dtype=t.dtype, device=c.device) if t is not None and want else None
              for t, want in zip(c.params, wanted)]
-    tail = (dy.data_ptr(), gb, gn, dx.data_ptr(), *c.rows(), *(0 if g is None else g.data_ptr() for g in grads))
+    status = _status_word(c.device)
+    tail = (dy.data_ptr(), gb, gn, dx.data_ptr(), *c.rows(), *(0 if g is None else g.data_ptr() for g in grads),
+            0 if status is None else status.data_ptr())
     head = (*c.head, *c.terms, 0, 0, 0, 0, 0, 0, mean.data_ptr(), rstd.data_ptr(), *tail)
     ws, wp, need = None, 0, 0
     if any(g is not None for g in grads):

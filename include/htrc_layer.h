@@ -133,6 +133,7 @@ typedef struct {
   int64_t dx_stride[2];
   void *dweight, *dbias;        /* [width], each in its parameter's type, or NULL */
   void *dscale, *dshift;        /* [batch][width] */
+  int32_t* status;              /* as in HtrcCrossArgs */
   void* workspace;              /* htrc_norm_workspace_size() bytes */
   size_t workspace_bytes;
 } HtrcNormArgs;

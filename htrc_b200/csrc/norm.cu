@@ -46,7 +46,6 @@ struct NormParams {
   float *mean, *rstd;
   int64_t entries, rows;                    // rows per entry
   int width, nvec, lanes;                   // pieces per row, lanes per row (a power of two)
-  bool pairs;                               // unaligned rows: two elements stand at multiples of their size
   int64_t chunks;                           // CTAs that share an entry
   float eps, inv_width;
   bool affine, modulated;
@@ -59,11 +58,14 @@ __device__ __forceinline__ float term_at(const void* p, int dtype, int64_t i) {
   return __half2float(static_cast<const __half*>(p)[i]);
 }
 
-// N neighbouring elements as they were read: 16 bytes, or two elements by themselves where rows are not 16-byte aligned
-// (`both`: the second is within the row; it is 0 where not)
-template <typename T, bool VEC>
+// How a row's elements are read: 16 bytes at a time, two neighbours by one load (an even width, rows at multiples of two
+// elements), or two neighbours by themselves
+enum Reads : int { BY_ELEMENT = 0, BY_PAIR = 1, BY_16 = 2 };
+
+// N neighbouring elements as they were read (`both`: the second of two is within the row; it is 0 where not)
+template <typename T, int READ>
 struct Piece {
-  static constexpr int N = VEC ? 16 / sizeof(T) : 2, W = VEC ? 4 : 2;
+  static constexpr int N = READ == BY_16 ? 16 / sizeof(T) : 2, W = READ == BY_16 ? 4 : READ == BY_PAIR ? sizeof(T) / 2 : 2;
   uint32_t w[W];
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -74,23 +76,15 @@ struct Piece {
 #pragma unroll
     for (int i = 0; i < W; ++i) asm volatile("" : "+r"(w[i]));
   }
-  // pairs: the two elements in one load
-  __device__ __forceinline__ void load(const T* p, bool both, bool pairs) {
-    if (!VEC && pairs && both) {
-      if constexpr (sizeof(T) == 4) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-        w[0] = v.x;
-        w[1] = v.y;
-      } else {
-        const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(p));
-        w[0] = v & 0xFFFFu;
-        w[1] = v >> 16;
-      }
-      return;
-    }
-    if constexpr (VEC) {
+  __device__ __forceinline__ void load(const T* p, bool both) {
+    if constexpr (READ == BY_16) {
       const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
       w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else if constexpr (READ == BY_PAIR && sizeof(T) == 4) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = v.x; w[1] = v.y;
+    } else if constexpr (READ == BY_PAIR) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
     } else if constexpr (sizeof(T) == 4) {
       w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
       w[1] = both ? __ldg(reinterpret_cast<const uint32_t*>(p) + 1) : 0;
@@ -106,7 +100,7 @@ struct Piece {
   }
   // elements 2 i and 2 i + 1
   __device__ __forceinline__ float2 pair(int i) const {
-    if constexpr (!VEC || sizeof(T) == 4) {
+    if constexpr (READ == BY_ELEMENT || sizeof(T) == 4) {
       return make_float2(one(w[2 * i]), one(w[2 * i + 1]));
     } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
       return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
@@ -120,7 +114,7 @@ struct Piece {
       w[2 * i + 1] = __float_as_uint(v.y);
     } else {
       const uint32_t two = std::is_same<T, __nv_bfloat16>::value ? pack_bf16x2(v.x, v.y) : pack_f16x2(v.x, v.y);
-      if constexpr (VEC) {
+      if constexpr (READ != BY_ELEMENT) {
         w[i] = two;
       } else {
         w[0] = two & 0xFFFFu;
@@ -128,14 +122,13 @@ struct Piece {
       }
     }
   }
-  __device__ __forceinline__ void store(T* p, bool both, bool pairs) const {
-    if (!VEC && pairs && both) {
-      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-      else *reinterpret_cast<uint32_t*>(p) = w[0] | w[1] << 16;
-      return;
-    }
-    if constexpr (VEC) {
+  __device__ __forceinline__ void store(T* p, bool both) const {
+    if constexpr (READ == BY_16) {
       __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+    } else if constexpr (READ == BY_PAIR && sizeof(T) == 4) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else if constexpr (READ == BY_PAIR) {
+      *reinterpret_cast<uint32_t*>(p) = w[0];
     } else if constexpr (sizeof(T) == 4) {
       *reinterpret_cast<uint32_t*>(p) = w[0];
       if (both) reinterpret_cast<uint32_t*>(p)[1] = w[1];
@@ -153,19 +146,26 @@ __device__ __forceinline__ int term_slot(int e, int nvec) {
   if constexpr (N == 8) return ((e >> 2 & 1) * nvec + (e >> 3)) * 4 + (e & 3);
   return e;
 }
+// a lane's view of them: piece i of it is `at + i * L`
 template <int N>
-__device__ __forceinline__ void term_load(const float* s, int vec, int nvec, float2 (&t)[N / 2]) {
-  if constexpr (N == 2) {
-    t[0] = *reinterpret_cast<const float2*>(s + 2 * vec);
-  } else {
-#pragma unroll
-    for (int h = 0; h < N / 4; ++h) {
-      const float4 v = *reinterpret_cast<const float4*>(s + (h * nvec + vec) * 4);
-      t[2 * h] = make_float2(v.x, v.y);
-      t[2 * h + 1] = make_float2(v.z, v.w);
+struct Terms {
+  const float *lo, *hi;
+  __device__ __forceinline__ Terms(const float* s, int at, int nvec) : lo(s + at * (N == 2 ? 2 : 4)), hi(lo + nvec * 4) {}
+  __device__ __forceinline__ void load(int off, float2 (&t)[N / 2]) const {
+    if constexpr (N == 2) {
+      t[0] = *reinterpret_cast<const float2*>(lo + off * 2);
+    } else {
+      const float4 v = *reinterpret_cast<const float4*>(lo + off * 4);
+      t[0] = make_float2(v.x, v.y);
+      t[1] = make_float2(v.z, v.w);
+      if constexpr (N == 8) {
+        const float4 u = *reinterpret_cast<const float4*>(hi + off * 4);
+        t[2] = make_float2(u.x, u.y);
+        t[3] = make_float2(u.z, u.w);
+      }
     }
   }
-}
+};
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -179,9 +179,10 @@ __device__ __forceinline__ float larger(float a, float b) {      // NaN if eithe
   return m;
 }
 
-// R rows' sums (or maxima) over their L lanes.  L > 32: the CTA is one row's; slots alternate, so one barrier each.
+// R rows' sums (or maxima) over their L lanes.  L > 32: through the group's slots, which alternate, so that one barrier of
+// the group (of its L threads) does for each.
 template <int R, bool MOST>
-__device__ __forceinline__ void over_lanes(float (&v)[R], int L, float (*slots)[kNormMaxWarps][8], int& turn) {
+__device__ __forceinline__ void over_lanes(float (&v)[R], int L, int group, float (*slots)[kNormMaxWarps][4], int& turn) {
   auto step = [&](int d) {
 #pragma unroll
     for (int k = 0; k < R; ++k) {
@@ -200,48 +201,58 @@ __device__ __forceinline__ void over_lanes(float (&v)[R], int L, float (*slots)[
 #pragma unroll
     for (int k = 0; k < R; ++k) slots[turn][threadIdx.x >> 5][k] = v[k];
   }
-  __syncthreads();
-  const int warps = L >> 5;
+  named_bar_sync(1 + group, L);
+  const int warps = L >> 5, first = group * warps;
 #pragma unroll
-  for (int k = 0; k < R; ++k) v[k] = slots[turn][0][k];
+  for (int k = 0; k < R; ++k) v[k] = slots[turn][first][k];
   for (int i = 1; i < warps; ++i) {
 #pragma unroll
-    for (int k = 0; k < R; ++k) v[k] = MOST ? larger(v[k], slots[turn][i][k]) : v[k] + slots[turn][i][k];
+    for (int k = 0; k < R; ++k) v[k] = MOST ? larger(v[k], slots[turn][first + i][k]) : v[k] + slots[turn][first + i][k];
   }
 }
 
-template <typename T, bool VEC, int V, int MODE>
-__global__ void __launch_bounds__(kNormMaxWarps * 32) __maxnreg__(MODE == NORM_CODES ? 128 : MODE == NORM_ROWS ? 80 : 64)
+// LANES: lanes to a row, or 0 for any number (p.lanes); fixed ones have the pieces' offsets in the instructions
+template <typename T, int READ, int V, int LANES, int MODE>
+__global__ void __launch_bounds__(kNormMaxWarps * 32) __maxnreg__(MODE == QUANT_CODES ? 64 : MODE == NORM_CODES || V == 8 ? 128 : 80)
     norm_rows_kernel(const __grid_constant__ NormParams p) {
-  using P = Piece<T, VEC>;
+  using P = Piece<T, READ>;
   constexpr int N = P::N, H = N / 2, R = V >= 8 ? 1 : V == 1 ? 4 : 8 / V;
   extern __shared__ __align__(16) float terms[];
-  __shared__ float slots[2][kNormMaxWarps][8];
-  const int L = p.lanes, at = threadIdx.x & (L - 1), G = blockDim.x / L, group = threadIdx.x / L;
+  __shared__ float slots[2][kNormMaxWarps][4];
+  const int L = LANES ? LANES : p.lanes, at = threadIdx.x & (L - 1), G = blockDim.x / L, group = threadIdx.x / L;
   const int room = p.nvec * N;
-  const float *sa = terms, *sb = terms + room;
+  const Terms<N> ta(terms, at, p.nvec), tb(terms + room, at, p.nvec);
+  // a fixed number of lanes: V is the least power of two that holds a row, so that half of the pieces are whole
+  auto has = [&](int i) { return (LANES && i < V / 2) || at + i * L < p.nvec; };
+  auto two = [&](int i) { return READ != BY_ELEMENT || 2 * (at + i * L) + 1 < p.width; };
   int turn = 0;
   int64_t held = -1;                                        // the entry whose A and B are in shared memory
   const int64_t tasks = p.entries * p.chunks;
   if (MODE != NORM_ROWS) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // a product waits for this kernel's end itself
   for (int64_t task = blockIdx.x; task < tasks; task += gridDim.x) {
     // an entry's CTAs sweep its rows together: neighbouring CTAs at neighbouring rows
-    const int64_t e = task / p.chunks, r0 = (task - e * p.chunks) * G * R, r1 = p.rows, step = p.chunks * G * R;
-    const T* x = static_cast<const T*>(p.x) + e * p.xs[0] + at * N;
-    auto fetch = [&](P (&v)[R][V], int64_t r) {
+    // (fewer than 2^31 rows and 2^20 to a step: unsigned 32 bits hold the row after the last)
+    const int64_t e = task / p.chunks;
+    const uint32_t chunk = static_cast<uint32_t>(task - e * p.chunks), r1 = static_cast<uint32_t>(p.rows);
+    const uint32_t r0 = chunk * G * R, step = static_cast<uint32_t>(p.chunks) * G * R;
+    // row r + group, and what leads from it to the lane's other rows and to the next step's
+    const T* x = static_cast<const T*>(p.x) + e * p.xs[0] + (static_cast<int64_t>(r0) + group) * p.xs[1] + at * N;
+    const int64_t x_step = step * p.xs[1], x_row = G * p.xs[1];
+    auto fetch = [&](P (&v)[R][V], uint32_t r) {
 #pragma unroll
       for (int k = 0; k < R; ++k) {
-        const int64_t row = r + k * G + group;
+        const T* from = x + k * x_row;
+        const bool in = r + k * G + group < r1;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const int vec = at + i * L;
-          if (row < r1 && vec < p.nvec) v[k][i].load(x + row * p.xs[1] + i * L * N, N > 2 || 2 * vec + 1 < p.width, p.pairs);
-          else v[k][i].clear();
+          v[k][i].clear();
+          if (in && has(i)) v[k][i].load(from + i * L * N, two(i));
         }
       }
     };
     P v[R][V];
     fetch(v, r0);
+    x += x_step;
     if (MODE != QUANT_CODES && p.affine && held != (p.modulated ? e : 0)) {
       if (held >= 0) __syncthreads();
       held = p.modulated ? e : 0;
@@ -263,8 +274,14 @@ __global__ void __launch_bounds__(kNormMaxWarps * 32) __maxnreg__(MODE == NORM_C
       }
       __syncthreads();
     }
-    for (int64_t r = r0; r < r1; r += step) {
-      if (MODE != NORM_CODES && r > r0) fetch(v, r);
+    const int64_t row0 = e * p.rows + r0 + group;           // in the statistics and among the 8-bit rows
+    T* out = static_cast<T*>(p.out) + e * p.os[0] + (static_cast<int64_t>(r0) + group) * p.os[1] + at * N;
+    int8_t* codes = p.codes + row0 * p.pitch + at * N;
+    for (uint32_t r = r0; r < r1; r += step) {
+      if (MODE != NORM_CODES && r > r0) {
+        fetch(v, r);
+        x += x_step;
+      }
       float mean[R], rstd[R];
       if (MODE != QUANT_CODES) {
 #pragma unroll
@@ -280,7 +297,7 @@ __global__ void __launch_bounds__(kNormMaxWarps * 32) __maxnreg__(MODE == NORM_C
 #pragma unroll
           for (int i = 0; i < V; ++i) v[k][i].packed();
         }
-        over_lanes<R, false>(mean, L, slots, turn);
+        over_lanes<R, false>(mean, L, group, slots, turn);
 #pragma unroll
         for (int k = 0; k < R; ++k) {
           mean[k] *= p.inv_width;
@@ -289,11 +306,11 @@ __global__ void __launch_bounds__(kNormMaxWarps * 32) __maxnreg__(MODE == NORM_C
           if (r + k * G < r1) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-              if (at + i * L < p.nvec) {
+              if (has(i)) {
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                   float2 d = sub2(v[k][i].pair(h), m2);
-                  if (N == 2 && 2 * (at + i * L) + 1 >= p.width) d.y = 0.f;
+                  if (!two(i)) d.y = 0.f;
                   ss = fma2(d, d, ss);
                 }
               }
@@ -303,23 +320,23 @@ __global__ void __launch_bounds__(kNormMaxWarps * 32) __maxnreg__(MODE == NORM_C
 #pragma unroll
           for (int i = 0; i < V; ++i) v[k][i].packed();
         }
-        over_lanes<R, false>(rstd, L, slots, turn);
+        over_lanes<R, false>(rstd, L, group, slots, turn);
 #pragma unroll
         for (int k = 0; k < R; ++k) {
           rstd[k] = rsqrtf(rstd[k] * p.inv_width + p.eps);
-          const int64_t row = r + k * G + group;
-          if (at == 0 && row < r1) {
-            if (p.mean) p.mean[e * p.rows + row] = mean[k];
-            if (p.rstd) p.rstd[e * p.rows + row] = rstd[k];
+          if (at == 0 && r + k * G + group < r1) {
+            const int64_t row = row0 + (r - r0) + k * G;
+            if (p.mean) p.mean[row] = mean[k];
+            if (p.rstd) p.rstd[row] = rstd[k];
           }
         }
       }
       // the results of piece i of every row, which share its A and B
-      auto results = [&](int i, int vec, auto use) {
+      auto results = [&](int i, auto use) {
         float2 a[H], b[H];
         if (p.affine) {
-          term_load<N>(sa, vec, p.nvec, a);
-          term_load<N>(sb, vec, p.nvec, b);
+          ta.load(i * L, a);
+          tb.load(i * L, b);
         }
 #pragma unroll
         for (int k = 0; k < R; ++k) {
@@ -335,17 +352,22 @@ __global__ void __launch_bounds__(kNormMaxWarps * 32) __maxnreg__(MODE == NORM_C
         }
       };
       if constexpr (MODE == NORM_ROWS) {
-        T* out = static_cast<T*>(p.out) + e * p.os[0] + at * N;
+        T* to[R];
+        bool in[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          to[k] = out + k * G * p.os[1];
+          in[k] = r + k * G + group < r1;
+        }
+        out += step * p.os[1];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const int vec = at + i * L;
-          if (vec < p.nvec) {
-            results(i, vec, [&](int k, float2 (&y)[H]) {
-              const int64_t row = r + k * G + group;
+          if (has(i)) {
+            results(i, [&](int k, float2 (&y)[H]) {
               P o;
 #pragma unroll
               for (int h = 0; h < H; ++h) o.set(h, y[h]);
-              if (row < r1) o.store(out + row * p.os[1] + i * L * N, N > 2 || 2 * vec + 1 < p.width, p.pairs);
+              if (in[k]) o.store(to[k] + i * L * N, two(i));
             });
           }
         }
@@ -361,11 +383,10 @@ __global__ void __launch_bounds__(kNormMaxWarps * 32) __maxnreg__(MODE == NORM_C
         };
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const int vec = at + i * L;
-          const bool both = N > 2 || 2 * vec + 1 < p.width;
-          if (vec < p.nvec) {
+          const bool both = two(i);
+          if (has(i)) {
             if constexpr (MODE == NORM_CODES) {
-              results(i, vec, [&](int k, float2 (&t)[H]) {
+              results(i, [&](int k, float2 (&t)[H]) {
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                   y[k][i][h] = t[h];
@@ -381,23 +402,37 @@ __global__ void __launch_bounds__(kNormMaxWarps * 32) __maxnreg__(MODE == NORM_C
           }
         }
         // the rows as they were read are done with: the next ones arrive while these are quantised
-        if (MODE == NORM_CODES) fetch(v, r + step);
-        over_lanes<R, true>(top, L, slots, turn);
+        if (MODE == NORM_CODES) {
+          fetch(v, r + step);
+          x += x_step;
+        }
+        over_lanes<R, true>(top, L, group, slots, turn);
+        // the lane's rows' factors 127 / top and scales top / 127 by one division in 2 R lanes.  A row with a NaN or an
+        // infinity has no codes: its scale is NaN, and with it what is made of it
+        float factor[R];
+        {
+          const int lane = threadIdx.x & 31, which = lane >> 1 & (R - 1), width = L < 32 ? L : 32;
+          float full = top[0];
+#pragma unroll
+          for (int k = 1; k < R; ++k) full = which == k ? top[k] : full;
+          full = full <= 3.4028235e38f ? fmaxf(full, kLeastTop) : __uint_as_float(0x7FC00000u);
+          const float q = __fdiv_rn(lane & 1 ? full : 127.f, lane & 1 ? 127.f : full);
+#pragma unroll
+          for (int k = 0; k < R; ++k) factor[k] = __shfl_sync(0xffffffffu, q, 2 * k, width);
+          if ((at & 1) && at < 2 * R && r + which * G + group < r1) p.scales[row0 + (r - r0) + which * G] = q;
+        }
+        int8_t* base = codes;
+        codes += step * p.pitch;
 #pragma unroll
         for (int k = 0; k < R; ++k) {
-          const int64_t row = r + k * G + group;
           if (r + k * G >= r1) break;
-          // a row with a NaN or an infinity has no codes: its scale is NaN, and with it what is made of it
-          const float full = top[k] <= 3.4028235e38f ? fmaxf(top[k], kLeastTop) : __uint_as_float(0x7FC00000u);
-          const float by = __fdiv_rn(127.f, full);
-          if (at == 0 && row < r1) p.scales[e * p.rows + row] = __fdiv_rn(full, 127.f);
-          const float2 by2 = make_float2(by, by);
-          int8_t* codes = p.codes + (e * p.rows + row) * p.pitch;
+          const float2 by2 = make_float2(factor[k], factor[k]);
+          int8_t* to = base + k * G * p.pitch;
+          const bool in = r + k * G + group < r1;
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const int vec = at + i * L;
             if (MODE == QUANT_CODES) v[k][i].packed();
-            if (vec < p.nvec && row < r1) {
+            if (has(i) && in) {
               uint32_t c[2 * H];
 #pragma unroll
               for (int h = 0; h < H; ++h) {
@@ -410,15 +445,15 @@ __global__ void __launch_bounds__(kNormMaxWarps * 32) __maxnreg__(MODE == NORM_C
                 c[2 * h + 1] = __float_as_uint(__fadd_rn(z.y, kRoundMagic));
               }
               if constexpr (N == 2) {             // an odd row's last store reaches into the pitch
-                *reinterpret_cast<unsigned short*>(codes + 2 * vec) = static_cast<unsigned short>(__byte_perm(c[0], c[1], 0x0040));
+                *reinterpret_cast<unsigned short*>(to + i * L * N) = static_cast<unsigned short>(__byte_perm(c[0], c[1], 0x0040));
               } else {
                 uint32_t w[N / 4];
 #pragma unroll
                 for (int q = 0; q < N / 4; ++q)
                   w[q] = __byte_perm(__byte_perm(c[4 * q], c[4 * q + 1], 0x0040), __byte_perm(c[4 * q + 2], c[4 * q + 3], 0x0040),
                                      0x5410);
-                if constexpr (N == 8) *reinterpret_cast<uint2*>(codes + vec * 8) = make_uint2(w[0], w[1]);
-                else *reinterpret_cast<uint32_t*>(codes + vec * 4) = w[0];
+                if constexpr (N == 8) *reinterpret_cast<uint2*>(to + i * L * N) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<uint32_t*>(to + i * L * N) = w[0];
               }
             }
           }
@@ -445,7 +480,7 @@ struct NormBackParams {
   int width, nvec;
   int64_t chunks;                           // CTAs that share an entry
   float inv_width;
-  bool sums, affine, pairs;                 // sums: P and Q are wanted
+  bool sums, affine;                        // sums: P and Q are wanted
   int lanes, stages;
   int* status;
   TermView weight, scale;
@@ -453,9 +488,10 @@ struct NormBackParams {
 };
 
 // RELOAD: rows too wide for the registers are read again (from L2) once their sums are known.
-template <typename T, bool VEC, int C, int R, bool RELOAD>
+template <typename T, int READ, int C, int R, bool RELOAD>
 __global__ void __launch_bounds__(512, 1) norm_back_any_kernel(const __grid_constant__ NormBackParams p) {
-  using P = Piece<T, VEC>;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the sums' kernel waits for this one's end itself
+  using P = Piece<T, READ>;
   constexpr int N = P::N, H = N / 2, HELD = RELOAD ? 1 : C;
   __shared__ float slots[2][16][2 * R];
   extern __shared__ __align__(16) float gain[];          // A, as term_slot() has it
@@ -478,7 +514,7 @@ __global__ void __launch_bounds__(512, 1) norm_back_any_kernel(const __grid_cons
   auto gains = [&](int vec, float2 (&a)[H]) {
 #pragma unroll
     for (int h = 0; h < H; ++h) a[h] = make_float2(1.f, 1.f);
-    if (p.affine) term_load<N>(gain, vec, p.nvec, a);
+    if (p.affine) Terms<N>(gain, vec, p.nvec).load(0, a);
   };
   const T* dy = static_cast<const T*>(p.dy) + e * p.gs[0];
   const T* x = static_cast<const T*>(p.x) + e * p.xs[0];
@@ -489,9 +525,9 @@ __global__ void __launch_bounds__(512, 1) norm_back_any_kernel(const __grid_cons
     auto fetch = [&](int k, int c, int to) {
       const int vec = threadIdx.x + c * L;
       if (r + k < r1 && vec < p.nvec) {
-        const bool both = N > 2 || 2 * vec + 1 < p.width;
-        vg[k][to].load(dy + (r + k) * p.gs[1] + vec * N, both, p.pairs);
-        vx[k][to].load(x + (r + k) * p.xs[1] + vec * N, both, p.pairs);
+        const bool both = READ != BY_ELEMENT || 2 * vec + 1 < p.width;
+        vg[k][to].load(dy + (r + k) * p.gs[1] + vec * N, both);
+        vx[k][to].load(x + (r + k) * p.xs[1] + vec * N, both);
       } else {
         vg[k][to].clear();
         vx[k][to].clear();
@@ -568,7 +604,7 @@ __global__ void __launch_bounds__(512, 1) norm_back_any_kernel(const __grid_cons
           const float2 u = mul2(sub2(vx[k][at].pair(h), m2), r2), g = mul2(vg[k][at].pair(h), a[h]);
           o.set(h, mul2(fma2(u, g1, sub2(g, g0)), r2));
         }
-        o.store(dx + (r + k) * p.os[1] + vec * N, N > 2 || 2 * vec + 1 < p.width, p.pairs);
+        o.store(dx + (r + k) * p.os[1] + vec * N, READ != BY_ELEMENT || 2 * vec + 1 < p.width);
       }
     }
   }
@@ -611,11 +647,13 @@ __device__ __forceinline__ int value_of(int lane) { return lane >> 2; }
 // C pieces of R = 4 / C rows to a thread, the CTA one row wide
 template <typename T, int C>
 __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_constant__ NormBackParams p) {
-  using P = Piece<T, true>;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the sums' kernel waits for this one's end itself
+  using P = Piece<T, BY_16>;
   constexpr int N = P::N, H = N / 2, R = 4 / C, kStages = 4;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ __align__(8) uint64_t full[kStages];
   __shared__ float slots[2][8][16];
+  __shared__ __align__(16) float stats[2][2][4];            // the rows' means and reciprocal deviations
   __shared__ int abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, L = blockDim.x;
   const uint32_t row_bytes = p.width * sizeof(T), stage_bytes = 2 * R * row_bytes;
@@ -663,12 +701,17 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
 #pragma unroll
       for (int h = 0; h < H; ++h) a[h] = own[h];
     } else if (p.affine) {
-      term_load<N>(gain, vec, p.nvec, a);
+      Terms<N>(gain, vec, p.nvec).load(0, a);
     } else {
 #pragma unroll
       for (int h = 0; h < H; ++h) a[h] = make_float2(1.f, 1.f);
     }
   };
+  // threads 0 .. 2 R - 1 each fetch one of the next rows' statistics
+  const bool keeps = threadIdx.x < 2 * R;
+  const int64_t ahead = threadIdx.x % R;
+  const float* stat = (threadIdx.x < R ? p.mean : p.rstd) + e * p.rows + ahead;
+  if (keeps) stats[0][threadIdx.x / R][ahead] = r0 + ahead < r1 ? __ldg(stat + r0) : 0.f;
   __syncthreads();
   bool ok = true;
   int it = 0;
@@ -676,24 +719,29 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
     const int s = it % p.stages;
     // (a wait that ran out: the launch ends without further waits, its status says so)
     ok = ok && mbar_wait(&full[s], (it / p.stages) & 1, p.status, &abort_flag);
-    const uint8_t* from = ring + s * stage_bytes;
+    const uint8_t* from = ring + s * stage_bytes + threadIdx.x * 16;
+    const float later = keeps && r + step + ahead < r1 ? __ldg(stat + r + step) : 0.f;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(R), r1 - r));
     P vg[R][C], vx[R][C];
-    float mean[R], rstd[R], sum[8];
+    float mean[4], rstd[4], sum[8];
+    {
+      const float4 m4 = *reinterpret_cast<const float4*>(stats[it & 1][0]), d4 = *reinterpret_cast<const float4*>(stats[it & 1][1]);
+      mean[0] = m4.x; mean[1] = m4.y; mean[2] = m4.z; mean[3] = m4.w;
+      rstd[0] = d4.x; rstd[1] = d4.y; rstd[2] = d4.z; rstd[3] = d4.w;
+    }
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum[k] = 0.f;
 #pragma unroll
     for (int k = 0; k < R; ++k) {
-      const bool in = r + k < r1;
-      mean[k] = in ? __ldg(p.mean + e * p.rows + r + k) : 0.f;
-      rstd[k] = in ? __ldg(p.rstd + e * p.rows + r + k) : 0.f;
+      const bool in = k < rows;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int vec = threadIdx.x + c * L;
         vg[k][c].clear();
         vx[k][c].clear();
         if (in && vec < p.nvec) {
-          const uint4 g = *reinterpret_cast<const uint4*>(from + 2 * k * row_bytes + vec * 16);
-          const uint4 v = *reinterpret_cast<const uint4*>(from + (2 * k + 1) * row_bytes + vec * 16);
+          const uint4 g = *reinterpret_cast<const uint4*>(from + 2 * k * row_bytes + c * L * 16);
+          const uint4 v = *reinterpret_cast<const uint4*>(from + (2 * k + 1) * row_bytes + c * L * 16);
           vg[k][c].w[0] = g.x; vg[k][c].w[1] = g.y; vg[k][c].w[2] = g.z; vg[k][c].w[3] = g.w;
           vx[k][c].w[0] = v.x; vx[k][c].w[1] = v.y; vx[k][c].w[2] = v.z; vx[k][c].w[3] = v.w;
         }
@@ -726,6 +774,7 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
     turn ^= 1;
     const float mine = warp_sum8(sum, lane);
     if ((lane & 3) == 0) slots[turn][value_of(lane)][warp] = mine;
+    if (keeps) stats[(it + 1) & 1][threadIdx.x / R][ahead] = later;
     __syncthreads();
     // the stage has been read: its next rows
     if (threadIdx.x == 0 && ok && r + p.stages * step < r1) fill(s, r + p.stages * step);
@@ -745,7 +794,7 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
       gains(vec, a);
 #pragma unroll
       for (int k = 0; k < R; ++k) {
-        if (r + k >= r1) break;
+        if (k >= rows) break;
         const float2 r2 = make_float2(rstd[k], rstd[k]), m2 = make_float2(mean[k], mean[k]);
         const float2 g0 = make_float2(sum[2 * k], sum[2 * k]), g1 = make_float2(-sum[2 * k + 1], -sum[2 * k + 1]);
         P o;
@@ -754,7 +803,7 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
           const float2 u = mul2(sub2(vx[k][c].pair(h), m2), r2), g = mul2(vg[k][c].pair(h), a[h]);
           o.set(h, mul2(fma2(u, g1, sub2(g, g0)), r2));
         }
-        o.store(dx + (r + k) * p.os[1] + vec * N, true, true);
+        o.store(dx + (r + k) * p.os[1] + vec * N, true);
       }
     }
   }
@@ -780,7 +829,8 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
 // 8 to 32 lanes to a row, V pieces of R = 2 / V rows to a lane, the next rows fetched before these are used
 template <typename T, int V>
 __global__ void __launch_bounds__(kNormThreads, 2) norm_back_narrow_kernel(const __grid_constant__ NormBackParams p) {
-  using P = Piece<T, true>;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the sums' kernel waits for this one's end itself
+  using P = Piece<T, BY_16>;
   constexpr int N = P::N, H = N / 2, R = 2 / V;
   extern __shared__ __align__(16) float sums[];             // [group][2][nvec * N]
   const int L = p.lanes, at = threadIdx.x & (L - 1), G = kNormThreads / L, group = threadIdx.x / L;
@@ -817,8 +867,8 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_back_narrow_kernel(const
         v.g[k][i].clear();
         v.x[k][i].clear();
         if (in && at + i * L < p.nvec) {
-          v.g[k][i].load(dy + row * p.gs[1] + i * L * N, true, true);
-          v.x[k][i].load(x + row * p.xs[1] + i * L * N, true, true);
+          v.g[k][i].load(dy + row * p.gs[1] + i * L * N, true);
+          v.x[k][i].load(x + row * p.xs[1] + i * L * N, true);
         }
       }
       v.mean[k] = in ? __ldg(p.mean + e * p.rows + row) : 0.f;
@@ -877,7 +927,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_back_narrow_kernel(const
           const float2 u = mul2(sub2(v.x[k][i].pair(h), m2), r2), g = mul2(v.g[k][i].pair(h), a[i][h]);
           o.set(h, mul2(fma2(u, g1, sub2(g, g0)), r2));
         }
-        if (row < r1 && at + i * L < p.nvec) o.store(dx + row * p.os[1] + i * L * N, true, true);
+        if (row < r1 && at + i * L < p.nvec) o.store(dx + row * p.os[1] + i * L * N, true);
       }
     }
     v = next;
@@ -917,32 +967,41 @@ __device__ __forceinline__ void term_store(void* p, int dtype, int64_t i, float 
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-// 32 columns per CTA: an entry's parts in 32 interleaved sums and those in order, then the entries in order
-__global__ void __launch_bounds__(1024) norm_terms_kernel(const __grid_constant__ NormTermsParams p) {
-  __shared__ float part[2][32][33];
-  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
-  const int i = blockIdx.x * 32 + lane;
+// 8 columns per CTA, 128 threads to a column: an entry's parts in 128 interleaved sums, those over the warps and then over
+// the CTA, then the entries in order
+__global__ void __launch_bounds__(1024, 1) norm_terms_kernel(const __grid_constant__ NormTermsParams p) {
+  __shared__ float part[2][2][32][8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = threadIdx.x >> 3, col = threadIdx.x & 7;
+  const int i = blockIdx.x * 8 + col;
   const bool in = i < p.width;
   const float w = in && p.weight.p ? term_at(p.weight.p, p.weight.dtype, i) : 1.f;
   const float b = in && p.bias.p ? term_at(p.bias.p, p.bias.dtype, i) : 0.f;
   float dw = 0.f, db = 0.f;
+  asm volatile("griddepcontrol.wait;" ::: "memory");        // the rows' kernel has ended
   for (int64_t e = 0; e < p.entries; ++e) {
     float sp = 0.f, sq = 0.f;
     if (in) {
-      const float* src = p.part + e * p.chunks * 2 * p.width + i;
-      for (int64_t c = row; c < p.chunks; c += 32) {
-        sp += src[c * 2 * p.width];
-        sq += src[c * 2 * p.width + p.width];
+      const float* src = p.part + (e * p.chunks + row) * 2 * p.width + i;
+      for (int64_t c = row; c < p.chunks; c += 128, src += static_cast<int64_t>(256) * p.width) {
+        sp += src[0];
+        sq += src[p.width];
       }
     }
-    part[0][row][lane] = sp;
-    part[1][row][lane] = sq;
-    __syncthreads();
-    if (row == 0 && in) {
+    sp += __shfl_xor_sync(0xffffffffu, sp, 8);
+    sq += __shfl_xor_sync(0xffffffffu, sq, 8);
+    sp += __shfl_xor_sync(0xffffffffu, sp, 16);
+    sq += __shfl_xor_sync(0xffffffffu, sq, 16);
+    if (lane < 8) {
+      part[e & 1][0][warp][col] = sp;
+      part[e & 1][1][warp][col] = sq;
+    }
+    __syncthreads();                                        // (the two buffers alternate)
+    if (threadIdx.x < 8 && in) {
       sp = sq = 0.f;
+#pragma unroll
       for (int k = 0; k < 32; ++k) {
-        sp += part[0][k][lane];
-        sq += part[1][k][lane];
+        sp += part[e & 1][0][k][col];
+        sq += part[e & 1][1][k][col];
       }
       const float s = p.scale.p ? 1.f + term_at(p.scale.p, p.scale.dtype, e * p.scale.stride + i) : 1.f;
       dw = fmaf(sp, s, dw);
@@ -950,9 +1009,8 @@ __global__ void __launch_bounds__(1024) norm_terms_kernel(const __grid_constant_
       if (p.dscale) term_store(p.dscale, p.scale_dtype, e * p.width + i, fmaf(sp, w, sq * b));
       if (p.dshift) term_store(p.dshift, p.shift_dtype, e * p.width + i, sq);
     }
-    __syncthreads();
   }
-  if (row == 0 && in) {
+  if (threadIdx.x < 8 && in) {
     if (p.dweight) term_store(p.dweight, p.weight_dtype, i, dw);
     if (p.dbias) term_store(p.dbias, p.bias_dtype, i, db);
   }
@@ -981,12 +1039,11 @@ int norm_validate(const HtrcNormArgs* a) {
   return HTRC_OK;
 }
 
-bool rows_even(const void* p, const int64_t* s, int es) {
-  return reinterpret_cast<uintptr_t>(p) % (2 * es) == 0 && s[0] % 2 == 0 && s[1] % 2 == 0;
-}
-
-bool rows16(const void* p, const int64_t* s, int es) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] * es % 16 == 0 && s[1] * es % 16 == 0;
+// how the rows of a tensor may be read
+Reads reads_of(const void* p, const int64_t* s, int width, int es) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  if (width * es % 16 == 0 && at % 16 == 0 && s[0] * es % 16 == 0 && s[1] * es % 16 == 0) return BY_16;
+  return width % 2 == 0 && at % (2 * es) == 0 && s[0] % 2 == 0 && s[1] % 2 == 0 ? BY_PAIR : BY_ELEMENT;
 }
 
 // Entries and rows of a launch, and how a tensor's (batch, token) strides step over them: one entry where neither terms
@@ -1024,12 +1081,14 @@ bool allow_smem(const void* kernel, size_t smem) {
          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) == cudaSuccess;
 }
 
-template <typename T, bool VEC, int MODE, int V>
+template <typename T, int READ, int MODE, int V, int LANES>
 int norm_run(NormParams& p, cudaStream_t st) {
-  constexpr int N = Piece<T, VEC>::N, R = V >= 8 ? 1 : V == 1 ? 4 : 8 / V;
-  auto kernel = norm_rows_kernel<T, VEC, V, MODE>;
-  const int threads = p.lanes > 32 ? p.lanes : kNormThreads, groups = threads / p.lanes;
+  constexpr int N = Piece<T, READ>::N, R = V >= 8 ? 1 : V == 1 ? 4 : 8 / V;
+  auto kernel = norm_rows_kernel<T, READ, V, LANES, MODE>;
+  if (LANES) p.lanes = LANES;
   const size_t smem = MODE != QUANT_CODES && p.affine ? static_cast<size_t>(p.nvec) * N * 2 * sizeof(float) : 0;
+  // rows so wide that an SM holds one CTA's A and B: twice the warps share them
+  const int threads = std::max(p.lanes, smem > kNormSms / 2 - 4096 ? 2 * kNormThreads : kNormThreads), groups = threads / p.lanes;
   static int registers = 0;
   const int resident = resident_ctas(kernel, threads, smem, &registers);
   if (resident == 0 || !allow_smem(reinterpret_cast<const void*>(kernel), smem)) return HTRC_ERR_CUDA;
@@ -1039,32 +1098,46 @@ int norm_run(NormParams& p, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
 }
 
-template <typename T, bool VEC, int MODE>
+template <typename T, int READ, int MODE>
 int norm_launch(NormParams& p, cudaStream_t st) {
-  constexpr int N = Piece<T, VEC>::N;
+  constexpr int N = Piece<T, READ>::N;
   p.nvec = (p.width + N - 1) / N;
   const int64_t rows = p.entries * p.rows;
-  // lanes to a row: four pieces each; a warp takes eight before a row takes several
+  // a warp to a row of up to 16 words to a lane (narrower rows: as many lanes as they have pieces, from eight on), more warps
+  // to a wider one
+  constexpr int kMost = READ == BY_16 ? 8 : 16;
   int lanes = 8;
-  while (lanes < 32 * kNormMaxWarps && p.nvec > lanes * (lanes == 32 ? 8 : 4)) lanes *= 2;
-  // few rows: more lanes to each
-  while (lanes < 32 * kNormMaxWarps && p.nvec > lanes && rows * lanes * 2 <= 128 * sm_count()) lanes *= 2;
+  while (lanes < 32 * kNormMaxWarps && p.nvec > lanes * (lanes >= 32 ? kMost : 1)) lanes *= 2;
+  // few rows: as many lanes as a row has pieces
+  int most = lanes;
+  while (most < p.nvec) most *= 2;
+  if (most <= 32 * kNormMaxWarps && rows * most <= 256 * sm_count()) lanes = most;
   p.lanes = lanes;
-  const int per = (p.nvec + lanes - 1) / lanes;
-  if (per <= 1) return norm_run<T, VEC, MODE, 1>(p, st);
-  if (per <= 2) return norm_run<T, VEC, MODE, 2>(p, st);
-  if (per <= 4) return norm_run<T, VEC, MODE, 4>(p, st);
-  if (VEC || per <= 8) return norm_run<T, VEC, MODE, 8>(p, st);
-  if constexpr (!VEC) return norm_run<T, VEC, MODE, 16>(p, st);
-  return HTRC_ERR_UNSUPPORTED;
+  if (p.nvec <= lanes) return norm_run<T, READ, MODE, 1, 0>(p, st);
+  if constexpr (READ == BY_16) {
+    if (lanes == 32 && p.nvec <= 64) return norm_run<T, READ, MODE, 2, 32>(p, st);
+    if (lanes == 32 && p.nvec <= 128) return norm_run<T, READ, MODE, 4, 32>(p, st);
+    if (lanes == 32) return norm_run<T, READ, MODE, 8, 32>(p, st);
+    if (lanes == 64) return norm_run<T, READ, MODE, 8, 64>(p, st);
+    if (lanes == 128) return norm_run<T, READ, MODE, 8, 128>(p, st);
+    if (lanes == 256) return norm_run<T, READ, MODE, 8, 256>(p, st);
+    return norm_run<T, READ, MODE, 8, 512>(p, st);
+  } else {
+    if (p.nvec > 64 && p.nvec <= 128) return norm_run<T, READ, MODE, 4, 32>(p, st);
+    if (p.nvec > 256 && p.nvec <= 512) return norm_run<T, READ, MODE, 16, 32>(p, st);
+    return norm_run<T, READ, MODE, 16, 0>(p, st);
+  }
 }
 
+template <int MODE, typename T>
+int norm_reads(NormParams& p, Reads reads, cudaStream_t st) {
+  if (reads == BY_16) return norm_launch<T, BY_16, MODE>(p, st);
+  return reads == BY_PAIR ? norm_launch<T, BY_PAIR, MODE>(p, st) : norm_launch<T, BY_ELEMENT, MODE>(p, st);
+}
 template <int MODE>
-int norm_types(NormParams& p, int dtype, bool vec, cudaStream_t st) {
-  if (dtype == HTRC_LAYER_F32) return vec ? norm_launch<float, true, MODE>(p, st) : norm_launch<float, false, MODE>(p, st);
-  if (dtype == HTRC_LAYER_BF16)
-    return vec ? norm_launch<__nv_bfloat16, true, MODE>(p, st) : norm_launch<__nv_bfloat16, false, MODE>(p, st);
-  return vec ? norm_launch<__half, true, MODE>(p, st) : norm_launch<__half, false, MODE>(p, st);
+int norm_types(NormParams& p, int dtype, Reads reads, cudaStream_t st) {
+  if (dtype == HTRC_LAYER_F32) return norm_reads<MODE, float>(p, reads, st);
+  return dtype == HTRC_LAYER_BF16 ? norm_reads<MODE, __nv_bfloat16>(p, reads, st) : norm_reads<MODE, __half>(p, reads, st);
 }
 
 int norm_forward(const HtrcNormArgs* a, cudaStream_t st) {
@@ -1094,19 +1167,15 @@ int norm_forward(const HtrcNormArgs* a, cudaStream_t st) {
   p.modulated = a->scale || a->shift;
   p.affine = p.modulated || a->weight || a->bias;
   const int es = type_size(a->dtype);
-  bool vec = a->width * es % 16 == 0 && rows16(a->x, a->x_stride, es);
-  p.pairs = rows_even(a->x, a->x_stride, es);
-  if (!codes) {
-    vec = vec && rows16(a->out, a->out_stride, es);
-    p.pairs = p.pairs && rows_even(a->out, a->out_stride, es);
-  }
+  Reads reads = reads_of(a->x, a->x_stride, a->width, es);
+  if (!codes) reads = std::min(reads, reads_of(a->out, a->out_stride, a->width, es));
   const RowShape shape = codes ? RowShape(a->batch, a->tokens, p.modulated, {a->x_stride})
                                : RowShape(a->batch, a->tokens, p.modulated, {a->x_stride, a->out_stride});
   p.entries = shape.entries;
   p.rows = shape.rows;
   shape.set(a->x_stride, p.xs);
   if (!codes) shape.set(a->out_stride, p.os);
-  return codes ? norm_types<NORM_CODES>(p, a->dtype, vec, st) : norm_types<NORM_ROWS>(p, a->dtype, vec, st);
+  return codes ? norm_types<NORM_CODES>(p, a->dtype, reads, st) : norm_types<NORM_ROWS>(p, a->dtype, reads, st);
 }
 
 // How the backward's rows are shared out: the kernel, its CTAs' threads, shared memory and rows
@@ -1115,7 +1184,8 @@ struct NormBackPlan {
   int per, lanes, threads, stages;          // per: pieces of a row to a thread
   size_t smem;
   int64_t chunks;                           // CTAs of an entry
-  NormBackPlan(int width, int es, bool vec, bool affine, int64_t entries, int64_t rows) {
+  NormBackPlan(int width, int es, Reads reads, bool affine, int64_t entries, int64_t rows) {
+    const bool vec = reads == BY_16;
     const int n = vec ? 16 / es : 2, nvec = (width + n - 1) / n;
     int resident;
     lanes = stages = 0;
@@ -1140,7 +1210,7 @@ struct NormBackPlan {
     } else {
       kind = ANY;
       const int wide = (nvec + 511) / 512;
-      per = vec ? 8 : wide <= 2 ? 2 : wide <= 4 ? 4 : 16;
+      per = vec ? 8 : wide <= 2 ? 2 : wide <= 4 ? 4 : wide <= 8 ? 8 : 16;
       least = per == 2 ? 4 : per == 4 ? 2 : 1;
       threads = ((nvec + per - 1) / per + 31) / 32 * 32;
       smem = affine ? static_cast<size_t>(nvec) * n * sizeof(float) : 0;
@@ -1158,8 +1228,8 @@ RowShape norm_back_shape(const HtrcNormArgs* a) {
 }
 
 template <typename T>
-int norm_back_launch(NormBackParams& p, const NormBackPlan& plan, bool vec, cudaStream_t st) {
-  const int n = vec ? static_cast<int>(16 / sizeof(T)) : 2;
+int norm_back_launch(NormBackParams& p, const NormBackPlan& plan, Reads reads, cudaStream_t st) {
+  const int n = reads == BY_16 ? static_cast<int>(16 / sizeof(T)) : 2;
   p.nvec = (p.width + n - 1) / n;
   p.lanes = plan.lanes;
   p.stages = plan.stages;
@@ -1176,17 +1246,23 @@ int norm_back_launch(NormBackParams& p, const NormBackPlan& plan, bool vec, cuda
   if (plan.kind == NormBackPlan::RING)
     return plan.per == 1 ? go(norm_back_ring_kernel<T, 1>)
                          : plan.per == 2 ? go(norm_back_ring_kernel<T, 2>) : go(norm_back_ring_kernel<T, 4>);
-  if (vec) return go(norm_back_any_kernel<T, true, 8, 1, true>);
-  if (plan.per == 2) return go(norm_back_any_kernel<T, false, 2, 4, false>);
-  if (plan.per == 4) return go(norm_back_any_kernel<T, false, 4, 2, false>);
-  return go(norm_back_any_kernel<T, false, 16, 1, true>);
+  auto by = [&](auto read) {
+    constexpr int READ = decltype(read)::value;
+    if (plan.per == 2) return go(norm_back_any_kernel<T, READ, 2, 4, false>);
+    if (plan.per == 4) return go(norm_back_any_kernel<T, READ, 4, 2, false>);
+    if (plan.per == 8) return go(norm_back_any_kernel<T, READ, 8, 1, false>);
+    return go(norm_back_any_kernel<T, READ, 16, 1, true>);
+  };
+  if (reads == BY_PAIR) return by(std::integral_constant<int, BY_PAIR>{});
+  if (reads == BY_ELEMENT) return by(std::integral_constant<int, BY_ELEMENT>{});
+  if constexpr (sizeof(T) == 4) return go(norm_back_any_kernel<T, BY_16, 8, 1, true>);
+  return HTRC_ERR_UNSUPPORTED;            // 16-bit rows of 16-byte pieces are narrow or the ring's
 }
 
-// whether a tensor's rows allow 16-byte pieces, and pairs of elements
-bool back_vec(const HtrcNormArgs* a) {
+Reads back_reads(const HtrcNormArgs* a) {
   const int es = type_size(a->dtype);
-  return a->width * es % 16 == 0 && rows16(a->x, a->x_stride, es) && rows16(a->dy, a->dy_stride, es) &&
-         rows16(a->dx, a->dx_stride, es);
+  return std::min({reads_of(a->x, a->x_stride, a->width, es), reads_of(a->dy, a->dy_stride, a->width, es),
+                   reads_of(a->dx, a->dx_stride, a->width, es)});
 }
 
 int norm_back_size(const HtrcNormArgs* a, size_t* bytes) {
@@ -1194,7 +1270,7 @@ int norm_back_size(const HtrcNormArgs* a, size_t* bytes) {
   const int rc = norm_validate(a);
   if (rc != HTRC_OK) return rc;
   const RowShape shape = norm_back_shape(a);
-  const NormBackPlan plan(a->width, type_size(a->dtype), back_vec(a), a->weight || a->scale, shape.entries, shape.rows);
+  const NormBackPlan plan(a->width, type_size(a->dtype), back_reads(a), a->weight || a->scale, shape.entries, shape.rows);
   *bytes = norm_sums(a) ? static_cast<size_t>(shape.entries) * plan.chunks * 2 * a->width * sizeof(float) : 0;
   return HTRC_OK;
 }
@@ -1230,15 +1306,13 @@ int norm_backward(const HtrcNormArgs* a, cudaStream_t st) {
   p.sums = norm_sums(a);
   p.affine = a->weight || a->scale;
   p.part = static_cast<float*>(a->workspace);
-  const bool vec = back_vec(a);
-  const int es = type_size(a->dtype);
-  p.pairs = rows_even(a->x, a->x_stride, es) && rows_even(a->dy, a->dy_stride, es) && rows_even(a->dx, a->dx_stride, es);
+  const Reads reads = back_reads(a);
   p.status = a->status;
-  const NormBackPlan plan(a->width, es, vec, p.affine, p.entries, p.rows);
+  const NormBackPlan plan(a->width, type_size(a->dtype), reads, p.affine, p.entries, p.rows);
   if (p.entries * plan.chunks >= kMaxRows) return HTRC_ERR_UNSUPPORTED;
-  rc = a->dtype == HTRC_LAYER_F32    ? norm_back_launch<float>(p, plan, vec, st)
-       : a->dtype == HTRC_LAYER_BF16 ? norm_back_launch<__nv_bfloat16>(p, plan, vec, st)
-                                     : norm_back_launch<__half>(p, plan, vec, st);
+  rc = a->dtype == HTRC_LAYER_F32    ? norm_back_launch<float>(p, plan, reads, st)
+       : a->dtype == HTRC_LAYER_BF16 ? norm_back_launch<__nv_bfloat16>(p, plan, reads, st)
+                                     : norm_back_launch<__half>(p, plan, reads, st);
   if (rc != HTRC_OK) return rc;
   if (p.sums) {
     NormTermsParams t{};
@@ -1257,7 +1331,16 @@ int norm_backward(const HtrcNormArgs* a, cudaStream_t st) {
     t.bias_dtype = a->bias_dtype;
     t.scale_dtype = a->scale_dtype;
     t.shift_dtype = a->shift_dtype;
-    norm_terms_kernel<<<(a->width + 31) / 32, 1024, 0, st>>>(t);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((a->width + 7) / 8);
+    cfg.blockDim = dim3(1024);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, norm_terms_kernel, t) != cudaSuccess) return HTRC_ERR_CUDA;
   }
   return cudaGetLastError() == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
 }
@@ -1279,14 +1362,11 @@ int quantize_rows(const void* x, int dtype, int64_t batch, int64_t tokens, int w
   p.pitch = pitch;
   p.scales = scales;
   p.width = width;
-  const int es = type_size(dtype);
-  const bool vec = width * es % 16 == 0 && rows16(x, stride, es);
-  p.pairs = rows_even(x, stride, es);
   const RowShape shape(batch, tokens, false, {stride});
   p.entries = shape.entries;
   p.rows = shape.rows;
   shape.set(stride, p.xs);
-  return norm_types<QUANT_CODES>(p, dtype, vec, st);
+  return norm_types<QUANT_CODES>(p, dtype, reads_of(x, stride, width, type_size(dtype)), st);
 }
 
 }  // namespace htrc

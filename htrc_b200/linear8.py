@@ -33,11 +33,11 @@ class Int8Rows(NamedTuple):
 
 
 def _check_codes(rows, name):
-    if not (isinstance(rows, tuple) and len(rows) == 2 and all(isinstance(t, torch.Tensor) for t in rows)):
+    if not isinstance(rows, tuple) or len(rows) != 2:
         raise ValueError(f"{name}: Int8Rows (codes, scales) expected")
     codes, scales = rows
-    if codes.dtype is not torch.int8 or codes.dim() < 1 or scales.dtype is not torch.float32 or \
-            scales.shape != codes.shape[:-1]:
+    if not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor) or codes.dtype is not torch.int8 or \
+            codes.dim() < 1 or scales.dtype is not torch.float32 or scales.shape != codes.shape[:-1]:
         raise ValueError(f"{name}: int8 codes [.., width] and float32 scales [..] expected")
     if not codes.is_cuda or scales.device != codes.device:
         raise ValueError(f"{name} must be on one CUDA device (there is no CPU path)")
@@ -50,9 +50,11 @@ def _pitch(codes):
     if codes.data_ptr() & 15 or (stride[-1] != 1 and shape[-1] != 1):
         return None
     pitch = covered = None
-    for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+    for i in range(len(shape) - 2, -1, -1):
+        n = shape[i]
         if n == 1:
             continue
+        s = stride[i]
         if pitch is None:
             pitch = s
         elif s != covered:
@@ -63,12 +65,13 @@ def _pitch(codes):
     return pitch if pitch >= shape[-1] and not pitch & 15 else None
 
 
-def _new_codes(shape, device):
-    """Codes [.., width] whose rows start at multiples of 16 bytes: (codes, pitch)."""
+def _new_codes(shape, like):
+    """Codes [.., width] on the tensor's device whose rows start at multiples of 16 bytes: (codes, pitch)."""
     width = shape[-1]
     pitch = (width + 15) // 16 * 16
-    codes = torch.empty((*shape[:-1], pitch), dtype=torch.int8, device=device)
-    return (codes if pitch == width else codes[..., :width]), pitch
+    if pitch == width:
+        return like.new_empty(shape, dtype=torch.int8), pitch
+    return like.new_empty((*shape[:-1], pitch), dtype=torch.int8)[..., :width], pitch
 
 
 def int8_rows(codes, scales):
@@ -76,31 +79,28 @@ def int8_rows(codes, scales):
     they are), so that no product has to."""
     codes, scales = _check_codes((codes, scales), "rows")
     if _pitch(codes) is None:
-        laid, _ = _new_codes(codes.shape, codes.device)
+        laid, _ = _new_codes(codes.shape, codes)
         codes = laid.copy_(codes)
     return Int8Rows(codes, scales.contiguous())
 
 
 def _two_strides(x):
     """x [.., width] as (tensor, batch, tokens, width, batch stride, token stride); a copy only where its strides need one."""
-    if x.dim() == 0 or x.shape[-1] < 1:
-        raise ValueError("rows of at least one element expected")
-    if x.stride(-1) != 1 and x.shape[-1] != 1:
-        x = x.contiguous()
     d = x.dim()
-    if d == 3:
-        (b, n, w), (sb, sn, _) = x.shape, x.stride()
-    elif d == 2:
-        (n, w), (sn, _) = x.shape, x.stride()
-        b, sb = 1, 0
-    elif d == 1:
-        b, n, w, sb, sn = 1, 1, x.shape[0], 0, 0
-    else:
+    if d > 3:
         x = x.reshape(-1, x.shape[-2], x.shape[-1]) if x.numel() else x.new_empty((0, 1, x.shape[-1]))
-        if x.stride(-1) != 1 and x.shape[-1] != 1:
-            x = x.contiguous()
-        (b, n, w), (sb, sn, _) = x.shape, x.stride()
-    return x, b, n, w, sb, sn
+    shape, stride = x.shape, x.stride()
+    w = shape[-1]
+    if w < 1:
+        raise ValueError("rows of at least one element expected")
+    if stride[-1] != 1 and w != 1:
+        x = x.contiguous()
+        stride = x.stride()
+    if d >= 3:
+        return x, shape[0], shape[1], w, stride[0], stride[1]
+    if d == 2:
+        return x, 1, shape[0], w, 0, stride[0]
+    return x, 1, 1, w, 0, 0
 
 
 def _check_float_rows(x):
@@ -127,8 +127,8 @@ def quantize_rows(x):
     kept, b, n, w, sb, sn = _two_strides(x)
     if w > _lib.NORM_MAX_WIDTH:
         raise NotImplementedError(f"rows of up to {_lib.NORM_MAX_WIDTH} elements are supported, got {w}")
-    codes, pitch = _new_codes(shape, x.device)
-    scales = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    codes, pitch = _new_codes(shape, x)
+    scales = x.new_empty(shape[:-1], dtype=torch.float32)
     check(lib().htrc_quantize_rows(kept.data_ptr(), _DTYPES[x.dtype], b, n, w, (ctypes.c_int64 * 2)(sb, sn),
                                    codes.data_ptr(), pitch, scales.data_ptr(), _lib.raw_stream(x.device.index)),
           "htrc_quantize_rows")
@@ -186,14 +186,13 @@ def int8_linear(x, weight, *, bias=None, dtype=None):
         ws = ws.contiguous()
     if bias is not None:
         bias = bias.contiguous()
-    out = torch.empty((*lead, channels), dtype=dtype, device=dev)
+    out = ws.new_empty((*lead, channels), dtype=dtype)
     if floats:
         kept, b, n, _, sb, sn = _two_strides(x)
         kind, scales, rows = _DTYPES[x.dtype], 0, b * n
-        room = (rows * ((width + 15) // 16 * 16) + 255) // 256 * 256
-        need = room + 4 * rows
-        ws8 = torch.empty(need, dtype=torch.uint8, device=dev)
-        wp = ws8.data_ptr()
+        need = (rows * ((width + 15) // 16 * 16) + 255) // 256 * 256 + 4 * rows      # htrc_linear8_workspace_size's
+        workspace = ws.new_empty((need,), dtype=torch.uint8)
+        wp = workspace.data_ptr()
     else:
         pitch = _pitch(codes)
         if pitch is None:

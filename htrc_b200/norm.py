@@ -24,65 +24,63 @@ from .cross import _on, _status_word
 from .linear8 import Int8Rows, _check_float_rows, _DTYPES, _new_codes, _refuse_gradients, _two_strides
 
 
+def _term(t, name, shapes, width, device):
+    """(tensor, pointer, type) of a parameter of one of the shapes, its last dimension dense; (None, 0, 0) of None."""
+    if t is None:
+        return None, 0, 0
+    if not isinstance(t, torch.Tensor) or t.shape not in shapes or t.dtype not in _DTYPES or t.device != device:
+        raise ValueError(f"{name}: {list(shapes[0])} float32, bfloat16 or float16 on x's device expected")
+    if width != 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    return t, t.data_ptr(), _DTYPES[t.dtype]
+
+
 class _Call:
     """The checked arguments of one call: rows and parameters as the kernels take them."""
-    __slots__ = ("x", "shape", "dtype", "device", "batch", "tokens", "width", "head", "terms", "keep", "params")
+    __slots__ = ("x", "given", "device", "head", "terms", "keep", "params", "dense")
 
     def __init__(self, x, weight, bias, scale, shift, eps):
         _check_float_rows(x)
         if not (eps >= 0 and math.isfinite(eps)):
             raise ValueError("eps must be non-negative and finite")
-        self.shape, self.dtype, self.device = x.shape, x.dtype, x.device
-        self.params = (weight, bias, scale, shift)
+        self.given = x
+        dev = self.device = x.device
+        dims = x.dim()
         modulated = scale is not None or shift is not None
-        if modulated and x.dim() > 3:
+        if modulated and dims > 3:
             x = x.reshape(x.shape[0], math.prod(x.shape[1:-1]), x.shape[-1])
-        x, self.batch, self.tokens, self.width, sb, sn = _two_strides(x)
-        width = self.width
+        x, batch, tokens, width, sb, sn = _two_strides(x)
         if width > _lib.NORM_MAX_WIDTH:
             raise NotImplementedError(f"rows of up to {_lib.NORM_MAX_WIDTH} elements are supported, got {width}")
         self.x = x
-        pointers, strides, kinds, self.keep = [], [], [], []
-        for name, t in (("weight", weight), ("bias", bias)):
-            if t is None:
-                pointers.append(0)
-                kinds.append(0)
-                continue
-            if not isinstance(t, torch.Tensor) or t.shape != (width,) or t.dtype not in _DTYPES or t.device != x.device:
-                raise ValueError(f"{name}: [{width}] float32, bfloat16 or float16 on x's device expected")
-            t = t.contiguous()
-            self.keep.append(t)
-            pointers.append(t.data_ptr())
-            kinds.append(_DTYPES[t.dtype])
-        # a modulation per entry of the first dimension; of rows without one, a single vector
-        want = (self.batch, width) if len(self.shape) > 2 else (width,)
-        for name, t in (("scale", scale), ("shift", shift)):
-            if t is None:
-                pointers.append(0)
-                kinds.append(0)
-                strides.append(0)
-                continue
-            if not isinstance(t, torch.Tensor) or t.shape not in (want, (*want[:-1], 1, width)) or \
-                    t.dtype not in _DTYPES or t.device != x.device:
-                raise ValueError(f"{name}: {list(want)} float32, bfloat16 or float16 on x's device expected")
-            if t.stride(-1) != 1 and width != 1:
-                t = t.contiguous()
-            self.keep.append(t)
-            pointers.append(t.data_ptr())
-            kinds.append(_DTYPES[t.dtype])
-            strides.append(t.stride(0) if len(want) == 2 else 0)
-        self.head = (x.data_ptr(), sb, sn, self.batch, self.tokens, width, _DTYPES[x.dtype])
-        self.terms = (*pointers, *strides, *kinds, eps)
-
-    def rows(self):
-        """(batch, token) strides of dense rows."""
-        return self.tokens * self.width, self.width
-
-    def statistics(self):
-        return (torch.empty(self.shape[:-1], dtype=torch.float32, device=self.device) for _ in range(2))
+        self.params = (weight, bias, scale, shift)
+        self.keep = ()
+        self.terms = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, eps)
+        if modulated or weight is not None or bias is not None:
+            w, wp, wk = _term(weight, "weight", ((width,),), width, dev)
+            b, bp, bk = _term(bias, "bias", ((width,),), width, dev)
+            sp = sk = ss = tp = tk = ts = 0
+            s = t = None
+            if modulated:
+                # a modulation per entry of the first dimension; of rows without one, a single vector
+                shapes = ((batch, width), (batch, 1, width)) if dims > 2 else ((width,), (1, width))
+                s, sp, sk = _term(scale, "scale", shapes, width, dev)
+                t, tp, tk = _term(shift, "shift", shapes, width, dev)
+                if dims > 2:
+                    ss = 0 if s is None else s.stride(0)
+                    ts = 0 if t is None else t.stride(0)
+            self.keep = (w, b, s, t)
+            self.terms = (wp, bp, sp, tp, ss, ts, wk, bk, sk, tk, eps)
+        self.head = (x.data_ptr(), sb, sn, batch, tokens, width, _DTYPES[x.dtype])
+        self.dense = (tokens * width, width)         # (batch, token) strides of dense rows
 
 
 _NO_BACK = (0,) * 13
+
+
+def _like(x):
+    """A dense tensor of x's shape and type."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _forward(c, stats):
@@ -90,46 +88,68 @@ def _forward(c, stats):
     if guard is not None:
         with guard:
             return _forward(c, stats)
-    out = torch.empty(c.shape, dtype=c.dtype, device=c.device)
-    mean, rstd = c.statistics() if stats else (None, None)
-    args = _lib.NORM_ARGS.pack(*c.head, *c.terms, out.data_ptr(), *c.rows(), 0, 0, 0, mean.data_ptr() if stats else 0,
-                               rstd.data_ptr() if stats else 0, *_NO_BACK)
+    x = c.given
+    out = _like(x)
+    mean = rstd = None
+    mp = rp = 0
+    if stats:
+        mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+        rstd = torch.empty_like(mean)
+        mp, rp = mean.data_ptr(), rstd.data_ptr()
+    args = _lib.NORM_ARGS.pack(*c.head, *c.terms, out.data_ptr(), *c.dense, 0, 0, 0, mp, rp, *_NO_BACK)
     rc = lib().htrc_norm_forward(args, _lib.raw_stream(c.device.index))
     if rc:
         check(rc, "htrc_norm_forward")
     return out, mean, rstd
 
 
+_workspaces = {}
+
+
+def _workspace_bytes(key, args):
+    """What the backward asks for: it goes by sizes, strides and alignments alone (``key``)."""
+    need = _workspaces.get(key)
+    if need is None:
+        size = ctypes.c_size_t()
+        check(lib().htrc_norm_workspace_size(args, size), "htrc_norm_workspace_size")
+        if len(_workspaces) >= 1024:
+            _workspaces.clear()
+        need = _workspaces[key] = size.value
+    return need
+
+
 def _backward(c, dy, mean, rstd, wanted=(True,) * 4):
     """dx and the gradients of weight, bias, scale and shift: None for those that are none or not wanted."""
-    if not isinstance(dy, torch.Tensor) or dy.shape != c.shape or dy.dtype != c.dtype or dy.device != c.device:
-        raise ValueError(f"dy: {list(c.shape)} {c.dtype} on x's device expected")
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        if not isinstance(t, torch.Tensor) or t.shape != c.shape[:-1] or t.dtype is not torch.float32 or t.device != c.device:
-            raise ValueError(f"{name}: {list(c.shape[:-1])} float32 on x's device expected")
-    guard = _on(c.device)
+    x, dev = c.given, c.device
+    shape = x.shape
+    if not isinstance(dy, torch.Tensor) or dy.shape != shape or dy.dtype != x.dtype or dy.device != dev:
+        raise ValueError(f"dy: {list(shape)} {x.dtype} on x's device expected")
+    for t in (mean, rstd):
+        if not isinstance(t, torch.Tensor) or t.shape != shape[:-1] or t.dtype is not torch.float32 or t.device != dev:
+            raise ValueError(f"mean and rstd: {list(shape[:-1])} float32 on x's device expected")
+    guard = _on(dev)
     if guard is not None:
         with guard:
             return _backward(c, dy, mean, rstd, wanted)
     mean, rstd = mean.contiguous(), rstd.contiguous()
     if dy.dim() > 3:
-        dy = dy.reshape(c.batch, c.tokens, c.width)
+        dy = dy.reshape(c.x.shape)
     dy, _, _, _, gb, gn = _two_strides(dy)
-    dx = torch.empty(c.shape, dtype=c.dtype, device=c.device)
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=c.device) if t is not None and want else None
-             for t, want in zip(c.params, wanted)]
-    status = _status_word(c.device)
-    tail = (dy.data_ptr(), gb, gn, dx.data_ptr(), *c.rows(), *(0 if g is None else g.data_ptr() for g in grads),
-            0 if status is None else status.data_ptr())
-    head = (*c.head, *c.terms, 0, 0, 0, 0, 0, 0, mean.data_ptr(), rstd.data_ptr(), *tail)
+    dx = _like(x)
+    grads = [_like(t) if t is not None and want else None for t, want in zip(c.params, wanted)]
+    pointers = [0 if g is None else g.data_ptr() for g in grads]
+    status = _status_word(dev)
+    gp = dy.data_ptr()
+    head = (*c.head, *c.terms, 0, 0, 0, 0, 0, 0, mean.data_ptr(), rstd.data_ptr(), gp, gb, gn, dx.data_ptr(), *c.dense,
+            *pointers, 0 if status is None else status.data_ptr())
     ws, wp, need = None, 0, 0
-    if any(g is not None for g in grads):
-        size = ctypes.c_size_t()
-        check(lib().htrc_norm_workspace_size(_lib.NORM_ARGS.pack(*head, 0, 0), size), "htrc_norm_workspace_size")
-        need = size.value
-        ws = torch.empty(need, dtype=torch.uint8, device=c.device)
+    if any(pointers):
+        w, _, s, t = (p != 0 for p in c.terms[:4])
+        need = _workspace_bytes((*c.head[1:], gb, gn, c.head[0] & 15, gp & 15, w, s, t, dev.index),
+                                _lib.NORM_ARGS.pack(*head, 0, 0))
+        ws = x.new_empty((need,), dtype=torch.uint8)
         wp = ws.data_ptr()
-    rc = lib().htrc_norm_backward(_lib.NORM_ARGS.pack(*head, wp, need), _lib.raw_stream(c.device.index))
+    rc = lib().htrc_norm_backward(_lib.NORM_ARGS.pack(*head, wp, need), _lib.raw_stream(dev.index))
     if rc:
         check(rc, "htrc_norm_backward")
     return (dx, *grads)
@@ -184,8 +204,9 @@ def _codes(c):
     if guard is not None:
         with guard:
             return _codes(c)
-    codes, pitch = _new_codes(c.shape, c.device)
-    scales = torch.empty(c.shape[:-1], dtype=torch.float32, device=c.device)
+    x = c.given
+    codes, pitch = _new_codes(x.shape, x)
+    scales = x.new_empty(x.shape[:-1], dtype=torch.float32)
     args = _lib.NORM_ARGS.pack(*c.head, *c.terms, 0, 0, 0, codes.data_ptr(), pitch, scales.data_ptr(), 0, 0, *_NO_BACK)
     rc = lib().htrc_norm_forward(args, _lib.raw_stream(c.device.index))
     if rc:

@@ -81,7 +81,7 @@ constexpr int kSmallChannels = 128;
 
 template <int T>
 struct SmallShape {
-  static constexpr int kStages = T <= 32 ? 5 : T <= 64 ? 4 : 3;      // two CTAs per SM
+  static constexpr int kStages = T <= 32 ? 5 : T <= 64 ? 4 : 3;      // two CTAs per SM (one of T = 256)
   static constexpr uint32_t kW = kSmallChannels * 128, kX = T * 128, kStage = kW + kX;
   static constexpr uint32_t kCols = T < 32 ? 32 : T;
   static constexpr uint32_t kBars = kStages * kStage, kBytes = kBars + 128;
@@ -210,13 +210,25 @@ __global__ void __launch_bounds__(kSmallThreads)
       const int n = n0 + 32 * warp + lane;
       if (n < p.channels) {
         const float ws = __ldg(p.ws + n), bias = bias_at(p, n);
-        const int rows = min(T, p.rows - row0);
-        for (int t = rank; t < rows; t += splits) {
-          const uint32_t mine = smem_u32(smem) + (t * kSmallChannels + 32 * warp + lane) * 4;
-          int sum = 0;
-          for (int c = 0; c < splits; ++c) sum += load_cluster(in_cta(mine, c));
-          const int64_t r = row0 + t;
-          static_cast<O*>(p.out)[r * p.channels + n] = from_f<O>(scaled(sum, __ldg(p.xs + r), ws, bias));
+        const int rows = min(T, p.rows - row0), share = T / splits, first = rank * share;
+        constexpr int kBatch = T / 8 < 8 ? T / 8 : 8;       // tokens whose parts are in flight together
+        for (int t0 = first; t0 < min(first + share, rows); t0 += kBatch) {
+          const uint32_t mine = smem_u32(smem) + (t0 * kSmallChannels + 32 * warp + lane) * 4;
+          int sum[kBatch];
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j) sum[j] = 0;
+          for (int c = 0; c < splits; ++c) {
+            const uint32_t at = in_cta(mine, c);
+            int v[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) v[j] = load_cluster(at + j * kSmallChannels * 4);
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) sum[j] += v[j];
+          }
+          O* out = static_cast<O*>(p.out) + static_cast<int64_t>(row0 + t0) * p.channels + n;
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j)
+            if (t0 + j < rows) out[static_cast<int64_t>(j) * p.channels] = from_f<O>(scaled(sum[j], __ldg(p.xs + row0 + t0 + j), ws, bias));
         }
       }
     }
@@ -598,7 +610,7 @@ int linear8_launch(Linear8Params& p, const int8_t* x, int64_t pitch, const HtrcL
   p.tiles_n = (p.channels + kSmallChannels - 1) / kSmallChannels;
   const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
   p.splits = 1;
-  while (p.splits < 8 && tiles * p.splits * 2 <= 2 * sm_count() && p.blocks >= 4 * p.splits) p.splits *= 2;
+  while (p.splits < 8 && tiles * p.splits * 2 <= sm_count() && p.blocks >= 4 * p.splits) p.splits *= 2;
   if (tile == 16) return small_launch<16, O>(mx, mw, p, st);
   if (tile == 32) return small_launch<32, O>(mx, mw, p, st);
   if (tile == 64) return small_launch<64, O>(mx, mw, p, st);

@@ -141,26 +141,71 @@ def int8_linear_status(device=None):
     return cross_status(device)
 
 
+_plans = {}
+
+
+def _meta(t):
+    return (t.shape, t.stride(), t.dtype, t.device)
+
+
 def int8_linear(x, weight, *, bias=None, dtype=None):
     """x [.., width], as float rows (quantised on the way) or ``Int8Rows``, times weight (``Int8Rows`` of
     [channels, width]) -> [.., channels] in ``dtype``: x's by default, bfloat16 for ``Int8Rows``.
 
     bias: [channels] float32, bfloat16 or float16."""
+    floats = isinstance(x, torch.Tensor)
+    # what follows from shapes, strides and types alone is kept for calls that repeat them: the checks cost more host time
+    # than the rest of a small call
+    try:
+        wc, ws = weight
+        rows, xs = (x, None) if floats else x
+        key = (_meta(rows), None if floats else _meta(xs), _meta(wc), _meta(ws), None if bias is None else _meta(bias), dtype)
+        plan = None if wc.data_ptr() & 15 or (not floats and rows.data_ptr() & 15) else _plans.get(key)
+        _refuse_gradients("int8_linear", rows, xs, ws, bias)
+    except (AttributeError, TypeError, ValueError):       # no tensors: the checks say so
+        key = plan = None
+    if plan is None:
+        rows, xs, wc, ws, bias, plan, whole = _plan(x, weight, bias, dtype, floats)
+        if whole and key is not None:
+            if len(_plans) >= 1024:
+                _plans.clear()
+            _plans[key] = plan
+    dev, sizes, wpitch, kinds, shape, dtype, need = plan
+    guard = _on(dev)
+    if guard is not None:
+        with guard:
+            return int8_linear(x, weight, bias=bias, dtype=dtype)
+    out = ws.new_empty(shape, dtype=dtype)
+    wp = 0
+    if floats:
+        workspace = ws.new_empty((need,), dtype=torch.uint8)
+        wp = workspace.data_ptr()
+    status = _status_word(dev)
+    sb, sn, *rest = sizes
+    rc = lib().htrc_linear8_forward(
+        _lib.LINEAR8_ARGS.pack(rows.data_ptr(), sb, sn, 0 if floats else xs.data_ptr(), *rest, wc.data_ptr(), wpitch,
+                               ws.data_ptr(), 0 if bias is None else bias.data_ptr(), *kinds, out.data_ptr(),
+                               0 if status is None else status.data_ptr(), wp, need), _lib.raw_stream(dev.index))
+    if rc:
+        check(rc, "htrc_linear8_forward")
+    return out
+
+
+def _plan(x, weight, bias, dtype, floats):
+    """The call's operands as the kernels read them, what follows from their shapes, strides and types, and whether every
+    operand is read as it was given."""
     wc, ws = _check_codes(weight, "weight")
     if wc.dim() != 2 or wc.shape[0] < 1 or wc.shape[1] < 1:
         raise ValueError("weight: Int8Rows of [channels, width] expected")
-    floats = isinstance(x, torch.Tensor)
     if floats:
         _check_float_rows(x)
-        codes, xs = x, None
-        _refuse_gradients("int8_linear", x, ws, bias)
+        rows, xs = x, None
     else:
-        codes, xs = _check_codes(x, "x")
-        _refuse_gradients("int8_linear", xs, ws, bias)
-    dev = codes.device
+        rows, xs = _check_codes(x, "x")
+    dev = rows.device
     channels, width = wc.shape
-    if codes.shape[-1] != width:
-        raise ValueError(f"x: rows of {width} elements expected, got {codes.shape[-1]}")
+    if rows.shape[-1] != width:
+        raise ValueError(f"x: rows of {width} elements expected, got {rows.shape[-1]}")
     most = _lib.NORM_MAX_WIDTH if floats else _lib.LINEAR8_MAX_WIDTH
     if width > most:
         raise NotImplementedError(f"rows of up to {most} elements are supported, got {width}")
@@ -173,40 +218,29 @@ def int8_linear(x, weight, *, bias=None, dtype=None):
         dtype = x.dtype if floats else torch.bfloat16
     elif dtype not in _DTYPES:
         raise ValueError("dtype: float32, bfloat16 or float16 expected")
-    guard = _on(dev)
-    if guard is not None:
-        with guard:
-            return int8_linear(x, weight, bias=bias, dtype=dtype)
-    lead = codes.shape[:-1]
-    wpitch = _pitch(wc)
-    if wpitch is None:
-        wc, ws = int8_rows(wc, ws)
+    given = (rows, xs, wc, ws, bias)
+    shape = (*rows.shape[:-1], channels)
+    with torch.cuda.device(dev):
         wpitch = _pitch(wc)
-    elif not ws.is_contiguous():
+        if wpitch is None:
+            wc, ws = int8_rows(wc, ws)
+            wpitch = _pitch(wc)
         ws = ws.contiguous()
-    if bias is not None:
-        bias = bias.contiguous()
-    out = ws.new_empty((*lead, channels), dtype=dtype)
-    if floats:
-        kept, b, n, _, sb, sn = _two_strides(x)
-        kind, scales, rows = _DTYPES[x.dtype], 0, b * n
-        need = (rows * ((width + 15) // 16 * 16) + 255) // 256 * 256 + 4 * rows      # htrc_linear8_workspace_size's
-        workspace = ws.new_empty((need,), dtype=torch.uint8)
-        wp = workspace.data_ptr()
-    else:
-        pitch = _pitch(codes)
-        if pitch is None:
-            codes, xs = int8_rows(codes, xs)
-            pitch = _pitch(codes)
-        xs = xs.contiguous()
-        kept, kind, scales = codes, _lib.LAYER_I8, xs.data_ptr()
-        b, n, sb, sn, wp, need = 1, xs.numel(), 0, pitch, 0, 0
-    status = _status_word(dev)
-    args = _lib.LINEAR8_ARGS.pack(
-        kept.data_ptr(), sb, sn, scales, b, n, width, channels, kind, wc.data_ptr(), wpitch, ws.data_ptr(),
-        0 if bias is None else bias.data_ptr(), 0 if bias is None else _DTYPES[bias.dtype], _DTYPES[dtype], out.data_ptr(),
-        0 if status is None else status.data_ptr(), wp, need)
-    rc = lib().htrc_linear8_forward(args, _lib.raw_stream(dev.index))
-    if rc:
-        check(rc, "htrc_linear8_forward")
-    return out
+        bias = None if bias is None else bias.contiguous()
+        need = 0
+        if floats:
+            rows, b, n, _, sb, sn = _two_strides(rows)
+            need = (b * n * ((width + 15) // 16 * 16) + 255) // 256 * 256 + 4 * b * n      # htrc_linear8_workspace_size's
+        else:
+            sn = _pitch(rows)
+            if sn is None:
+                rows, xs = int8_rows(rows, xs)
+                sn = _pitch(rows)
+            xs = xs.contiguous()
+            b, n, sb = 1, xs.numel(), 0
+    sizes = (sb, sn, b, n, width, channels, _DTYPES[rows.dtype] if floats else _lib.LAYER_I8)
+    kinds = (0 if bias is None else _DTYPES[bias.dtype], _DTYPES[dtype])
+    used = (rows, xs, wc, ws, bias)
+    whole = all(a is b or (a is not None and b is not None and a.data_ptr() == b.data_ptr() and a.numel() == b.numel())
+                for a, b in zip(given, used))
+    return *used, (dev, sizes, wpitch, kinds, shape, dtype, need), whole

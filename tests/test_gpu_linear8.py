@@ -112,6 +112,20 @@ def test_shapes_and_strides(dev):
     assert htrc_b200.int8_rows(*laid).codes.data_ptr() == laid.codes.data_ptr()
 
 
+def test_repeated_calls_with_other_alignments(dev):
+    """What a call keeps for the next goes by shapes, strides and types, and no pointer is taken to be aligned."""
+    gen = torch.Generator(device=dev).manual_seed(13)
+    room = torch.randint(-127, 128, (90 * 112 + 64,), generator=gen, device=dev, dtype=torch.int8)
+    scales = torch.rand(90, generator=gen, device=dev)
+    for start in (0, 16, 0, 3, 32, 1, 0):
+        x = Int8Rows(room[start:].as_strided((90, 96), (112, 1)), scales)
+        w = Int8Rows(x.codes[:70], scales[:70])
+        f = torch.randn(90 * 96 + 64, generator=gen, device=dev).bfloat16()[start:start + 90 * 96].view(90, 96)
+        for _ in range(2):
+            _check(htrc_b200.int8_linear(x, w, dtype=torch.float32), x, w, None, torch.float32)
+            _check(htrc_b200.int8_linear(f, w), htrc_b200.quantize_rows(f), w, None, torch.bfloat16)
+
+
 @pytest.mark.parametrize("tokens,channels", [(1, 1), (3, 77), (130, 130), (300, 520), (2100, 1030), (700, 2048),
                                              (5000, 1032), (9000, 515)])
 def test_what_lies_around_the_result_is_left_alone(dev, tokens, channels):

@@ -169,6 +169,28 @@ def test_strides_and_shapes(dev, dtype):
     _close(y[None], want, off)
 
 
+def test_repeated_calls_with_other_alignments_and_modulated_dimensions(dev):
+    """What a call keeps for the next goes by shapes, strides and types: pointers of other alignments are read as they are."""
+    gen = torch.Generator(device=dev).manual_seed(12)
+    for dtype in TYPES:
+        room = torch.randn(2 * 3 * 5 * 72 + 64, generator=gen, device=dev).to(dtype)
+        kw = _params(gen, dev, "wbst", 2, 64, dtype)
+        kw["shift"] = kw["shift"][:, 0]
+        for start in (0, 8, 0, 1, 2, 8):
+            x = room[start:].as_strided((2, 3, 5, 64), (3 * 5 * 72, 5 * 72, 72, 1))
+            for _ in range(2):
+                y, mean, rstd = htrc_b200.layer_norm(x, **kw, return_stats=True)
+                flat = x.reshape(2, 15, 64)
+                want, off, *_ = _plain(flat, kw)
+                _close(y.reshape(2, 15, 64), want, off)
+                dy = torch.randn((2, 3, 5, 80), generator=gen, device=dev).to(dtype)[..., start:start + 64]
+                got = htrc_b200.layer_norm_backward(dy, x, mean, rstd, **kw)
+                _check_backward((got[0].reshape(2, 15, 64), *got[1:]), dy.reshape(2, 15, 64), flat, mean.reshape(2, 15),
+                                rstd.reshape(2, 15), kw)
+                rows = htrc_b200.quantize_rows(x)
+                assert torch.equal(rows.codes.double(), _codes(x)[0])
+
+
 def test_large_offset_and_constant_rows(dev):
     """A mean far above the deviations loses no more than its own rounding; a constant row gives the shift."""
     gen = torch.Generator(device=dev).manual_seed(6)

@@ -3,7 +3,7 @@
 // on tcgen05 (kind::i8: int32 sums in TMEM, exact), the scales and the bias in float32 on the way out.
 //
 // Few tokens (linear8_small_kernel): the weights are what is read, so they take the product's 128-row side, a tile of
-// 16 to 128 tokens its other.  Where the tiles alone leave SMs idle a cluster shares a tile, each CTA a range of the width;
+// 16 to 64 tokens its other.  Where the tiles alone leave SMs idle a cluster shares a tile, each CTA a range of the width;
 // their integer sums are added over distributed shared memory, which changes no result.
 //
 // Many tokens (linear8_pair_kernel): two CTAs on neighbouring SMs share a tile of 256 tokens x 256 channels (cta_group::2),
@@ -81,7 +81,7 @@ constexpr int kSmallChannels = 128;
 
 template <int T>
 struct SmallShape {
-  static constexpr int kStages = T <= 32 ? 5 : T <= 64 ? 4 : 3;      // two CTAs per SM (one of T = 256)
+  static constexpr int kStages = T <= 32 ? 5 : 4;          // two CTAs per SM
   static constexpr uint32_t kW = kSmallChannels * 128, kX = T * 128, kStage = kW + kX;
   static constexpr uint32_t kCols = T < 32 ? 32 : T;
   static constexpr uint32_t kBars = kStages * kStage, kBytes = kBars + 128;
@@ -265,10 +265,10 @@ int small_launch(const CUtensorMap& mx, const CUtensorMap& mw, const Linear8Para
 // ------------------------------------------------------------------------------------------------ many tokens
 // Of the pair's 256 x 256 tile each CTA holds the sums of its own 128 tokens (TMEM lanes) and all 256 channels (columns),
 // twice.  Warps 0-7: the way out, 32 tokens x 128 channels each; 8: TMA; 9: MMA issue (the leader's, rank 0).
-constexpr int kPairThreads = 320, kPairStages = 6;
+constexpr int kPairThreads = 320, kPairStages = 5, kPairOuts = 2;
 constexpr int kPairRows = 256, kPairChannels = 256;         // of the pair
 constexpr uint32_t kPairTile = 128 * 128, kPairStage = 2 * kPairTile;
-constexpr uint32_t kPairOut = kPairStages * kPairStage, kPairTable = kPairOut + 8 * 4096, kPairBars = kPairTable + 2 * kPairChannels * 4;
+constexpr uint32_t kPairOut = kPairStages * kPairStage, kPairTable = kPairOut + 8 * kPairOuts * 4096, kPairBars = kPairTable + 2 * kPairChannels * 4;
 constexpr uint32_t kPairBytes = kPairBars + 192;
 constexpr int kPairGroup = 8;                               // row tiles that are walked together: their operands stay in L2
 
@@ -449,26 +449,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   } else {
     constexpr int kCols = 128 / sizeof(O);                  // of a staged 128-byte row
     float* table = reinterpret_cast<float*>(smem + kPairTable);
-    uint8_t* stage = smem + kPairOut + warp * 4096;
+    uint8_t* const stages = smem + kPairOut + warp * kPairOuts * 4096;
     const int quarter = warp & 3, side = warp >> 2;
     const uint32_t at = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + 128 * side;
     const uint32_t leaders[2] = {in_cta(smem_u32(&bars->sums_empty[0]), 0), in_cta(smem_u32(&bars->sums_empty[1]), 0)};
+    // a tile's scales and biases, a thread a channel, and the thread's row's scale: read one tile ahead
+    float2 term = make_float2(0.f, 0.f);
+    float xs = 0.f;
+    auto fetch = [&](int t) {
+      if (t >= tiles) return;
+      int row, channel;
+      pair_tile(p, t, row, channel);
+      row += 128 * rank + 32 * quarter + lane;
+      const int n = channel + threadIdx.x;
+      term = n < p.channels ? make_float2(__ldg(p.ws + n), bias_at(p, n)) : make_float2(0.f, 0.f);
+      xs = row < p.rows ? __ldg(p.xs + row) : 0.f;
+    };
+    fetch(first);
     bool ok = aligned;
-    int turn = 0;
+    int turn = 0, out_turn = 0;
     // (a warp whose wait ran out goes on to the barriers that the others stand at, without work)
     for (int t = first; t < tiles; t += pairs, ++turn) {
       int row, channel;
       pair_tile(p, t, row, channel);
       row += 128 * rank + 32 * quarter;
       const int half = turn & 1;
-      // the tile's scales and biases, a thread a channel
-      const int n = channel + threadIdx.x;
-      const float2 term = n < p.channels ? make_float2(__ldg(p.ws + n), bias_at(p, n)) : make_float2(0.f, 0.f);
-      const float xs = row + lane < p.rows ? __ldg(p.xs + row + lane) : 0.f;
       named_bar_sync(1, 256);
       table[threadIdx.x] = term.x;
       table[kPairChannels + threadIdx.x] = term.y;
+      const float row_scale = xs;
       named_bar_sync(1, 256);
+      fetch(t + pairs);
       ok = ok && wait_cluster(&bars->sums_full[half], (turn / 2) & 1, p.status, abort_flag);
       if (!ok) continue;
       tc_fence_after();
@@ -476,7 +487,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const float* ws = table + 128 * side;
 #pragma unroll 1
       for (int c = 0; c < 128; c += kCols) {
-        bulk_wait_group_read0();                            // lane 0's: the stage has left
+        uint8_t* const stage = stages + (out_turn++ % kPairOuts) * 4096;
+        asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kPairOuts - 1) : "memory");      // lane 0's: the stage has left
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < kCols; i += 32) {
@@ -492,8 +504,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           for (int j = 0; j < 32; j += 4) {
             const float4 s4 = *reinterpret_cast<const float4*>(ws + c + i + j);
             const float4 b4 = *reinterpret_cast<const float4*>(ws + kPairChannels + c + i + j);
-            const float y0 = scaled(static_cast<int>(v[j]), xs, s4.x, b4.x), y1 = scaled(static_cast<int>(v[j + 1]), xs, s4.y, b4.y);
-            const float y2 = scaled(static_cast<int>(v[j + 2]), xs, s4.z, b4.z), y3 = scaled(static_cast<int>(v[j + 3]), xs, s4.w, b4.w);
+            const float y0 = scaled(static_cast<int>(v[j]), row_scale, s4.x, b4.x), y1 = scaled(static_cast<int>(v[j + 1]), row_scale, s4.y, b4.y);
+            const float y2 = scaled(static_cast<int>(v[j + 2]), row_scale, s4.z, b4.z), y3 = scaled(static_cast<int>(v[j + 3]), row_scale, s4.w, b4.w);
             if constexpr (sizeof(O) == 4) {
               v[j] = __float_as_uint(y0);
               v[j + 1] = __float_as_uint(y1);
@@ -520,13 +532,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             bulk_commit_group();
           }
         } else {
-          // rows of any alignment: element by element, a row's neighbours together
+          // rows of any alignment, by 4-byte words, a row's neighbours together (19,000 x 1,024 x 3,499 in bfloat16: see the
+          // launch's comment)
           __syncwarp();
+          const int cols = min(kCols, p.channels - (channel + c)), high = min(32, p.rows - row);
           O* out = static_cast<O*>(p.out) + static_cast<int64_t>(row) * p.channels + channel + c;
-          for (int r = 0; r < 32 && row + r < p.rows; ++r)
-            for (int e = lane; e < kCols && channel + c + e < p.channels; e += 32)
-              out[static_cast<int64_t>(r) * p.channels + e] =
-                  *reinterpret_cast<const O*>(stage + sw128_off(r, e * sizeof(O) / 16) + e * sizeof(O) % 16);
+#pragma unroll 4
+          for (int r = 0; r < high; ++r, out += p.channels) {
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(stage + sw128_off(r, lane / 4) + lane % 4 * 4);
+            if constexpr (sizeof(O) == 4) {
+              if (lane < cols) reinterpret_cast<uint32_t*>(out)[lane] = word;
+            } else {
+              // where the row starts inside a word its first element stands alone, and the words hold the ones after it
+              const uint32_t next = __shfl_down_sync(0xffffffffu, word, 1);
+              const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(out) >> 1 & 1), e = 2 * lane + odd;
+              const uint32_t two = odd ? __byte_perm(word, next, 0x5432) : word;
+              unsigned short* to = reinterpret_cast<unsigned short*>(out);
+              if (e + 1 < cols && e + 1 < kCols) *reinterpret_cast<uint32_t*>(to + e) = two;
+              else if (e < cols) to[e] = static_cast<unsigned short>(two);
+              if (odd && lane == 0 && cols > 0) to[0] = static_cast<unsigned short>(word);
+            }
+          }
           __syncwarp();
         }
       }
@@ -581,8 +607,10 @@ int linear8_validate(const HtrcLinear8Args* a) {
 
 template <typename O>
 int linear8_launch(Linear8Params& p, const int8_t* x, int64_t pitch, const HtrcLinear8Args* a, cudaStream_t st) {
+  // Pairs where their tiles occupy half of the SMs (1,024 x 4,096 x 4,096: 18.5 us, by tiles of 64 tokens 30.1), not for so few
+  // tokens that most of a tile would be empty.
   const int64_t pairs = (static_cast<int64_t>(p.rows) + 255) / 256 * ((static_cast<int64_t>(p.channels) + 255) / 256);
-  if (pairs >= sm_count() / 2) {
+  if (p.rows > 128 && pairs >= 32) {
     CUtensorMap mx, mw, mo;
     constexpr int es = sizeof(O);
     p.direct = p.channels * es % 16 != 0 || reinterpret_cast<uintptr_t>(p.out) % 16 != 0;
@@ -602,19 +630,21 @@ int linear8_launch(Linear8Params& p, const int8_t* x, int64_t pitch, const HtrcL
     p.tiles_n = (p.channels + kPairChannels - 1) / kPairChannels;
     return pair_launch<O>(mx, mw, mo, p, st);
   }
-  const int tile = p.rows <= 16 ? 16 : p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : 128;
+  // tokens of a tile: 64 (512 x 1,024 x 4,096: 8.3 us, of 128 tokens 11.5, of 32 11.9), fewer where there are fewer
+  const int tile = p.rows <= 16 ? 16 : p.rows <= 32 ? 32 : 64;
   CUtensorMap mx, mw;
   if (!code_map(&mx, x, p.rows, a->width, pitch, tile) || !code_map(&mw, a->w, p.channels, a->width, a->w_pitch, kSmallChannels))
     return HTRC_ERR_CUDA;
   p.tiles_m = (p.rows + tile - 1) / tile;
   p.tiles_n = (p.channels + kSmallChannels - 1) / kSmallChannels;
+  // a tile's width is split while its parts are longer than 8 blocks and leave SMs idle: 64 x 4,096 x 4,096 10.2 us in 4 parts
+  // and 15 whole; 16 x 1,024 x 4,096 4.1 whole and 5.4 in 2; 16 x 4,096 x 16,384 14.1 whole and 16.4 in 2
   const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
   p.splits = 1;
-  while (p.splits < 8 && tiles * p.splits * 2 <= sm_count() && p.blocks >= 4 * p.splits) p.splits *= 2;
+  while (p.splits < 8 && tiles * p.splits * 4 <= 3 * sm_count() && p.blocks > 8 * p.splits) p.splits *= 2;
   if (tile == 16) return small_launch<16, O>(mx, mw, p, st);
   if (tile == 32) return small_launch<32, O>(mx, mw, p, st);
-  if (tile == 64) return small_launch<64, O>(mx, mw, p, st);
-  return small_launch<128, O>(mx, mw, p, st);
+  return small_launch<64, O>(mx, mw, p, st);
 }
 
 int linear8_forward(const HtrcLinear8Args* a, cudaStream_t st) {

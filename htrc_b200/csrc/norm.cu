@@ -759,11 +759,11 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
         float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-          const float2 d = vg[k][c].pair(h), u = mul2(sub2(vx[k][c].pair(h), m2), r2), g = mul2(d, a[h]);
+          const float2 d = vg[k][c].pair(h), dl = mul2(d, sub2(vx[k][c].pair(h), m2));
           sq[c][h] = add2(sq[c][h], d);
-          sp[c][h] = fma2(d, u, sp[c][h]);
-          s0 = add2(s0, g);
-          s1 = fma2(g, u, s1);
+          sp[c][h] = fma2(dl, r2, sp[c][h]);
+          s0 = fma2(d, a[h], s0);
+          s1 = fma2(dl, a[h], s1);
         }
         sum[2 * k] += s0.x + s0.y;
         sum[2 * k + 1] += s1.x + s1.y;
@@ -795,14 +795,14 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
 #pragma unroll
       for (int k = 0; k < R; ++k) {
         if (k >= rows) break;
+        // dx = (x - mean) (-rstd^3 mean(g (x - mean))) + dy (A rstd) - rstd mean(g)
+        const float f0 = -rstd[k] * sum[2 * k], f1 = -rstd[k] * (rstd[k] * (rstd[k] * sum[2 * k + 1]));
         const float2 r2 = make_float2(rstd[k], rstd[k]), m2 = make_float2(mean[k], mean[k]);
-        const float2 g0 = make_float2(sum[2 * k], sum[2 * k]), g1 = make_float2(-sum[2 * k + 1], -sum[2 * k + 1]);
+        const float2 g0 = make_float2(f0, f0), g1 = make_float2(f1, f1);
         P o;
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-          const float2 u = mul2(sub2(vx[k][c].pair(h), m2), r2), g = mul2(vg[k][c].pair(h), a[h]);
-          o.set(h, mul2(fma2(u, g1, sub2(g, g0)), r2));
-        }
+        for (int h = 0; h < H; ++h)
+          o.set(h, fma2(sub2(vx[k][c].pair(h), m2), g1, fma2(vg[k][c].pair(h), mul2(a[h], r2), g0)));
         o.store(dx + (r + k) * p.os[1] + vec * N, true);
       }
     }
@@ -953,12 +953,14 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_back_narrow_kernel(const
 }
 
 struct NormTermsParams {
-  const float* part;
-  int64_t entries, chunks;
-  int width;
+  float* part;                              // P and Q of a part: [2][width]
+  int64_t lists, count, list_stride, part_stride;    // lists of `count` parts
+  int width, columns;                       // columns: CTAs to a list
+  bool entries;                             // a list is a batch entry's, else all of the entries' weighted sums
   TermView weight, bias, scale;             // scale: of the modulation
   void *dweight, *dbias, *dscale, *dshift;
   int weight_dtype, bias_dtype, scale_dtype, shift_dtype;
+  bool keep;                                // an entry's sums times its modulation, for the sum over entries, in its first part
 };
 
 __device__ __forceinline__ void term_store(void* p, int dtype, int64_t i, float v) {
@@ -967,52 +969,66 @@ __device__ __forceinline__ void term_store(void* p, int dtype, int64_t i, float 
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-// 8 columns per CTA, 128 threads to a column: an entry's parts in 128 interleaved sums, those over the warps and then over
-// the CTA, then the entries in order
+// A list's parts added up, 32 columns to a CTA: each warp every blockDim / 32th part, the warps' sums by a tree
 __global__ void __launch_bounds__(1024, 1) norm_terms_kernel(const __grid_constant__ NormTermsParams p) {
-  __shared__ float part[2][2][32][8];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = threadIdx.x >> 3, col = threadIdx.x & 7;
-  const int i = blockIdx.x * 8 + col;
-  const bool in = i < p.width;
-  const float w = in && p.weight.p ? term_at(p.weight.p, p.weight.dtype, i) : 1.f;
-  const float b = in && p.bias.p ? term_at(p.bias.p, p.bias.dtype, i) : 0.f;
-  float dw = 0.f, db = 0.f;
-  asm volatile("griddepcontrol.wait;" ::: "memory");        // the rows' kernel has ended
-  for (int64_t e = 0; e < p.entries; ++e) {
-    float sp = 0.f, sq = 0.f;
-    if (in) {
-      const float* src = p.part + (e * p.chunks + row) * 2 * p.width + i;
-      for (int64_t c = row; c < p.chunks; c += 128, src += static_cast<int64_t>(256) * p.width) {
-        sp += src[0];
-        sq += src[p.width];
-      }
-    }
-    sp += __shfl_xor_sync(0xffffffffu, sp, 8);
-    sq += __shfl_xor_sync(0xffffffffu, sq, 8);
-    sp += __shfl_xor_sync(0xffffffffu, sp, 16);
-    sq += __shfl_xor_sync(0xffffffffu, sq, 16);
-    if (lane < 8) {
-      part[e & 1][0][warp][col] = sp;
-      part[e & 1][1][warp][col] = sq;
-    }
-    __syncthreads();                                        // (the two buffers alternate)
-    if (threadIdx.x < 8 && in) {
-      sp = sq = 0.f;
+  __shared__ float part[2][32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int64_t list = blockIdx.x / p.columns;
+  const int first = static_cast<int>(blockIdx.x - list * p.columns) * 32;
+  float* base = p.part + list * p.list_stride;
+  asm volatile("griddepcontrol.wait;" ::: "memory");        // the kernel that writes the parts has ended
+  float sp = 0.f, sq = 0.f;
+  if (first + lane < p.width) {
+    const float* src = base + warp * p.part_stride + first + lane;
+    const int64_t step = warps * p.part_stride;
+    int64_t c = warp;
+    for (; c + 3 * warps < p.count; c += 4 * warps, src += 4 * step) {
+      float a[4], b[4];
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        sp += part[e & 1][0][k][col];
-        sq += part[e & 1][1][k][col];
+      for (int k = 0; k < 4; ++k) {
+        a[k] = __ldcg(src + k * step);
+        b[k] = __ldcg(src + k * step + p.width);
       }
-      const float s = p.scale.p ? 1.f + term_at(p.scale.p, p.scale.dtype, e * p.scale.stride + i) : 1.f;
-      dw = fmaf(sp, s, dw);
-      db = fmaf(sq, s, db);
-      if (p.dscale) term_store(p.dscale, p.scale_dtype, e * p.width + i, fmaf(sp, w, sq * b));
-      if (p.dshift) term_store(p.dshift, p.shift_dtype, e * p.width + i, sq);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        sp += a[k];
+        sq += b[k];
+      }
     }
+    float a[3] = {0.f, 0.f, 0.f}, b[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (c + k * warps < p.count) {
+        a[k] = __ldcg(src + k * step);
+        b[k] = __ldcg(src + k * step + p.width);
+      }
+    sp += a[0] + a[1] + a[2];
+    sq += b[0] + b[1] + b[2];
   }
-  if (threadIdx.x < 8 && in) {
-    if (p.dweight) term_store(p.dweight, p.weight_dtype, i, dw);
-    if (p.dbias) term_store(p.dbias, p.bias_dtype, i, db);
+  part[0][warp][lane] = sp;
+  part[1][warp][lane] = sq;
+  __syncthreads();
+  for (int col = warp; col < 32; col += warps) {
+    sp = warp_sum(lane < warps ? part[0][lane][col] : 0.f);
+    sq = warp_sum(lane < warps ? part[1][lane][col] : 0.f);
+    const int i = first + col;
+    if (lane != 0 || i >= p.width) continue;
+    if (p.entries) {
+      const float w = p.weight.p ? term_at(p.weight.p, p.weight.dtype, i) : 1.f;
+      const float b = p.bias.p ? term_at(p.bias.p, p.bias.dtype, i) : 0.f;
+      if (p.dscale) term_store(p.dscale, p.scale_dtype, list * p.width + i, fmaf(sp, w, sq * b));
+      if (p.dshift) term_store(p.dshift, p.shift_dtype, list * p.width + i, sq);
+      const float s = p.scale.p ? 1.f + term_at(p.scale.p, p.scale.dtype, list * p.scale.stride + i) : 1.f;
+      sp *= s;
+      sq *= s;
+      if (p.keep) {                         // (this column of this part is read by this CTA alone, before the barrier)
+        base[i] = sp;
+        base[p.width + i] = sq;
+        continue;
+      }
+    }
+    if (p.dweight) term_store(p.dweight, p.weight_dtype, i, sp);
+    if (p.dbias) term_store(p.dbias, p.bias_dtype, i, sq);
   }
 }
 
@@ -1275,6 +1291,23 @@ int norm_back_size(const HtrcNormArgs* a, size_t* bytes) {
   return HTRC_OK;
 }
 
+int norm_terms(const NormTermsParams& t, cudaStream_t st) {
+  if (t.lists == 0) return HTRC_OK;
+  if (t.lists * t.columns >= kMaxRows) return HTRC_ERR_UNSUPPORTED;
+  int warps = 1;
+  while (warps < 32 && warps * 4 < t.count) warps *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(t.lists * t.columns));
+  cfg.blockDim = dim3(32 * warps);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, norm_terms_kernel, t) == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
+}
+
 int norm_backward(const HtrcNormArgs* a, cudaStream_t st) {
   size_t need = 0;
   int rc = norm_back_size(a, &need);
@@ -1317,9 +1350,9 @@ int norm_backward(const HtrcNormArgs* a, cudaStream_t st) {
   if (p.sums) {
     NormTermsParams t{};
     t.part = p.part;
-    t.entries = p.entries;
-    t.chunks = p.chunks;
     t.width = a->width;
+    t.columns = (a->width + 31) / 32;
+    t.part_stride = 2 * static_cast<int64_t>(a->width);
     t.weight = p.weight;
     t.bias = TermView{a->bias, 0, a->bias_dtype};
     t.scale = p.scale;
@@ -1331,16 +1364,23 @@ int norm_backward(const HtrcNormArgs* a, cudaStream_t st) {
     t.bias_dtype = a->bias_dtype;
     t.scale_dtype = a->scale_dtype;
     t.shift_dtype = a->shift_dtype;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((a->width + 7) / 8);
-    cfg.blockDim = dim3(1024);
-    cfg.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, norm_terms_kernel, t) != cudaSuccess) return HTRC_ERR_CUDA;
+    // an entry's parts with a modulation, and then the entries' sums where a weight or bias wants them; without one all
+    // parts are alike
+    t.entries = a->scale || a->shift;
+    t.lists = t.entries ? p.entries : 1;
+    t.count = t.entries ? p.chunks : p.entries * p.chunks;
+    t.list_stride = t.count * t.part_stride;
+    t.keep = t.entries && p.entries != 1 && (a->dweight || a->dbias);
+    rc = norm_terms(t, st);
+    if (rc != HTRC_OK) return rc;
+    if (t.keep) {
+      t.entries = t.keep = false;
+      t.part_stride = t.list_stride;
+      t.count = t.lists;
+      t.lists = 1;
+      rc = norm_terms(t, st);
+      if (rc != HTRC_OK) return rc;
+    }
   }
   return cudaGetLastError() == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
 }

@@ -213,7 +213,7 @@ __device__ __forceinline__ void over_lanes(float (&v)[R], int L, int group, floa
 
 // LANES: lanes to a row, or 0 for any number (p.lanes); fixed ones have the pieces' offsets in the instructions
 template <typename T, int READ, int V, int LANES, int MODE>
-__global__ void __launch_bounds__(kNormMaxWarps * 32) __maxnreg__(MODE == QUANT_CODES ? 64 : MODE == NORM_CODES || V == 8 ? 128 : 80)
+__global__ void __maxnreg__(MODE == QUANT_CODES ? 64 : MODE == NORM_CODES || V == 8 ? 128 : 80)
     norm_rows_kernel(const __grid_constant__ NormParams p) {
   using P = Piece<T, READ>;
   constexpr int N = P::N, H = N / 2, R = V >= 8 ? 1 : V == 1 ? 4 : 8 / V;
@@ -468,8 +468,9 @@ __global__ void __launch_bounds__(kNormMaxWarps * 32) __maxnreg__(MODE == QUANT_
 // A thread keeps its columns over all of the CTA's rows, so that their P and Q stay in registers; the rows' two sums go over
 // the lanes.  Rows of half a warp to a warp's pieces (norm_back_narrow_kernel) need no barrier.  A wider row is the whole
 // CTA's (norm_back_ring_kernel): rows arrive in shared memory by bulk copies several stages ahead, since a barrier per
-// four rows leaves loads by the threads themselves no time in flight.  norm_back_any_kernel: rows that are not 16-byte aligned, and float32 rows too wide for
-// the registers.  The parts' P and Q are added in order by norm_terms_kernel.  HBM bounds it: 6 bytes per 16-bit element.
+// four rows leaves loads by the threads themselves no time in flight (32,768 x 2,048: 120 us by such loads, 77 by the ring).
+// Rows that are not 16-byte aligned arrive as the 16-byte pieces that cover them.  The parts' P and Q are added in order by
+// norm_terms_kernel.  HBM bounds it: 6 bytes per 16-bit element.
 struct NormBackParams {
   const void *dy, *x;
   int64_t gs[2], xs[2];
@@ -486,146 +487,6 @@ struct NormBackParams {
   TermView weight, scale;
   float* part;                              // [entry * chunks][2][width]
 };
-
-// RELOAD: rows too wide for the registers are read again (from L2) once their sums are known.
-template <typename T, int READ, int C, int R, bool RELOAD>
-__global__ void __launch_bounds__(512, 1) norm_back_any_kernel(const __grid_constant__ NormBackParams p) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the sums' kernel waits for this one's end itself
-  using P = Piece<T, READ>;
-  constexpr int N = P::N, H = N / 2, HELD = RELOAD ? 1 : C;
-  __shared__ float slots[2][16][2 * R];
-  extern __shared__ __align__(16) float gain[];          // A, as term_slot() has it
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, L = blockDim.x;
-  int turn = 0;
-  const int64_t e = blockIdx.x / p.chunks, r1 = p.rows, r0 = (blockIdx.x - e * p.chunks) * R, step = p.chunks * R;
-  if (p.affine) {
-    for (int i = threadIdx.x; i < p.nvec * N; i += L) {
-      float t = i >= p.width ? 0.f : p.weight.p ? term_at(p.weight.p, p.weight.dtype, i) : 1.f;
-      if (i < p.width && p.scale.p) t *= 1.f + term_at(p.scale.p, p.scale.dtype, e * p.scale.stride + i);
-      gain[term_slot<N>(i, p.nvec)] = t;
-    }
-    __syncthreads();
-  }
-  float2 sp[C][H], sq[C][H];
-#pragma unroll
-  for (int c = 0; c < C; ++c)
-#pragma unroll
-    for (int h = 0; h < H; ++h) sp[c][h] = sq[c][h] = make_float2(0.f, 0.f);
-  auto gains = [&](int vec, float2 (&a)[H]) {
-#pragma unroll
-    for (int h = 0; h < H; ++h) a[h] = make_float2(1.f, 1.f);
-    if (p.affine) Terms<N>(gain, vec, p.nvec).load(0, a);
-  };
-  const T* dy = static_cast<const T*>(p.dy) + e * p.gs[0];
-  const T* x = static_cast<const T*>(p.x) + e * p.xs[0];
-  T* dx = static_cast<T*>(p.dx) + e * p.os[0];
-  for (int64_t r = r0; r < r1; r += step) {
-    P vg[R][HELD], vx[R][HELD];
-    float mean[R], rstd[R];
-    auto fetch = [&](int k, int c, int to) {
-      const int vec = threadIdx.x + c * L;
-      if (r + k < r1 && vec < p.nvec) {
-        const bool both = READ != BY_ELEMENT || 2 * vec + 1 < p.width;
-        vg[k][to].load(dy + (r + k) * p.gs[1] + vec * N, both);
-        vx[k][to].load(x + (r + k) * p.xs[1] + vec * N, both);
-      } else {
-        vg[k][to].clear();
-        vx[k][to].clear();
-      }
-    };
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      if (!RELOAD) {
-#pragma unroll
-        for (int c = 0; c < C; ++c) fetch(k, c, c);
-      }
-      const bool in = r + k < r1;
-      mean[k] = in ? __ldg(p.mean + e * p.rows + r + k) : 0.f;
-      rstd[k] = in ? __ldg(p.rstd + e * p.rows + r + k) : 0.f;
-    }
-    float2 s0[R], s1[R];
-#pragma unroll
-    for (int k = 0; k < R; ++k) s0[k] = s1[k] = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int vec = threadIdx.x + c * L, at = RELOAD ? 0 : c;
-      if (vec >= p.nvec) break;
-      float2 a[H];
-      gains(vec, a);
-#pragma unroll
-      for (int k = 0; k < R; ++k) {
-        if (RELOAD) fetch(k, c, 0);
-        const float2 r2 = make_float2(rstd[k], rstd[k]), m2 = make_float2(mean[k], mean[k]);
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-          const float2 d = vg[k][at].pair(h), u = mul2(sub2(vx[k][at].pair(h), m2), r2), g = mul2(d, a[h]);
-          sq[c][h] = add2(sq[c][h], d);
-          sp[c][h] = fma2(d, u, sp[c][h]);
-          s0[k] = add2(s0[k], g);
-          s1[k] = fma2(g, u, s1[k]);
-        }
-        vg[k][at].packed();
-        vx[k][at].packed();
-      }
-    }
-    turn ^= 1;
-    float sum[2 * R];
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      sum[2 * k] = warp_sum(s0[k].x + s0[k].y);
-      sum[2 * k + 1] = warp_sum(s1[k].x + s1[k].y);
-    }
-    if (lane == 0) {
-#pragma unroll
-      for (int k = 0; k < 2 * R; ++k) slots[turn][warp][k] = sum[k];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 2 * R; ++k) {
-      sum[k] = slots[turn][0][k];
-      for (int w = 1; w < warps; ++w) sum[k] += slots[turn][w][k];
-      sum[k] *= p.inv_width;
-    }
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int vec = threadIdx.x + c * L, at = RELOAD ? 0 : c;
-      if (vec >= p.nvec) break;
-      float2 a[H];
-      gains(vec, a);
-#pragma unroll
-      for (int k = 0; k < R; ++k) {
-        if (r + k >= r1) break;
-        if (RELOAD) fetch(k, c, 0);
-        const float2 r2 = make_float2(rstd[k], rstd[k]), m2 = make_float2(mean[k], mean[k]);
-        const float2 g0 = make_float2(sum[2 * k], sum[2 * k]), g1 = make_float2(-sum[2 * k + 1], -sum[2 * k + 1]);
-        P o;
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-          const float2 u = mul2(sub2(vx[k][at].pair(h), m2), r2), g = mul2(vg[k][at].pair(h), a[h]);
-          o.set(h, mul2(fma2(u, g1, sub2(g, g0)), r2));
-        }
-        o.store(dx + (r + k) * p.os[1] + vec * N, READ != BY_ELEMENT || 2 * vec + 1 < p.width);
-      }
-    }
-  }
-  if (p.sums) {
-    float* part = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.width;
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int h = 0; h < H; ++h) {
-        const int i = (threadIdx.x + c * L) * N + 2 * h;
-        if (i < p.width) {
-          part[i] = sp[c][h].x;
-          part[p.width + i] = sq[c][h].x;
-          if (i + 1 < p.width) {
-            part[i + 1] = sp[c][h].y;
-            part[p.width + i + 1] = sq[c][h].y;
-          }
-        }
-      }
-  }
-}
 
 // 8 values over a warp: afterwards lane 4 i' holds one of them, value_of(lane)
 __device__ __forceinline__ float warp_sum8(float (&v)[8], int lane) {
@@ -644,19 +505,29 @@ __device__ __forceinline__ float warp_sum8(float (&v)[8], int lane) {
 }
 __device__ __forceinline__ int value_of(int lane) { return lane >> 2; }
 
-// C pieces of R = 4 / C rows to a thread, the CTA one row wide
-template <typename T, int C>
+// rows of a ring's stage with C pieces of each to a thread
+template <typename T, int READ>
+__host__ __device__ constexpr int ring_rows(int c) {
+  return READ == BY_16 ? (c >= 4 ? 1 : 4 / c) : sizeof(T) == 4 ? (c >= 8 ? 1 : 8 / c) : c <= 4 ? 4 : 16 / c;
+}
+// bytes between the rows of a stage: a row that starts inside a 16-byte piece begins with what is before it there
+__host__ __device__ inline uint32_t ring_pitch(uint32_t row_bytes, int read) {
+  return read == BY_16 ? row_bytes : (row_bytes + 15 + 15) / 16 * 16;
+}
+
+// C pieces of each of R rows to a thread, the CTA one row wide
+template <typename T, int READ, int C>
 __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_constant__ NormBackParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the sums' kernel waits for this one's end itself
-  using P = Piece<T, BY_16>;
-  constexpr int N = P::N, H = N / 2, R = 4 / C, kStages = 4;
+  using P = Piece<T, READ == BY_16 ? BY_16 : BY_PAIR>;        // in registers two elements stand together
+  constexpr int N = P::N, H = N / 2, R = ring_rows<T, READ>(C), kStages = 4;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ __align__(8) uint64_t full[kStages];
   __shared__ float slots[2][8][16];
   __shared__ __align__(16) float stats[2][2][4];            // the rows' means and reciprocal deviations
   __shared__ int abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, L = blockDim.x;
-  const uint32_t row_bytes = p.width * sizeof(T), stage_bytes = 2 * R * row_bytes;
+  const uint32_t row_bytes = p.width * sizeof(T), pitch = ring_pitch(row_bytes, READ), stage_bytes = 2 * R * pitch;
   float* gain = reinterpret_cast<float*>(ring + p.stages * stage_bytes);       // C > 1: A, as term_slot() has it
   int turn = 0;
   const int64_t e = blockIdx.x / p.chunks, r1 = p.rows, r0 = (blockIdx.x - e * p.chunks) * R, step = p.chunks * R;
@@ -666,11 +537,23 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
   const uint64_t policy = policy_evict_first();
   auto fill = [&](int s, int64_t r) {
     const int n = static_cast<int>(min(static_cast<int64_t>(R), r1 - r));
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&full[s])), "r"(2 * n * row_bytes) : "memory");
+    // the 16-byte pieces that cover a row
+    auto start = [](const T* row) { return reinterpret_cast<uintptr_t>(row) & ~static_cast<uintptr_t>(READ == BY_16 ? 0 : 15); };
+    auto bytes = [&](const T* row) {
+      if (READ == BY_16) return row_bytes;
+      return static_cast<uint32_t>((reinterpret_cast<uintptr_t>(row) + row_bytes + 15 & ~static_cast<uintptr_t>(15)) - start(row));
+    };
+    uint32_t all = 2 * n * row_bytes;
+    if (READ != BY_16) {
+      all = 0;
+      for (int k = 0; k < n; ++k) all += bytes(dy + (r + k) * p.gs[1]) + bytes(x + (r + k) * p.xs[1]);
+    }
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&full[s])), "r"(all) : "memory");
     for (int k = 0; k < n; ++k) {
-      uint8_t* to = ring + s * stage_bytes + 2 * k * row_bytes;
-      bulk_load(to, dy + (r + k) * p.gs[1], row_bytes, &full[s], policy);
-      bulk_load(to + row_bytes, x + (r + k) * p.xs[1], row_bytes, &full[s], policy);
+      uint8_t* to = ring + s * stage_bytes + 2 * k * pitch;
+      const T *g = dy + (r + k) * p.gs[1], *v = x + (r + k) * p.xs[1];
+      bulk_load(to, reinterpret_cast<const void*>(start(g)), bytes(g), &full[s], policy);
+      bulk_load(to + pitch, reinterpret_cast<const void*>(start(v)), bytes(v), &full[s], policy);
     }
   };
   if (threadIdx.x == 0) {
@@ -712,6 +595,22 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
   const int64_t ahead = threadIdx.x % R;
   const float* stat = (threadIdx.x < R ? p.mean : p.rstd) + e * p.rows + ahead;
   if (keeps) stats[0][threadIdx.x / R][ahead] = r0 + ahead < r1 ? __ldg(stat + r0) : 0.f;
+  auto two = [&](int vec) { return READ != BY_ELEMENT || 2 * vec + 1 < p.width; };
+  auto take = [](P& v, const uint8_t* at, bool both) {
+    if constexpr (READ == BY_16) {
+      const uint4 w = *reinterpret_cast<const uint4*>(at);
+      v.w[0] = w.x; v.w[1] = w.y; v.w[2] = w.z; v.w[3] = w.w;
+    } else if constexpr (sizeof(T) == 4) {
+      v.w[0] = *reinterpret_cast<const uint32_t*>(at);
+      if (both) v.w[1] = *reinterpret_cast<const uint32_t*>(at + 4);
+    } else if constexpr (READ == BY_PAIR) {
+      v.w[0] = *reinterpret_cast<const uint32_t*>(at);
+    } else {
+      uint32_t w = *reinterpret_cast<const unsigned short*>(at);
+      if (both) w |= static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(at + 2)) << 16;
+      v.w[0] = w;
+    }
+  };
   __syncthreads();
   bool ok = true;
   int it = 0;
@@ -719,9 +618,14 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
     const int s = it % p.stages;
     // (a wait that ran out: the launch ends without further waits, its status says so)
     ok = ok && mbar_wait(&full[s], (it / p.stages) & 1, p.status, &abort_flag);
-    const uint8_t* from = ring + s * stage_bytes + threadIdx.x * 16;
+    const uint8_t* from = ring + s * stage_bytes + threadIdx.x * N * sizeof(T);
     const float later = keeps && r + step + ahead < r1 ? __ldg(stat + r + step) : 0.f;
     const int rows = static_cast<int>(min(static_cast<int64_t>(R), r1 - r));
+    // where row k begins in its first 16 bytes
+    auto skip = [&](const T* base, int64_t stride, int k) -> uint32_t {
+      if (READ == BY_16) return 0;
+      return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base)) + (static_cast<uint32_t>(r) + k) * static_cast<uint32_t>(stride * sizeof(T)) & 15u;
+    };
     P vg[R][C], vx[R][C];
     float mean[4], rstd[4], sum[8];
     {
@@ -740,10 +644,9 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
         vg[k][c].clear();
         vx[k][c].clear();
         if (in && vec < p.nvec) {
-          const uint4 g = *reinterpret_cast<const uint4*>(from + 2 * k * row_bytes + c * L * 16);
-          const uint4 v = *reinterpret_cast<const uint4*>(from + (2 * k + 1) * row_bytes + c * L * 16);
-          vg[k][c].w[0] = g.x; vg[k][c].w[1] = g.y; vg[k][c].w[2] = g.z; vg[k][c].w[3] = g.w;
-          vx[k][c].w[0] = v.x; vx[k][c].w[1] = v.y; vx[k][c].w[2] = v.z; vx[k][c].w[3] = v.w;
+          const int off = c * L * N * sizeof(T);
+          take(vg[k][c], from + 2 * k * pitch + skip(dy, p.gs[1], k) + off, two(vec));
+          take(vx[k][c], from + (2 * k + 1) * pitch + skip(x, p.xs[1], k) + off, two(vec));
         }
       }
     }
@@ -767,8 +670,6 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
         }
         sum[2 * k] += s0.x + s0.y;
         sum[2 * k + 1] += s1.x + s1.y;
-        vg[k][c].packed();
-        vx[k][c].packed();
       }
     }
     turn ^= 1;
@@ -799,11 +700,11 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
         const float f0 = -rstd[k] * sum[2 * k], f1 = -rstd[k] * (rstd[k] * (rstd[k] * sum[2 * k + 1]));
         const float2 r2 = make_float2(rstd[k], rstd[k]), m2 = make_float2(mean[k], mean[k]);
         const float2 g0 = make_float2(f0, f0), g1 = make_float2(f1, f1);
-        P o;
+        Piece<T, READ> o;
 #pragma unroll
         for (int h = 0; h < H; ++h)
           o.set(h, fma2(sub2(vx[k][c].pair(h), m2), g1, fma2(vg[k][c].pair(h), mul2(a[h], r2), g0)));
-        o.store(dx + (r + k) * p.os[1] + vec * N, true);
+        o.store(dx + (r + k) * p.os[1] + vec * N, two(vec));
       }
     }
   }
@@ -819,8 +720,17 @@ __global__ void __launch_bounds__(512, 1) norm_back_ring_kernel(const __grid_con
       if (vec >= p.nvec) break;
 #pragma unroll
       for (int h = 0; h < H; ++h) {
-        *reinterpret_cast<float2*>(part + vec * N + 2 * h) = sp[c][h];
-        *reinterpret_cast<float2*>(part + p.width + vec * N + 2 * h) = sq[c][h];
+        if constexpr (READ == BY_ELEMENT) {
+          part[2 * vec] = sp[c][h].x;
+          part[p.width + 2 * vec] = sq[c][h].x;
+          if (two(vec)) {
+            part[2 * vec + 1] = sp[c][h].y;
+            part[p.width + 2 * vec + 1] = sq[c][h].y;
+          }
+        } else {
+          *reinterpret_cast<float2*>(part + vec * N + 2 * h) = sp[c][h];
+          *reinterpret_cast<float2*>(part + p.width + vec * N + 2 * h) = sq[c][h];
+        }
       }
     }
   }
@@ -1196,41 +1106,36 @@ int norm_forward(const HtrcNormArgs* a, cudaStream_t st) {
 
 // How the backward's rows are shared out: the kernel, its CTAs' threads, shared memory and rows
 struct NormBackPlan {
-  enum { NARROW, RING, ANY } kind;
+  Reads reads;
+  bool narrow;
   int per, lanes, threads, stages;          // per: pieces of a row to a thread
   size_t smem;
   int64_t chunks;                           // CTAs of an entry
-  NormBackPlan(int width, int es, Reads reads, bool affine, int64_t entries, int64_t rows) {
-    const bool vec = reads == BY_16;
-    const int n = vec ? 16 / es : 2, nvec = (width + n - 1) / n;
-    int resident;
+  NormBackPlan(int width, int es, Reads by, bool affine, int64_t entries, int64_t rows) : reads(by) {
+    // float32 rows of more 16-byte pieces than a thread has registers for
+    if (reads == BY_16 && width * es > 2048 * 16) reads = BY_PAIR;
+    const int n = reads == BY_16 ? 16 / es : 2, nvec = (width + n - 1) / n;
+    int resident, least;                    // CTAs of an SM, rows that a CTA takes at a time
     lanes = stages = 0;
-    int least;                              // rows that a CTA takes at a time
-    if (vec && nvec <= 64) {
-      kind = NARROW;
+    narrow = reads == BY_16 && nvec <= 64;
+    if (narrow) {
       lanes = nvec <= 8 ? 8 : nvec <= 16 ? 16 : 32;
       per = nvec <= lanes ? 1 : 2;
       threads = kNormThreads;
       smem = static_cast<size_t>(threads / lanes) * 2 * nvec * n * sizeof(float);
       resident = 2;
       least = threads / lanes * (2 / per);
-    } else if (vec && nvec <= 2048) {
-      kind = RING;
-      per = nvec <= 512 ? 1 : nvec <= 1024 ? 2 : 4;
-      threads = ((nvec + per - 1) / per + 31) / 32 * 32;
-      least = 4 / per;
-      resident = std::max(1, 512 / threads);
-      const size_t stage = static_cast<size_t>(8 / per) * width * es, gain = per > 1 && affine ? static_cast<size_t>(nvec) * n * 4 : 0;
-      stages = static_cast<int>(std::max<size_t>(2, std::min<size_t>(4, (200 * 1024 / resident - gain) / stage)));
-      smem = stages * stage + gain;
     } else {
-      kind = ANY;
-      const int wide = (nvec + 511) / 512;
-      per = vec ? 8 : wide <= 2 ? 2 : wide <= 4 ? 4 : wide <= 8 ? 8 : 16;
-      least = per == 2 ? 4 : per == 4 ? 2 : 1;
+      if (reads == BY_16) per = nvec <= 512 ? 1 : nvec <= 1024 ? 2 : 4;
+      else per = nvec <= 128 ? 2 : nvec <= 2048 ? 4 : nvec <= 4096 ? 8 : 16;
       threads = ((nvec + per - 1) / per + 31) / 32 * 32;
-      smem = affine ? static_cast<size_t>(nvec) * n * sizeof(float) : 0;
       resident = std::max(1, 512 / threads);
+      least = es == 4 ? (reads == BY_16 ? ring_rows<float, BY_16>(per) : ring_rows<float, BY_PAIR>(per))
+                      : (reads == BY_16 ? ring_rows<__half, BY_16>(per) : ring_rows<__half, BY_PAIR>(per));
+      const size_t stage = 2 * static_cast<size_t>(least) * ring_pitch(width * es, reads);
+      const size_t gain = per > 1 && affine ? static_cast<size_t>(nvec) * n * 4 : 0, room = 216 * 1024 / resident - gain - 2048;
+      stages = static_cast<int>(std::max<size_t>(1, std::min<size_t>(4, room / stage)));
+      smem = stages * stage + gain;
     }
     const int64_t share = std::max<int64_t>(1, static_cast<int64_t>(resident) * sm_count() / std::max<int64_t>(1, entries));
     chunks = std::max<int64_t>(1, std::min(share, (rows + least - 1) / least));
@@ -1244,8 +1149,8 @@ RowShape norm_back_shape(const HtrcNormArgs* a) {
 }
 
 template <typename T>
-int norm_back_launch(NormBackParams& p, const NormBackPlan& plan, Reads reads, cudaStream_t st) {
-  const int n = reads == BY_16 ? static_cast<int>(16 / sizeof(T)) : 2;
+int norm_back_launch(NormBackParams& p, const NormBackPlan& plan, cudaStream_t st) {
+  const int n = plan.reads == BY_16 ? static_cast<int>(16 / sizeof(T)) : 2;
   p.nvec = (p.width + n - 1) / n;
   p.lanes = plan.lanes;
   p.stages = plan.stages;
@@ -1257,22 +1162,18 @@ int norm_back_launch(NormBackParams& p, const NormBackPlan& plan, Reads reads, c
     kernel<<<grid, plan.threads, plan.smem, st>>>(p);
     return cudaGetLastError() == cudaSuccess ? HTRC_OK : HTRC_ERR_CUDA;
   };
-  if (plan.kind == NormBackPlan::NARROW)
-    return plan.per == 1 ? go(norm_back_narrow_kernel<T, 1>) : go(norm_back_narrow_kernel<T, 2>);
-  if (plan.kind == NormBackPlan::RING)
-    return plan.per == 1 ? go(norm_back_ring_kernel<T, 1>)
-                         : plan.per == 2 ? go(norm_back_ring_kernel<T, 2>) : go(norm_back_ring_kernel<T, 4>);
+  if (plan.narrow) return plan.per == 1 ? go(norm_back_narrow_kernel<T, 1>) : go(norm_back_narrow_kernel<T, 2>);
+  if (plan.reads == BY_16) {
+    if (plan.per == 1) return go(norm_back_ring_kernel<T, BY_16, 1>);
+    return plan.per == 2 ? go(norm_back_ring_kernel<T, BY_16, 2>) : go(norm_back_ring_kernel<T, BY_16, 4>);
+  }
   auto by = [&](auto read) {
     constexpr int READ = decltype(read)::value;
-    if (plan.per == 2) return go(norm_back_any_kernel<T, READ, 2, 4, false>);
-    if (plan.per == 4) return go(norm_back_any_kernel<T, READ, 4, 2, false>);
-    if (plan.per == 8) return go(norm_back_any_kernel<T, READ, 8, 1, false>);
-    return go(norm_back_any_kernel<T, READ, 16, 1, true>);
+    if (plan.per == 2) return go(norm_back_ring_kernel<T, READ, 2>);
+    if (plan.per == 4) return go(norm_back_ring_kernel<T, READ, 4>);
+    return plan.per == 8 ? go(norm_back_ring_kernel<T, READ, 8>) : go(norm_back_ring_kernel<T, READ, 16>);
   };
-  if (reads == BY_PAIR) return by(std::integral_constant<int, BY_PAIR>{});
-  if (reads == BY_ELEMENT) return by(std::integral_constant<int, BY_ELEMENT>{});
-  if constexpr (sizeof(T) == 4) return go(norm_back_any_kernel<T, BY_16, 8, 1, true>);
-  return HTRC_ERR_UNSUPPORTED;            // 16-bit rows of 16-byte pieces are narrow or the ring's
+  return plan.reads == BY_PAIR ? by(std::integral_constant<int, BY_PAIR>{}) : by(std::integral_constant<int, BY_ELEMENT>{});
 }
 
 Reads back_reads(const HtrcNormArgs* a) {
@@ -1339,13 +1240,12 @@ int norm_backward(const HtrcNormArgs* a, cudaStream_t st) {
   p.sums = norm_sums(a);
   p.affine = a->weight || a->scale;
   p.part = static_cast<float*>(a->workspace);
-  const Reads reads = back_reads(a);
   p.status = a->status;
-  const NormBackPlan plan(a->width, type_size(a->dtype), reads, p.affine, p.entries, p.rows);
+  const NormBackPlan plan(a->width, type_size(a->dtype), back_reads(a), p.affine, p.entries, p.rows);
   if (p.entries * plan.chunks >= kMaxRows) return HTRC_ERR_UNSUPPORTED;
-  rc = a->dtype == HTRC_LAYER_F32    ? norm_back_launch<float>(p, plan, reads, st)
-       : a->dtype == HTRC_LAYER_BF16 ? norm_back_launch<__nv_bfloat16>(p, plan, reads, st)
-                                     : norm_back_launch<__half>(p, plan, reads, st);
+  rc = a->dtype == HTRC_LAYER_F32    ? norm_back_launch<float>(p, plan, st)
+       : a->dtype == HTRC_LAYER_BF16 ? norm_back_launch<__nv_bfloat16>(p, plan, st)
+                                     : norm_back_launch<__half>(p, plan, st);
   if (rc != HTRC_OK) return rc;
   if (p.sums) {
     NormTermsParams t{};

@@ -33,6 +33,11 @@ struct Linear8Params {
   int* status;
   int tiles_m, tiles_n, splits;
   bool early;                               // few tokens: the kernel before this one did not write the weights
+  // few float rows, quantised by the product: their elements, strides, tokens of a batch entry and width
+  const void* x;
+  int64_t x_stride[2], tokens;
+  int width;
+  bool vec;                                 // the rows are 16-byte aligned
   bool direct;                              // pair kernel: the output's rows are not 16-byte aligned
 };
 
@@ -76,32 +81,120 @@ __device__ __forceinline__ void expect_tx(uint64_t* bar, uint32_t bytes) {
 }
 
 // ------------------------------------------------------------------------------------------------ few tokens
-constexpr int kSmallThreads = 192;          // warps 0-3: the way out; 4: TMA; 5: MMA
 constexpr int kSmallChannels = 128;
+constexpr int kFewTokens = 16, kFewBlocks = 32;      // rows that the product quantises itself: so many, of so many blocks a part
 
-template <int T>
+// X: int8_t, or the float type of rows that are quantised here.  Warps 0-3: the way out; the next two: TMA, MMA.  Of float
+// rows warps 0-15 first write a row's codes each.
+template <int T, typename X>
 struct SmallShape {
+  static constexpr bool kCodes = std::is_same<X, int8_t>::value;
+  static constexpr int kRowWarps = kCodes ? 4 : 16, kThreads = 32 * (kRowWarps + 2);
   static constexpr int kStages = T <= 32 ? 5 : 4;          // two CTAs per SM
-  static constexpr uint32_t kW = kSmallChannels * 128, kX = T * 128, kStage = kW + kX;
+  static constexpr uint32_t kW = kSmallChannels * 128, kX = T * 128, kStage = kCodes ? kW + kX : kW;
   static constexpr uint32_t kCols = T < 32 ? 32 : T;
-  static constexpr uint32_t kBars = kStages * kStage, kBytes = kBars + 128;
+  static constexpr uint32_t kBars = kStages * kStage, kRows = kBars + 256;    // kRows: float rows' codes, block by block
   static_assert(T * kSmallChannels * 4 <= kBars, "the parts of a split tile reuse the stages");
+  static uint32_t bytes(int blocks) { return kCodes ? kBars + 256 : (kRows + 1023) / 1024 * 1024 + blocks * kX; }
 };
 
 struct SmallBars {
-  uint64_t full[5], empty[5], done;
+  uint64_t full[5], empty[5], done, rows;
   uint32_t tmem;
   int abort_flag;
+  float scales[kFewTokens];
 };
-static_assert(sizeof(SmallBars) <= 128, "barriers");
+static_assert(sizeof(SmallBars) <= 256, "barriers");
 
-template <int T, typename O>
-__global__ void __launch_bounds__(kSmallThreads)
+// A float row's scale, and the codes of its elements from k0 up to k1 into blocks of [T][128] bytes, 128-byte swizzled (what
+// is past the row in its last block is whatever was there: the weights are zero there).  One warp.
+template <int T, typename X>
+__device__ __forceinline__ float quantise_row(const X* x, int width, bool vec, int k0, int k1, uint8_t* blocks, int row, int lane) {
+  constexpr int N = 16 / sizeof(X);
+  auto one = [](X v) -> float {
+    if constexpr (sizeof(X) == 4) return v;
+    else if constexpr (std::is_same<X, __nv_bfloat16>::value) return __bfloat162float(v);
+    else return __half2float(v);
+  };
+  auto larger = [](float a, float b) {                      // NaN if either is
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+  };
+  union Sixteen {
+    uint4 v;
+    X e[N];
+  };
+  float top = 0.f;
+  if (vec) {
+    const int vecs = width / N;
+    for (int i = lane; i < vecs; i += 8 * 32) {
+      Sixteen t[8];                                         // in flight together
+#pragma unroll
+      for (int b = 0; b < 8; ++b) t[b].v = i + 32 * b < vecs ? __ldg(reinterpret_cast<const uint4*>(x) + i + 32 * b) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int b = 0; b < 8; ++b)
+#pragma unroll
+        for (int j = 0; j < N; ++j) top = larger(top, fabsf(one(t[b].e[j])));
+    }
+  } else {
+    for (int i = lane; i < width; i += 8 * 32) {
+      float t[8];
+#pragma unroll
+      for (int b = 0; b < 8; ++b) t[b] = i + 32 * b < width ? one(x[i + 32 * b]) : 0.f;
+#pragma unroll
+      for (int b = 0; b < 8; ++b) top = larger(top, fabsf(t[b]));
+    }
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) top = larger(top, __shfl_xor_sync(0xffffffffu, top, d));
+  // as the rows' own kernel has it
+  top = top <= 3.4028235e38f ? fmaxf(top, 1e-30f) : __uint_as_float(0x7FC00000u);
+  const float by = __fdiv_rn(127.f, top);
+  auto code = [&](float v) { return __float_as_uint(__fadd_rn(__fmul_rn(v, by), 12582912.f)) & 0xFFu; };
+  k1 = min(k1, width);
+  if (vec) {
+    for (int k = k0 + lane * N; k < k1; k += 4 * 32 * N) {
+      Sixteen t[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        t[b].v = k + 32 * N * b < k1 ? __ldg(reinterpret_cast<const uint4*>(x + k + 32 * N * b)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j / 4] |= code(one(t[b].e[j])) << (8 * (j % 4));
+        const uint32_t at = k + 32 * N * b - k0;
+        if (k + 32 * N * b >= k1) continue;
+        uint8_t* to = blocks + at / 128 * (T * 128) + sw128_off(row, at % 128 / 16) + at % 16;
+        if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(to) = w[0];
+      }
+    }
+  } else {
+    for (int k = k0 + lane; k < k1; k += 8 * 32) {
+      float t[8];
+#pragma unroll
+      for (int b = 0; b < 8; ++b) t[b] = k + 32 * b < k1 ? one(x[k + 32 * b]) : 0.f;
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        const uint32_t at = k + 32 * b - k0;
+        if (k + 32 * b < k1) blocks[at / 128 * (T * 128) + sw128_off(row, at % 128 / 16) + at % 16] = static_cast<uint8_t>(code(t[b]));
+      }
+    }
+  }
+  return __fdiv_rn(top, 127.f);
+}
+
+template <int T, typename O, typename X>
+__global__ void __launch_bounds__(SmallShape<T, X>::kThreads)
     linear8_small_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                          const __grid_constant__ Linear8Params p) {
-  using SM = SmallShape<T>;
+  using SM = SmallShape<T, X>;
+  constexpr int kTma = SM::kRowWarps, kMma = kTma + 1;
   extern __shared__ __align__(1024) uint8_t smem[];
   SmallBars* bars = reinterpret_cast<SmallBars*>(smem + SM::kBars);
+  uint8_t* codes = smem + (SM::kRows + 1023) / 1024 * 1024;
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool aligned = (smem_u32(smem) & 1023) == 0;      // the swizzled tiles need it
@@ -111,11 +204,12 @@ __global__ void __launch_bounds__(kSmallThreads)
       mbar_init(&bars->empty[i], 1);
     }
     mbar_init(&bars->done, 1);
+    mbar_init(&bars->rows, SM::kRowWarps);
     bars->abort_flag = !aligned;
     if (!aligned) flag_status(p.status, ST_WAIT_TIMEOUT);
     fence_barrier_init();
   }
-  if (warp == 5) tmem_alloc(&bars->tmem, SM::kCols);
+  if (warp == kMma) tmem_alloc(&bars->tmem, SM::kCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -126,8 +220,9 @@ __global__ void __launch_bounds__(kSmallThreads)
   const int n0 = tile / p.tiles_m * kSmallChannels, row0 = tile % p.tiles_m * T;
   const int b0 = static_cast<int>(static_cast<int64_t>(p.blocks) * rank / splits);
   const int b1 = static_cast<int>(static_cast<int64_t>(p.blocks) * (rank + 1) / splits);
+  auto row_scale = [&](int64_t r) { return SM::kCodes ? __ldg(p.xs + r) : bars->scales[r & (kFewTokens - 1)]; };
 
-  if (warp == 4) {
+  if (warp == kTma) {
     if (lane == 0 && aligned) {
       const uint64_t once = policy_evict_first(), keep = policy_evict_last();
       auto load_w = [&](int s, int b) {
@@ -135,7 +230,7 @@ __global__ void __launch_bounds__(kSmallThreads)
         tma_load_2d(smem + s * SM::kStage, &tm_w, &bars->full[s], b * 128, n0, p.tiles_m > 1 ? keep : once);
       };
       auto load_x = [&](int s, int b) {
-        tma_load_2d(smem + s * SM::kStage + SM::kW, &tm_x, &bars->full[s], b * 128, row0, keep);
+        if (SM::kCodes) tma_load_2d(smem + s * SM::kStage + SM::kW, &tm_x, &bars->full[s], b * 128, row0, keep);
       };
       const int first = min(b1 - b0, SM::kStages);
       if (!p.early) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -155,17 +250,18 @@ __global__ void __launch_bounds__(kSmallThreads)
       drain_ring<false>(bars->full, SM::kStages, issued, p.status, &gave_up);
     }
     __syncwarp();
-  } else if (warp == 5) {
+  } else if (warp == kMma) {
     const uint32_t leader = elect_one();
     constexpr uint32_t idesc = idesc_i8(kSmallChannels, T);
     bool ok = aligned;
+    if (!SM::kCodes) ok = ok && mbar_wait_warp(&bars->rows, 0, p.status, abort_flag);
     for (int i = 0; ok && i < b1 - b0; ++i) {
       const int s = i % SM::kStages;
       ok = mbar_wait_warp(&bars->full[s], (i / SM::kStages) & 1, p.status, abort_flag);
       if (!ok) break;
       tc_fence_after();
       const uint64_t a = sw128_desc(smem_u32(smem + s * SM::kStage), 16, 1024);
-      const uint64_t b = sw128_desc(smem_u32(smem + s * SM::kStage + SM::kW), 16, 1024);
+      const uint64_t b = sw128_desc(smem_u32(SM::kCodes ? smem + s * SM::kStage + SM::kW : codes + i * SM::kX), 16, 1024);
 #pragma unroll
       for (int k = 0; k < 4; ++k) mma_i8_by(leader, tmem, a + 2 * k, b + 2 * k, idesc, i > 0 || k > 0);
       mma_commit_by(leader, &bars->empty[s]);
@@ -176,28 +272,43 @@ __global__ void __launch_bounds__(kSmallThreads)
     mbar_wait_warp(&bars->done, 0, p.status, &gave_up);
     drain_ring<true>(bars->empty, SM::kStages, ok ? b1 - b0 : 0, p.status, &gave_up);
   } else {
-    const int n = n0 + 32 * warp + lane;
-    const bool in = n < p.channels;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const float ws = in ? __ldg(p.ws + n) : 0.f, bias = in ? bias_at(p, n) : 0.f;
-    O* out = static_cast<O*>(p.out) + n;
-    const bool ok = mbar_wait_warp(&bars->done, 0, p.status, abort_flag) && *abort_flag == 0;
-    tc_fence_after();
-    const uint32_t at = tmem + (static_cast<uint32_t>(32 * warp) << 16);
-    int* part = reinterpret_cast<int*>(smem);
-    if (__all_sync(0xffffffffu, ok)) {
-      for (int t0 = 0; t0 < T && row0 + t0 < p.rows; t0 += 16) {
-        uint32_t v[16];
-        tmem_ld16(at + t0, v);
-        tmem_ld_wait();
-        if (splits > 1) {
+    if constexpr (!SM::kCodes) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      if (warp < p.rows) {
+        const int64_t e = warp / p.tokens, t = warp - e * p.tokens;
+        const X* x = static_cast<const X*>(p.x) + e * p.x_stride[0] + t * p.x_stride[1];
+        const float scale = quantise_row<T>(x, p.width, p.vec, b0 * 128, b1 * 128, codes, warp, lane);
+        if (lane == 0) bars->scales[warp] = scale;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->rows);
+    }
+    if (warp < 4) {
+      const int n = n0 + 32 * warp + lane;
+      const bool in = n < p.channels;
+      if (SM::kCodes) asm volatile("griddepcontrol.wait;" ::: "memory");
+      const float ws = in ? __ldg(p.ws + n) : 0.f, bias = in ? bias_at(p, n) : 0.f;
+      O* out = static_cast<O*>(p.out) + n;
+      bool ok = SM::kCodes || mbar_wait_warp(&bars->rows, 0, p.status, abort_flag);      // the other warps' scales
+      ok = mbar_wait_warp(&bars->done, 0, p.status, abort_flag) && ok && *abort_flag == 0;
+      tc_fence_after();
+      const uint32_t at = tmem + (static_cast<uint32_t>(32 * warp) << 16);
+      int* part = reinterpret_cast<int*>(smem);
+      if (__all_sync(0xffffffffu, ok)) {
+        for (int t0 = 0; t0 < T && row0 + t0 < p.rows; t0 += 16) {
+          uint32_t v[16];
+          tmem_ld16(at + t0, v);
+          tmem_ld_wait();
+          if (splits > 1) {
 #pragma unroll
-          for (int t = 0; t < 16; ++t) part[(t0 + t) * kSmallChannels + 32 * warp + lane] = static_cast<int>(v[t]);
-        } else {
+            for (int t = 0; t < 16; ++t) part[(t0 + t) * kSmallChannels + 32 * warp + lane] = static_cast<int>(v[t]);
+          } else {
 #pragma unroll
-          for (int t = 0; t < 16; ++t) {
-            const int64_t r = row0 + t0 + t;
-            if (in && r < p.rows) out[r * p.channels] = from_f<O>(scaled(static_cast<int>(v[t]), __ldg(p.xs + r), ws, bias));
+            for (int t = 0; t < 16; ++t) {
+              const int64_t r = row0 + t0 + t;
+              if (in && r < p.rows) out[r * p.channels] = from_f<O>(scaled(static_cast<int>(v[t]), row_scale(r), ws, bias));
+            }
           }
         }
       }
@@ -228,7 +339,7 @@ __global__ void __launch_bounds__(kSmallThreads)
           O* out = static_cast<O*>(p.out) + static_cast<int64_t>(row0 + t0) * p.channels + n;
 #pragma unroll
           for (int j = 0; j < kBatch; ++j)
-            if (t0 + j < rows) out[static_cast<int64_t>(j) * p.channels] = from_f<O>(scaled(sum[j], __ldg(p.xs + row0 + t0 + j), ws, bias));
+            if (t0 + j < rows) out[static_cast<int64_t>(j) * p.channels] = from_f<O>(scaled(sum[j], row_scale(row0 + t0 + j), ws, bias));
         }
       }
     }
@@ -238,18 +349,20 @@ __global__ void __launch_bounds__(kSmallThreads)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) tmem_dealloc(tmem, SM::kCols);
+  if (warp == kMma) tmem_dealloc(tmem, SM::kCols);
 }
 
-template <int T, typename O>
+template <int T, typename O, typename X>
 int small_launch(const CUtensorMap& mx, const CUtensorMap& mw, const Linear8Params& p, cudaStream_t st) {
-  using SM = SmallShape<T>;
-  auto kernel = linear8_small_kernel<T, O>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kBytes) != cudaSuccess) return HTRC_ERR_CUDA;
+  using SM = SmallShape<T, X>;
+  auto kernel = linear8_small_kernel<T, O, X>;
+  const uint32_t bytes = SM::bytes((p.blocks + p.splits - 1) / p.splits);
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::bytes(kFewBlocks)) != cudaSuccess)
+    return HTRC_ERR_CUDA;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits));
-  cfg.blockDim = dim3(kSmallThreads);
-  cfg.dynamicSmemBytes = SM::kBytes;
+  cfg.blockDim = dim3(SM::kThreads);
+  cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -605,6 +718,32 @@ int linear8_validate(const HtrcLinear8Args* a) {
   return HTRC_OK;
 }
 
+// Parts of the width that a tile of few tokens is shared out to: split while the parts are longer than 8 blocks and leave SMs
+// idle.  64 x 4,096 x 4,096 10.2 us in 4 parts and 15 whole; 16 x 1,024 x 4,096 4.1 whole and 5.4 in 2; 16 x 4,096 x 16,384 14.1
+// whole and 16.4 in 2.
+int split_width(int64_t tiles, int blocks) {
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 4 <= 3 * sm_count() && blocks > 8 * splits) splits *= 2;
+  return splits;
+}
+
+// whether the product quantises its float rows itself: few of them, and no more of the width to a CTA than it has room for
+bool quantises(const HtrcLinear8Args* a) {
+  if (a->dtype == HTRC_LAYER_I8 || a->batch * a->tokens > kFewTokens) return false;
+  const int blocks = (a->width + 127) / 128, splits = split_width((a->channels + kSmallChannels - 1) / kSmallChannels, blocks);
+  return (blocks + splits - 1) / splits <= kFewBlocks;
+}
+
+template <typename O, typename X>
+int few_launch(Linear8Params& p, const HtrcLinear8Args* a, cudaStream_t st) {
+  CUtensorMap mw;
+  if (!code_map(&mw, a->w, p.channels, a->width, a->w_pitch, kSmallChannels)) return HTRC_ERR_CUDA;
+  p.tiles_m = 1;
+  p.tiles_n = (p.channels + kSmallChannels - 1) / kSmallChannels;
+  p.splits = split_width(p.tiles_n, p.blocks);
+  return small_launch<kFewTokens, O, X>(mw, mw, p, st);
+}
+
 template <typename O>
 int linear8_launch(Linear8Params& p, const int8_t* x, int64_t pitch, const HtrcLinear8Args* a, cudaStream_t st) {
   // Pairs where their tiles occupy half of the SMs (1,024 x 4,096 x 4,096: 18.5 us, by tiles of 64 tokens 30.1), not for so few
@@ -637,14 +776,17 @@ int linear8_launch(Linear8Params& p, const int8_t* x, int64_t pitch, const HtrcL
     return HTRC_ERR_CUDA;
   p.tiles_m = (p.rows + tile - 1) / tile;
   p.tiles_n = (p.channels + kSmallChannels - 1) / kSmallChannels;
-  // a tile's width is split while its parts are longer than 8 blocks and leave SMs idle: 64 x 4,096 x 4,096 10.2 us in 4 parts
-  // and 15 whole; 16 x 1,024 x 4,096 4.1 whole and 5.4 in 2; 16 x 4,096 x 16,384 14.1 whole and 16.4 in 2
-  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
-  p.splits = 1;
-  while (p.splits < 8 && tiles * p.splits * 4 <= 3 * sm_count() && p.blocks > 8 * p.splits) p.splits *= 2;
-  if (tile == 16) return small_launch<16, O>(mx, mw, p, st);
-  if (tile == 32) return small_launch<32, O>(mx, mw, p, st);
-  return small_launch<64, O>(mx, mw, p, st);
+  p.splits = split_width(static_cast<int64_t>(p.tiles_m) * p.tiles_n, p.blocks);
+  if (tile == 16) return small_launch<16, O, int8_t>(mx, mw, p, st);
+  if (tile == 32) return small_launch<32, O, int8_t>(mx, mw, p, st);
+  return small_launch<64, O, int8_t>(mx, mw, p, st);
+}
+
+template <typename O>
+int linear8_run(Linear8Params& p, const int8_t* x, int64_t pitch, const HtrcLinear8Args* a, cudaStream_t st) {
+  if (p.x == nullptr) return linear8_launch<O>(p, x, pitch, a, st);
+  if (a->dtype == HTRC_LAYER_F32) return few_launch<O, float>(p, a, st);
+  return a->dtype == HTRC_LAYER_BF16 ? few_launch<O, __nv_bfloat16>(p, a, st) : few_launch<O, __half>(p, a, st);
 }
 
 int linear8_forward(const HtrcLinear8Args* a, cudaStream_t st) {
@@ -669,7 +811,16 @@ int linear8_forward(const HtrcLinear8Args* a, cudaStream_t st) {
   const int8_t* x = static_cast<const int8_t*>(a->x);
   int64_t pitch = rows > 1 ? (a->tokens > 1 ? a->x_stride[1] : a->x_stride[0]) : code_pitch(a->width);
   p.xs = a->x_scales;
-  if (!codes) {
+  if (quantises(a)) {
+    const int es = a->dtype == HTRC_LAYER_F32 ? 4 : 2;
+    p.x = a->x;
+    p.x_stride[0] = a->x_stride[0];
+    p.x_stride[1] = a->x_stride[1];
+    p.tokens = a->tokens;
+    p.width = a->width;
+    p.vec = a->width * es % 16 == 0 && reinterpret_cast<uintptr_t>(a->x) % 16 == 0 && a->x_stride[0] * es % 16 == 0 &&
+            a->x_stride[1] * es % 16 == 0;
+  } else if (!codes) {
     const size_t at = code_bytes(a);
     if (a->workspace == nullptr || a->workspace_bytes < at + rows * sizeof(float) ||
         reinterpret_cast<uintptr_t>(a->workspace) % 256)
@@ -691,10 +842,10 @@ int linear8_forward(const HtrcLinear8Args* a, cudaStream_t st) {
   p.out = a->out;
   p.status = a->status;
   // the rows' own kernel starts when all before it has ended, the product under the rows' kernel
-  p.early = !codes;
-  if (a->out_dtype == HTRC_LAYER_F32) return linear8_launch<float>(p, x, pitch, a, st);
-  if (a->out_dtype == HTRC_LAYER_BF16) return linear8_launch<__nv_bfloat16>(p, x, pitch, a, st);
-  return linear8_launch<__half>(p, x, pitch, a, st);
+  p.early = !codes && p.x == nullptr;
+  if (a->out_dtype == HTRC_LAYER_F32) return linear8_run<float>(p, x, pitch, a, st);
+  if (a->out_dtype == HTRC_LAYER_BF16) return linear8_run<__nv_bfloat16>(p, x, pitch, a, st);
+  return linear8_run<__half>(p, x, pitch, a, st);
 }
 
 }  // namespace
@@ -707,7 +858,9 @@ int htrc_linear8_workspace_size(const HtrcLinear8Args* args, size_t* bytes) {
   if (bytes == nullptr) return HTRC_ERR_ARG;
   const int rc = htrc::linear8_validate(args);
   if (rc != HTRC_OK) return rc;
-  *bytes = args->dtype == HTRC_LAYER_I8 ? 0 : htrc::code_bytes(args) + static_cast<size_t>(args->batch * args->tokens) * 4;
+  *bytes = args->dtype == HTRC_LAYER_I8 || htrc::quantises(args)
+               ? 0
+               : htrc::code_bytes(args) + static_cast<size_t>(args->batch * args->tokens) * 4;
   return HTRC_OK;
 }
 

@@ -65,12 +65,21 @@ def _pitch(codes):
     return pitch if pitch >= shape[-1] and not pitch & 15 else None
 
 
+def _dense(shape):
+    """The strides of a dense tensor (with them ``empty_strided`` is the cheapest allocation there is)."""
+    strides, n = [], 1
+    for size in reversed(shape):
+        strides.append(n)
+        n *= max(1, size)
+    return tuple(reversed(strides))
+
+
 def _new_codes(shape, like):
     """Codes [.., width] on the tensor's device whose rows start at multiples of 16 bytes: (codes, pitch)."""
     width = shape[-1]
     pitch = (width + 15) // 16 * 16
     if pitch == width:
-        return like.new_empty(shape, dtype=torch.int8), pitch
+        return torch.empty_strided(shape, _dense(shape), dtype=torch.int8, device=like.device), pitch
     return like.new_empty((*shape[:-1], pitch), dtype=torch.int8)[..., :width], pitch
 
 
@@ -170,15 +179,15 @@ def int8_linear(x, weight, *, bias=None, dtype=None):
             if len(_plans) >= 1024:
                 _plans.clear()
             _plans[key] = plan
-    dev, sizes, wpitch, kinds, shape, dtype, need = plan
+    dev, sizes, wpitch, kinds, shape, strides, dtype, need = plan
     guard = _on(dev)
     if guard is not None:
         with guard:
             return int8_linear(x, weight, bias=bias, dtype=dtype)
-    out = ws.new_empty(shape, dtype=dtype)
+    out = torch.empty_strided(shape, strides, dtype=dtype, device=dev)
     wp = 0
-    if floats:
-        workspace = ws.new_empty((need,), dtype=torch.uint8)
+    if need:
+        workspace = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=dev)
         wp = workspace.data_ptr()
     status = _status_word(dev)
     sb, sn, *rest = sizes
@@ -227,10 +236,8 @@ def _plan(x, weight, bias, dtype, floats):
             wpitch = _pitch(wc)
         ws = ws.contiguous()
         bias = None if bias is None else bias.contiguous()
-        need = 0
         if floats:
             rows, b, n, _, sb, sn = _two_strides(rows)
-            need = (b * n * ((width + 15) // 16 * 16) + 255) // 256 * 256 + 4 * b * n      # htrc_linear8_workspace_size's
         else:
             sn = _pitch(rows)
             if sn is None:
@@ -240,7 +247,12 @@ def _plan(x, weight, bias, dtype, floats):
             b, n, sb = 1, xs.numel(), 0
     sizes = (sb, sn, b, n, width, channels, _DTYPES[rows.dtype] if floats else _lib.LAYER_I8)
     kinds = (0 if bias is None else _DTYPES[bias.dtype], _DTYPES[dtype])
+    size = ctypes.c_size_t()
+    with torch.cuda.device(dev):
+        check(lib().htrc_linear8_workspace_size(_lib.LINEAR8_ARGS.pack(0, sb, sn, 0, *sizes[2:], 0, wpitch, 0, 0, *kinds, 0, 0, 0, 0),
+                                                size), "htrc_linear8_workspace_size")
+    need = size.value
     used = (rows, xs, wc, ws, bias)
     whole = all(a is b or (a is not None and b is not None and a.data_ptr() == b.data_ptr() and a.numel() == b.numel())
                 for a, b in zip(given, used))
-    return *used, (dev, sizes, wpitch, kinds, shape, dtype, need), whole
+    return *used, (dev, sizes, wpitch, kinds, shape, _dense(shape), dtype, need), whole

@@ -21,7 +21,7 @@ from . import _lib
 from ._autograd import first_order, recorded
 from ._lib import check, lib
 from .cross import _on, _status_word
-from .linear8 import Int8Rows, _check_float_rows, _DTYPES, _new_codes, _refuse_gradients, _two_strides
+from .linear8 import Int8Rows, _check_float_rows, _dense, _DTYPES, _new_codes, _refuse_gradients, _two_strides
 
 
 def _term(t, name, shapes, width, device):
@@ -89,7 +89,8 @@ def _meta(t):
 
 
 def _call(x, weight, bias, scale, shift, eps):
-    """(x, parameters, sizes, strides, kinds, dense) of checked arguments.  What follows from their shapes, strides and
+    """(x, parameters, sizes, strides, kinds, dense, lead) of checked arguments, lead being the shape and strides of a value
+    per row.  What follows from their shapes, strides and
     types alone is kept for calls that repeat them: the checks cost more host time than the rest of a small call."""
     given = (weight, bias, scale, shift)
     try:
@@ -100,7 +101,8 @@ def _call(x, weight, bias, scale, shift, eps):
     if kept is not None:
         return x, given, *kept
     c = _Call(x, weight, bias, scale, shift, eps)
-    kept = (c.sizes, c.strides, c.kinds, c.dense)
+    lead = tuple(x.shape[:-1])
+    kept = (c.sizes, c.strides, c.kinds, c.dense, (lead, _dense(lead)))
     if key is not None and c.x.data_ptr() == x.data_ptr() and all(a is b for a, b in zip(c.keep, given)):
         if len(_plans) >= 1024:
             _plans.clear()
@@ -121,7 +123,7 @@ _NO_BACK = (0,) * 13
 
 
 def _forward(given, weight, bias, scale, shift, eps, stats):
-    x, params, sizes, strides, kinds, dense = _call(given, weight, bias, scale, shift, eps)
+    x, params, sizes, strides, kinds, dense, lead = _call(given, weight, bias, scale, shift, eps)
     guard = _on(x.device)
     if guard is not None:
         with guard:
@@ -130,7 +132,7 @@ def _forward(given, weight, bias, scale, shift, eps, stats):
     mean = rstd = None
     mp = rp = 0
     if stats:
-        mean = given.new_empty(given.shape[:-1], dtype=torch.float32)
+        mean = torch.empty_strided(*lead, dtype=torch.float32, device=x.device)
         rstd = torch.empty_like(mean)
         mp, rp = mean.data_ptr(), rstd.data_ptr()
     rc = lib().htrc_norm_forward(
@@ -144,12 +146,12 @@ def _forward(given, weight, bias, scale, shift, eps, stats):
 _workspaces = {}
 
 
-def _workspace_bytes(key, args):
+def _workspace_bytes(key, head):
     """What the backward asks for: it goes by sizes, strides and alignments alone (``key``)."""
     need = _workspaces.get(key)
     if need is None:
         size = ctypes.c_size_t()
-        check(lib().htrc_norm_workspace_size(args, size), "htrc_norm_workspace_size")
+        check(lib().htrc_norm_workspace_size(_lib.NORM_ARGS.pack(*head, 0, 0), size), "htrc_norm_workspace_size")
         if len(_workspaces) >= 1024:
             _workspaces.clear()
         need = _workspaces[key] = size.value
@@ -158,7 +160,7 @@ def _workspace_bytes(key, args):
 
 def _backward(dy, given, mean, rstd, weight, bias, scale, shift, wanted=(True,) * 4):
     """dx and the gradients of weight, bias, scale and shift: None for those that are none or not wanted."""
-    x, params, sizes, strides, kinds, dense = _call(given, weight, bias, scale, shift, 0.0)
+    x, params, sizes, strides, kinds, dense, _ = _call(given, weight, bias, scale, shift, 0.0)
     dev, shape = x.device, given.shape
     if not isinstance(dy, torch.Tensor) or dy.shape != shape or dy.dtype != x.dtype or dy.device != dev:
         raise ValueError(f"dy: {list(shape)} {x.dtype} on x's device expected")
@@ -170,21 +172,24 @@ def _backward(dy, given, mean, rstd, weight, bias, scale, shift, wanted=(True,) 
         with guard:
             return _backward(dy, given, mean, rstd, weight, bias, scale, shift, wanted)
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    if dy.dim() > 3:
-        dy = dy.reshape(sizes[2:5])
-    dy, _, _, _, gb, gn = _two_strides(dy)
+    if dy.is_contiguous():
+        gb, gn = dense
+    else:
+        dy, _, _, _, gb, gn = _two_strides(dy.reshape(sizes[2:5]))
     dx = _like(given)
-    grads = [_like(t) if t is not None and want else None for t, want in zip((weight, bias, scale, shift), wanted)]
-    to = _pointers(grads)
+    grads, to = [], []
+    for t, want in zip((weight, bias, scale, shift), wanted):
+        g = _like(t) if want and t is not None else None
+        grads.append(g)
+        to.append(0 if g is None else g.data_ptr())
     status = _status_word(dev)
     xp, gp, terms = x.data_ptr(), dy.data_ptr(), _pointers(params)
     head = (xp, *sizes, *terms, *strides, *kinds, 0, 0, 0, 0, 0, 0, mean.data_ptr(), rstd.data_ptr(), gp, gb, gn,
             dx.data_ptr(), *dense, *to, 0 if status is None else status.data_ptr())
     ws, wp, need = None, 0, 0
     if any(to):
-        w, _, s, t = (p != 0 for p in terms)
-        need = _workspace_bytes((sizes, gb, gn, xp & 15, gp & 15, w, s, t, dev.index), _lib.NORM_ARGS.pack(*head, 0, 0))
-        ws = given.new_empty((need,), dtype=torch.uint8)
+        need = _workspace_bytes((sizes, gb, gn, xp & 15, gp & 15, terms[0] != 0, terms[2] != 0, terms[3] != 0, dev.index), head)
+        ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=dev)
         wp = ws.data_ptr()
     rc = lib().htrc_norm_backward(_lib.NORM_ARGS.pack(*head, wp, need), _lib.raw_stream(dev.index))
     if rc:
@@ -236,13 +241,13 @@ def layer_norm_int8(x, *, weight=None, bias=None, scale=None, shift=None, eps=1e
 
 
 def _codes(given, *terms):
-    x, params, sizes, strides, kinds, _ = _call(given, *terms)
+    x, params, sizes, strides, kinds, _, lead = _call(given, *terms)
     guard = _on(x.device)
     if guard is not None:
         with guard:
             return _codes(given, *terms)
     codes, pitch = _new_codes(given.shape, given)
-    scales = given.new_empty(given.shape[:-1], dtype=torch.float32)
+    scales = torch.empty_strided(*lead, dtype=torch.float32, device=x.device)
     rc = lib().htrc_norm_forward(
         _lib.NORM_ARGS.pack(x.data_ptr(), *sizes, *_pointers(params), *strides, *kinds, 0, 0, 0, codes.data_ptr(), pitch,
                             scales.data_ptr(), 0, 0, *_NO_BACK), _lib.raw_stream(x.device.index))

@@ -150,7 +150,8 @@ int htrc_quantize_rows(const void* x, int32_t dtype, int64_t batch, int64_t toke
                        int8_t* codes, int64_t pitch, float* scales, htrc_stream_t stream);
 
 /* Product in 8-bit integers: out[row][n] = (sum over k of x[row][k] w[n][k]) x_scales[row] w_scales[n] + bias[n], the sum
- * an exact 32-bit integer, the rest float32, rounded once.  Rows that are not 8-bit yet are quantised into the workspace. */
+ * an exact 32-bit integer, the rest float32, rounded once.  Rows that are not 8-bit yet are quantised into the workspace, or
+ * (few of them) by the product. */
 enum { HTRC_LINEAR8_MAX_WIDTH = 65536 };
 
 typedef struct {
@@ -167,7 +168,7 @@ typedef struct {
   int32_t bias_dtype, out_dtype;   /* HTRC_LAYER_F32 / BF16 / F16 */
   void* out;                    /* [batch * tokens][channels], dense */
   int32_t* status;              /* as in HtrcCrossArgs */
-  void* workspace;              /* htrc_linear8_workspace_size() bytes (0 for 8-bit rows), 256-byte aligned */
+  void* workspace;              /* htrc_linear8_workspace_size() bytes (it may be 0), 256-byte aligned */
   size_t workspace_bytes;
 } HtrcLinear8Args;
 

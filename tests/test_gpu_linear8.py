@@ -75,6 +75,22 @@ def test_floats_are_quantised_on_the_way(dev, size, dtype):
     assert torch.equal(got, htrc_b200.int8_linear(rows, w, bias=bias, dtype=dtype))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [1, 5, 128, 130, 1000, 4096, 4104, 8200, 16384])
+def test_few_float_rows(dev, width, dtype):
+    """Up to 16 rows are quantised by the product itself (up to a width): the same codes as the rows' own kernel's, rows of
+    any alignment and stride, split over the width or not."""
+    gen = torch.Generator(device=dev).manual_seed(width)
+    for channels in (100, 3000, 20000 if width < 1000 else 9000):
+        w = htrc_b200.quantize_rows(torch.randn((channels, width), generator=gen, device=dev))
+        for shape in ((1, 1), (16, 1), (3, 5)):
+            room = torch.randn((*shape, width + 17), generator=gen, device=dev).to(dtype)
+            for x in (room[..., :width], room[..., 17:], room[..., 1:1 + width].contiguous()):
+                want = htrc_b200.int8_linear(htrc_b200.quantize_rows(x), w, dtype=dtype)
+                assert torch.equal(htrc_b200.int8_linear(x, w), want)
+    htrc_b200.int8_linear_status()
+
+
 def test_extreme_codes_and_widest_rows(dev):
     """Sums at the ends of what the width allows: 65,536 products of 128 * 128 are 2^30."""
     for width in (65536, 1024):

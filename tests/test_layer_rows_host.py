@@ -141,8 +141,8 @@ def test_linear8_workspace_size():
     L = _lib.lib()
     n = ctypes.c_size_t(1)
     assert L.htrc_linear8_workspace_size(ctypes.byref(_linear()), ctypes.byref(n)) == _lib.HTRC_OK and n.value == 0
-    assert L.htrc_linear8_workspace_size(ctypes.byref(_linear(dtype=_lib.LAYER_F32)), ctypes.byref(n)) == _lib.HTRC_OK
-    assert n.value >= 10 * 64 + 10 * 4
+    assert L.htrc_linear8_workspace_size(ctypes.byref(_linear(dtype=_lib.LAYER_F32, tokens=20)), ctypes.byref(n)) == _lib.HTRC_OK
+    assert n.value >= 40 * 64 + 40 * 4
     assert L.htrc_linear8_workspace_size(ctypes.byref(_linear()), None) == _lib.HTRC_ERR_ARG
     assert L.htrc_linear8_forward(None, None) == _lib.HTRC_ERR_ARG
 

@@ -32,6 +32,8 @@ struct Linear8Params {
   void* out;
   int* status;
   int tiles_m, tiles_n, splits;
+  int stages;                               // few tokens: of the ring, behind rows_bytes of codes
+  uint32_t rows_bytes;
   bool early;                               // few tokens: the kernel before this one did not write the weights
   // few float rows, quantised by the product: their elements, strides, tokens of a batch entry and width
   const void* x;
@@ -90,21 +92,22 @@ template <int T, typename X>
 struct SmallShape {
   static constexpr bool kCodes = std::is_same<X, int8_t>::value;
   static constexpr int kRowWarps = kCodes ? 4 : 16, kThreads = 32 * (kRowWarps + 2);
-  static constexpr int kStages = T <= 32 ? 5 : 4;          // two CTAs per SM
   static constexpr uint32_t kW = kSmallChannels * 128, kX = T * 128, kStage = kCodes ? kW + kX : kW;
   static constexpr uint32_t kCols = T < 32 ? 32 : T;
-  static constexpr uint32_t kBars = kStages * kStage, kRows = kBars + 256;    // kRows: float rows' codes, block by block
-  static_assert(T * kSmallChannels * 4 <= kBars, "the parts of a split tile reuse the stages");
-  static uint32_t bytes(int blocks) { return kCodes ? kBars + 256 : (kRows + 1023) / 1024 * 1024 + blocks * kX; }
+  static constexpr uint32_t kBars = 1024;                  // then float rows' codes, block by block, then the stages
+  static constexpr uint32_t kMost = 224 * 1024;            // of an SM's CTA; half of it where two share the SM
+  static_assert(T * kSmallChannels * 4 <= 2 * kStage, "the parts of a split tile reuse the stages");
+  static uint32_t rows(int blocks) { return kCodes ? 0 : blocks * kX; }
 };
+constexpr int kSmallStages = 12;                           // at most
 
 struct SmallBars {
-  uint64_t full[5], empty[5], done, rows;
+  uint64_t full[kSmallStages], empty[kSmallStages], done, rows;
   uint32_t tmem;
   int abort_flag;
   float scales[kFewTokens];
 };
-static_assert(sizeof(SmallBars) <= 256, "barriers");
+static_assert(sizeof(SmallBars) <= 1024, "barriers");
 
 // A float row's scale, and the codes of its elements from k0 up to k1 into blocks of [T][128] bytes, 128-byte swizzled (what
 // is past the row in its last block is whatever was there: the weights are zero there).  One warp.
@@ -154,13 +157,13 @@ __device__ __forceinline__ float quantise_row(const X* x, int width, bool vec, i
   auto code = [&](float v) { return __float_as_uint(__fadd_rn(__fmul_rn(v, by), 12582912.f)) & 0xFFu; };
   k1 = min(k1, width);
   if (vec) {
-    for (int k = k0 + lane * N; k < k1; k += 4 * 32 * N) {
-      Sixteen t[4];
+    for (int k = k0 + lane * N; k < k1; k += 8 * 32 * N) {
+      Sixteen t[8];
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      for (int b = 0; b < 8; ++b)
         t[b].v = k + 32 * N * b < k1 ? __ldg(reinterpret_cast<const uint4*>(x + k + 32 * N * b)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
+      for (int b = 0; b < 8; ++b) {
         uint32_t w[2] = {0, 0};
 #pragma unroll
         for (int j = 0; j < N; ++j) w[j / 4] |= code(one(t[b].e[j])) << (8 * (j % 4));
@@ -187,19 +190,21 @@ __device__ __forceinline__ float quantise_row(const X* x, int width, bool vec, i
 }
 
 template <int T, typename O, typename X>
-__global__ void __launch_bounds__(SmallShape<T, X>::kThreads)
+__global__ void __launch_bounds__(SmallShape<T, X>::kThreads, 1)
     linear8_small_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                          const __grid_constant__ Linear8Params p) {
   using SM = SmallShape<T, X>;
   constexpr int kTma = SM::kRowWarps, kMma = kTma + 1;
   extern __shared__ __align__(1024) uint8_t smem[];
-  SmallBars* bars = reinterpret_cast<SmallBars*>(smem + SM::kBars);
-  uint8_t* codes = smem + (SM::kRows + 1023) / 1024 * 1024;
+  SmallBars* bars = reinterpret_cast<SmallBars*>(smem);
+  uint8_t* const codes = smem + SM::kBars;
+  uint8_t* const ring = codes + p.rows_bytes;
+  const int stages = p.stages;
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool aligned = (smem_u32(smem) & 1023) == 0;      // the swizzled tiles need it
   if (threadIdx.x == 0) {
-    for (int i = 0; i < SM::kStages; ++i) {
+    for (int i = 0; i < stages; ++i) {
       mbar_init(&bars->full[i], 1);
       mbar_init(&bars->empty[i], 1);
     }
@@ -227,27 +232,27 @@ __global__ void __launch_bounds__(SmallShape<T, X>::kThreads)
       const uint64_t once = policy_evict_first(), keep = policy_evict_last();
       auto load_w = [&](int s, int b) {
         expect_tx(&bars->full[s], SM::kStage);
-        tma_load_2d(smem + s * SM::kStage, &tm_w, &bars->full[s], b * 128, n0, p.tiles_m > 1 ? keep : once);
+        tma_load_2d(ring + s * SM::kStage, &tm_w, &bars->full[s], b * 128, n0, p.tiles_m > 1 ? keep : once);
       };
       auto load_x = [&](int s, int b) {
-        if (SM::kCodes) tma_load_2d(smem + s * SM::kStage + SM::kW, &tm_x, &bars->full[s], b * 128, row0, keep);
+        if (SM::kCodes) tma_load_2d(ring + s * SM::kStage + SM::kW, &tm_x, &bars->full[s], b * 128, row0, keep);
       };
-      const int first = min(b1 - b0, SM::kStages);
+      const int first = min(b1 - b0, stages);
       if (!p.early) asm volatile("griddepcontrol.wait;" ::: "memory");
       for (int i = 0; i < first; ++i) load_w(i, b0 + i);
       if (p.early) asm volatile("griddepcontrol.wait;" ::: "memory");
       for (int i = 0; i < first; ++i) load_x(i, b0 + i);
       int issued = first;
       for (int i = first; i < b1 - b0; ++i) {
-        const int s = i % SM::kStages;
-        if (!mbar_wait(&bars->empty[s], (i / SM::kStages - 1) & 1, p.status, abort_flag)) break;
+        const int s = i % stages;
+        if (!mbar_wait(&bars->empty[s], (i / stages - 1) & 1, p.status, abort_flag)) break;
         load_w(s, b0 + i);
         load_x(s, b0 + i);
         issued = i + 1;
       }
       // before the CTA leaves: every load has landed (again with a limit)
       int gave_up = 0;
-      drain_ring<false>(bars->full, SM::kStages, issued, p.status, &gave_up);
+      drain_ring<false>(bars->full, stages, issued, p.status, &gave_up);
     }
     __syncwarp();
   } else if (warp == kMma) {
@@ -256,12 +261,12 @@ __global__ void __launch_bounds__(SmallShape<T, X>::kThreads)
     bool ok = aligned;
     if (!SM::kCodes) ok = ok && mbar_wait_warp(&bars->rows, 0, p.status, abort_flag);
     for (int i = 0; ok && i < b1 - b0; ++i) {
-      const int s = i % SM::kStages;
-      ok = mbar_wait_warp(&bars->full[s], (i / SM::kStages) & 1, p.status, abort_flag);
+      const int s = i % stages;
+      ok = mbar_wait_warp(&bars->full[s], (i / stages) & 1, p.status, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      const uint64_t a = sw128_desc(smem_u32(smem + s * SM::kStage), 16, 1024);
-      const uint64_t b = sw128_desc(smem_u32(SM::kCodes ? smem + s * SM::kStage + SM::kW : codes + i * SM::kX), 16, 1024);
+      const uint64_t a = sw128_desc(smem_u32(ring + s * SM::kStage), 16, 1024);
+      const uint64_t b = sw128_desc(smem_u32(SM::kCodes ? ring + s * SM::kStage + SM::kW : codes + i * SM::kX), 16, 1024);
 #pragma unroll
       for (int k = 0; k < 4; ++k) mma_i8_by(leader, tmem, a + 2 * k, b + 2 * k, idesc, i > 0 || k > 0);
       mma_commit_by(leader, &bars->empty[s]);
@@ -270,7 +275,7 @@ __global__ void __launch_bounds__(SmallShape<T, X>::kThreads)
     // the products are done before the CTA leaves, those of an aborted one too
     int gave_up = 0;
     mbar_wait_warp(&bars->done, 0, p.status, &gave_up);
-    drain_ring<true>(bars->empty, SM::kStages, ok ? b1 - b0 : 0, p.status, &gave_up);
+    drain_ring<true>(bars->empty, stages, ok ? b1 - b0 : 0, p.status, &gave_up);
   } else {
     if constexpr (!SM::kCodes) {
       asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -294,7 +299,7 @@ __global__ void __launch_bounds__(SmallShape<T, X>::kThreads)
       ok = mbar_wait_warp(&bars->done, 0, p.status, abort_flag) && ok && *abort_flag == 0;
       tc_fence_after();
       const uint32_t at = tmem + (static_cast<uint32_t>(32 * warp) << 16);
-      int* part = reinterpret_cast<int*>(smem);
+      int* part = reinterpret_cast<int*>(ring);
       if (__all_sync(0xffffffffu, ok)) {
         for (int t0 = 0; t0 < T && row0 + t0 < p.rows; t0 += 16) {
           uint32_t v[16];
@@ -324,7 +329,7 @@ __global__ void __launch_bounds__(SmallShape<T, X>::kThreads)
         const int rows = min(T, p.rows - row0), share = T / splits, first = rank * share;
         constexpr int kBatch = T / 8 < 8 ? T / 8 : 8;       // tokens whose parts are in flight together
         for (int t0 = first; t0 < min(first + share, rows); t0 += kBatch) {
-          const uint32_t mine = smem_u32(smem) + (t0 * kSmallChannels + 32 * warp + lane) * 4;
+          const uint32_t mine = smem_u32(ring) + (t0 * kSmallChannels + 32 * warp + lane) * 4;
           int sum[kBatch];
 #pragma unroll
           for (int j = 0; j < kBatch; ++j) sum[j] = 0;
@@ -353,14 +358,21 @@ __global__ void __launch_bounds__(SmallShape<T, X>::kThreads)
 }
 
 template <int T, typename O, typename X>
-int small_launch(const CUtensorMap& mx, const CUtensorMap& mw, const Linear8Params& p, cudaStream_t st) {
+int small_launch(const CUtensorMap& mx, const CUtensorMap& mw, Linear8Params& p, cudaStream_t st) {
   using SM = SmallShape<T, X>;
   auto kernel = linear8_small_kernel<T, O, X>;
-  const uint32_t bytes = SM::bytes((p.blocks + p.splits - 1) / p.splits);
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::bytes(kFewBlocks)) != cudaSuccess)
-    return HTRC_ERR_CUDA;
+  // as many stages as there is room for: where the CTAs do not fill the SMs twice one has an SM to itself (16 x 4,096 x 16,384:
+  // the loads in flight are all that counts)
+  const int64_t ctas = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits;
+  const int part = (p.blocks + p.splits - 1) / p.splits;
+  const uint32_t room = (ctas <= sm_count() ? SM::kMost : SM::kMost / 2) - 1024, fixed = SM::kBars + SM::rows(part);
+  p.rows_bytes = SM::rows(part);
+  p.stages = fixed + 2 * SM::kStage > room ? 2 : static_cast<int>((room - fixed) / SM::kStage);
+  p.stages = std::max(2, std::min({p.stages, kSmallStages, part}));
+  const uint32_t bytes = fixed + p.stages * SM::kStage;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kMost) != cudaSuccess) return HTRC_ERR_CUDA;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.splits));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(SM::kThreads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
@@ -727,9 +739,12 @@ int split_width(int64_t tiles, int blocks) {
   return splits;
 }
 
-// whether the product quantises its float rows itself: few of them, and no more of the width to a CTA than it has room for
+// Whether the product quantises its float rows itself: few of them, and no more of the width to a CTA than it has room for.
+// Every CTA reads all of them, which costs more than the launch that it saves where the weights take longer than that launch:
+// 16 x 4,096 x 16,384 19.2 us by itself and 16.5 behind the rows' kernel; 16 x 4,096 x 4,096 10.8 either way, and one launch.
 bool quantises(const HtrcLinear8Args* a) {
   if (a->dtype == HTRC_LAYER_I8 || a->batch * a->tokens > kFewTokens) return false;
+  if (a->batch * a->tokens * a->width > 32768 && static_cast<int64_t>(a->width) * a->channels > (32 << 20)) return false;
   const int blocks = (a->width + 127) / 128, splits = split_width((a->channels + kSmallChannels - 1) / kSmallChannels, blocks);
   return (blocks + splits - 1) / splits <= kFewBlocks;
 }

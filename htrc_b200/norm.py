@@ -89,8 +89,8 @@ def _meta(t):
 
 
 def _call(x, weight, bias, scale, shift, eps):
-    """(x, parameters, sizes, strides, kinds, dense, lead) of checked arguments, lead being the shape and strides of a value
-    per row.  What follows from their shapes, strides and
+    """(x, parameters, sizes, strides, kinds, dense, lead, whole) of checked arguments, lead and whole being the shape and
+    dense strides of a value per row and of rows.  What follows from their shapes, strides and
     types alone is kept for calls that repeat them: the checks cost more host time than the rest of a small call."""
     given = (weight, bias, scale, shift)
     try:
@@ -102,7 +102,7 @@ def _call(x, weight, bias, scale, shift, eps):
         return x, given, *kept
     c = _Call(x, weight, bias, scale, shift, eps)
     lead = tuple(x.shape[:-1])
-    kept = (c.sizes, c.strides, c.kinds, c.dense, (lead, _dense(lead)))
+    kept = (c.sizes, c.strides, c.kinds, c.dense, (lead, _dense(lead)), (tuple(x.shape), _dense(x.shape)))
     if key is not None and c.x.data_ptr() == x.data_ptr() and all(a is b for a, b in zip(c.keep, given)):
         if len(_plans) >= 1024:
             _plans.clear()
@@ -123,12 +123,12 @@ _NO_BACK = (0,) * 13
 
 
 def _forward(given, weight, bias, scale, shift, eps, stats):
-    x, params, sizes, strides, kinds, dense, lead = _call(given, weight, bias, scale, shift, eps)
+    x, params, sizes, strides, kinds, dense, lead, whole = _call(given, weight, bias, scale, shift, eps)
     guard = _on(x.device)
     if guard is not None:
         with guard:
             return _forward(given, weight, bias, scale, shift, eps, stats)
-    out = _like(given)
+    out = torch.empty_strided(*whole, dtype=x.dtype, device=x.device)
     mean = rstd = None
     mp = rp = 0
     if stats:
@@ -160,7 +160,7 @@ def _workspace_bytes(key, head):
 
 def _backward(dy, given, mean, rstd, weight, bias, scale, shift, wanted=(True,) * 4):
     """dx and the gradients of weight, bias, scale and shift: None for those that are none or not wanted."""
-    x, params, sizes, strides, kinds, dense, _ = _call(given, weight, bias, scale, shift, 0.0)
+    x, params, sizes, strides, kinds, dense, _, whole = _call(given, weight, bias, scale, shift, 0.0)
     dev, shape = x.device, given.shape
     if not isinstance(dy, torch.Tensor) or dy.shape != shape or dy.dtype != x.dtype or dy.device != dev:
         raise ValueError(f"dy: {list(shape)} {x.dtype} on x's device expected")
@@ -176,7 +176,7 @@ def _backward(dy, given, mean, rstd, weight, bias, scale, shift, wanted=(True,) 
         gb, gn = dense
     else:
         dy, _, _, _, gb, gn = _two_strides(dy.reshape(sizes[2:5]))
-    dx = _like(given)
+    dx = torch.empty_strided(*whole, dtype=x.dtype, device=dev)
     grads, to = [], []
     for t, want in zip((weight, bias, scale, shift), wanted):
         g = _like(t) if want and t is not None else None
@@ -241,12 +241,15 @@ def layer_norm_int8(x, *, weight=None, bias=None, scale=None, shift=None, eps=1e
 
 
 def _codes(given, *terms):
-    x, params, sizes, strides, kinds, _, lead = _call(given, *terms)
+    x, params, sizes, strides, kinds, _, lead, whole = _call(given, *terms)
     guard = _on(x.device)
     if guard is not None:
         with guard:
             return _codes(given, *terms)
-    codes, pitch = _new_codes(given.shape, given)
+    if sizes[4] % 16:
+        codes, pitch = _new_codes(given.shape, given)
+    else:
+        codes, pitch = torch.empty_strided(*whole, dtype=torch.int8, device=x.device), sizes[4]
     scales = torch.empty_strided(*lead, dtype=torch.float32, device=x.device)
     rc = lib().htrc_norm_forward(
         _lib.NORM_ARGS.pack(x.data_ptr(), *sizes, *_pointers(params), *strides, *kinds, 0, 0, 0, codes.data_ptr(), pitch,

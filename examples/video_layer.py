@@ -1,13 +1,17 @@
 """The attention part of a video transformer's layer on htrc_b200's operators, and a few training steps of its prompt
 branch (synthetic latents, states and weights).
 
-    python examples/video_layer.py [--grid 16,32,32] [--heads 24] [--keys 256] [--train 0]
+    python examples/video_layer.py [--grid 16,32,32] [--heads 24] [--keys 256] [--train 0] [--modulated]
 
 Self attention: q and k are normalised per head, turned by their (time, height, width) positions and laid out head by
 head in one pass (``rotary_qk``), then attend through the flat operator (``flat_attention_heads``).  Cross attention:
 the tokens read the states of an encoder, each batch entry its own number of them (``cross_attention``).  ``--train``
 trains the prompt branch alone, as an adapter would: its gradients run through ``rotary_axes`` (the query norm, no
 rotation) and ``cross_attention``.
+
+``--modulated``: the same branches behind a layer norm that a timestep's scale and shift modulate, trained as they are
+(``layer_norm``), and the self branch also as it is served, its norm written in 8 bits and its projections multiplied in 8
+bits (``layer_norm_int8``, ``int8_linear``).
 """
 from __future__ import annotations
 
@@ -37,12 +41,15 @@ class SelfBranch(nn.Module):
 
     @torch.no_grad()
     def forward(self, x, positions):
-        q, k, v = self.qkv(x).unflatten(-1, (3, self.heads, 128)).unbind(-3)       # strided views, no copies
+        return self.out(self.attend(self.qkv(x), positions).to(x.dtype))
+
+    def attend(self, qkv, positions):
+        q, k, v = qkv.unflatten(-1, (3, self.heads, 128)).unbind(-3)               # strided views, no copies
         q, k = htrc_b200.rotary_qk(q, k, positions, axes=AXES, q_weight=self.norm[0], k_weight=self.norm[1],
                                    heads_first=True)
         a = torch.stack([htrc_b200.flat_attention_heads(*rows, **self.cfg)
                          for rows in zip(q, k, v.transpose(1, 2).contiguous())])    # [batch, heads, tokens, 128]
-        return self.out(a.transpose(1, 2).flatten(2).to(x.dtype))
+        return a.transpose(1, 2).flatten(2)
 
 
 class PromptBranch(nn.Module):
@@ -62,6 +69,36 @@ class PromptBranch(nn.Module):
         q, k = (htrc_b200.rotary_axes(r, r.new_zeros(r.shape[:2] + (1,), dtype=torch.int32), axes=(0,), weight=w)
                 for r, w in zip((q, k), self.norm))                                 # no axis is turned: the norm alone
         return self.out(htrc_b200.cross_attention(q, k, v, key_lengths=lengths).flatten(2))
+
+
+class Modulated(nn.Module):
+    """A branch behind its norm, with the scale and shift that a timestep's embedding gives each batch entry."""
+
+    def __init__(self, branch, width, embedding):
+        super().__init__()
+        self.branch = branch
+        self.terms = nn.Linear(embedding, 2 * width)
+
+    def forward(self, x, step, *args):
+        scale, shift = self.terms(step).chunk(2, -1)
+        return self.branch(htrc_b200.layer_norm(x, scale=scale, shift=shift), *args)
+
+
+class ServedBranch:
+    """A modulated self branch for inference, its weights in 8 bits with a scale per channel."""
+
+    @torch.no_grad()
+    def __init__(self, modulated):
+        self.modulated = modulated
+        self.qkv, self.out = (htrc_b200.quantize_rows(m.weight) for m in (modulated.branch.qkv, modulated.branch.out))
+
+    @torch.no_grad()
+    def __call__(self, x, step, positions):
+        own = self.modulated.branch
+        scale, shift = self.modulated.terms(step).chunk(2, -1)
+        rows = htrc_b200.layer_norm_int8(x, scale=scale, shift=shift)              # the norm is never written in 16 bits
+        qkv = htrc_b200.int8_linear(rows, self.qkv, dtype=x.dtype)
+        return htrc_b200.int8_linear(own.attend(qkv, positions).to(x.dtype), self.out)
 
 
 class VideoLayer(nn.Module):
@@ -105,6 +142,21 @@ def train(layer, x, positions, states, lengths, steps, rate=3e-4):
     return losses
 
 
+def modulated(layer, x, positions, states, lengths, embedding=256):
+    """(the served self branch's answer, the same branch's in the layer's type, the gradients' norms of one training step of
+    the prompt branch and its modulation) on the layer's weights."""
+    torch.manual_seed(2)
+    width = x.shape[-1]
+    step = torch.randn((x.shape[0], embedding), device="cuda").to(x.dtype)
+    own, prompt = (Modulated(b, width, embedding).cuda().to(x.dtype) for b in (layer.own, layer.prompt))
+    served = ServedBranch(own)(x, step, positions)
+    with torch.no_grad():
+        plain = own(x, step, positions)
+    prompt.zero_grad()
+    prompt(x, step, states, lengths).float().pow(2).mean().backward()
+    return served, plain, {n: float(p.grad.float().norm()) for n, p in prompt.named_parameters()}
+
+
 def main():
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--grid", default="16,32,32")
@@ -112,6 +164,7 @@ def main():
     ap.add_argument("--kv-heads", type=int, default=8)
     ap.add_argument("--keys", type=int, default=256)
     ap.add_argument("--train", type=int, default=0, help="training steps of the prompt branch")
+    ap.add_argument("--modulated", action="store_true", help="the branches behind a modulated norm, served in 8 bits")
     a = ap.parse_args()
     grid = tuple(int(g) for g in a.grid.split(","))
     layer, *args = make(grid, a.heads, a.kv_heads, a.keys)
@@ -126,6 +179,11 @@ def main():
     htrc_b200.cross_status()
     print(f"{args[0].shape[0]} x {args[0].shape[1]} tokens: {start.elapsed_time(end):.2f} ms, "
           f"rms {float(y.float().pow(2).mean().sqrt()):.3f}")
+    if a.modulated:
+        served, plain, norms = modulated(layer, *args)
+        off = float((served.float() - plain.float()).pow(2).mean().sqrt() / plain.float().pow(2).mean().sqrt())
+        print(f"self branch in 8 bits: {off:.4f} of its rms off; gradient norms of the prompt branch:",
+              " ".join(f"{n} {v:.3g}" for n, v in norms.items()))
     if a.train:
         losses = train(layer, *args, a.train)
         print("prompt branch, relative error:", " ".join(f"{x:.3f}" for x in losses))

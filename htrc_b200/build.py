@@ -11,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -36,18 +37,22 @@ def build(verbose: bool = False, ptxas_verbose: bool = False, force: bool = Fals
         return LIB
     out_dir = ROOT / "_build"
     out_dir.mkdir(exist_ok=True)
-    objs = []
     flags = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
                     "-I", str(ROOT / "include")]
     if ptxas_verbose:
         flags += ["-Xptxas", "-v"]
-    for s in srcs:
-        o = out_dir / (s.stem + ".o")
-        cmd = [nvcc_path(), "-c", str(s), "-o", str(o)] + flags
+
+    def compile_one(src):
+        o = out_dir / (src.stem + ".o")
+        cmd = [nvcc_path(), "-c", str(src), "-o", str(o)] + flags
         if verbose:
             print(" ".join(cmd))
         subprocess.run(cmd, check=True)
-        objs.append(str(o))
+        return str(o)
+
+    # the longest first; nvcc runs in processes of its own
+    with ThreadPoolExecutor(max(1, min(len(srcs), os.cpu_count() or 1))) as pool:
+        objs = list(pool.map(compile_one, sorted(srcs, key=lambda f: -f.stat().st_size)))
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [nvcc_path(), "-shared", "-o", str(tmp)] + objs + ARCH + ["-Xcompiler", "-fPIC"]
     if verbose:

@@ -9,6 +9,10 @@
 // Many tokens (linear8_pair_kernel): two CTAs on neighbouring SMs share a tile of 256 tokens x 256 channels (cta_group::2),
 // each loading half of either operand; persistent, two accumulators in TMEM, so that a tile leaves under the next one's
 // products.
+//
+// Measured, 8-bit rows, bfloat16 out: 129,024 x 2,048 x 6,144 1,090 us after a rest (2,980 TOP/s) and 1,270 once the 1,000 W cap
+// holds the SM clock at 1,290 MHz; 8,192 x 8,192 x 8,192 335 (3,280) and 395.  The tensor pipe is busy for 82 % of 16,384 x
+// 2,048 x 6,144; the cap bounds the rest.  16 x 4,096 x 16,384: 14.1 us, the weights at 4.8 TB/s.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -657,8 +661,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             bulk_commit_group();
           }
         } else {
-          // rows of any alignment, by 4-byte words, a row's neighbours together (19,000 x 1,024 x 3,499 in bfloat16: see the
-          // launch's comment)
+          // rows of any alignment, by 4-byte words, a row's neighbours together (19,000 x 1,024 x 3,499 in bfloat16 143 us,
+          // aligned 75)
           __syncwarp();
           const int cols = min(kCols, p.channels - (channel + c)), high = min(32, p.rows - row);
           O* out = static_cast<O*>(p.out) + static_cast<int64_t>(row) * p.channels + channel + c;

@@ -4,10 +4,14 @@
 //   u = (x - mean) rstd,   y = (u weight + bias) (1 + scale) + shift = u A + B
 //   codes = rint(y (127 / top)), scales = top / 127, top = max |y| of the row
 //
-// Forward: a row is read once and stays in registers as it was read, 8 lanes to 16 warps to a row, several rows to a lane's
-// eight pieces, and the next rows are fetched before these are used.  The mean, then the squared deviations from it (no
-// cancellation under a large mean), then the result, all float32.  A and B are formed once per batch entry in shared memory.
-// HBM bounds it: 4 bytes per 16-bit element, 3 to 8-bit rows.
+// Forward: a row is read once and stays in registers as it was read, 8 lanes to 16 warps to a row, up to four rows to a lane,
+// which share the reading of A and B.  The mean, then the squared deviations from it (no cancellation under a large mean),
+// then the result, all float32.  A and B are formed once per batch entry in shared memory.  An entry's CTAs sweep its rows
+// together: each with rows of its own far from the others' cost 10 % (129,024 x 2,048: 188 us, 168).
+//
+// HBM bounds it: 4 bytes per 16-bit element, 3 to 8-bit rows.  129,024 x 2,048 in bfloat16, device time after a rest: plain
+// 170 us (6.2 TB/s), modulated 177 (5.9), its 8-bit rows 160 (4.9; issue and 16 warps of 128 registers), 8-bit rows of x
+// itself 131 (6.0).
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
@@ -21,7 +25,7 @@ namespace htrc {
 
 namespace {
 
-constexpr int kNormThreads = 256;           // of a CTA whose rows take a warp or less; wider rows: one row's lanes
+constexpr int kNormThreads = 256;           // of a CTA; of rows that take more: those lanes
 constexpr int kNormMaxWarps = 16;           // per row
 constexpr int kNormSms = 228 * 1024;        // shared memory of an SM
 constexpr float kRoundMagic = 12582912.f;   // 1.5 * 2^23: adding it rounds to the nearest integer, ties to even
@@ -211,7 +215,9 @@ __device__ __forceinline__ void over_lanes(float (&v)[R], int L, int group, floa
   }
 }
 
-// LANES: lanes to a row, or 0 for any number (p.lanes); fixed ones have the pieces' offsets in the instructions
+// LANES: lanes to a row, or 0 for any number (p.lanes); fixed ones have the pieces' offsets in the instructions (8,192 x
+// 8,192: 61 us, 79 by runtime offsets).  Registers: eight pieces of a row want the 128 that 16 warps leave (129,024 x 2,048 in
+// 80 of them, spilling: 322 us); fewer pieces, and rows that only look for their largest, do better with more warps.
 template <typename T, int READ, int V, int LANES, int MODE>
 __global__ void __maxnreg__(MODE == QUANT_CODES ? 64 : MODE == NORM_CODES || V == 8 ? 128 : 80)
     norm_rows_kernel(const __grid_constant__ NormParams p) {
@@ -466,11 +472,14 @@ __global__ void __maxnreg__(MODE == QUANT_CODES ? 64 : MODE == NORM_CODES || V =
 // ------------------------------------------------------------------------------------------------ backward
 //   g = dy A,  dx = rstd (g - mean(g) - u mean(g u)),  P = sum over rows of dy u,  Q = sum over rows of dy
 // A thread keeps its columns over all of the CTA's rows, so that their P and Q stay in registers; the rows' two sums go over
-// the lanes.  Rows of half a warp to a warp's pieces (norm_back_narrow_kernel) need no barrier.  A wider row is the whole
-// CTA's (norm_back_ring_kernel): rows arrive in shared memory by bulk copies several stages ahead, since a barrier per
-// four rows leaves loads by the threads themselves no time in flight (32,768 x 2,048: 120 us by such loads, 77 by the ring).
-// Rows that are not 16-byte aligned arrive as the 16-byte pieces that cover them.  The parts' P and Q are added in order by
-// norm_terms_kernel.  HBM bounds it: 6 bytes per 16-bit element.
+// the lanes.  Rows of up to two pieces to a lane of a warp (norm_back_narrow_kernel) need no barrier.  A wider row is the
+// whole CTA's (norm_back_ring_kernel): rows arrive in shared memory by bulk copies several stages ahead, since a barrier per
+// four rows leaves loads by the threads themselves no time in flight (32,768 x 2,048: 120 us by such loads).  Rows that are
+// not 16-byte aligned arrive as the 16-byte pieces that cover them (16,384 x 4,999: 1,062 us by elements, 252 so).  The
+// parts' P and Q are added in a fixed order by norm_terms_kernel.
+//
+// HBM bounds it: 6 bytes per 16-bit element.  32,768 x 2,048 in bfloat16, modulated: 79 us, 5.1 TB/s; the barriers are the
+// largest stall.  Rows to warps and columns to other warps that meet at mbarriers alone, without any, took 93 us.
 struct NormBackParams {
   const void *dy, *x;
   int64_t gs[2], xs[2];

@@ -105,7 +105,8 @@ int htrc_cross_backward_workspace_size(const HtrcCrossArgs* args, size_t* bytes)
 int htrc_cross_backward(const HtrcCrossArgs* args, htrc_stream_t stream);
 
 /* Layer norm: u = (x - mean) rstd over the width, y = (u weight + bias) (1 + scale) + shift, rstd = 1 / sqrt(variance +
- * eps).  Rows are [batch][token][width] through their strides (batch, token; the width's is 1). */
+ * eps).  Rows are [batch][token][width] through their strides (batch, token; the width's is 1); rows that are not 16-byte
+ * aligned may be read in the whole 16-byte pieces that cover them. */
 enum { HTRC_NORM_MAX_WIDTH = 16384 };
 
 typedef struct {

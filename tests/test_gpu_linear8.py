@@ -249,6 +249,27 @@ def test_streams_graphs_and_repeats(dev):
     htrc_b200.int8_linear_status()
 
 
+def test_no_rows_and_calls_on_two_streams_at_once(dev):
+    gen = torch.Generator(device=dev).manual_seed(17)
+    w = _rows(gen, dev, 300, 256)
+    none = Int8Rows(w.codes[:0], w.scales[:0])
+    assert htrc_b200.int8_linear(none, w).shape == (0, 300)
+    assert htrc_b200.int8_linear(torch.empty((2, 0, 256), device=dev), w).shape == (2, 0, 300)
+    cases = [(torch.randn((n, k), generator=gen, device=dev).half(), _rows(gen, dev, m, k))
+             for n, k, m in ((5, 512, 700), (16, 4096, 300), (40, 1000, 520), (900, 256, 8200), (5000, 384, 1100))]
+    want = [htrc_b200.int8_linear(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    got = []
+    for k in range(4):
+        for i, c in enumerate(cases):
+            with torch.cuda.stream(streams[(i + k) % 2]):
+                got.append((i, htrc_b200.int8_linear(*c)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i, g in got)
+    htrc_b200.int8_linear_status()
+
+
 def test_refusals(dev):
     x = torch.zeros((4, 64), device=dev).bfloat16()
     w = htrc_b200.quantize_rows(torch.ones((8, 64), device=dev))

@@ -356,6 +356,61 @@ def test_streams_and_graphs(dev):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_empty_batches_and_broadcast_gradients(dev):
+    gen = torch.Generator(device=dev).manual_seed(14)
+    for shape in ((0, 4, 96), (3, 0, 96), (0, 96)):
+        x = torch.empty(shape, device=dev)
+        kw = _params(gen, dev, "wb" if len(shape) == 2 else "wbst", shape[0], 96, torch.float32)
+        y, mean, rstd = htrc_b200.layer_norm(x, **kw, return_stats=True)
+        assert y.shape == x.shape and mean.shape == rstd.shape == x.shape[:-1]
+        dx, *grads = htrc_b200.layer_norm_backward(y, x, mean, rstd, **kw)
+        assert dx.shape == x.shape and all(g is None or (g == 0).all() for g in grads)
+        assert htrc_b200.layer_norm_int8(x, **kw).codes.shape == htrc_b200.quantize_rows(x).codes.shape == x.shape
+    # an upstream gradient that is one value, and one that is the same row for all tokens
+    x = torch.randn((2, 70, 520), generator=gen, device=dev).bfloat16().requires_grad_()
+    row = torch.randn(520, generator=gen, device=dev).bfloat16()
+    for dy in (torch.ones((), device=dev).bfloat16().expand(2, 70, 520), row.expand(2, 70, 520)):
+        y, mean, rstd = htrc_b200.layer_norm(x, return_stats=True)
+        (g,) = torch.autograd.grad(y, x, dy)
+        _check_backward((g, None, None, None, None), dy, x.detach(), mean, rstd, {})
+
+
+def test_offsets_past_32_bits(dev):
+    gen = torch.Generator(device=dev).manual_seed(15)
+    x = torch.randn((1, 140000, 16384), generator=gen, device=dev, dtype=torch.bfloat16)
+    y, mean, rstd = htrc_b200.layer_norm(x, return_stats=True)
+    dx = htrc_b200.layer_norm_backward(y, x, mean, rstd)[0]
+    for a in (0, 131060, 139990):
+        some = slice(a, a + 10)
+        want, off, *_ = _plain(x[:, some], {})
+        _close(y[:, some], want, off)
+        _check_backward((dx[:, some], None, None, None, None), y[:, some], x[:, some], mean[:, some], rstd[:, some], {})
+
+
+def test_calls_on_two_streams_at_once(dev):
+    gen = torch.Generator(device=dev).manual_seed(16)
+    cases = []
+    for width in (2048, 768, 1001, 128):
+        x = torch.randn((2, 900, width), generator=gen, device=dev).bfloat16()
+        cases.append((x, torch.randn(x.shape, generator=gen, device=dev).bfloat16(),
+                      _params(gen, dev, "wbst", 2, width, torch.bfloat16)))
+
+    def step(x, dy, kw):
+        y, mean, rstd = htrc_b200.layer_norm(x, **kw, return_stats=True)
+        return (y, *htrc_b200.layer_norm_backward(dy, x, mean, rstd, **kw), *htrc_b200.layer_norm_int8(x, **kw))
+    want = [step(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    got = []
+    for k in range(3):
+        for i, c in enumerate(cases):
+            with torch.cuda.stream(streams[(i + k) % 2]):
+                got.append((i, step(*c)))
+    torch.cuda.synchronize()
+    for i, g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i]))
+
+
 def test_refusals(dev):
     x = torch.zeros((2, 3, 64), device=dev)
     w = torch.ones(64, device=dev)

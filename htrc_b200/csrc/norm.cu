@@ -215,14 +215,22 @@ __device__ __forceinline__ void over_lanes(float (&v)[R], int L, int group, floa
   }
 }
 
+// Rows to a lane of V pieces of each.  Two 16-bit rows of several warps share the reading of A and B (16,384 x 5,120: 85 us one by
+// one, 66 so; a warp's: 129,024 x 2,048 171 and 190; float32, 32,768 x 1,536: 69 and 73).
+template <typename T, int READ, int V, int LANES, int MODE>
+constexpr int rows_of() {
+  if (V == 8 && LANES >= 64 && MODE == NORM_ROWS && READ == BY_16 && sizeof(T) == 2) return 2;
+  return V >= 8 ? 1 : V == 1 ? 4 : 8 / V;
+}
+
 // LANES: lanes to a row, or 0 for any number (p.lanes); fixed ones have the pieces' offsets in the instructions (8,192 x
-// 8,192: 61 us, 79 by runtime offsets).  Registers: eight pieces of a row want the 128 that 16 warps leave (129,024 x 2,048 in
+// 8,192, a row at a time: 61 us, 79 by runtime offsets).  Registers: eight pieces of a row want the 128 that 16 warps leave (129,024 x 2,048 in
 // 80 of them, spilling: 322 us); fewer pieces, and rows that only look for their largest, do better with more warps.
 template <typename T, int READ, int V, int LANES, int MODE>
 __global__ void __maxnreg__(MODE == QUANT_CODES ? 64 : MODE == NORM_CODES || V == 8 ? 128 : 80)
     norm_rows_kernel(const __grid_constant__ NormParams p) {
   using P = Piece<T, READ>;
-  constexpr int N = P::N, H = N / 2, R = V >= 8 ? 1 : V == 1 ? 4 : 8 / V;
+  constexpr int N = P::N, H = N / 2, R = rows_of<T, READ, V, LANES, MODE>();
   extern __shared__ __align__(16) float terms[];
   __shared__ float slots[2][kNormMaxWarps][4];
   const int L = LANES ? LANES : p.lanes, at = threadIdx.x & (L - 1), G = blockDim.x / L, group = threadIdx.x / L;
@@ -1018,7 +1026,7 @@ bool allow_smem(const void* kernel, size_t smem) {
 
 template <typename T, int READ, int MODE, int V, int LANES>
 int norm_run(NormParams& p, cudaStream_t st) {
-  constexpr int N = Piece<T, READ>::N, R = V >= 8 ? 1 : V == 1 ? 4 : 8 / V;
+  constexpr int N = Piece<T, READ>::N, R = rows_of<T, READ, V, LANES, MODE>();
   auto kernel = norm_rows_kernel<T, READ, V, LANES, MODE>;
   if (LANES) p.lanes = LANES;
   const size_t smem = MODE != QUANT_CODES && p.affine ? static_cast<size_t>(p.nvec) * N * 2 * sizeof(float) : 0;

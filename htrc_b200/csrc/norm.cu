@@ -216,19 +216,27 @@ __device__ __forceinline__ void over_lanes(float (&v)[R], int L, int group, floa
 }
 
 // Rows to a lane of V pieces of each.  Two 16-bit rows of several warps share the reading of A and B (16,384 x 5,120: 85 us one by
-// one, 66 so; a warp's: 129,024 x 2,048 171 and 190; float32, 32,768 x 1,536: 69 and 73).
+// one, 66 so; a warp's: 129,024 x 2,048 171 and 190; float32, 32,768 x 1,536: 69 and 73).  A norm's 8-bit rows, whose results stay
+// in registers, do better one by one with more warps (16 bits, 65,536 x 1,024: 57 us by two, 50 so; 100,000 x 512: 52 by four,
+// 42; float32, 65,536 x 512: 34 by four, 37).
 template <typename T, int READ, int V, int LANES, int MODE>
 constexpr int rows_of() {
   if (V == 8 && LANES >= 64 && MODE == NORM_ROWS && READ == BY_16 && sizeof(T) == 2) return 2;
+  if ((V == 2 || V == 4) && MODE == NORM_CODES && READ == BY_16 && sizeof(T) == 2) return 1;
   return V >= 8 ? 1 : V == 1 ? 4 : 8 / V;
+}
+template <typename T, int READ, int V, int MODE>
+constexpr int registers_of() {
+  if (MODE == QUANT_CODES) return 64;
+  if (MODE == NORM_CODES) return READ != BY_16 || sizeof(T) == 4 || V == 1 || V == 8 ? 128 : V == 4 ? 80 : 64;
+  return V == 8 ? 128 : 80;
 }
 
 // LANES: lanes to a row, or 0 for any number (p.lanes); fixed ones have the pieces' offsets in the instructions (8,192 x
 // 8,192, a row at a time: 61 us, 79 by runtime offsets).  Registers: eight pieces of a row want the 128 that 16 warps leave (129,024 x 2,048 in
 // 80 of them, spilling: 322 us); fewer pieces, and rows that only look for their largest, do better with more warps.
 template <typename T, int READ, int V, int LANES, int MODE>
-__global__ void __maxnreg__(MODE == QUANT_CODES ? 64 : MODE == NORM_CODES || V == 8 ? 128 : 80)
-    norm_rows_kernel(const __grid_constant__ NormParams p) {
+__global__ void __maxnreg__((registers_of<T, READ, V, MODE>())) norm_rows_kernel(const __grid_constant__ NormParams p) {
   using P = Piece<T, READ>;
   constexpr int N = P::N, H = N / 2, R = rows_of<T, READ, V, LANES, MODE>();
   extern __shared__ __align__(16) float terms[];
@@ -386,7 +394,7 @@ __global__ void __maxnreg__(MODE == QUANT_CODES ? 64 : MODE == NORM_CODES || V =
           }
         }
       } else {
-        // a norm's results stay in float32 until the row's largest is known
+        // a norm's results stay in float32 until the row's largest is known (129,024 x 2,048: 157 us; formed again then: 267)
         float2 y[MODE == NORM_CODES ? R : 1][MODE == NORM_CODES ? V : 1][H];
         float top[R];
 #pragma unroll

@@ -137,7 +137,7 @@ def quantize_rows(x):
     if w > _lib.NORM_MAX_WIDTH:
         raise NotImplementedError(f"rows of up to {_lib.NORM_MAX_WIDTH} elements are supported, got {w}")
     codes, pitch = _new_codes(shape, x)
-    scales = x.new_empty(shape[:-1], dtype=torch.float32)
+    scales = torch.empty_strided(shape[:-1], _dense(shape[:-1]), dtype=torch.float32, device=x.device)
     check(lib().htrc_quantize_rows(kept.data_ptr(), _DTYPES[x.dtype], b, n, w, (ctypes.c_int64 * 2)(sb, sn),
                                    codes.data_ptr(), pitch, scales.data_ptr(), _lib.raw_stream(x.device.index)),
           "htrc_quantize_rows")

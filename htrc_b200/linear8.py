@@ -49,6 +49,8 @@ def _pitch(codes):
     shape, stride = codes.shape, codes.stride()
     if codes.data_ptr() & 15 or (stride[-1] != 1 and shape[-1] != 1):
         return None
+    if 0 in shape[:-1]:                   # no rows, whatever their strides
+        return (shape[-1] + 15) // 16 * 16
     pitch = covered = None
     for i in range(len(shape) - 2, -1, -1):
         n = shape[i]

@@ -49,7 +49,7 @@ struct Linear8Params {
 
 __device__ __forceinline__ float bias_at(const Linear8Params& p, int n) {
   if (p.bias == nullptr) return 0.f;
-  if (p.bias_dtype == HTRC_LAYER_F32) return __ldg(static_cast<const float*>(p.bias) + n);
+  if (p.bias_dtype == HTRC_LAYER_F32) return static_cast<const float*>(p.bias)[n];
   if (p.bias_dtype == HTRC_LAYER_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n]);
   return __half2float(static_cast<const __half*>(p.bias)[n]);
 }
@@ -109,7 +109,7 @@ struct SmallBars {
   uint64_t full[kSmallStages], empty[kSmallStages], done, rows;
   uint32_t tmem;
   int abort_flag;
-  float scales[kFewTokens];
+  alignas(16) float scales[64];                            // the tokens'
 };
 static_assert(sizeof(SmallBars) <= 1024, "barriers");
 
@@ -138,7 +138,7 @@ __device__ __forceinline__ float quantise_row(const X* x, int width, bool vec, i
     for (int i = lane; i < vecs; i += 8 * 32) {
       Sixteen t[8];                                         // in flight together
 #pragma unroll
-      for (int b = 0; b < 8; ++b) t[b].v = i + 32 * b < vecs ? __ldg(reinterpret_cast<const uint4*>(x) + i + 32 * b) : make_uint4(0, 0, 0, 0);
+      for (int b = 0; b < 8; ++b) t[b].v = i + 32 * b < vecs ? reinterpret_cast<const uint4*>(x)[i + 32 * b] : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int b = 0; b < 8; ++b)
 #pragma unroll
@@ -165,7 +165,7 @@ __device__ __forceinline__ float quantise_row(const X* x, int width, bool vec, i
       Sixteen t[8];
 #pragma unroll
       for (int b = 0; b < 8; ++b)
-        t[b].v = k + 32 * N * b < k1 ? __ldg(reinterpret_cast<const uint4*>(x + k + 32 * N * b)) : make_uint4(0, 0, 0, 0);
+        t[b].v = k + 32 * N * b < k1 ? *reinterpret_cast<const uint4*>(x + k + 32 * N * b) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int b = 0; b < 8; ++b) {
         uint32_t w[2] = {0, 0};
@@ -193,6 +193,8 @@ __device__ __forceinline__ float quantise_row(const X* x, int width, bool vec, i
   return __fdiv_rn(top, 127.f);
 }
 
+// The kernel may be resident while the one before it still writes the rows, scales or bias: behind griddepcontrol.wait they are
+// read by ordinary loads, since those of the read-only path want data that is constant for the kernel's whole life.
 template <int T, typename O, typename X>
 __global__ void __launch_bounds__(SmallShape<T, X>::kThreads, 1)
     linear8_small_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
@@ -229,7 +231,8 @@ __global__ void __launch_bounds__(SmallShape<T, X>::kThreads, 1)
   const int n0 = tile / p.tiles_m * kSmallChannels, row0 = tile % p.tiles_m * T;
   const int b0 = static_cast<int>(static_cast<int64_t>(p.blocks) * rank / splits);
   const int b1 = static_cast<int>(static_cast<int64_t>(p.blocks) * (rank + 1) / splits);
-  auto row_scale = [&](int64_t r) { return SM::kCodes ? __ldg(p.xs + r) : bars->scales[r & (kFewTokens - 1)]; };
+  const int n = n0 + 32 * (warp & 3) + lane;              // warps 0-3: the thread's channel
+  float ws = 0.f, bias = 0.f;
 
   if (warp == kTma) {
     if (lane == 0 && aligned) {
@@ -294,12 +297,20 @@ __global__ void __launch_bounds__(SmallShape<T, X>::kThreads, 1)
       if (lane == 0) mbar_arrive(&bars->rows);
     }
     if (warp < 4) {
-      const int n = n0 + 32 * warp + lane;
       const bool in = n < p.channels;
       if (SM::kCodes) asm volatile("griddepcontrol.wait;" ::: "memory");
-      const float ws = in ? __ldg(p.ws + n) : 0.f, bias = in ? bias_at(p, n) : 0.f;
+      if (in) {
+        ws = p.ws[n];
+        bias = bias_at(p, n);
+      }
       O* out = static_cast<O*>(p.out) + n;
-      bool ok = SM::kCodes || mbar_wait_warp(&bars->rows, 0, p.status, abort_flag);      // the other warps' scales
+      bool ok = true;
+      if constexpr (SM::kCodes) {
+        if (threadIdx.x < T) bars->scales[threadIdx.x] = row0 + threadIdx.x < p.rows ? p.xs[row0 + threadIdx.x] : 0.f;
+        named_bar_sync(1, 128);
+      } else {
+        ok = mbar_wait_warp(&bars->rows, 0, p.status, abort_flag);       // the other warps' scales
+      }
       ok = mbar_wait_warp(&bars->done, 0, p.status, abort_flag) && ok && *abort_flag == 0;
       tc_fence_after();
       const uint32_t at = tmem + (static_cast<uint32_t>(32 * warp) << 16);
@@ -314,9 +325,14 @@ __global__ void __launch_bounds__(SmallShape<T, X>::kThreads, 1)
             for (int t = 0; t < 16; ++t) part[(t0 + t) * kSmallChannels + 32 * warp + lane] = static_cast<int>(v[t]);
           } else {
 #pragma unroll
-            for (int t = 0; t < 16; ++t) {
-              const int64_t r = row0 + t0 + t;
-              if (in && r < p.rows) out[r * p.channels] = from_f<O>(scaled(static_cast<int>(v[t]), row_scale(r), ws, bias));
+            for (int t = 0; t < 16; t += 4) {
+              const float4 s4 = *reinterpret_cast<const float4*>(bars->scales + t0 + t);
+              const float xs[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int64_t r = row0 + t0 + t + j;
+                if (in && r < p.rows) out[r * p.channels] = from_f<O>(scaled(static_cast<int>(v[t + j]), xs[j], ws, bias));
+              }
             }
           }
         }
@@ -326,30 +342,26 @@ __global__ void __launch_bounds__(SmallShape<T, X>::kThreads, 1)
   if (splits > 1) {
     __syncwarp();
     cluster_sync();
-    if (warp < 4) {
-      const int n = n0 + 32 * warp + lane;
-      if (n < p.channels) {
-        const float ws = __ldg(p.ws + n), bias = bias_at(p, n);
-        const int rows = min(T, p.rows - row0), share = T / splits, first = rank * share;
-        constexpr int kBatch = T / 8 < 8 ? T / 8 : 8;       // tokens whose parts are in flight together
-        for (int t0 = first; t0 < min(first + share, rows); t0 += kBatch) {
-          const uint32_t mine = smem_u32(ring) + (t0 * kSmallChannels + 32 * warp + lane) * 4;
-          int sum[kBatch];
+    if (warp < 4 && n < p.channels) {
+      const int rows = min(T, p.rows - row0), share = T / splits, first = rank * share;
+      constexpr int kBatch = T / 8 < 8 ? T / 8 : 8;         // tokens whose parts are in flight together
+      for (int t0 = first; t0 < min(first + share, rows); t0 += kBatch) {
+        const uint32_t mine = smem_u32(ring) + (t0 * kSmallChannels + 32 * warp + lane) * 4;
+        int sum[kBatch];
 #pragma unroll
-          for (int j = 0; j < kBatch; ++j) sum[j] = 0;
-          for (int c = 0; c < splits; ++c) {
-            const uint32_t at = in_cta(mine, c);
-            int v[kBatch];
+        for (int j = 0; j < kBatch; ++j) sum[j] = 0;
+        for (int c = 0; c < splits; ++c) {
+          const uint32_t at = in_cta(mine, c);
+          int v[kBatch];
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) v[j] = load_cluster(at + j * kSmallChannels * 4);
+          for (int j = 0; j < kBatch; ++j) v[j] = load_cluster(at + j * kSmallChannels * 4);
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) sum[j] += v[j];
-          }
-          O* out = static_cast<O*>(p.out) + static_cast<int64_t>(row0 + t0) * p.channels + n;
-#pragma unroll
-          for (int j = 0; j < kBatch; ++j)
-            if (t0 + j < rows) out[static_cast<int64_t>(j) * p.channels] = from_f<O>(scaled(sum[j], row_scale(row0 + t0 + j), ws, bias));
+          for (int j = 0; j < kBatch; ++j) sum[j] += v[j];
         }
+        O* out = static_cast<O*>(p.out) + static_cast<int64_t>(row0 + t0) * p.channels + n;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+          if (t0 + j < rows) out[static_cast<int64_t>(j) * p.channels] = from_f<O>(scaled(sum[j], bars->scales[t0 + j], ws, bias));
       }
     }
     __syncwarp();

@@ -171,7 +171,8 @@ def int8_linear(x, weight, *, bias=None, dtype=None):
         wc, ws = weight
         rows, xs = (x, None) if floats else x
         key = (_meta(rows), None if floats else _meta(xs), _meta(wc), _meta(ws), None if bias is None else _meta(bias), dtype)
-        plan = None if wc.data_ptr() & 15 or (not floats and rows.data_ptr() & 15) else _plans.get(key)
+        kept = isinstance(weight, tuple) and (floats or isinstance(x, tuple))       # (pairs of another type are refused)
+        plan = _plans.get(key) if kept and not (wc.data_ptr() & 15 or (not floats and rows.data_ptr() & 15)) else None
         _refuse_gradients("int8_linear", rows, xs, ws, bias)
     except (AttributeError, TypeError, ValueError):       # no tensors: the checks say so
         key = plan = None

@@ -25,14 +25,14 @@ from .linear8 import Int8Rows, _check_float_rows, _dense, _DTYPES, _new_codes, _
 
 
 def _term(t, name, shapes, width, device):
-    """(tensor, pointer, type) of a parameter of one of the shapes, its last dimension dense; (None, 0, 0) of None."""
+    """(tensor, type) of a parameter of one of the shapes, its last dimension dense; (None, 0) of None."""
     if t is None:
-        return None, 0, 0
+        return None, 0
     if not isinstance(t, torch.Tensor) or t.shape not in shapes or t.dtype not in _DTYPES or t.device != device:
         raise ValueError(f"{name}: {list(shapes[0])} float32, bfloat16 or float16 on x's device expected")
     if width != 1 and t.stride(-1) != 1:
         t = t.contiguous()
-    return t, t.data_ptr(), _DTYPES[t.dtype]
+    return t, _DTYPES[t.dtype]
 
 
 class _Call:
@@ -68,17 +68,6 @@ class _Call:
     def dense(self):
         """(batch, token) strides of dense rows."""
         return self.sizes[3] * self.sizes[4], self.sizes[4]
-
-
-def _term(t, name, shapes, width, device):
-    """(tensor, type) of a parameter of one of the shapes, its last dimension dense; (None, 0) of None."""
-    if t is None:
-        return None, 0
-    if not isinstance(t, torch.Tensor) or t.shape not in shapes or t.dtype not in _DTYPES or t.device != device:
-        raise ValueError(f"{name}: {list(shapes[0])} float32, bfloat16 or float16 on x's device expected")
-    if width != 1 and t.stride(-1) != 1:
-        t = t.contiguous()
-    return t, _DTYPES[t.dtype]
 
 
 _plans = {}

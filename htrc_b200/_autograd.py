@@ -8,13 +8,16 @@ from torch.autograd import forward_ad
 
 def recorded(*tensors):
     """Whether a call with these inputs goes through its autograd function: to record it, or to be refused there because
-    one of them carries a forward-mode tangent (the functions have no jvp)."""
+    one of them carries a forward-mode tangent (the functions have no jvp).  What is no tensor is left to the call's checks."""
     if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
+        try:
+            for t in tensors:
+                if t is not None and t.requires_grad:
+                    return True
+        except AttributeError:
+            return False
     if forward_ad._current_level >= 0:
-        return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+        return any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
     return False
 
 

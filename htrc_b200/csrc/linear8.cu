@@ -12,7 +12,7 @@
 //
 // Measured, 8-bit rows, bfloat16 out: 129,024 x 2,048 x 6,144 1,090 us after a rest (2,980 TOP/s) and 1,270 once the 1,000 W cap
 // holds the SM clock at 1,290 MHz; 8,192 x 8,192 x 8,192 335 (3,280) and 395.  The tensor pipe is busy for 82 % of 16,384 x
-// 2,048 x 6,144; the cap bounds the rest.  16 x 4,096 x 16,384: 14.1 us, the weights at 4.8 TB/s.
+// 2,048 x 6,144; the cap bounds the rest.  16 x 4,096 x 16,384: 14.6 us, the weights at 4.6 TB/s.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -225,6 +225,8 @@ constexpr int rows_of() {
   if ((V == 2 || V == 4) && MODE == NORM_CODES && READ == BY_16 && sizeof(T) == 2) return 1;
   return V >= 8 ? 1 : V == 1 ? 4 : 8 / V;
 }
+// (-Xptxas -v: 8-bit rows from two and four 16-byte pieces of 16-bit elements spill 32 bytes in their 64 and 80 registers, from
+// eight 52 to 64 in 128; results of sixteen unaligned pieces 156 in 80)
 template <typename T, int READ, int V, int MODE>
 constexpr int registers_of() {
   if (MODE == QUANT_CODES) return 64;
@@ -495,7 +497,8 @@ __global__ void __maxnreg__((registers_of<T, READ, V, MODE>())) norm_rows_kernel
 // parts' P and Q are added in a fixed order by norm_terms_kernel.
 //
 // HBM bounds it: 6 bytes per 16-bit element.  32,768 x 2,048 in bfloat16, modulated: 79 us, 5.1 TB/s; the barriers are the
-// largest stall.  Rows to warps and columns to other warps that meet at mbarriers alone, without any, took 93 us.
+// largest stall.  In float32 133 us, 6.1 TB/s.  Rows to warps and columns to other warps that meet at mbarriers alone, without
+// any, took 93 us.
 struct NormBackParams {
   const void *dy, *x;
   int64_t gs[2], xs[2];
@@ -1142,7 +1145,8 @@ struct NormBackPlan {
     const int n = reads == BY_16 ? 16 / es : 2, nvec = (width + n - 1) / n;
     int resident, least;                    // CTAs of an SM, rows that a CTA takes at a time
     lanes = stages = 0;
-    // rows to warps: 128 wide 36 us (200,000 rows in 16 bits), by the ring 67; 256 wide 36 and 42; 512 wide 68 either way
+    // rows to warps: 200,000 x 128 in 16 bits 38 us, by the ring 68; 200,000 x 256 66 and 70; 100,000 x 512 70 and 68; float32,
+    // 200,000 x 128 63 and 63, 100,000 x 256 60 and 58
     narrow = reads == BY_16 && nvec <= 64;
     if (narrow) {
       lanes = nvec <= 8 ? 8 : nvec <= 16 ? 16 : 32;
